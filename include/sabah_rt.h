@@ -276,6 +276,91 @@ int sabah_moe_prefill_layer(const sabah_moe_layer_desc *layer, const float *d_x,
 int sabah_moe_route(const float *d_logits, int n_tokens, int n_experts, int n_used, int norm_w,
                     float w_scale, int32_t *d_ids, float *d_w, void *stream);
 
+/* ---- adapting a frozen bank ------------------------------------------------ */
+
+/* The operators below have no reference counterpart (the reference only runs a
+ * model).  Their device scratch is the caller's: *_workspace gives its bytes for
+ * a call, 16-byte aligned device memory that no other call may use until
+ * this one has run, whose content need not be set before and means nothing after.  They
+ * allocate nothing and never synchronise, so they can be captured as they are;
+ * the same inputs give the same bits.  The calling thread's current device may be another one. */
+
+/* The router's balance loss and z loss with the per-expert counts they need, over
+ * the tokens that d_mask (uint8 [n_tokens], NULL: all) leaves valid; a token whose
+ * logits are all minus infinity counts as masked.  The tokens form n_groups
+ * groups of equal length (the sequences of a padded batch; 1: the whole batch).
+ *   p = softmax(logits[t]), lse = log(sum(exp(logits[t])))
+ *   d_counts[g][e]  = valid (token, slot) pairs of the group with d_ids[t][j] == e
+ *   d_mean_p[g][e]  = mean of p[e] over the group's valid tokens (0 without any)
+ *   d_losses[0]     = mean over the groups with a valid token of
+ *                     n_experts * sum_e counts[g][e] / (valid_g * n_used) * mean_p[g][e]
+ *   d_losses[1]     = mean of lse^2 over the valid tokens;  both 0 without any
+ *   d_n_valid[g]    = valid tokens of group g; [n_groups]: of all; [n_groups + 1]: groups with any
+ * logits: rows of n_experts f32, logits_stride bytes apart; d_ids: int32 [n_tokens][n_used] as
+ * sabah_moe_route writes them.  n_experts <= 4096, n_used <= min(n_experts, 64),
+ * n_tokens <= 2^24 and a multiple of n_groups.  An id out of range is not counted and fails the
+ * next call.  Of masked tokens neither logits nor ids are read. */
+size_t sabah_moe_balance_workspace(int n_tokens, int n_experts, int n_groups);
+int sabah_moe_balance(const float *d_logits, size_t logits_stride, const int32_t *d_ids, const uint8_t *d_mask,
+                      int n_tokens, int n_experts, int n_used, int n_groups, int32_t *d_counts, float *d_mean_p,
+                      float *d_losses, int32_t *d_n_valid, void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* The gradient of the router's logits, in one pass over them: what comes back
+ * through sabah_moe_route's weights (d_dw [n_tokens][n_used], NULL: nothing; the same ids, norm_w
+ * and w_scale as there), plus c_balance times the gradient of losses[0] and c_z times that of
+ * losses[1] (with sabah_moe_balance's d_counts and d_n_valid for the same mask and groups; the
+ * counts are constants of the gradient; both may be NULL when c_balance and c_z are 0).
+ * Every row of d_dlogits is written: zeros for a masked token, whose inputs are not
+ * read, and for a row of minus infinities only.  An expert named twice by a token gets both parts.
+ * An id out of range makes its token's row NaN and fails the next call. */
+int sabah_moe_route_backward(const float *d_logits, size_t logits_stride, const int32_t *d_ids, const uint8_t *d_mask,
+                             int n_tokens, int n_experts, int n_used, int norm_w, float w_scale, const float *d_dw,
+                             const int32_t *d_counts, const int32_t *d_n_valid, int n_groups, float c_balance, float c_z,
+                             float *d_dlogits, size_t dlogits_stride, void *stream);
+
+/* Low-rank adapters of a projection, one (A, B) pair for each (adapter, expert); a
+ * dense projection has one expert.  type: ggml's code of A and B, F32 0, F16 1 or
+ * BF16 30.  rank <= 128; an adapter of a lower rank says so in ranks (the
+ * values past it are not used) or pads A and B with zeros. */
+typedef struct sabah_lora_desc {
+    const void *a;            /* device [n_adapters][n_experts][rank][k] */
+    const void *b;            /* device [n_adapters][n_experts][rows][rank] */
+    const float *scale;       /* device [n_adapters], NULL: 1 */
+    const int32_t *ranks;     /* device [n_adapters], each in [0, rank] (clamped to it), NULL: rank */
+    int type;
+    int n_adapters, n_experts, rank, k, rows;
+} sabah_lora_desc;
+
+/* Each token's adapter beside a projection that all of them share:
+ *   dst[t][i][0..rows) = base[t][i] + scale[a] * B[a][e] (A[a][e] x[t][i % x_rows]),
+ *   a = d_adapters[t] (-1: none, dst = base), e = d_ids[t][i] (0 when d_ids is NULL, which needs
+ *   n_experts == 1)
+ * with x, ids and dst addressed as in sabah_rt_mul_mat_id_v2, whose dst is the base
+ * (base may be dst itself, with the same strides: rows without an adapter are then not touched;
+ * NULL: zeros).  All strides are bytes and multiples of 4; x and dst must not overlap; at most 2^24
+ * rows.  Sums are f32.  An adapter or expert id out of range makes its row NaN and fails
+ * the next call. */
+size_t sabah_lora_workspace(const sabah_lora_desc *lora, int n_ids, int n_tokens, int backward);
+int sabah_lora_apply(const sabah_lora_desc *lora, const float *d_x, size_t x_id_stride, int x_rows,
+                     size_t x_token_stride, const int32_t *d_adapters, const int32_t *d_ids, size_t ids_id_stride,
+                     size_t ids_token_stride, int n_ids, int n_tokens, const float *d_base, size_t base_id_stride,
+                     size_t base_token_stride, float *d_dst, size_t dst_id_stride, size_t dst_token_stride,
+                     void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* The gradients of sabah_lora_apply for dy[t][i][0..rows), that of dst:
+ *   dx[t][i][0..k) = scale A^T B^T dy[t][i]: one row per (token, slot), also when
+ *                    x has one row per token (the caller adds the slots up);
+ *                    zeros for a row without an adapter; added to dx with add_dx
+ *   d_da, d_db     f32 in the layouts of A and B, written for every adapter and expert (zeros where no
+ *                  row uses the pair and past an adapter's own rank); added to them with add_dw
+ * Each of d_dx, d_da and d_db may be NULL.  A row with an id out of range gives no part of d_da and
+ * d_db, its dx is NaN, and the next call fails. */
+int sabah_lora_backward(const sabah_lora_desc *lora, const float *d_x, size_t x_id_stride, int x_rows,
+                        size_t x_token_stride, const int32_t *d_adapters, const int32_t *d_ids, size_t ids_id_stride,
+                        size_t ids_token_stride, int n_ids, int n_tokens, const float *d_dy, size_t dy_id_stride,
+                        size_t dy_token_stride, float *d_dx, size_t dx_id_stride, size_t dx_token_stride, int add_dx,
+                        float *d_da, float *d_db, int add_dw, void *d_workspace, size_t workspace_bytes, void *stream);
+
 /* How sabah_rt_mul_mat_id_v2 runs calls over many tokens.  No reference
  * counterpart: the reference's kernel re-reads an expert per (token, slot)
  * (sabah_rt.cu:2791-2839).  Grouped, the (token, slot) pairs are grouped by

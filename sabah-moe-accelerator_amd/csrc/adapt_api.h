@@ -1,0 +1,339 @@
+// C-ABI entry points of the operators that adapt a frozen bank: adapters
+// (lora_kernels.h), the router's losses and gradient (balance_kernels.h).
+// Included by sabah_rt.hip after its helpers (fail, ck, check_sticky).
+// Their device scratch is the caller's: calls on different streams, or captured in
+// different graphs, share nothing.
+#pragma once
+
+// The calling thread's device is the library's while one lives (a program with
+// several GPUs may have another one current).
+struct OnDevice {
+    int before = -1;
+    bool ok = true;
+    OnDevice() {
+        int now = -1;
+        if (!ck(hipGetDevice(&now), "current device")) {
+            ok = false;
+        } else if (now != g_device) {
+            ok = ck(hipSetDevice(g_device), "set device");
+            before = now;
+        }
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// ---------------------------------------------------------------------------
+// balance loss, counts; the logits' gradient
+// ---------------------------------------------------------------------------
+constexpr int kBalanceChunkTokens = 16;      // tokens per workgroup of k_balance_rows, four per wave
+constexpr int kBalanceMaxChunks = 2048;      // workgroups at most: a larger batch has longer runs
+
+static void balance_plan(int n_tokens, int n_groups, int& chunks, int& chunk_len) {
+    const int len = n_tokens / n_groups;
+    const int most = std::max(1, kBalanceMaxChunks / n_groups);
+    chunk_len = std::max(kBalanceChunkTokens, (len + most - 1) / most);
+    chunks = std::max(1, (len + chunk_len - 1) / chunk_len);
+}
+
+struct BalanceSpace {
+    size_t p, c, z, loss, ticket, bytes;
+};
+static BalanceSpace balance_space(int n_tokens, int n_experts, int n_groups) {
+    int chunks, len;
+    balance_plan(n_tokens, n_groups, chunks, len);
+    const size_t parts = (size_t)n_groups * chunks;
+    BalanceSpace s{};
+    s.p = 0;
+    s.c = s.p + align256(parts * n_experts * 4);
+    s.z = s.c + align256(parts * n_experts * 4);
+    s.loss = s.z + align256(parts * 8);
+    s.ticket = s.loss + align256((size_t)n_groups * ((n_experts + 63) / 64) * 8);
+    s.bytes = s.ticket + 256;
+    return s;
+}
+
+static int check_router_shape(const char* what, int n_tokens, int n_experts, int n_used, int n_groups) {
+    if (n_experts <= 0 || n_experts > kRouteThreads * kRouteMaxPerThread)
+        return fail("%s: n_experts %d outside [1, %d]", what, n_experts, kRouteThreads * kRouteMaxPerThread);
+    if (n_used <= 0 || n_used > n_experts || n_used > kRouteMaxUsed)
+        return fail("%s: n_used %d outside [1, min(n_experts, %d)]", what, n_used, kRouteMaxUsed);
+    if (n_tokens < 0 || n_tokens > 1 << 24) return fail("%s: n_tokens %d outside [0, %d]", what, n_tokens, 1 << 24);
+    if (n_groups <= 0 || n_groups > 65535 || n_tokens % n_groups)
+        return fail("%s: n_groups %d does not divide %d tokens, or is outside [1, 65535]", what, n_groups, n_tokens);
+    return 0;
+}
+
+SABAH_API size_t sabah_moe_balance_workspace(int n_tokens, int n_experts, int n_groups) {
+    if (check_router_shape("balance", n_tokens, n_experts, 1, n_groups)) return 0;
+    return balance_space(n_tokens, n_experts, n_groups).bytes;
+}
+
+template <int PER, int W>
+static void launch_balance_rows(const BalanceArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_balance_rows<PER, W>), dim3((unsigned)a.chunks, (unsigned)a.n_groups), dim3(row_threads(W)),
+                       (uint32_t)a.n_experts * 8, st, a);
+}
+
+SABAH_API int sabah_moe_balance(const float* d_logits, size_t logits_stride, const int32_t* d_ids,
+                                const uint8_t* d_mask, int n_tokens, int n_experts, int n_used, int n_groups,
+                                int32_t* d_counts, float* d_mean_p, float* d_losses, int32_t* d_n_valid,
+                                void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (check_router_shape("balance", n_tokens, n_experts, n_used, n_groups)) return -1;
+    if (((!d_logits || !d_ids) && n_tokens) || !d_counts || !d_mean_p || !d_losses || !d_n_valid)
+        return fail("balance: null pointer");
+    if (logits_stride % 4 || logits_stride < (size_t)n_experts * 4)
+        return fail("balance: logits stride %zu below a row of %d floats, or no multiple of 4", logits_stride, n_experts);
+    const BalanceSpace sp = balance_space(n_tokens, n_experts, n_groups);
+    if (!d_workspace || workspace_bytes < sp.bytes || (uintptr_t)d_workspace % 16)
+        return fail("balance: the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", sp.bytes, workspace_bytes);
+    if (g_device < 0) return fail("sabah_rt_init has not been called");
+    if (!check_sticky()) return -1;
+    OnDevice dev;
+    if (!dev.ok) return -1;
+    uint8_t* ws = static_cast<uint8_t*>(d_workspace);
+    BalanceArgs a{};
+    a.logits = reinterpret_cast<const uint8_t*>(d_logits);
+    a.stride = logits_stride;
+    a.ids = d_ids;
+    a.mask = d_mask;
+    a.n_experts = n_experts;
+    a.n_used = n_used;
+    a.n_groups = n_groups;
+    a.group_len = n_tokens / n_groups;
+    balance_plan(n_tokens, n_groups, a.chunks, a.chunk_len);
+    a.part_p = reinterpret_cast<float*>(ws + sp.p);
+    a.part_c = reinterpret_cast<int*>(ws + sp.c);
+    a.part_z = reinterpret_cast<float2*>(ws + sp.z);
+    a.part_loss = reinterpret_cast<double*>(ws + sp.loss);
+    a.ticket = reinterpret_cast<unsigned*>(ws + sp.ticket);
+    a.counts = d_counts;
+    a.mean_p = d_mean_p;
+    a.losses = d_losses;
+    a.n_valid = d_n_valid;
+    a.err = g_err_dev;
+    hipStream_t st = pick_stream(stream);
+    if (n_experts <= 64) launch_balance_rows<1, 1>(a, st);
+    else if (n_experts <= 128) launch_balance_rows<2, 1>(a, st);
+    else if (n_experts <= 256) launch_balance_rows<4, 1>(a, st);
+    else if (n_experts <= 512) launch_balance_rows<8, 1>(a, st);
+    else if (n_experts <= 2048) launch_balance_rows<8, 4>(a, st);
+    else launch_balance_rows<8, 8>(a, st);
+    if (!ck(hipGetLastError(), "balance launch")) return -1;
+    hipLaunchKernelGGL(k_balance_sum, dim3((unsigned)((n_experts + 63) / 64), (unsigned)n_groups), dim3(kBalanceThreads),
+                       0, st, a);
+    return ck(hipGetLastError(), "balance sum launch") ? 0 : -1;
+}
+
+template <int PER, int W>
+static void launch_route_backward(const RouteBackArgs& a, hipStream_t st) {
+    constexpr int kSide = row_threads(W) / (64 * W);               // tokens of a workgroup
+    hipLaunchKernelGGL((k_route_backward<PER, W>), dim3((unsigned)((a.n_tokens + kSide - 1) / kSide)),
+                       dim3(row_threads(W)), 0, st, a);
+}
+
+SABAH_API int sabah_moe_route_backward(const float* d_logits, size_t logits_stride, const int32_t* d_ids,
+                                       const uint8_t* d_mask, int n_tokens, int n_experts, int n_used, int norm_w,
+                                       float w_scale, const float* d_dw, const int32_t* d_counts,
+                                       const int32_t* d_n_valid, int n_groups, float c_balance, float c_z,
+                                       float* d_dlogits, size_t dlogits_stride, void* stream) {
+    if (check_router_shape("route backward", n_tokens, n_experts, n_used, n_groups)) return -1;
+    if (n_tokens && (!d_logits || !d_dlogits || (!d_ids && d_dw))) return fail("route backward: null pointer");
+    if (!(w_scale > 0.0f) || w_scale == __builtin_inff())
+        return fail("route backward: w_scale must be positive and finite");
+    const bool losses = c_balance != 0.0f || c_z != 0.0f;
+    if (losses && (!d_counts || !d_n_valid))
+        return fail("route backward: a loss's gradient needs the counts and n_valid of sabah_moe_balance");
+    if (logits_stride % 4 || dlogits_stride % 4 || logits_stride < (size_t)n_experts * 4 ||
+        dlogits_stride < (size_t)n_experts * 4)
+        return fail("route backward: a stride (%zu, %zu) below a row of %d floats, or no multiple of 4", logits_stride,
+                    dlogits_stride, n_experts);
+    if (g_device < 0) return fail("sabah_rt_init has not been called");
+    if (!check_sticky()) return -1;
+    if (n_tokens == 0) return 0;
+    OnDevice dev;
+    if (!dev.ok) return -1;
+    RouteBackArgs a{};
+    a.logits = reinterpret_cast<const uint8_t*>(d_logits);
+    a.stride = logits_stride;
+    a.ids = d_ids;
+    a.mask = d_mask;
+    a.dw = d_dw;
+    a.counts = losses ? d_counts : nullptr;
+    a.n_valid = d_n_valid;
+    a.dlogits = reinterpret_cast<uint8_t*>(d_dlogits);
+    a.dstride = dlogits_stride;
+    a.n_tokens = n_tokens;
+    a.n_experts = n_experts;
+    a.n_used = n_used;
+    a.norm_w = norm_w ? 1 : 0;
+    a.n_groups = n_groups;
+    a.group_len = n_tokens / n_groups;
+    a.w_scale = w_scale;
+    a.c_balance = c_balance;
+    a.c_z = c_z;
+    a.err = g_err_dev;
+    hipStream_t st = pick_stream(stream);
+    if (n_experts <= 64) launch_route_backward<1, 1>(a, st);
+    else if (n_experts <= 128) launch_route_backward<2, 1>(a, st);
+    else if (n_experts <= 256) launch_route_backward<4, 1>(a, st);
+    else if (n_experts <= 512) launch_route_backward<8, 1>(a, st);
+    else if (n_experts <= 2048) launch_route_backward<8, 4>(a, st);
+    else launch_route_backward<8, 8>(a, st);
+    return ck(hipGetLastError(), "route backward launch") ? 0 : -1;
+}
+
+// ---------------------------------------------------------------------------
+// adapters
+// ---------------------------------------------------------------------------
+// type codes of adapter weights (ggml's F32, F16 and BF16)
+constexpr int kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 30;
+
+static int check_lora(const char* what, const sabah_lora_desc* L, int n_ids, int n_tokens) {
+    if (!L || !L->a || !L->b) return fail("%s: null adapter bank", what);
+    if (L->type != kTypeF32 && L->type != kTypeF16 && L->type != kTypeBF16)
+        return fail("%s: adapter type %d is none of F32 (0), F16 (1), BF16 (30)", what, L->type);
+    if (L->rank <= 0 || L->rank > kLoraMaxRank) return fail("%s: rank %d outside [1, %d]", what, L->rank, kLoraMaxRank);
+    if (L->n_adapters <= 0 || L->n_experts <= 0 || L->k <= 0 || L->rows <= 0 ||
+        (long long)L->n_adapters * L->n_experts > 1 << 24 || L->k > 1 << 24 || L->rows > 1 << 24)
+        return fail("%s: invalid geometry (n_adapters=%d n_experts=%d k=%d rows=%d)", what, L->n_adapters, L->n_experts,
+                    L->k, L->rows);
+    if (n_ids <= 0 || n_tokens < 0 || (long long)n_ids * n_tokens > 1 << 24)
+        return fail("%s: n_ids=%d, n_tokens=%d give no rows, or too many", what, n_ids, n_tokens);
+    return 0;
+}
+
+static bool stride_ok(size_t s) { return s % 4 == 0; }
+
+SABAH_API size_t sabah_lora_workspace(const sabah_lora_desc* lora, int n_ids, int n_tokens, int backward) {
+    if (check_lora("adapters", lora, n_ids, n_tokens)) return 0;
+    return backward ? align256((size_t)n_ids * n_tokens * lora->rank * 8) : 0;
+}
+
+static LoraArgs lora_args(const sabah_lora_desc* L, const float* d_x, size_t x_id_stride, int x_rows,
+                          size_t x_token_stride, const int32_t* d_adapters, const int32_t* d_ids, size_t ids_id_stride,
+                          size_t ids_token_stride, int n_ids, int n_tokens) {
+    LoraArgs a{};
+    a.x = reinterpret_cast<const uint8_t*>(d_x);
+    a.x_id = x_id_stride;
+    a.x_tok = x_token_stride;
+    a.x_rows = x_rows;
+    a.adapters = d_adapters;
+    a.ids = reinterpret_cast<const uint8_t*>(d_ids);
+    a.ids_id = ids_id_stride;
+    a.ids_tok = ids_token_stride;
+    a.n_ids = n_ids;
+    a.n_tokens = n_tokens;
+    a.a = L->a;
+    a.b = L->b;
+    a.scale = L->scale;
+    a.ranks = L->ranks;
+    a.n_adapters = L->n_adapters;
+    a.n_experts = L->n_experts;
+    a.rank = L->rank;
+    a.k = L->k;
+    a.rows = L->rows;
+    a.err = g_err_dev;
+    return a;
+}
+
+static int check_lora_rows(const char* what, const sabah_lora_desc* L, const float* d_x, size_t x_id_stride, int x_rows,
+                           size_t x_token_stride, const int32_t* d_adapters, const int32_t* d_ids, size_t ids_id_stride,
+                           size_t ids_token_stride, int n_ids, int n_tokens) {
+    if (check_lora(what, L, n_ids, n_tokens)) return -1;
+    if (n_tokens && (!d_x || !d_adapters)) return fail("%s: null pointer", what);
+    if (!d_ids && L->n_experts != 1) return fail("%s: %d experts need ids", what, L->n_experts);
+    if (x_rows != 1 && x_rows != n_ids) return fail("%s: %d input rows, expected 1 or n_ids=%d", what, x_rows, n_ids);
+    if (!stride_ok(x_id_stride) || !stride_ok(x_token_stride) || !stride_ok(ids_id_stride) || !stride_ok(ids_token_stride))
+        return fail("%s: strides are in bytes and multiples of 4", what);
+    return 0;
+}
+
+SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, size_t x_id_stride, int x_rows,
+                               size_t x_token_stride, const int32_t* d_adapters, const int32_t* d_ids,
+                               size_t ids_id_stride, size_t ids_token_stride, int n_ids, int n_tokens,
+                               const float* d_base, size_t base_id_stride, size_t base_token_stride, float* d_dst,
+                               size_t dst_id_stride, size_t dst_token_stride, void* d_workspace, size_t workspace_bytes,
+                               void* stream) {
+    (void)d_workspace;
+    (void)workspace_bytes;
+    if (check_lora_rows("adapters", lora, d_x, x_id_stride, x_rows, x_token_stride, d_adapters, d_ids, ids_id_stride,
+                        ids_token_stride, n_ids, n_tokens))
+        return -1;
+    if (n_tokens && !d_dst) return fail("adapters: null pointer");
+    if (!stride_ok(base_id_stride) || !stride_ok(base_token_stride) || !stride_ok(dst_id_stride) ||
+        !stride_ok(dst_token_stride))
+        return fail("adapters: strides are in bytes and multiples of 4");
+    if (d_base == d_dst && (base_id_stride != dst_id_stride || base_token_stride != dst_token_stride))
+        return fail("adapters: base in place of dst needs dst's strides");
+    if (g_device < 0) return fail("sabah_rt_init has not been called");
+    if (!check_sticky()) return -1;
+    if (n_tokens == 0) return 0;
+    OnDevice dev;
+    if (!dev.ok) return -1;
+    LoraArgs a = lora_args(lora, d_x, x_id_stride, x_rows, x_token_stride, d_adapters, d_ids, ids_id_stride,
+                           ids_token_stride, n_ids, n_tokens);
+    a.base = reinterpret_cast<const uint8_t*>(d_base);
+    a.base_id = base_id_stride;
+    a.base_tok = base_token_stride;
+    a.dst = reinterpret_cast<uint8_t*>(d_dst);
+    a.dst_id = dst_id_stride;
+    a.dst_tok = dst_token_stride;
+    hipStream_t st = pick_stream(stream);
+    const dim3 grid((unsigned)(n_ids * n_tokens)), block(kLoraThreads);
+    switch (lora->type) {
+    case kTypeF32: hipLaunchKernelGGL(k_lora_rows<LoraF32>, grid, block, 0, st, a); break;
+    case kTypeF16: hipLaunchKernelGGL(k_lora_rows<LoraF16>, grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL(k_lora_rows<LoraBF16>, grid, block, 0, st, a); break;
+    }
+    return ck(hipGetLastError(), "adapters launch") ? 0 : -1;
+}
+
+SABAH_API int sabah_lora_backward(const sabah_lora_desc* lora, const float* d_x, size_t x_id_stride, int x_rows,
+                                  size_t x_token_stride, const int32_t* d_adapters, const int32_t* d_ids,
+                                  size_t ids_id_stride, size_t ids_token_stride, int n_ids, int n_tokens,
+                                  const float* d_dy, size_t dy_id_stride, size_t dy_token_stride, float* d_dx,
+                                  size_t dx_id_stride, size_t dx_token_stride, int add_dx, float* d_da, float* d_db,
+                                  int add_dw, void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (check_lora_rows("adapters backward", lora, d_x, x_id_stride, x_rows, x_token_stride, d_adapters, d_ids,
+                        ids_id_stride, ids_token_stride, n_ids, n_tokens))
+        return -1;
+    if (n_tokens && !d_dy) return fail("adapters backward: null pointer");
+    if (!stride_ok(dy_id_stride) || !stride_ok(dy_token_stride) || !stride_ok(dx_id_stride) || !stride_ok(dx_token_stride))
+        return fail("adapters backward: strides are in bytes and multiples of 4");
+    const size_t need = sabah_lora_workspace(lora, n_ids, n_tokens, 1);
+    if (need && (!d_workspace || workspace_bytes < need || (uintptr_t)d_workspace % 16))
+        return fail("adapters backward: the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", need,
+                    workspace_bytes);
+    if (g_device < 0) return fail("sabah_rt_init has not been called");
+    if (!check_sticky()) return -1;
+    OnDevice dev;
+    if (!dev.ok) return -1;
+    LoraArgs a = lora_args(lora, d_x, x_id_stride, x_rows, x_token_stride, d_adapters, d_ids, ids_id_stride,
+                           ids_token_stride, n_ids, n_tokens);
+    a.dy = reinterpret_cast<const uint8_t*>(d_dy);
+    a.dy_id = dy_id_stride;
+    a.dy_tok = dy_token_stride;
+    a.dx = reinterpret_cast<uint8_t*>(d_dx);
+    a.dx_id = dx_id_stride;
+    a.dx_tok = dx_token_stride;
+    a.da = d_da;
+    a.db = d_db;
+    a.add_dx = add_dx != 0;
+    a.add_dw = add_dw != 0;
+    a.su = static_cast<float*>(d_workspace);
+    hipStream_t st = pick_stream(stream);
+    const dim3 grid((unsigned)(n_ids * n_tokens)), block(kLoraThreads);
+    if (n_tokens) switch (lora->type) {
+        case kTypeF32: hipLaunchKernelGGL(k_lora_back_rows<LoraF32>, grid, block, 0, st, a); break;
+        case kTypeF16: hipLaunchKernelGGL(k_lora_back_rows<LoraF16>, grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL(k_lora_back_rows<LoraBF16>, grid, block, 0, st, a); break;
+        }
+    if (d_da || d_db)
+        hipLaunchKernelGGL(k_lora_back_weights, dim3((unsigned)(lora->n_adapters * lora->n_experts), (unsigned)lora->rank),
+                           block, 0, st, a);
+    return ck(hipGetLastError(), "adapters backward launch") ? 0 : -1;
+}

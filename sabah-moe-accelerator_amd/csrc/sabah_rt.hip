@@ -19,10 +19,12 @@
 #include <unordered_set>
 #include <vector>
 
+#include "balance_kernels.h"
 #include "dense_kernels.h"
 #include "grouped_rows.h"
 #include "host_decode.h"
 #include "layer_kernels.h"
+#include "lora_kernels.h"
 #include "mmid_kernels.h"
 #include "prefill_kernels.h"
 #include "route_kernels.h"
@@ -347,6 +349,12 @@ bool check_sticky() {
         g_sync_reset_pending = true;
         fail("an earlier fused layer kernel's down workgroups waited too long for its gate/up workgroups "
              "(calls overlapping on different streams?); their rows were set to NaN");
+    } else if (w == kErrRouteId) {
+        fail("an earlier balance or route backward call read an expert id outside [0, n_experts); it was not counted, "
+             "or its token's gradient was set to NaN");
+    } else if (w == kErrLora) {
+        fail("an earlier adapters call read an adapter id outside [-1, n_adapters) or an expert id outside "
+             "[0, n_experts); its row was set to NaN");
     } else {
         fail("an earlier expert kernel read an expert id outside [0, n_experts); "
              "its slot outputs were set to NaN");
@@ -2447,3 +2455,5 @@ SABAH_API int sabah_synth_weights(void* d_dst, int qt, long long n_rows, int k, 
     }
     return ck(hipGetLastError(), "synth launch") ? 0 : -1;
 }
+
+#include "adapt_api.h"

@@ -26,6 +26,7 @@ import torch
 
 from . import rt
 from .bank import ROLES, DenseExpert, ExpertBank
+from .lora import LoraBank
 
 
 # A small call is bound by what Python does before the launch, so the hot
@@ -39,6 +40,19 @@ def _stream(device) -> int:
 
 def _vp(t: torch.Tensor) -> int:
     return t.data_ptr()
+
+
+class RouterBalance:
+    """What MoEExecutor.balance computes, kept for the gradient: `counts` [n_groups, n_experts] int32,
+    `mean_p` [n_groups, n_experts], `losses` [2] (balance loss, z loss) and `n_valid`
+    [n_groups + 2] int32 (valid tokens of each group, of all, groups with any)."""
+
+    def __init__(self, n_experts: int, n_groups: int = 1, device: str = "cuda:0"):
+        self.n_experts, self.n_groups = n_experts, n_groups
+        self.counts = torch.empty(n_groups, n_experts, dtype=torch.int32, device=device)
+        self.mean_p = torch.empty(n_groups, n_experts, dtype=torch.float32, device=device)
+        self.losses = torch.empty(2, dtype=torch.float32, device=device)
+        self.n_valid = torch.empty(n_groups + 2, dtype=torch.int32, device=device)
 
 
 class MoEExecutor:
@@ -98,12 +112,15 @@ class MoEExecutor:
 
     # ---- the drop-in operator ----------------------------------------------
     def mul_mat_id(self, layer: int, role: str, x: torch.Tensor, ids: torch.Tensor,
-                   out: torch.Tensor | None = None, source: int | None = None) -> torch.Tensor:
+                   out: torch.Tensor | None = None, source: int | None = None, lora: LoraBank | None = None,
+                   adapters: torch.Tensor | None = None) -> torch.Tensor:
         """ggml MUL_MAT_ID through sabah_rt_mul_mat_id_v2 on (layer, role).
 
         x [n_tokens, x_rows, k] f32 (x_rows = 1 or n_ids), ids [n_tokens, n_ids] i32
         -> [n_tokens, n_ids, rows] f32.  `source` overrides the src0 address
-        (e.g. a registered caller-side key)."""
+        (e.g. a registered caller-side key).  With `lora` and `adapters` [n_tokens] i32
+        each token's adapter is added (lora_apply): a pair per expert, or one
+        pair for all when the adapter bank has one expert."""
         b = self.bank
         T, n_ids = ids.shape
         rows, k, qt = b.rows[role], b.cols[role], b.layer_qtype(layer, role)
@@ -121,7 +138,97 @@ class MoEExecutor:
             rows, k, b.n_experts, qt, _stream(self.device), ids_ptr)
         if rc:
             rt.check(rc, "MUL_MAT_ID")
+        if lora is not None:
+            if lora.n_experts not in (1, b.n_experts):
+                raise ValueError("adapters of %d experts beside a bank of %d" % (lora.n_experts, b.n_experts))
+            self.lora_apply(lora, x, adapters, out, ids=ids if lora.n_experts > 1 else None, out=out)
         return out
+
+    # ---- adapters beside a projection --------------------------------------------
+    def _lora_rows(self, lora: LoraBank, x: torch.Tensor, adapters: torch.Tensor, ids: torch.Tensor | None,
+                   y: torch.Tensor | None):
+        """The checks that the two calls share; (tokens, slots, C arguments of x, adapters and ids).
+        y: a tensor with the output's shape [T, rows] or [T, n_ids, rows], if there is one."""
+        T = adapters.shape[0]
+        slots = ids.shape[1] if ids is not None else y.shape[1] if y is not None and y.dim() == 3 else 1
+        xs, xr = x.stride(), x.shape[1] if x.dim() == 3 else 1
+        if (x.dtype != torch.float32 or x.shape[-1] != lora.k or (xs[-1] != 1 and T) or x.shape[0] != T or xr not in (1, slots)
+                or adapters.dtype != torch.int32 or not adapters.is_contiguous() or x.dim() not in (2, 3)):
+            raise ValueError("adapters: x %s %s for %d values, adapters %s %s"
+                             % (tuple(x.shape), x.dtype, lora.k, tuple(adapters.shape), adapters.dtype))
+        if x.device != self.device or adapters.device != self.device or lora.a.device != self.device:
+            raise ValueError("adapters: the tensors are not on %s" % self.device)
+        if ids is None:
+            if lora.n_experts != 1:
+                raise ValueError("adapters of %d experts need ids" % lora.n_experts)
+            return T, slots, (x.data_ptr(), xs[1] * 4 if x.dim() == 3 else 0, xr, xs[0] * 4, adapters.data_ptr(),
+                              None, 0, 0, slots, T)
+        if ids.dtype != torch.int32 or ids.shape[0] != T or ids.device != self.device:
+            raise ValueError("adapters: ids %s %s for %d tokens" % (tuple(ids.shape), ids.dtype, T))
+        ns = ids.stride()
+        return T, slots, (x.data_ptr(), xs[1] * 4 if x.dim() == 3 else 0, xr, xs[0] * 4, adapters.data_ptr(),
+                          ids.data_ptr(), ns[1] * 4, ns[0] * 4, slots, T)
+
+    def _lora_y(self, what: str, y: torch.Tensor, T: int, slots: int, width: int):
+        """(address, slot stride, token stride) of rows [T, width] or [T, slots, width] f32."""
+        s = y.stride()
+        if (y.dtype != torch.float32 or (s[-1] != 1 and T) or y.device != self.device
+                or tuple(y.shape) not in ((T, slots, width),) + (((T, width),) if slots == 1 else ())):
+            raise ValueError("adapters: %s is %s %s, expected f32 [%d, %d, %d] with contiguous rows on %s"
+                             % (what, tuple(y.shape), y.dtype, T, slots, width, self.device))
+        return y.data_ptr(), s[1] * 4 if y.dim() == 3 else 0, s[0] * 4
+
+    def lora_apply(self, lora: LoraBank, x: torch.Tensor, adapters: torch.Tensor, base: torch.Tensor | None = None,
+                   ids: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """base + scale * B (A x) with each token's adapter (sabah_lora_apply): x [T, k] or
+        [T, x_rows, k] f32, adapters [T] i32 (-1: none), ids [T, n_ids] i32 where the
+        bank has a pair per expert, base [T, rows] or [T, n_ids, rows] f32 (None: zeros).
+        `out` may be `base` itself."""
+        T, slots, rows = self._lora_rows(lora, x, adapters, ids, base if base is not None else out)
+        if out is None:
+            out = (torch.empty_like(base) if base is not None else
+                   torch.empty((T, lora.rows) if x.dim() == 2 and ids is None else (T, slots, lora.rows),
+                               dtype=torch.float32, device=self.device))
+        b = self._lora_y("base", base, T, slots, lora.rows) if base is not None else (None, 0, 0)
+        n = rt.lib().sabah_lora_workspace(lora.ref, slots, T, 0)
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        rc = rt.lib().sabah_lora_apply(lora.ref, *rows, *b, *self._lora_y("out", out, T, slots, lora.rows),
+                                       ws.data_ptr() if n else None, n, _stream(self.device))
+        if rc:
+            rt.check(rc, "lora_apply")
+        return out
+
+    def lora_backward(self, lora: LoraBank, x: torch.Tensor, adapters: torch.Tensor, dy: torch.Tensor,
+                      ids: torch.Tensor | None = None, dx: torch.Tensor | None = None,
+                      da: torch.Tensor | None = None, db: torch.Tensor | None = None, add_dx: bool = False,
+                      add_dw: bool = False, need_dx: bool = True, need_dw: bool = True):
+        """The gradients (dx, da, db) of lora_apply for dy, the gradient of its result
+        (sabah_lora_backward): dx [T, k] or [T, n_ids, k], da and db f32 in the shapes of lora.a
+        and lora.b, written, or with add_dx / add_dw added to the tensors given; None for
+        what need_dx / need_dw leave out."""
+        T, slots, rows = self._lora_rows(lora, x, adapters, ids, dy)
+        if (add_dx and dx is None) or (add_dw and (da is None or db is None)):
+            raise ValueError("lora_backward: add_dx needs dx, add_dw needs da and db")
+        if dx is None and need_dx:
+            dx = torch.empty((T, lora.k) if dy.dim() == 2 else (T, slots, lora.k), dtype=torch.float32,
+                             device=self.device)
+        if need_dw:
+            da = torch.empty(lora.a.shape, dtype=torch.float32, device=self.device) if da is None else da
+            db = torch.empty(lora.b.shape, dtype=torch.float32, device=self.device) if db is None else db
+            for g, w in ((da, lora.a), (db, lora.b)):
+                if g.shape != w.shape or g.dtype != torch.float32 or not g.is_contiguous() or g.device != self.device:
+                    raise ValueError("lora_backward: a weight gradient is %s %s, expected contiguous f32 %s"
+                                     % (tuple(g.shape), g.dtype, tuple(w.shape)))
+        d = self._lora_y("dx", dx, T, slots, lora.k) if need_dx else (None, 0, 0)
+        n = rt.lib().sabah_lora_workspace(lora.ref, slots, T, 1)
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        rc = rt.lib().sabah_lora_backward(lora.ref, *rows, *self._lora_y("dy", dy, T, slots, lora.rows), *d,
+                                          int(add_dx), da.data_ptr() if need_dw else None,
+                                          db.data_ptr() if need_dw else None, int(add_dw),
+                                          ws.data_ptr() if n else None, n, _stream(self.device))
+        if rc:
+            rt.check(rc, "lora_backward")
+        return dx if need_dx else None, da if need_dw else None, db if need_dw else None
 
     # ---- fused layer / chain --------------------------------------------------
     def run_layer(self, layer: int, x: torch.Tensor, ids: torch.Tensor, w: torch.Tensor,
@@ -148,6 +255,67 @@ class MoEExecutor:
         rt.check(rt.lib().sabah_moe_route(_vp(logits), T, E, k, int(norm_w), ctypes.c_float(w_scale), _vp(ids),
                                           _vp(w), _stream(self.device)), "moe_route")
         return ids, w
+
+    def _router_rows(self, logits: torch.Tensor, ids: torch.Tensor, mask: torch.Tensor | None, n_groups: int):
+        T, E = logits.shape
+        if (logits.dtype != torch.float32 or (logits.stride(1) != 1 and T) or logits.device != self.device
+                or ids.dtype != torch.int32 or ids.shape[0] != T or not ids.is_contiguous() or ids.device != self.device):
+            raise ValueError("router: logits %s %s, ids %s %s" % (tuple(logits.shape), logits.dtype, tuple(ids.shape),
+                                                                 ids.dtype))
+        if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.numel() != T
+                                 or not mask.is_contiguous() or mask.device != self.device):
+            raise ValueError("router: mask %s %s for %d tokens" % (tuple(mask.shape), mask.dtype, T))
+        return T, E, ids.shape[1]
+
+    def balance(self, logits: torch.Tensor, ids: torch.Tensor, mask: torch.Tensor | None = None, n_groups: int = 1,
+                out: RouterBalance | None = None) -> RouterBalance:
+        """The router's balance loss, z loss, mean probabilities and per-expert counts
+        (sabah_moe_balance) from logits [T, n_experts] f32 and route()'s ids [T, n_used]
+        over the tokens where mask [T] (bool or uint8) holds, in n_groups groups of equal length
+        (`out` brings its own number)."""
+        if out is None:
+            out = RouterBalance(logits.shape[1], n_groups, device=self.device)
+        n_groups = out.n_groups
+        T, E, k = self._router_rows(logits, ids, mask, n_groups)
+        if out.n_experts != E:
+            raise ValueError("balance: %d experts, out has %d" % (E, out.n_experts))
+        n = rt.lib().sabah_moe_balance_workspace(T, E, n_groups)
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        rc = rt.lib().sabah_moe_balance(logits.data_ptr(), logits.stride(0) * 4 if T > 1 else E * 4, ids.data_ptr(),
+                                        mask.data_ptr() if mask is not None else None, T, E, k, n_groups,
+                                        out.counts.data_ptr(), out.mean_p.data_ptr(), out.losses.data_ptr(),
+                                        out.n_valid.data_ptr(), ws.data_ptr(), n, _stream(self.device))
+        if rc:
+            rt.check(rc, "moe_balance")
+        return out
+
+    def route_backward(self, logits: torch.Tensor, ids: torch.Tensor, dw: torch.Tensor | None = None,
+                       balance: RouterBalance | None = None, c_balance: float = 0.0, c_z: float = 0.0,
+                       mask: torch.Tensor | None = None, norm_w: bool = True, w_scale: float = 1.0,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+        """The logits' gradient [T, n_experts] (sabah_moe_route_backward): through
+        route()'s weights, dw [T, n_used] f32 (None: nothing), and of c_balance * losses[0] +
+        c_z * losses[1] of `balance`, which balance() computed with the same mask."""
+        n_groups = balance.n_groups if balance is not None else 1
+        T, E, k = self._router_rows(logits, ids, mask, n_groups)
+        if balance is not None and balance.n_experts != E:
+            raise ValueError("route_backward: %d experts, balance has %d" % (E, balance.n_experts))
+        if dw is not None and (dw.dtype != torch.float32 or dw.shape != ids.shape or not dw.is_contiguous()
+                               or dw.device != self.device):
+            raise ValueError("route_backward: dw %s %s, ids %s" % (tuple(dw.shape), dw.dtype, tuple(ids.shape)))
+        if out is None:
+            out = torch.empty((T, E), dtype=torch.float32, device=self.device)
+        elif out.dtype != torch.float32 or out.shape != logits.shape or out.stride(1) != 1 or out.device != self.device:
+            raise ValueError("route_backward: out %s %s" % (tuple(out.shape), out.dtype))
+        rc = rt.lib().sabah_moe_route_backward(
+            logits.data_ptr(), logits.stride(0) * 4 if T > 1 else E * 4, ids.data_ptr(), mask.data_ptr() if mask is not None else None,
+            T, E, k, int(norm_w), w_scale, dw.data_ptr() if dw is not None else None,
+            balance.counts.data_ptr() if balance is not None else None,
+            balance.n_valid.data_ptr() if balance is not None else None, n_groups, c_balance, c_z,
+            out.data_ptr(), out.stride(0) * 4 if T > 1 else E * 4, _stream(self.device))
+        if rc:
+            rt.check(rc, "moe_route_backward")
+        return out
 
     def run_prefill_layer(self, layer: int, x: torch.Tensor, ids: torch.Tensor, w: torch.Tensor,
                           out: torch.Tensor | None = None, resid: torch.Tensor | None = None) -> torch.Tensor:

@@ -58,6 +58,12 @@ class MoeLayerDesc(ctypes.Structure):
                 ("d_ff_shared", c_i), ("shared_gate_inp", c_vp)]
 
 
+class LoraDesc(ctypes.Structure):
+    """sabah_lora_desc (include/sabah_rt.h)."""
+    _fields_ = [("a", c_vp), ("b", c_vp), ("scale", c_vp), ("ranks", c_vp), ("type", c_i),
+                ("n_adapters", c_i), ("n_experts", c_i), ("rank", c_i), ("k", c_i), ("rows", c_i)]
+
+
 # every symbol include/sabah_rt.h declares, with its ctypes signature
 SIGNATURES = {
     "sabah_rt_init": ([c_i], c_i),
@@ -83,6 +89,15 @@ SIGNATURES = {
     "sabah_moe_prefill_layer": ([ctypes.POINTER(MoeLayerDesc), c_vp, c_vp, c_vp, c_i, c_i, c_vp, c_vp, c_vp], c_i),
     "sabah_moe_route": ([c_vp, c_i, c_i, c_i, c_i, ctypes.c_float, c_vp, c_vp, c_vp], c_i),
     "sabah_rt_set_mmid_grouping": ([c_i], c_i),
+    "sabah_moe_balance_workspace": ([c_i, c_i, c_i], c_sz),
+    "sabah_moe_balance": ([c_vp, c_sz, c_vp, c_vp, c_i, c_i, c_i, c_i, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp], c_i),
+    "sabah_moe_route_backward": ([c_vp, c_sz, c_vp, c_vp, c_i, c_i, c_i, c_i, ctypes.c_float, c_vp, c_vp, c_vp, c_i,
+                                  ctypes.c_float, ctypes.c_float, c_vp, c_sz, c_vp], c_i),
+    "sabah_lora_workspace": ([ctypes.POINTER(LoraDesc), c_i, c_i, c_i], c_sz),
+    "sabah_lora_apply": ([ctypes.POINTER(LoraDesc), c_vp, c_sz, c_i, c_sz, c_vp, c_vp, c_sz, c_sz, c_i, c_i,
+                          c_vp, c_sz, c_sz, c_vp, c_sz, c_sz, c_vp, c_sz, c_vp], c_i),
+    "sabah_lora_backward": ([ctypes.POINTER(LoraDesc), c_vp, c_sz, c_i, c_sz, c_vp, c_vp, c_sz, c_sz, c_i, c_i,
+                             c_vp, c_sz, c_sz, c_vp, c_sz, c_sz, c_i, c_vp, c_vp, c_i, c_vp, c_sz, c_vp], c_i),
     # memory, copies, events and streams for the harness (the reference binds them, rt.py:70-107)
     "sabah_dev_alloc": ([c_sz], c_vp),
     "sabah_dev_free": ([c_vp], None),
