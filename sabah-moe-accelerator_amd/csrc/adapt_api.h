@@ -190,6 +190,7 @@ SABAH_API int sabah_moe_route_backward(const float* d_logits, size_t logits_stri
 // adapters
 // ---------------------------------------------------------------------------
 // type codes of adapter weights (ggml's F32, F16 and BF16)
+constexpr int kLoraMaxKeys = 1 << 21;         // (adapter, expert) pairs: a key and its row sort as one 32-bit word
 constexpr int kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 30;
 
 static int check_lora(const char* what, const sabah_lora_desc* L, int n_ids, int n_tokens) {
@@ -198,7 +199,7 @@ static int check_lora(const char* what, const sabah_lora_desc* L, int n_ids, int
         return fail("%s: adapter type %d is none of F32 (0), F16 (1), BF16 (30)", what, L->type);
     if (L->rank <= 0 || L->rank > kLoraMaxRank) return fail("%s: rank %d outside [1, %d]", what, L->rank, kLoraMaxRank);
     if (L->n_adapters <= 0 || L->n_experts <= 0 || L->k <= 0 || L->rows <= 0 ||
-        (long long)L->n_adapters * L->n_experts > 1 << 24 || L->k > 1 << 24 || L->rows > 1 << 24)
+        (long long)L->n_adapters * L->n_experts > kLoraMaxKeys || L->k > 1 << 24 || L->rows > 1 << 24)
         return fail("%s: invalid geometry (n_adapters=%d n_experts=%d k=%d rows=%d)", what, L->n_adapters, L->n_experts,
                     L->k, L->rows);
     if (n_ids <= 0 || n_tokens < 0 || (long long)n_ids * n_tokens > 1 << 24)
@@ -208,9 +209,31 @@ static int check_lora(const char* what, const sabah_lora_desc* L, int n_ids, int
 
 static bool stride_ok(size_t s) { return s % 4 == 0; }
 
+// Tiles of a call's rows: none up to kLoraDirectRows; above, per window of
+// rows at most one per 16 and one more per key.
+struct LoraSpace {
+    size_t order, items, n_items, bytes;
+    int windows, slots;
+};
+static LoraSpace lora_space(const sabah_lora_desc* L, int n_rows) {
+    LoraSpace s{};
+    const int keys = L->n_adapters * L->n_experts + 2;      // without an adapter, and with a bad id
+    const int span = std::min(n_rows, kLoraWindow);
+    s.windows = (n_rows + kLoraWindow - 1) / kLoraWindow;
+    s.slots = std::min(span, span / kLoraTile + std::min(keys, span));
+    if (n_rows <= kLoraDirectRows) {
+        s.windows = 1;
+        return s;
+    }
+    s.items = align256((size_t)s.windows * kLoraWindow * 4);
+    s.n_items = s.items + align256((size_t)s.windows * s.slots * 16);
+    s.bytes = s.n_items + align256((size_t)s.windows * 4);
+    return s;
+}
+
 SABAH_API size_t sabah_lora_workspace(const sabah_lora_desc* lora, int n_ids, int n_tokens, int backward) {
     if (check_lora("adapters", lora, n_ids, n_tokens)) return 0;
-    return backward ? align256((size_t)n_ids * n_tokens * lora->rank * 8) : 0;
+    return backward ? align256((size_t)n_ids * n_tokens * lora->rank * 8) : lora_space(lora, n_ids * n_tokens).bytes;
 }
 
 static LoraArgs lora_args(const sabah_lora_desc* L, const float* d_x, size_t x_id_stride, int x_rows,
@@ -252,14 +275,20 @@ static int check_lora_rows(const char* what, const sabah_lora_desc* L, const flo
     return 0;
 }
 
+template <typename W>
+static void launch_lora_apply(const LoraArgs& a, const LoraTiles& t, dim3 grid, hipStream_t st) {
+    if (a.rank <= 16) hipLaunchKernelGGL((k_lora_apply<W, 1, 4, 4>), grid, dim3(256), 0, st, a, t);
+    else if (a.rank <= 32) hipLaunchKernelGGL((k_lora_apply<W, 2, 4, 4>), grid, dim3(256), 0, st, a, t);
+    else if (a.rank <= 64) hipLaunchKernelGGL((k_lora_apply<W, 4, 4, 2>), grid, dim3(256), 0, st, a, t);
+    else hipLaunchKernelGGL((k_lora_apply<W, 8, 4, 1>), grid, dim3(256), 0, st, a, t);
+}
+
 SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, size_t x_id_stride, int x_rows,
                                size_t x_token_stride, const int32_t* d_adapters, const int32_t* d_ids,
                                size_t ids_id_stride, size_t ids_token_stride, int n_ids, int n_tokens,
                                const float* d_base, size_t base_id_stride, size_t base_token_stride, float* d_dst,
                                size_t dst_id_stride, size_t dst_token_stride, void* d_workspace, size_t workspace_bytes,
                                void* stream) {
-    (void)d_workspace;
-    (void)workspace_bytes;
     if (check_lora_rows("adapters", lora, d_x, x_id_stride, x_rows, x_token_stride, d_adapters, d_ids, ids_id_stride,
                         ids_token_stride, n_ids, n_tokens))
         return -1;
@@ -269,6 +298,11 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
         return fail("adapters: strides are in bytes and multiples of 4");
     if (d_base == d_dst && (base_id_stride != dst_id_stride || base_token_stride != dst_token_stride))
         return fail("adapters: base in place of dst needs dst's strides");
+    const int n_rows = n_ids * n_tokens;
+    const LoraSpace sp = lora_space(lora, n_rows);
+    if (sp.bytes && (!d_workspace || workspace_bytes < sp.bytes || (uintptr_t)d_workspace % 16))
+        return fail("adapters: the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", sp.bytes,
+                    workspace_bytes);
     if (g_device < 0) return fail("sabah_rt_init has not been called");
     if (!check_sticky()) return -1;
     if (n_tokens == 0) return 0;
@@ -283,11 +317,30 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
     a.dst_id = dst_id_stride;
     a.dst_tok = dst_token_stride;
     hipStream_t st = pick_stream(stream);
-    const dim3 grid((unsigned)(n_ids * n_tokens)), block(kLoraThreads);
+    LoraTiles t{};
+    t.n_rows = n_rows;
+    t.slots = sp.slots;
+    t.skip_none = d_base == d_dst;
+    if (sp.bytes) {
+        uint8_t* ws = static_cast<uint8_t*>(d_workspace);
+        const LoraGroup g{reinterpret_cast<int*>(ws + sp.order), reinterpret_cast<int4*>(ws + sp.items),
+                          reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, t.skip_none};
+        hipLaunchKernelGGL(k_lora_group, dim3((unsigned)sp.windows), dim3(kLoraWindow), 0, st, a, g);
+        if (!ck(hipGetLastError(), "adapters grouping launch")) return -1;
+        t.order = g.order;
+        t.items = g.items;
+        t.n_items = g.n_items;
+    }
+    const long long tiles = std::min<long long>(n_rows, (long long)sp.windows * sp.slots);
+    int parts = (int)std::max<long long>(1, 512 / std::max<long long>(1, tiles));
+    parts = std::min(parts, (lora->rows + 63) / 64);
+    t.cols = ((lora->rows + parts - 1) / parts + 31) / 32 * 32;
+    parts = (lora->rows + t.cols - 1) / t.cols;
+    const dim3 grid((unsigned)sp.slots, (unsigned)parts, (unsigned)sp.windows);
     switch (lora->type) {
-    case kTypeF32: hipLaunchKernelGGL(k_lora_rows<LoraF32>, grid, block, 0, st, a); break;
-    case kTypeF16: hipLaunchKernelGGL(k_lora_rows<LoraF16>, grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL(k_lora_rows<LoraBF16>, grid, block, 0, st, a); break;
+    case kTypeF32: launch_lora_apply<LoraF32>(a, t, grid, st); break;
+    case kTypeF16: launch_lora_apply<LoraF16>(a, t, grid, st); break;
+    default: launch_lora_apply<LoraBF16>(a, t, grid, st); break;
     }
     return ck(hipGetLastError(), "adapters launch") ? 0 : -1;
 }
