@@ -213,14 +213,16 @@ static bool stride_ok(size_t s) { return s % 4 == 0; }
 // rows at most one per 16 and one more per key.
 struct LoraSpace {
     size_t order, items, n_items, bytes;
-    int windows, slots;
+    int windows, slots, key_bits;
 };
+constexpr int kLoraDirectRows = 256;          // a thread of k_lora_apply's workgroup for each
 static LoraSpace lora_space(const sabah_lora_desc* L, int n_rows) {
     LoraSpace s{};
     const int keys = L->n_adapters * L->n_experts + 2;      // without an adapter, and with a bad id
     const int span = std::min(n_rows, kLoraWindow);
     s.windows = (n_rows + kLoraWindow - 1) / kLoraWindow;
     s.slots = std::min(span, span / kLoraTile + std::min(keys, span));
+    while (keys >> s.key_bits) ++s.key_bits;                // the word past the rows has key + 2 == keys
     if (n_rows <= kLoraDirectRows) {
         s.windows = 1;
         return s;
@@ -277,9 +279,9 @@ static int check_lora_rows(const char* what, const sabah_lora_desc* L, const flo
 
 template <typename W>
 static void launch_lora_apply(const LoraArgs& a, const LoraTiles& t, dim3 grid, hipStream_t st) {
-    if (a.rank <= 16) hipLaunchKernelGGL((k_lora_apply<W, 1, 4, 4>), grid, dim3(256), 0, st, a, t);
-    else if (a.rank <= 32) hipLaunchKernelGGL((k_lora_apply<W, 2, 4, 4>), grid, dim3(256), 0, st, a, t);
-    else if (a.rank <= 64) hipLaunchKernelGGL((k_lora_apply<W, 4, 4, 2>), grid, dim3(256), 0, st, a, t);
+    if (a.rank <= 16) hipLaunchKernelGGL((k_lora_apply<W, 1, 4, 2>), grid, dim3(256), 0, st, a, t);
+    else if (a.rank <= 32) hipLaunchKernelGGL((k_lora_apply<W, 2, 4, 2>), grid, dim3(256), 0, st, a, t);
+    else if (a.rank <= 64) hipLaunchKernelGGL((k_lora_apply<W, 4, 4, 1>), grid, dim3(256), 0, st, a, t);
     else hipLaunchKernelGGL((k_lora_apply<W, 8, 4, 1>), grid, dim3(256), 0, st, a, t);
 }
 
@@ -321,11 +323,13 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
     t.n_rows = n_rows;
     t.slots = sp.slots;
     t.skip_none = d_base == d_dst;
+    t.key_bits = sp.key_bits;
     if (sp.bytes) {
         uint8_t* ws = static_cast<uint8_t*>(d_workspace);
         const LoraGroup g{reinterpret_cast<int*>(ws + sp.order), reinterpret_cast<int4*>(ws + sp.items),
-                          reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, t.skip_none};
-        hipLaunchKernelGGL(k_lora_group, dim3((unsigned)sp.windows), dim3(kLoraWindow), 0, st, a, g);
+                          reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, t.skip_none, sp.key_bits};
+        hipLaunchKernelGGL(k_lora_group, dim3((unsigned)sp.windows),
+                           dim3((unsigned)std::min(kLoraWindow, (n_rows + 63) / 64 * 64)), 0, st, a, g);
         if (!ck(hipGetLastError(), "adapters grouping launch")) return -1;
         t.order = g.order;
         t.items = g.items;

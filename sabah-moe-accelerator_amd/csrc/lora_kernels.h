@@ -10,6 +10,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace sabah {
 
 constexpr int kLoraThreads = 256;
@@ -121,19 +123,19 @@ __device__ inline void lora_shrink(const typename W::T* A, const float* x, int k
 }
 
 // ---------------------------------------------------------------------------
-// Tiles: up to 16 rows of one key.  Up to 64 rows each workgroup finds its tile among
-// them by itself (lora_tile); above, k_lora_group sorts each window of 1,024 rows by
-// key and lists its tiles.
+// Tiles: up to 16 rows of one key.  A workgroup with a thread for every row of the call finds its
+// tile by itself (lora_tile); above, k_lora_group sorts each window of 1,024 rows by key
+// and lists its tiles.
 // ---------------------------------------------------------------------------
 constexpr int kLoraTile = 16;
-constexpr int kLoraDirectRows = 64;
 constexpr int kLoraWindow = 1024;
 
 struct LoraTiles {
-    const int* order;             // [windows * 1024]: rows by key, each window on its own
+    const int* order;             // [windows * 1024]: rows by key, each window on its own; null: found by each workgroup
     const int4* items;            // [windows][slots]: (key, position in order, rows)
     const int* n_items;           // [windows]
     int n_rows, slots, skip_none; // skip_none: rows without an adapter are left alone
+    int key_bits;                 // of key + 2 and of one more
     int cols;                     // columns of the output per workgroup
 };
 
@@ -141,73 +143,111 @@ struct LoraGroup {
     int* order;
     int4* items;
     int* n_items;
-    int n_rows, slots, skip_none;
+    int n_rows, slots, skip_none, key_bits;
 };
 
-// One window per workgroup: a bitonic sort of (key, row), a row per thread, in
-// registers with the exchanges within a wave by shuffles; then every 16th row of a
-// run of equal keys begins a tile.  Stable, and without atomics: the same rows
-// give the same tiles.
-__global__ __launch_bounds__(kLoraWindow) void k_lora_group(LoraArgs a, LoraGroup g) {
-    __shared__ uint32_t s_c[kLoraWindow];
-    __shared__ int s_w[kLoraWindow / 64];
-    constexpr uint32_t kPad = 0xFFFFFFFFu;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, w = (int)blockIdx.x;
-    const int row = w * kLoraWindow + tid;
-    uint32_t c = kPad;                                      // (key + 2, row of the window)
-    if (row < g.n_rows) {
-        const int key = lora_key(a, row);
-        if (key == kLoraBad) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrLora;
-        c = ((uint32_t)(key + 2) << 10) | (uint32_t)tid;
+// A row's word, (key + 2, row of the window); past the rows one above every key
+__device__ inline uint32_t lora_word(const LoraArgs& a, int row, int n_rows, int at) {
+    if (row >= n_rows) return ((uint32_t)(a.n_adapters * a.n_experts + 2) << 10) | (uint32_t)at;
+    const int key = lora_key(a, row);
+    if (key == kLoraBad) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrLora;
+    return ((uint32_t)(key + 2) << 10) | (uint32_t)at;
+}
+
+// LDS of the sort: NW waves at most
+template <int NW>
+struct LoraSort {
+    uint32_t c[64 * NW];
+    int w[NW];                    // zeros for waves that the workgroup lacks
+    uint64_t m[NW];
+};
+
+// The workgroup's words in the order of their keys (stable), one per thread, left in f.c too: a radix sort by single
+// bits, as many as the keys have.  Every wave reads all the waves' counts at once: a loop over
+// them cost 0.8 us a bit with 16 waves.
+template <int NW>
+__device__ inline uint32_t lora_sort(uint32_t c, int bits, LoraSort<NW>& f) {
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, nt = (int)blockDim.x;
+    if (tid < NW) {
+        f.w[tid] = 0;
+        f.m[tid] = 0;
     }
-    for (int size = 2; size <= kLoraWindow; size <<= 1)
-        for (int d = size >> 1; d > 0; d >>= 1) {
-            uint32_t o;
-            if (d < 64) {
-                o = (uint32_t)__shfl_xor((int)c, d);
-            } else {
-                __syncthreads();
-                s_c[tid] = c;
-                __syncthreads();
-                o = s_c[tid ^ d];
-            }
-            const bool lower = (tid & d) == 0, up = (tid & size) == 0;
-            c = lower == up ? min(c, o) : max(c, o);
-        }
+    f.c[tid] = c;
     __syncthreads();
-    s_c[tid] = c;
-    __syncthreads();
-    const bool valid = c != kPad;
-    const uint32_t k2 = c >> 10;
-    int start = tid > 0 && (s_c[tid - 1] >> 10) == k2 ? 0 : tid;   // the run's first thread: an inclusive maximum
+    for (int b = 10; b < 10 + bits; ++b) {
+        const bool one = (c >> b) & 1u;
+        const uint64_t m = __ballot(one);
+        if (lane == 0) f.w[wave] = __popcll(m);
+        __syncthreads();
+        int ones = __popcll(m & ((1ull << lane) - 1ull)), total = 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(start, o);
-        if (lane >= o) start = max(start, y);
+        for (int v = 0; v < NW; ++v) {
+            const int x = f.w[v];
+            ones += v < wave ? x : 0;
+            total += x;
+        }
+        f.c[one ? nt - total + ones : tid - ones] = c;
+        __syncthreads();
+        c = f.c[tid];
     }
-    if (lane == 63) s_w[wave] = start;
+    return c;
+}
+
+// In sorted order: every 16th row of a run of equal keys begins a tile.  The thread's tile, if it begins one
+// (its number of rows, else 0), and the tiles before it.
+template <int NW>
+__device__ inline int lora_leader(uint32_t c, LoraSort<NW>& f, int n_keys2, bool skip_none, int& slot) {
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, nt = (int)blockDim.x;
+    const uint32_t k2 = c >> 10;
+    const uint64_t head = __ballot(tid == 0 || (f.c[max(tid - 1, 0)] >> 10) != k2);   // rows that begin a run
+    if (lane == 0) f.m[wave] = head;
     __syncthreads();
-    for (int v = 0; v < wave; ++v) start = max(start, s_w[v]);
-    const bool leader = valid && ((tid - start) & (kLoraTile - 1)) == 0 && !(g.skip_none && (int)k2 - 2 == kLoraNone);
+    int start = 0;                                          // of the thread's run
+    uint64_t next = 0;                                      // the heads of the wave after this one
+#pragma unroll
+    for (int v = 0; v < NW; ++v) {
+        const uint64_t h = f.m[v];
+        if (v < wave && h) start = 64 * v + 63 - __builtin_clzll(h);
+        if (v == wave + 1) next = h;
+    }
+    const uint64_t upto = head & ((2ull << lane) - 1ull), after = head & ~((2ull << lane) - 1ull);
+    if (upto) start = 64 * wave + 63 - __builtin_clzll(upto);
+    int end = after ? 64 * wave + __builtin_ctzll(after) : next ? 64 * wave + 64 + __builtin_ctzll(next) : nt;
+    const bool leader = (int)k2 < n_keys2 && ((tid - start) & (kLoraTile - 1)) == 0 && !(skip_none && (int)k2 == kLoraNone + 2);
     const uint64_t m = __ballot(leader);
     __syncthreads();
-    if (lane == 0) s_w[wave] = __popcll(m);
+    if (lane == 0) f.w[wave] = __popcll(m);
     __syncthreads();
-    int slot = __popcll(m & ((1ull << lane) - 1ull));
-    for (int v = 0; v < wave; ++v) slot += s_w[v];
-    if (leader) {
-        int n = 1;
-        while (n < kLoraTile && tid + n < kLoraWindow && (s_c[tid + n] >> 10) == k2) ++n;
-        g.items[(size_t)w * g.slots + slot] = make_int4((int)k2 - 2, w * kLoraWindow + tid, n, 0);
-    }
-    if (tid == kLoraWindow - 1) g.n_items[w] = slot + (leader ? 1 : 0);
-    if (valid) g.order[w * kLoraWindow + tid] = w * kLoraWindow + (int)(c & 1023u);
+    slot = __popcll(m & ((1ull << lane) - 1ull));
+#pragma unroll
+    for (int v = 0; v < NW; ++v) slot += v < wave ? f.w[v] : 0;
+    return leader ? min(kLoraTile, end - tid) : 0;          // a head two waves on is more than 16 rows away
 }
+
+// One window per workgroup, a row per thread.  Without atomics: the same rows give the same tiles.
+__global__ __launch_bounds__(kLoraWindow) void k_lora_group(LoraArgs a, LoraGroup g) {
+    __shared__ LoraSort<kLoraWindow / 64> f;
+    const int tid = (int)threadIdx.x, w = (int)blockIdx.x, n_keys2 = a.n_adapters * a.n_experts + 2;
+    const uint32_t c = lora_sort(lora_word(a, w * kLoraWindow + tid, g.n_rows, tid), g.key_bits, f);
+    int slot;
+    const int n = lora_leader(c, f, n_keys2, g.skip_none, slot);
+    if (n) g.items[(size_t)w * g.slots + slot] = make_int4((int)(c >> 10) - 2, w * kLoraWindow + tid, n, 0);
+    if (tid == (int)blockDim.x - 1) g.n_items[w] = slot + (n ? 1 : 0);
+    if ((int)(c >> 10) < n_keys2) g.order[w * kLoraWindow + tid] = w * kLoraWindow + (int)(c & 1023u);
+}
+
+// LDS of a workgroup that finds its own tile
+template <int NW>
+struct LoraFind {
+    LoraSort<NW> s;
+    int item[3];
+};
 
 // The workgroup's tile: its key and number of rows, and the row of the lane's place
 // lane % 16 in it (the last one's again past the number).  False: no tile is left for it.
-__device__ inline bool lora_tile(const LoraArgs& a, const LoraTiles& t, int lane, int& key, int& n, int& row) {
-    const int p = lane & (kLoraTile - 1);
+template <int NW>
+__device__ inline bool lora_tile(const LoraArgs& a, const LoraTiles& t, LoraFind<NW>& f, int& key, int& n, int& row) {
+    const int tid = (int)threadIdx.x, p = tid & (kLoraTile - 1);
     if (t.order) {
         const int w = (int)blockIdx.z;
         if ((int)blockIdx.x >= t.n_items[w]) return false;
@@ -217,22 +257,27 @@ __device__ inline bool lora_tile(const LoraArgs& a, const LoraTiles& t, int lane
         row = t.order[it.y + min(p, n - 1)];
         return true;
     }
-    const int k = lane < t.n_rows ? lora_key(a, lane) : 0x7FFFFFFF;
-    if (k == kLoraBad) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrLora;
-    int idx = 0;                                            // earlier rows of the lane's key
-    for (int j = 0; j < t.n_rows; ++j) idx += __builtin_amdgcn_readlane(k, j) == k && j < lane;
-    const bool leader = lane < t.n_rows && (idx & (kLoraTile - 1)) == 0 && !(t.skip_none && k == kLoraNone);
-    const uint64_t m = __ballot(leader);
-    const uint64_t mine = __ballot(leader && __popcll(m & ((1ull << lane) - 1ull)) == (int)blockIdx.x);
-    if (mine == 0) return false;
-    const int first = __builtin_ctzll(mine);
-    key = __builtin_amdgcn_readlane(k, first);
-    const int i0 = __builtin_amdgcn_readlane(idx, first);
-    const bool in = lane < t.n_rows && k == key && idx >= i0 && idx < i0 + kLoraTile;
-    n = __popcll(__ballot(in));
-    // the lane's number to its place in the tile; the others' to place 63, which nobody reads
-    const int at = __builtin_amdgcn_ds_permute((in ? idx - i0 : 63) * 4, lane);
-    row = __shfl(at, min(p, n - 1));
+    if (t.n_rows == 1) {
+        row = 0;
+        n = 1;
+        key = __builtin_amdgcn_readfirstlane(lora_key(a, 0));
+        if (key == kLoraBad && tid == 0) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrLora;
+        return !(t.skip_none && key == kLoraNone);
+    }
+    const uint32_t c = lora_sort(lora_word(a, tid, t.n_rows, tid), t.key_bits, f.s);
+    if (tid == 0) f.item[2] = 0;
+    int slot;
+    const int m = lora_leader(c, f.s, a.n_adapters * a.n_experts + 2, t.skip_none, slot);
+    if (m && slot == (int)blockIdx.x) {
+        f.item[0] = (int)(c >> 10) - 2;
+        f.item[1] = tid;
+        f.item[2] = m;
+    }
+    __syncthreads();
+    n = __builtin_amdgcn_readfirstlane(f.item[2]);
+    if (n == 0) return false;
+    key = __builtin_amdgcn_readfirstlane(f.item[0]);
+    row = (int)(f.s.c[f.item[1] + min(p, n - 1)] & 1023u);
     return true;
 }
 
@@ -259,157 +304,233 @@ __device__ inline typename W::V8 lora_load8(const typename W::T* row, int i, int
     return v;
 }
 
-// S = X A^T of a tile with v_mfma_f32_16x16x4: the waves share k in steps of 32, of which lane l holds the eight
-// values at 8 (l / 16) of row l % 16 of X (B operand) and of A (A operand), any order of k being
-// the same sum; part [NW][16 NR][16] gets each wave's (rank, row).  Rows of A past the rank are
-// the last one's again.
+// ---------------------------------------------------------------------------
+// Products of a weight operand (A: row m = lane % 16 of it) with an f32 operand (B: column lane % 16), eight
+// neighbours of the summed axis per lane, on a tile whose lane holds column lane % 16 and rows 4 (lane / 16) .. +3.
+//   f32 and f16 weights   eight v_mfma_f32_16x16x4 (any order of the summed axis is the same sum)
+//   bf16 weights          the f32 operand in three bf16 pieces that add up to it exactly (each
+//                         keeps the next 8 of its 24 bits), three v_mfma_f32_16x16x32_bf16: 48
+//                         cycles against 256, with the same products and an f32 sum
+// An infinity has no pieces (its rest is inf - inf): its columns are done with the f32 form (big).
+// ---------------------------------------------------------------------------
+typedef __bf16 lb8 __attribute__((ext_vector_type(8)));
+
+struct LoraPieces {
+    lb8 v[3];
+};
+__device__ inline LoraPieces lora_split(const float (&x)[8]) {
+    union {
+        uint32_t u[4];
+        lb8 b;
+    } p[3];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        float r[2] = {x[2 * c], x[2 * c + 1]};
+#pragma unroll
+        for (int g = 0; g < 3; ++g) {
+            // the upper halves of the two words
+            p[g].u[c] = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302u);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) r[e] = r[e] - __uint_as_float(__float_as_uint(r[e]) & 0xFFFF0000u);
+        }
+    }
+    return LoraPieces{{p[0].b, p[1].b, p[2].b}};
+}
+__device__ inline float lora_most(const float (&x)[8], float m) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) m = fmaxf(m, __builtin_fabsf(x[c]));
+    return m;
+}
+// lane p's flag of column p, from the four lanes that hold it
+__device__ inline bool lora_column_big(float most) {
+    most = fmaxf(most, __shfl_xor(most, 16));
+    return fmaxf(most, __shfl_xor(most, 32)) == __builtin_inff();
+}
+template <typename W>
+constexpr bool kLoraPieces = false;
+template <>
+constexpr bool kLoraPieces<LoraBF16> = true;
+
+// S = X A^T of a tile: the waves share k in steps of 32, of which lane l holds the eight
+// values at 8 (l / 16) of row l % 16 of X and of A; part [NW][16 NR][16] gets each wave's (rank, row).  Rows of
+// A past the rank are the last one's again.  U steps are loaded while U others are multiplied.
 template <typename W, int NR, int NW, int U>
-__device__ inline void lora_shrink_tile(const typename W::T* A, const float* x, int k, int rank, float* part) {
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, p = lane & 15, q = lane >> 4;
-    const typename W::T* ar[NR];
-#pragma unroll
-    for (int b = 0; b < NR; ++b) ar[b] = A + (size_t)min(16 * b + p, rank - 1) * k;
-    lf4 acc[NR];
-#pragma unroll
-    for (int b = 0; b < NR; ++b) acc[b] = lf4{0, 0, 0, 0};
-    const int steps = k / 32;
-    auto step = [&](const LoraF32::V8& xv, const typename W::V8 (&av)[NR]) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-#pragma unroll
-            for (int b = 0; b < NR; ++b)
-                acc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(W::get(av[b], c), LoraF32::get(xv, c), acc[b], 0, 0, 0);
+struct LoraShrink {
+    struct In {
+        LoraF32::V8 x;
+        typename W::V8 a[NR];
     };
-    int s = wave;
-    for (; s + (U - 1) * NW < steps; s += NW * U) {
-        LoraF32::V8 xv[U];
-        typename W::V8 av[U][NR];
+    const typename W::T* ar[NR];
+    const float* x;
+    int k, q;
+    float most = 0.0f;
+
+    __device__ inline LoraShrink(const typename W::T* A, const float* x_, int k_, int rank) : x(x_), k(k_) {
+        const int lane = (int)threadIdx.x & 63, p = lane & 15;
+        q = lane >> 4;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = (s + u * NW) * 32 + 8 * q;
-            xv[u] = LoraF32::load8(x + i);
-#pragma unroll
-            for (int b = 0; b < NR; ++b) av[u][b] = W::load8(ar[b] + i);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) step(xv[u], av[u]);
+        for (int b = 0; b < NR; ++b) ar[b] = A + (size_t)min(16 * b + p, rank - 1) * k;
     }
-    for (; s <= steps; s += NW) {                           // what is left of the unrolled steps, then k's rest
+    __device__ inline void load(In& in, int s) const {
         const int i = s * 32 + 8 * q;
-        if (s == steps && k % 32 == 0) break;
-        typename W::V8 av[NR];
+        in.x = LoraF32::load8(x + i);
 #pragma unroll
-        for (int b = 0; b < NR; ++b) av[b] = lora_load8<W>(ar[b], i, k);
-        step(lora_load8<LoraF32>(x, i, k), av);
+        for (int b = 0; b < NR; ++b) in.a[b] = W::load8(ar[b] + i);
     }
+    __device__ inline void load_rest(In& in, int s) const {
+        const int i = s * 32 + 8 * q;
+        in.x = lora_load8<LoraF32>(x, i, k);
 #pragma unroll
-    for (int b = 0; b < NR; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[((size_t)wave * 16 * NR + 16 * b + 4 * q + i) * 16 + p] = acc[b][i];
-}
-
-// The ranks of a lane's 4 NR values of a row of B and of S: groups of four from 4 NR (lane / 16) on; a
-// group that reaches past the rank is moved back to the row's last four (rows of fewer than four: the
-// last value again), so that loads stay inside the row.  A value counts if it is not one that an
-// earlier group has, and below the adapter's own rank.
-__device__ inline int lora_group_at(int r, int rank) { return min(r, max(0, rank - 4)); }
-__device__ inline bool lora_counts(int r, int c, int rank, int rk) {
-    const int at = lora_group_at(r, rank) + c;
-    return at >= r && at < rk;
-}
-
-// the lane's operand of S^T, of row lane % 16, times c; 0 where a value does not count
-template <int NR, int NW>
-__device__ inline void lora_sum_parts(const float* part, int rank, int rk, float c, float (&s)[4 * NR]) {
-    const int lane = (int)threadIdx.x & 63, p = lane & 15, q = lane >> 4;
-#pragma unroll
-    for (int j = 0; j < 4 * NR; ++j) {
-        const int r0 = 4 * NR * q + (j & ~3), r = lora_group_at(r0, rank) + (j & 3);
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) v += part[((size_t)w * 16 * NR + r) * 16 + p];
-        s[j] = lora_counts(r0, j & 3, rank, rk) ? v * c : 0.0f;
+        for (int b = 0; b < NR; ++b) in.a[b] = lora_load8<W>(ar[b], i, k);
     }
-}
-
-// The lane's 4 NR weights of a row of B.  WHOLE: every value counts; else the others become zeros by a
-// mask in registers (a NaN or an infinity past an adapter's own rank must not meet its zero in S).
-template <typename W, int NR, bool WHOLE>
-struct LoraRow {
-    int at[NR];
-    uint32_t mask[WHOLE ? 1 : NR][4];
-    bool small;
-    __device__ inline LoraRow(int rank, int rk) {
-        const int q = ((int)threadIdx.x & 63) >> 4;
-        small = rank < 4;
+    template <bool PIECES>
+    __device__ inline void mul(const In& in, lf4 (&acc)[NR]) {
+        if constexpr (PIECES) {
+            float v[8];
 #pragma unroll
-        for (int g = 0; g < NR; ++g) {
-            const int r = 4 * (NR * q + g);
-            at[g] = lora_group_at(r, rank);
-            if constexpr (!WHOLE) {
+            for (int c = 0; c < 8; ++c) v[c] = LoraF32::get(in.x, c);
+            most = lora_most(v, most);
+            const LoraPieces P = lora_split(v);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    mask[g][c] = lora_counts(r, c, rank, rk) ? 0xFFFFFFFFu : 0u;
-                    asm volatile("" : "+v"(mask[g][c]));    // kept as a word, not as a condition
-                }
-            }
+            for (int g = 2; g >= 0; --g)
+#pragma unroll
+                for (int b = 0; b < NR; ++b)
+                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lb8, in.a[b]), P.v[g], acc[b], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int b = 0; b < NR; ++b)
+                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(W::get(in.a[b], c), LoraF32::get(in.x, c), acc[b], 0, 0, 0);
         }
     }
-    __device__ inline void load(const typename W::T* row, int rank, typename W::V4 (&v)[NR]) const {
+    template <bool PIECES>
+    __device__ inline void sum(lf4 (&acc)[NR]) {
+        const int wave = (int)threadIdx.x >> 6, steps = k / 32;
 #pragma unroll
-        for (int g = 0; g < NR; ++g) {
-            if (!WHOLE && NR == 1 && small) {
+        for (int b = 0; b < NR; ++b) acc[b] = lf4{0, 0, 0, 0};
+        In in[2][U];
+        auto load_all = [&](In (&z)[U], int s) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) W::set(v[g], c, row[min(c, rank - 1)]);
-            } else {
-                v[g] = W::load4(row + at[g]);
+            for (int u = 0; u < U; ++u) load(z[u], s + u * NW);
+        };
+        auto mul_all = [&](const In (&z)[U]) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) mul<PIECES>(z[u], acc);
+        };
+        int s = wave;                                       // the first step that is not loaded
+        auto more = [&] { return s + (U - 1) * NW < steps; };
+        if (more()) {
+            load_all(in[0], s);
+            s += U * NW;
+            for (;;) {
+                bool m = more();
+                if (m) load_all(in[1], s), s += U * NW;
+                mul_all(in[0]);
+                if (!m) break;
+                m = more();
+                if (m) load_all(in[0], s), s += U * NW;
+                mul_all(in[1]);
+                if (!m) break;
             }
         }
+        for (; s <= steps; s += NW) {                       // what is left of whole steps, then k's rest
+            if (s == steps && k % 32 == 0) break;
+            load_rest(in[0][0], s);
+            mul<PIECES>(in[0][0], acc);
+        }
     }
-    __device__ inline float get(const typename W::V4 (&v)[NR], int j) const {
-        const float w = W::get(v[j >> 2], j & 3);
-        if constexpr (WHOLE) return w;
-        else return __uint_as_float(__float_as_uint(w) & mask[j >> 2][j & 3]);
+    __device__ inline void run(float* part) {
+        const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, p = lane & 15;
+        lf4 acc[NR];
+        sum<kLoraPieces<W>>(acc);
+        if constexpr (kLoraPieces<W>) {
+            if (__any(most == __builtin_inff())) {          // rare: the columns with an infinity again
+                const bool big = lora_column_big(most);
+                lf4 again[NR];
+                sum<false>(again);
+#pragma unroll
+                for (int b = 0; b < NR; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[b][i] = big ? again[b][i] : acc[b][i];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NR; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[((size_t)wave * 16 * NR + 16 * b + 4 * q + i) * 16 + p] = acc[b][i];
     }
 };
 
-// y = base + B S over columns c0 .. c1 of the tile: D = B S^T, so that a lane holds eight neighbouring
-// columns (two products' four each) of row lane % 16
-template <typename W, int NR, int NW, bool WHOLE>
-__device__ inline void lora_expand_tile(const typename W::T* B, const float (&s)[4 * NR], int rank, int rk, int rows,
-                                        const float* base, float* dst, bool live, int c0, int c1) {
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, p = lane & 15, q = lane >> 4;
-    const LoraRow<W, NR, WHOLE> L(rank, rk);
-    for (int o0 = c0 + 32 * wave; o0 < c1; o0 += 32 * NW) {
-        typename W::V4 w[2][NR];
+// y = base + B S over columns c0 .. c1 of the tile, in steps of 32 columns per wave: D = B S^T, two products of 16
+// columns, so that a lane holds eight neighbouring columns (four of each) of row lane % 16.
+// The ranks of a lane's 4 NR values of a row of B and of S: groups of GW from 4 NR (lane / 16) on; a
+// group that reaches past the rank is moved back to the row's last GW (rows of fewer than four: the
+// last value again), so that loads stay inside the row.  A value counts if it is not one that an
+// earlier group has, and below the adapter's own rank; the others' weights become zeros by a
+// mask in registers (a NaN or an infinity past an adapter's own rank must not meet its zero in S).
+template <typename W, int NR, int NW>
+struct LoraExpand {
+    static constexpr int GW = NR == 1 ? 4 : 8, NG = 4 * NR / GW;
+    typedef typename std::conditional<NR == 1, typename W::V4, typename W::V8>::type V;
+    struct In {
+        V w[2][NG];
+        lf4 y[2];
+    };
+    const typename W::T* B;
+    const float* base;
+    float* dst;
+    int rank, rows, c1, p, q, at[NG];
+    bool live;
+
+    __device__ inline LoraExpand(const typename W::T* B_, int rank_, int rows_, const float* base_, float* dst_, bool live_,
+                                 int c1_)
+        : B(B_), base(base_), dst(dst_), rank(rank_), rows(rows_), c1(c1_), live(live_) {
+        const int lane = (int)threadIdx.x & 63;
+        p = lane & 15;
+        q = lane >> 4;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) at[g] = min(4 * NR * q + GW * g, max(0, rank - GW));
+    }
+    __device__ inline bool counts(int j, int rk) const {
+        const int r = at[j / GW] + j % GW;
+        return r >= 4 * NR * q + j / GW * GW && r < rk;
+    }
+    __device__ inline void load(In& in, int o0) const {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int o = min(o0 + 8 * (p >> 2) + 4 * h + (p & 3), rows - 1);
-            L.load(B + (size_t)o * rank, rank, w[h]);
-        }
-        const int o = o0 + 8 * q;
-        const bool full = o + 8 <= c1;
-        lf4 y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-        if (base) {
-            if (full) {
-                y[0] = *reinterpret_cast<const lf4u*>(base + o);
-                y[1] = *reinterpret_cast<const lf4u*>(base + o + 4);
-            } else {
+            const typename W::T* row = B + (size_t)min(o0 + 8 * (p >> 2) + 4 * h + (p & 3), rows - 1) * rank;
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    if (o + c < c1) y[c >> 2][c & 3] = base[o + c];
+            for (int g = 0; g < NG; ++g) {
+                if constexpr (NR == 1) {
+                    if (rank < 4) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) W::set(in.w[h][g], c, row[min(c, rank - 1)]);
+                    } else {
+                        in.w[h][g] = W::load4(row + at[g]);
+                    }
+                } else {
+                    in.w[h][g] = W::load8(row + at[g]);
+                }
             }
         }
-        lf4 d[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        const int o = o0 + 8 * q;
+        in.y[0] = lf4{0, 0, 0, 0};
+        in.y[1] = lf4{0, 0, 0, 0};
+        if (!base) return;
+        if (o + 8 <= c1) {
+            in.y[0] = *reinterpret_cast<const lf4u*>(base + o);
+            in.y[1] = *reinterpret_cast<const lf4u*>(base + o + 4);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4 * NR; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                d[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(L.get(w[h], j), s[j], d[h], 0, 0, 0);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) y[h] = y[h] + d[h];
-        if (!live) continue;
-        if (full) {
+            for (int c = 0; c < 8; ++c)
+                if (o + c < c1) in.y[c >> 2][c & 3] = base[o + c];
+        }
+    }
+    __device__ inline void store(const lf4 (&y)[2], int o0) const {
+        const int o = o0 + 8 * q;
+        if (!live) return;
+        if (o + 8 <= c1) {
             *reinterpret_cast<lf4u*>(dst + o) = y[0];
             *reinterpret_cast<lf4u*>(dst + o + 4) = y[1];
         } else {
@@ -418,34 +539,142 @@ __device__ inline void lora_expand_tile(const typename W::T* B, const float (&s)
                 if (o + c < c1) dst[o + c] = y[c >> 2][c & 3];
         }
     }
+    // in: the first step's, loaded by the caller (ahead of the shrink); s: the lane's S, already scaled, zeros
+    // where a value does not count
+    template <bool WHOLE>
+    __device__ inline void run(In& in, int o0, const float (&s)[4 * NR], int rk) const {
+        uint32_t mask[4 * NR];                              // of single values (f32 products), or pairs
+        if constexpr (!WHOLE) {
+#pragma unroll
+            for (int j = 0; j < 4 * NR; ++j) {
+                if constexpr (kLoraPieces<W>)
+                    mask[j] = j % 2 ? 0 : (counts(j, rk) ? 0xFFFFu : 0u) | (counts(j + 1, rk) ? 0xFFFF0000u : 0u);
+                else
+                    mask[j] = counts(j, rk) ? 0xFFFFFFFFu : 0u;
+                asm volatile("" : "+v"(mask[j]));           // kept as a word, not as a condition
+            }
+        }
+        constexpr int NP = (NR + 1) / 2;                    // bf16 products of 32 ranks
+        LoraPieces P[kLoraPieces<W> ? NP : 1];
+        bool big = false, any_big = false;
+        if constexpr (kLoraPieces<W>) {
+            float most = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NP; ++b) {
+                float v[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[c] = 8 * b + c < 4 * NR ? s[(8 * b + c) % (4 * NR)] : 0.0f;
+                most = lora_most(v, most);
+                P[b] = lora_split(v);
+            }
+            any_big = __any(most == __builtin_inff());
+            if (any_big) big = lora_column_big(most);
+        }
+        auto weight = [&](const V& v, int g, int c) {
+            const float w = W::get(v, c);
+            if constexpr (WHOLE) return w;
+            else if constexpr (kLoraPieces<W>)
+                return __uint_as_float(__float_as_uint(w) & (mask[(GW * g + c) & ~1] << (c & 1 ? 0 : 16)) & 0xFFFF0000u);
+            else return __uint_as_float(__float_as_uint(w) & mask[GW * g + c]);
+        };
+        auto f32_products = [&](const In& z, lf4 (&d)[2]) {
+#pragma unroll
+            for (int j = 0; j < 4 * NR; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    d[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(weight(z.w[h][j / GW], j / GW, j % GW), s[j], d[h], 0, 0, 0);
+        };
+        for (;;) {
+            const int next = o0 + 32 * NW;
+            In ahead;
+            if (next < c1) load(ahead, next);
+            lf4 d[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            if constexpr (kLoraPieces<W>) {
+#pragma unroll
+                for (int b = 0; b < NP; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        union {
+                            uint32_t u[4];
+                            lb8 v;
+                        } w;
+                        if constexpr (NR == 1) {
+                            const uint2 r = __builtin_bit_cast(uint2, in.w[h][0]);
+                            w.u[0] = r.x, w.u[1] = r.y, w.u[2] = 0, w.u[3] = 0;
+                        } else {
+                            w.v = __builtin_bit_cast(lb8, in.w[h][b]);
+                        }
+                        if constexpr (!WHOLE) {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                if (8 * b + 2 * c < 4 * NR) w.u[c] &= mask[(8 * b + 2 * c) % (4 * NR)];
+                        }
+#pragma unroll
+                        for (int g = 2; g >= 0; --g) d[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v, P[b].v[g], d[h], 0, 0, 0);
+                    }
+                if (any_big) {
+                    lf4 again[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                    f32_products(in, again);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) d[h][i] = big ? again[h][i] : d[h][i];
+                }
+            } else {
+                f32_products(in, d);
+            }
+            const lf4 y[2] = {in.y[0] + d[0], in.y[1] + d[1]};
+            store(y, o0);
+            if (next >= c1) return;
+            in = ahead;
+            o0 = next;
+        }
+    }
+};
+
+// the lane's operand of S^T, of row lane % 16, times c; 0 where a value does not count
+template <typename W, int NR, int NW>
+__device__ inline void lora_sum_parts(const LoraExpand<W, NR, NW>& E, const float* part, int rk, float c, float (&s)[4 * NR]) {
+    constexpr int GW = LoraExpand<W, NR, NW>::GW;
+#pragma unroll
+    for (int j = 0; j < 4 * NR; ++j) {
+        const int r = E.at[j / GW] + j % GW;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) v += part[((size_t)w * 16 * NR + r) * 16 + E.p];
+        s[j] = E.counts(j, rk) ? v * c : 0.0f;
+    }
 }
 
 // One tile and t.cols columns per workgroup.  grid (slots, column parts, windows).
 template <typename W, int NR, int NW, int U>
 __global__ __launch_bounds__(64 * NW) void k_lora_apply(LoraArgs a, LoraTiles t) {
     __shared__ float part[NW * 16 * NR * 16];
-    const int lane = (int)threadIdx.x & 63;
+    __shared__ LoraFind<NW> find;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
     int key, n, row;
-    if (!lora_tile(a, t, lane, key, n, row)) return;
-    const int c0 = (int)blockIdx.y * t.cols, c1 = min(a.rows, c0 + t.cols);
+    if (!lora_tile<NW>(a, t, find, key, n, row)) return;
+    const int c0 = (int)blockIdx.y * t.cols, c1 = min(a.rows, c0 + t.cols), o0 = c0 + 32 * wave;
     if (key < 0) {
         lora_plain_rows(a, key, n, row, c0, c1);
         return;
     }
     const int rk = lora_rank(a, key);
     const float c = lora_scale(a, key);
-    lora_shrink_tile<W, NR, NW, U>(static_cast<const typename W::T*>(a.a) + (size_t)key * a.rank * a.k, lora_x(a, row), a.k,
-                                   a.rank, part);
+    typedef LoraExpand<W, NR, NW> Expand;
+    const Expand E(static_cast<const typename W::T*>(a.b) + (size_t)key * a.rows * a.rank, a.rank, a.rows,
+                   a.base ? reinterpret_cast<const float*>(a.base + lora_at(row, a.n_ids, a.base_id, a.base_tok)) : nullptr,
+                   reinterpret_cast<float*>(a.dst + lora_at(row, a.n_ids, a.dst_id, a.dst_tok)), (lane & 15) < n, c1);
+    typename Expand::In in;
+    if (o0 < c1) E.load(in, o0);
+    LoraShrink<W, NR, NW, U>(static_cast<const typename W::T*>(a.a) + (size_t)key * a.rank * a.k, lora_x(a, row), a.k, a.rank)
+        .run(part);
     __syncthreads();
+    if (o0 >= c1) return;
     float s[4 * NR];
-    lora_sum_parts<NR, NW>(part, a.rank, rk, c, s);
-    const typename W::T* B = static_cast<const typename W::T*>(a.b) + (size_t)key * a.rows * a.rank;
-    const float* base =
-        a.base ? reinterpret_cast<const float*>(a.base + lora_at(row, a.n_ids, a.base_id, a.base_tok)) : nullptr;
-    float* dst = reinterpret_cast<float*>(a.dst + lora_at(row, a.n_ids, a.dst_id, a.dst_tok));
-    const bool live = (lane & 15) < n;
-    if (rk == 16 * NR) lora_expand_tile<W, NR, NW, true>(B, s, a.rank, rk, a.rows, base, dst, live, c0, c1);
-    else lora_expand_tile<W, NR, NW, false>(B, s, a.rank, rk, a.rows, base, dst, live, c0, c1);
+    lora_sum_parts(E, part, rk, c, s);
+    if (rk == 16 * NR) E.template run<true>(in, o0, s, rk);
+    else E.template run<false>(in, o0, s, rk);
 }
 
 // one workgroup per row: s, u and dx
