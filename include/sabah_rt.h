@@ -320,7 +320,7 @@ int sabah_moe_route_backward(const float *d_logits, size_t logits_stride, const 
 
 /* Low-rank adapters of a projection, one (A, B) pair for each (adapter, expert); a
  * dense projection has one expert.  type: ggml's code of A and B, F32 0, F16 1 or
- * BF16 30.  rank <= 128; an adapter of a lower rank says so in ranks (the
+ * BF16 30.  rank <= 128, n_adapters * n_experts <= 2^21, rank * k and rank * rows <= 2^28; an adapter of a lower rank says so in ranks (the
  * values past it are not used) or pads A and B with zeros. */
 typedef struct sabah_lora_desc {
     const void *a;            /* device [n_adapters][n_experts][rank][k] */

@@ -199,7 +199,7 @@ static int check_lora(const char* what, const sabah_lora_desc* L, int n_ids, int
         return fail("%s: adapter type %d is none of F32 (0), F16 (1), BF16 (30)", what, L->type);
     if (L->rank <= 0 || L->rank > kLoraMaxRank) return fail("%s: rank %d outside [1, %d]", what, L->rank, kLoraMaxRank);
     if (L->n_adapters <= 0 || L->n_experts <= 0 || L->k <= 0 || L->rows <= 0 ||
-        (long long)L->n_adapters * L->n_experts > kLoraMaxKeys || L->k > 1 << 24 || L->rows > 1 << 24)
+        (long long)L->n_adapters * L->n_experts > kLoraMaxKeys || (long long)L->rank * L->k > 1 << 28 || (long long)L->rank * L->rows > 1 << 28)
         return fail("%s: invalid geometry (n_adapters=%d n_experts=%d k=%d rows=%d)", what, L->n_adapters, L->n_experts,
                     L->k, L->rows);
     if (n_ids <= 0 || n_tokens < 0 || (long long)n_ids * n_tokens > 1 << 24)
@@ -209,27 +209,38 @@ static int check_lora(const char* what, const sabah_lora_desc* L, int n_ids, int
 
 static bool stride_ok(size_t s) { return s % 4 == 0; }
 
-// Tiles of a call's rows: none up to kLoraDirectRows; above, per window of
-// rows at most one per 16 and one more per key.
+// A call of at most kLoraDirectRows rows is one launch (k_lora_apply).  Above: per window of rows at most
+// one tile per 16 rows and one more per key; the shrink's k in parts of at least eight steps
+// of 32 while there are few tiles, so that the launch fills the chip.
+constexpr int kLoraDirectRows = 256;
+constexpr int kLoraFusedTiles = 256;          // from here on a tile's shrink and expand in one workgroup
+constexpr int kLoraShrinkGroups = 1024, kLoraShrinkParts = 8, kLoraShrinkSteps = 8;
 struct LoraSpace {
-    size_t order, items, n_items, bytes;
-    int windows, slots, key_bits;
+    size_t order, items, n_items, s, bytes;
+    int windows, slots, key_bits, k_parts, k_steps, rank16;
 };
-constexpr int kLoraDirectRows = 256;          // a thread of k_lora_apply's workgroup for each
 static LoraSpace lora_space(const sabah_lora_desc* L, int n_rows) {
     LoraSpace s{};
     const int keys = L->n_adapters * L->n_experts + 2;      // without an adapter, and with a bad id
     const int span = std::min(n_rows, kLoraWindow);
     s.windows = (n_rows + kLoraWindow - 1) / kLoraWindow;
     s.slots = std::min(span, span / kLoraTile + std::min(keys, span));
+    s.rank16 = L->rank <= 16 ? 16 : L->rank <= 32 ? 32 : L->rank <= 64 ? 64 : 128;
     while (keys >> s.key_bits) ++s.key_bits;                // the word past the rows has key + 2 == keys
     if (n_rows <= kLoraDirectRows) {
         s.windows = 1;
         return s;
     }
+    const int steps = (L->k + 31) / 32, tiles = (n_rows + kLoraTile - 1) / kLoraTile;
+    const int parts = std::max(1, std::min({kLoraShrinkParts, kLoraShrinkGroups / tiles, steps / kLoraShrinkSteps}));
+    s.k_steps = (steps + parts - 1) / parts;
+    s.k_parts = (steps + s.k_steps - 1) / s.k_steps;
+    const size_t positions = tiles < kLoraFusedTiles ? (size_t)s.windows * kLoraWindow : 0;
     s.items = align256((size_t)s.windows * kLoraWindow * 4);
     s.n_items = s.items + align256((size_t)s.windows * s.slots * 16);
-    s.bytes = s.n_items + align256((size_t)s.windows * 4);
+    s.s = s.n_items + align256((size_t)s.windows * 4);
+    s.bytes = s.s + align256(s.k_parts * positions * s.rank16 * 4);
+    if (!positions) s.s = 0;
     return s;
 }
 
@@ -277,12 +288,27 @@ static int check_lora_rows(const char* what, const sabah_lora_desc* L, const flo
     return 0;
 }
 
+template <typename W, int NR, int NW, int US, int U, int OCC>
+static void launch_lora_apply_rank(const LoraArgs& a, const LoraTiles& t, int column_parts, int windows, hipStream_t st) {
+    const dim3 grid((unsigned)t.slots, (unsigned)column_parts, (unsigned)windows);
+    if (!t.order) {
+        hipLaunchKernelGGL((k_lora_apply<W, NR, NW, US, 1, true>), grid, dim3(64 * NW), 0, st, a, t);
+        return;
+    }
+    if (!t.s) {
+        hipLaunchKernelGGL((k_lora_apply<W, NR, 4, U, OCC, false>), grid, dim3(256), 0, st, a, t);
+        return;
+    }
+    hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC>), dim3((unsigned)t.slots, (unsigned)t.k_parts, (unsigned)windows),
+                       dim3(256), 0, st, a, t);
+    hipLaunchKernelGGL((k_lora_expand<W, NR, std::min(OCC, 3)>), grid, dim3(256), 0, st, a, t);
+}
 template <typename W>
-static void launch_lora_apply(const LoraArgs& a, const LoraTiles& t, dim3 grid, hipStream_t st) {
-    if (a.rank <= 16) hipLaunchKernelGGL((k_lora_apply<W, 1, 4, 2>), grid, dim3(256), 0, st, a, t);
-    else if (a.rank <= 32) hipLaunchKernelGGL((k_lora_apply<W, 2, 4, 2>), grid, dim3(256), 0, st, a, t);
-    else if (a.rank <= 64) hipLaunchKernelGGL((k_lora_apply<W, 4, 4, 1>), grid, dim3(256), 0, st, a, t);
-    else hipLaunchKernelGGL((k_lora_apply<W, 8, 4, 1>), grid, dim3(256), 0, st, a, t);
+static void launch_lora_apply(const LoraArgs& a, const LoraTiles& t, int column_parts, int windows, hipStream_t st) {
+    if (a.rank <= 16) launch_lora_apply_rank<W, 1, 8, 4, 2, 4>(a, t, column_parts, windows, st);
+    else if (a.rank <= 32) launch_lora_apply_rank<W, 2, 8, 4, 2, 4>(a, t, column_parts, windows, st);
+    else if (a.rank <= 64) launch_lora_apply_rank<W, 4, 4, 2, 1, 2>(a, t, column_parts, windows, st);
+    else launch_lora_apply_rank<W, 8, 4, 1, 1, 1>(a, t, column_parts, windows, st);
 }
 
 SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, size_t x_id_stride, int x_rows,
@@ -334,17 +360,20 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
         t.order = g.order;
         t.items = g.items;
         t.n_items = g.n_items;
+        t.s = sp.s ? reinterpret_cast<float*>(ws + sp.s) : nullptr;
+        t.k_parts = sp.k_parts;
+        t.k_steps = sp.k_steps;
+        t.positions = sp.windows * kLoraWindow;
     }
-    const long long tiles = std::min<long long>(n_rows, (long long)sp.windows * sp.slots);
-    int parts = (int)std::max<long long>(1, 512 / std::max<long long>(1, tiles));
-    parts = std::min(parts, (lora->rows + 63) / 64);
-    t.cols = ((lora->rows + parts - 1) / parts + 31) / 32 * 32;
+    // columns per workgroup: a step of 64 for each wave of the expand; in small calls what fills the chip
+    int parts = t.s ? (lora->rows + 255) / 256 : 1;
+    if (!sp.bytes) parts = std::max(1, std::min((lora->rows + 63) / 64, 2 * g_num_cu / sp.slots));
+    t.cols = ((lora->rows + parts - 1) / parts + 63) / 64 * 64;
     parts = (lora->rows + t.cols - 1) / t.cols;
-    const dim3 grid((unsigned)sp.slots, (unsigned)parts, (unsigned)sp.windows);
     switch (lora->type) {
-    case kTypeF32: launch_lora_apply<LoraF32>(a, t, grid, st); break;
-    case kTypeF16: launch_lora_apply<LoraF16>(a, t, grid, st); break;
-    default: launch_lora_apply<LoraBF16>(a, t, grid, st); break;
+    case kTypeF32: launch_lora_apply<LoraF32>(a, t, parts, sp.windows, st); break;
+    case kTypeF16: launch_lora_apply<LoraF16>(a, t, parts, sp.windows, st); break;
+    default: launch_lora_apply<LoraBF16>(a, t, parts, sp.windows, st); break;
     }
     return ck(hipGetLastError(), "adapters launch") ? 0 : -1;
 }

@@ -123,20 +123,22 @@ __device__ inline void lora_shrink(const typename W::T* A, const float* x, int k
 }
 
 // ---------------------------------------------------------------------------
-// Tiles: up to 16 rows of one key.  A workgroup with a thread for every row of the call finds its
-// tile by itself (lora_tile); above, k_lora_group sorts each window of 1,024 rows by key
-// and lists its tiles.
+// Tiles: up to 16 rows of one key.  In small calls each workgroup finds its tile by itself
+// (lora_tile, a thread for every row of the call); above, k_lora_group sorts each window of 1,024
+// rows by key and lists its tiles.
 // ---------------------------------------------------------------------------
 constexpr int kLoraTile = 16;
 constexpr int kLoraWindow = 1024;
 
 struct LoraTiles {
-    const int* order;             // [windows * 1024]: rows by key, each window on its own; null: found by each workgroup
+    const int* order;             // [windows * 1024]: rows by key, each window on its own
     const int4* items;            // [windows][slots]: (key, position in order, rows)
     const int* n_items;           // [windows]
     int n_rows, slots, skip_none; // skip_none: rows without an adapter are left alone
     int key_bits;                 // of key + 2 and of one more
     int cols;                     // columns of the output per workgroup
+    float* s;                     // larger calls: [k_parts][positions][rank, in 16s]
+    int k_parts, k_steps, positions;
 };
 
 struct LoraGroup {
@@ -154,39 +156,49 @@ __device__ inline uint32_t lora_word(const LoraArgs& a, int row, int n_rows, int
     return ((uint32_t)(key + 2) << 10) | (uint32_t)at;
 }
 
-// LDS of the sort: NW waves at most
+// LDS of the sort: NW waves at most (16); w and m are zeros for waves that the workgroup lacks
 template <int NW>
 struct LoraSort {
     uint32_t c[64 * NW];
-    int w[NW];                    // zeros for waves that the workgroup lacks
-    uint64_t m[NW];
+    uint2 w[16];
+    uint64_t m[NW + 1];
 };
 
-// The workgroup's words in the order of their keys (stable), one per thread, left in f.c too: a radix sort by single
-// bits, as many as the keys have.  Every wave reads all the waves' counts at once: a loop over
-// them cost 0.8 us a bit with 16 waves.
+// inclusive sum over the 16 lanes of a row up to the lane's
+__device__ inline uint32_t lora_row_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, true);     // row_shr 1, 2, 4, 8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, true);
+    return v;
+}
+
+// The workgroup's words in the order of their keys (stable), one per thread, left in f.c too: a radix sort by two
+// bits, as many as the keys have.  A wave's counts of the four digits are packed in four halves, and
+// every wave sums all the waves' in its lanes (a loop over them cost 0.8 us a bit with 16 waves).
 template <int NW>
 __device__ inline uint32_t lora_sort(uint32_t c, int bits, LoraSort<NW>& f) {
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, nt = (int)blockDim.x;
-    if (tid < NW) {
-        f.w[tid] = 0;
-        f.m[tid] = 0;
-    }
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (tid < 16) f.w[tid] = make_uint2(0, 0);
+    if (tid <= NW) f.m[tid] = 0;
     f.c[tid] = c;
     __syncthreads();
-    for (int b = 10; b < 10 + bits; ++b) {
-        const bool one = (c >> b) & 1u;
-        const uint64_t m = __ballot(one);
-        if (lane == 0) f.w[wave] = __popcll(m);
+    for (int b = 10; b < 10 + bits; b += 2) {
+        const uint32_t d = (c >> b) & 3u;
+        const uint64_t hi = __ballot((d & 2u) != 0), lo = __ballot((d & 1u) != 0);
+        const uint2 own = make_uint2((uint32_t)__popcll(~hi & ~lo) | (uint32_t)__popcll(~hi & lo) << 16,
+                                     (uint32_t)__popcll(hi & ~lo) | (uint32_t)__popcll(hi & lo) << 16);
+        if (lane == 0) f.w[wave] = own;
         __syncthreads();
-        int ones = __popcll(m & ((1ull << lane) - 1ull)), total = 0;
-#pragma unroll
-        for (int v = 0; v < NW; ++v) {
-            const int x = f.w[v];
-            ones += v < wave ? x : 0;
-            total += x;
-        }
-        f.c[one ? nt - total + ones : tid - ones] = c;
+        const uint2 x = f.w[lane & 15];
+        const uint32_t sx = lora_row_scan(x.x), sy = lora_row_scan(x.y);
+        const uint32_t tx = (uint32_t)__builtin_amdgcn_readlane((int)sx, 15), ty = (uint32_t)__builtin_amdgcn_readlane((int)sy, 15);
+        const uint32_t bx = (uint32_t)__builtin_amdgcn_readlane((int)sx, wave) - own.x,
+                       by = (uint32_t)__builtin_amdgcn_readlane((int)sy, wave) - own.y;
+        const uint32_t n0 = tx & 0xFFFFu, n1 = n0 + (tx >> 16), n2 = n1 + (ty & 0xFFFFu);
+        const uint64_t same = (d & 2u ? hi : ~hi) & (d & 1u ? lo : ~lo);
+        const uint32_t first = d & 2u ? (d & 1u ? n2 + (by >> 16) : n1 + (by & 0xFFFFu)) : d & 1u ? n0 + (bx >> 16) : bx & 0xFFFFu;
+        f.c[first + (uint32_t)__popcll(same & ((1ull << lane) - 1ull))] = c;
         __syncthreads();
         c = f.c[tid];
     }
@@ -197,30 +209,31 @@ __device__ inline uint32_t lora_sort(uint32_t c, int bits, LoraSort<NW>& f) {
 // (its number of rows, else 0), and the tiles before it.
 template <int NW>
 __device__ inline int lora_leader(uint32_t c, LoraSort<NW>& f, int n_keys2, bool skip_none, int& slot) {
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, nt = (int)blockDim.x;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), nt = (int)blockDim.x;
     const uint32_t k2 = c >> 10;
     const uint64_t head = __ballot(tid == 0 || (f.c[max(tid - 1, 0)] >> 10) != k2);   // rows that begin a run
-    if (lane == 0) f.m[wave] = head;
     __syncthreads();
-    int start = 0;                                          // of the thread's run
-    uint64_t next = 0;                                      // the heads of the wave after this one
-#pragma unroll
-    for (int v = 0; v < NW; ++v) {
-        const uint64_t h = f.m[v];
-        if (v < wave && h) start = 64 * v + 63 - __builtin_clzll(h);
-        if (v == wave + 1) next = h;
+    if (lane == 0) {
+        f.m[wave] = head;
+        f.w[wave].x = head ? 64u * wave + 63u - (uint32_t)__builtin_clzll(head) : 0u;
     }
+    __syncthreads();
+    // the last head of the earlier waves
+    const uint64_t next = f.m[wave + 1];
+    const uint32_t last = f.w[lane & 15].x;
     const uint64_t upto = head & ((2ull << lane) - 1ull), after = head & ~((2ull << lane) - 1ull);
+    int start = 0;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) start = max(start, v < wave ? __builtin_amdgcn_readlane((int)last, v) : 0);
     if (upto) start = 64 * wave + 63 - __builtin_clzll(upto);
-    int end = after ? 64 * wave + __builtin_ctzll(after) : next ? 64 * wave + 64 + __builtin_ctzll(next) : nt;
+    const int end = after ? 64 * wave + __builtin_ctzll(after) : next ? 64 * wave + 64 + __builtin_ctzll(next) : nt;
     const bool leader = (int)k2 < n_keys2 && ((tid - start) & (kLoraTile - 1)) == 0 && !(skip_none && (int)k2 == kLoraNone + 2);
     const uint64_t m = __ballot(leader);
     __syncthreads();
-    if (lane == 0) f.w[wave] = __popcll(m);
+    if (lane == 0) f.w[wave].x = (uint32_t)__popcll(m);
     __syncthreads();
-    slot = __popcll(m & ((1ull << lane) - 1ull));
-#pragma unroll
-    for (int v = 0; v < NW; ++v) slot += v < wave ? f.w[v] : 0;
+    const uint32_t before = lora_row_scan(f.w[lane & 15].x);
+    slot = __builtin_amdgcn_readlane((int)before, wave) - __popcll(m) + __popcll(m & ((1ull << lane) - 1ull));
     return leader ? min(kLoraTile, end - tid) : 0;          // a head two waves on is more than 16 rows away
 }
 
@@ -248,21 +261,31 @@ struct LoraFind {
 template <int NW>
 __device__ inline bool lora_tile(const LoraArgs& a, const LoraTiles& t, LoraFind<NW>& f, int& key, int& n, int& row) {
     const int tid = (int)threadIdx.x, p = tid & (kLoraTile - 1);
-    if (t.order) {
-        const int w = (int)blockIdx.z;
-        if ((int)blockIdx.x >= t.n_items[w]) return false;
-        const int4 it = t.items[(size_t)w * t.slots + blockIdx.x];
-        key = __builtin_amdgcn_readfirstlane(it.x);
-        n = __builtin_amdgcn_readfirstlane(it.z);
-        row = t.order[it.y + min(p, n - 1)];
-        return true;
-    }
     if (t.n_rows == 1) {
         row = 0;
         n = 1;
         key = __builtin_amdgcn_readfirstlane(lora_key(a, 0));
         if (key == kLoraBad && tid == 0) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrLora;
         return !(t.skip_none && key == kLoraNone);
+    }
+    if (t.n_rows <= 64) {                                   // every wave for itself, without a barrier
+        const int lane = tid & 63, k = lane < t.n_rows ? lora_key(a, lane) : 0x7FFFFFFF;
+        if (k == kLoraBad) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrLora;
+        int idx = 0;                                        // earlier rows of the lane's key
+        for (int j = 0; j < t.n_rows; ++j) idx += __builtin_amdgcn_readlane(k, j) == k && j < lane;
+        const bool leader = lane < t.n_rows && (idx & (kLoraTile - 1)) == 0 && !(t.skip_none && k == kLoraNone);
+        const uint64_t m = __ballot(leader);
+        const uint64_t mine = __ballot(leader && __popcll(m & ((1ull << lane) - 1ull)) == (int)blockIdx.x);
+        if (mine == 0) return false;
+        const int first = __builtin_ctzll(mine);
+        key = __builtin_amdgcn_readlane(k, first);
+        const int i0 = __builtin_amdgcn_readlane(idx, first);
+        const bool in = lane < t.n_rows && k == key && idx >= i0 && idx < i0 + kLoraTile;
+        n = __popcll(__ballot(in));
+        // the lane's number to its place in the tile; the others' to place 63, which nobody reads
+        const int at = __builtin_amdgcn_ds_permute((in ? idx - i0 : 63) * 4, lane);
+        row = __shfl(at, min(p, n - 1));
+        return true;
     }
     const uint32_t c = lora_sort(lora_word(a, tid, t.n_rows, tid), t.key_bits, f.s);
     if (tid == 0) f.item[2] = 0;
@@ -281,6 +304,18 @@ __device__ inline bool lora_tile(const LoraArgs& a, const LoraTiles& t, LoraFind
     return true;
 }
 
+// The same from the lists of k_lora_group, with the tile's position in order
+__device__ inline bool lora_item(const LoraTiles& t, int& key, int& n, int& row, int& pos) {
+    const int w = (int)blockIdx.z;
+    if ((int)blockIdx.x >= t.n_items[w]) return false;
+    const int4 it = t.items[(size_t)w * t.slots + blockIdx.x];
+    key = __builtin_amdgcn_readfirstlane(it.x);
+    pos = __builtin_amdgcn_readfirstlane(it.y);
+    n = __builtin_amdgcn_readfirstlane(it.z);
+    row = t.order[pos + min((int)threadIdx.x & (kLoraTile - 1), n - 1)];
+    return true;
+}
+
 // columns c0 .. c1 of a tile whose rows have no adapter (a copy of base, or zeros) or a bad id (NaN)
 __device__ inline void lora_plain_rows(const LoraArgs& a, int key, int n, int row, int c0, int c1) {
     for (int p = 0; p < n; ++p) {
@@ -293,213 +328,332 @@ __device__ inline void lora_plain_rows(const LoraArgs& a, int key, int n, int ro
     }
 }
 
-// eight values of a row from column i on, zeros from column n on
-template <typename W>
-__device__ inline typename W::V8 lora_load8(const typename W::T* row, int i, int n) {
-    if (i + 8 <= n) return W::load8(row + i);
-    typename W::V8 v{};
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-        if (i + c < n) W::set(v, c, row[i + c]);
-    return v;
-}
-
 // ---------------------------------------------------------------------------
-// Products of a weight operand (A: row m = lane % 16 of it) with an f32 operand (B: column lane % 16), eight
-// neighbours of the summed axis per lane, on a tile whose lane holds column lane % 16 and rows 4 (lane / 16) .. +3.
-//   f32 and f16 weights   eight v_mfma_f32_16x16x4 (any order of the summed axis is the same sum)
-//   bf16 weights          the f32 operand in three bf16 pieces that add up to it exactly (each
-//                         keeps the next 8 of its 24 bits), three v_mfma_f32_16x16x32_bf16: 48
-//                         cycles against 256, with the same products and an f32 sum
-// An infinity has no pieces (its rest is inf - inf): its columns are done with the f32 form (big).
+// Products of a weight operand with an f32 operand, eight neighbours of the summed axis per lane, on a 16 x 16 tile.
+//   f32 weights    eight v_mfma_f32_16x16x4 (any order of the summed axis is the same sum): 256 cycles
+//   bf16 weights   the f32 operand in three bf16 pieces that add up to it exactly (each keeps the next 8 of
+//                  its 24 bits), three v_mfma_f32_16x16x32_bf16: 48 cycles, the same products
+//   f16 weights    two f16 pieces of 11 bits, rounded to nearest, of the operand scaled by a power of two that
+//                  brings its row's largest of these values to 2^14 .. 2^15: what is left out is below
+//                  2^-24 of a value, or 2^-39 of the largest.  32 cycles, and a product with the scale
+// Sums are f32.  An infinity has no pieces (its rest is inf - inf): a wave that meets one does the rows
+// that have it again with plain products.
 // ---------------------------------------------------------------------------
 typedef __bf16 lb8 __attribute__((ext_vector_type(8)));
+typedef _Float16 lh2 __attribute__((ext_vector_type(2)));
+typedef _Float16 lh8 __attribute__((ext_vector_type(8)));
+typedef float lf2 __attribute__((ext_vector_type(2)));
 
-struct LoraPieces {
-    lb8 v[3];
+template <typename W>
+constexpr int kLoraPieces = 0;                              // pieces of the f32 operand; 0: it stays whole
+template <>
+constexpr int kLoraPieces<LoraBF16> = 3;
+template <>
+constexpr int kLoraPieces<LoraF16> = 2;
+
+struct LoraWords {
+    uint32_t u[4];                                          // eight 16-bit values
 };
-__device__ inline LoraPieces lora_split(const float (&x)[8]) {
-    union {
-        uint32_t u[4];
-        lb8 b;
-    } p[3];
+__device__ inline lf4 lora_mfma(LoraBF16, const LoraWords& a, const LoraWords& b, lf4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lb8, a), __builtin_bit_cast(lb8, b), c, 0, 0, 0);
+}
+__device__ inline lf4 lora_mfma(LoraF16, const LoraWords& a, const LoraWords& b, lf4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(lh8, a), __builtin_bit_cast(lh8, b), c, 0, 0, 0);
+}
+__device__ inline void lora_split(LoraBF16, const float (&x)[8], float, LoraWords (&w)[3]) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         float r[2] = {x[2 * c], x[2 * c + 1]};
 #pragma unroll
         for (int g = 0; g < 3; ++g) {
             // the upper halves of the two words
-            p[g].u[c] = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302u);
+            w[g].u[c] = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302u);
 #pragma unroll
             for (int e = 0; e < 2; ++e) r[e] = r[e] - __uint_as_float(__float_as_uint(r[e]) & 0xFFFF0000u);
         }
     }
-    return LoraPieces{{p[0].b, p[1].b, p[2].b}};
 }
-__device__ inline float lora_most(const float (&x)[8], float m) {
+__device__ inline void lora_split(LoraF16, const float (&x)[8], float scale, LoraWords (&w)[2]) {
 #pragma unroll
-    for (int c = 0; c < 8; ++c) m = fmaxf(m, __builtin_fabsf(x[c]));
+    for (int c = 0; c < 4; ++c) {
+        lf2 r = {x[2 * c] * scale, x[2 * c + 1] * scale};
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const lh2 h = __builtin_convertvector(r, lh2);
+            w[g].u[c] = __builtin_bit_cast(uint32_t, h);
+            r[0] = r[0] - (float)h[0];                      // exact
+            r[1] = r[1] - (float)h[1];
+        }
+    }
+}
+// The power of two that brings `most` to 2^14 .. 2^15 (at most 2^126), and its inverse
+__device__ inline float lora_scale_of(float most, float& back) {
+    const uint32_t e = max(__float_as_uint(most) >> 23, 15u);
+    back = __uint_as_float((e - 14u) << 23);
+    return __uint_as_float((268u - e) << 23);
+}
+template <int N>
+__device__ inline float lora_most(const float (&x)[N], float m) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) m = fmaxf(m, __builtin_fabsf(x[c]));
     return m;
 }
-// lane p's flag of column p, from the four lanes that hold it
-__device__ inline bool lora_column_big(float most) {
-    most = fmaxf(most, __shfl_xor(most, 16));
-    return fmaxf(most, __shfl_xor(most, 32)) == __builtin_inff();
+// of column p, from the four lanes that hold it
+__device__ inline float lora_column_most(float most) {
+    const uint32_t m = __float_as_uint(most);
+    const auto h = __builtin_amdgcn_permlane32_swap(m, m, false, false);    // both halves in both
+    const uint32_t n = max(h[0], h[1]);                                     // magnitudes order as words
+    const auto r = __builtin_amdgcn_permlane16_swap(n, n, false, false);
+    return __uint_as_float(max(r[0], r[1]));
 }
-template <typename W>
-constexpr bool kLoraPieces = false;
-template <>
-constexpr bool kLoraPieces<LoraBF16> = true;
+__device__ inline unsigned lora_big_rows(float most) {
+    return (unsigned)(__ballot(lora_column_most(most) == __builtin_inff()) & 0xFFFFu);
+}
 
-// S = X A^T of a tile: the waves share k in steps of 32, of which lane l holds the eight
-// values at 8 (l / 16) of row l % 16 of X and of A; part [NW][16 NR][16] gets each wave's (rank, row).  Rows of
-// A past the rank are the last one's again.  U steps are loaded while U others are multiplied.
+// S = X A^T of a tile: the waves share k in steps of 32, of which lane l's operands are the eight
+// values at 8 (l / 16) of row l % 16 of X and of A.  Both are read along their rows and turned in LDS: in operand
+// order neighbouring lanes read different rows, and the L1 takes 64 cycles a load instead of 16.
+// part [NW][16 NR][17] gets each wave's (rank, row).  Rows of A past the rank are the last one's again.
+// U steps are loaded at a time.
+constexpr int kLoraPart = 17;                 // floats of part per rank
+constexpr int kLoraXLds = 16 * 9;             // of a wave: 16 rows of 128 bytes, 144 apart: no bank conflicts either way
+template <typename W>
+constexpr int kLoraALds = sizeof(typename W::T) == 4 ? 16 * 9 : 16 * 5;   // rows of 128 or 64 bytes
 template <typename W, int NR, int NW, int U>
 struct LoraShrink {
+    static constexpr int CH = sizeof(typename W::T) / 2;    // loads of 16 bytes for 16 rows of A
     struct In {
-        LoraF32::V8 x;
-        typename W::V8 a[NR];
+        lf4 x[2], a[NR][CH];
     };
-    const typename W::T* ar[NR];
-    const float* x;
-    int k, q;
+    const typename W::T* A;
+    const float* xr[2];
+    uint32_t at[NR][CH];                                    // elements; rank * k is below 2^28
+    lf4 *lx, *la;                                           // the wave's
+    int k, s0, steps, p, q, lane, rank;                     // whole steps s0 .. steps, and k's rest if steps is the last
     float most = 0.0f;
 
-    __device__ inline LoraShrink(const typename W::T* A, const float* x_, int k_, int rank) : x(x_), k(k_) {
-        const int lane = (int)threadIdx.x & 63, p = lane & 15;
+    // row: of the lane's place lane % 16 in the tile; lds: NW * (kLoraXLds + kLoraALds<W>); of k the steps from s0 on, below s1
+    __device__ inline LoraShrink(const LoraArgs& a, const typename W::T* A_, int row, lf4* lds, int s0_, int s1)
+        : A(A_), k(a.k), s0(s0_), steps(min(s1, a.k / 32)), rank(a.rank) {
+        lane = (int)threadIdx.x & 63;
+        p = lane & 15;
         q = lane >> 4;
+        lx = lds + ((int)threadIdx.x >> 6) * (kLoraXLds + kLoraALds<W>);
+        la = lx + kLoraXLds;
 #pragma unroll
-        for (int b = 0; b < NR; ++b) ar[b] = A + (size_t)min(16 * b + p, rank - 1) * k;
-    }
-    __device__ inline void load(In& in, int s) const {
-        const int i = s * 32 + 8 * q;
-        in.x = LoraF32::load8(x + i);
-#pragma unroll
-        for (int b = 0; b < NR; ++b) in.a[b] = W::load8(ar[b] + i);
-    }
-    __device__ inline void load_rest(In& in, int s) const {
-        const int i = s * 32 + 8 * q;
-        in.x = lora_load8<LoraF32>(x, i, k);
-#pragma unroll
-        for (int b = 0; b < NR; ++b) in.a[b] = lora_load8<W>(ar[b], i, k);
-    }
-    template <bool PIECES>
-    __device__ inline void mul(const In& in, lf4 (&acc)[NR]) {
-        if constexpr (PIECES) {
-            float v[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) v[c] = LoraF32::get(in.x, c);
-            most = lora_most(v, most);
-            const LoraPieces P = lora_split(v);
-#pragma unroll
-            for (int g = 2; g >= 0; --g)
-#pragma unroll
-                for (int b = 0; b < NR; ++b)
-                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lb8, in.a[b]), P.v[g], acc[b], 0, 0, 0);
-        } else {
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-#pragma unroll
-                for (int b = 0; b < NR; ++b)
-                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(W::get(in.a[b], c), LoraF32::get(in.x, c), acc[b], 0, 0, 0);
-        }
-    }
-    template <bool PIECES>
-    __device__ inline void sum(lf4 (&acc)[NR]) {
-        const int wave = (int)threadIdx.x >> 6, steps = k / 32;
-#pragma unroll
-        for (int b = 0; b < NR; ++b) acc[b] = lf4{0, 0, 0, 0};
-        In in[2][U];
-        auto load_all = [&](In (&z)[U], int s) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) load(z[u], s + u * NW);
-        };
-        auto mul_all = [&](const In (&z)[U]) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) mul<PIECES>(z[u], acc);
-        };
-        int s = wave;                                       // the first step that is not loaded
-        auto more = [&] { return s + (U - 1) * NW < steps; };
-        if (more()) {
-            load_all(in[0], s);
-            s += U * NW;
-            for (;;) {
-                bool m = more();
-                if (m) load_all(in[1], s), s += U * NW;
-                mul_all(in[0]);
-                if (!m) break;
-                m = more();
-                if (m) load_all(in[0], s), s += U * NW;
-                mul_all(in[1]);
-                if (!m) break;
-            }
-        }
-        for (; s <= steps; s += NW) {                       // what is left of whole steps, then k's rest
-            if (s == steps && k % 32 == 0) break;
-            load_rest(in[0][0], s);
-            mul<PIECES>(in[0][0], acc);
-        }
-    }
-    __device__ inline void run(float* part) {
-        const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, p = lane & 15;
-        lf4 acc[NR];
-        sum<kLoraPieces<W>>(acc);
-        if constexpr (kLoraPieces<W>) {
-            if (__any(most == __builtin_inff())) {          // rare: the columns with an infinity again
-                const bool big = lora_column_big(most);
-                lf4 again[NR];
-                sum<false>(again);
-#pragma unroll
-                for (int b = 0; b < NR; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[b][i] = big ? again[b][i] : acc[b][i];
-            }
-        }
+        for (int h = 0; h < 2; ++h) xr[h] = lora_x(a, __shfl(row, 8 * h + (lane >> 3)));
 #pragma unroll
         for (int b = 0; b < NR; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[((size_t)wave * 16 * NR + 16 * b + 4 * q + i) * 16 + p] = acc[b][i];
+            for (int h = 0; h < CH; ++h) at[b][h] = (uint32_t)min(16 * b + a_row(h), a.rank - 1) * (uint32_t)k + a_col();
+    }
+    // of 16 rows of A in one step of 32 columns, the row and the first column of the lane's load h
+    __device__ inline int a_row(int h) const { return CH == 1 ? lane >> 2 : 8 * h + (lane >> 3); }
+    __device__ inline int a_col() const { return CH == 1 ? 8 * (lane & 3) : 4 * (lane & 7); }
+    __device__ inline void load(In& in, int s) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) in.x[h] = *reinterpret_cast<const lf4u*>(xr[h] + s * 32 + 4 * (lane & 7));
+#pragma unroll
+        for (int b = 0; b < NR; ++b)
+#pragma unroll
+            for (int h = 0; h < CH; ++h) {
+                const typename W::T* w = A + at[b][h] + (uint32_t)s * 32u;
+                if constexpr (CH == 1) in.a[b][h] = __builtin_bit_cast(lf4, W::load8(w));
+                else in.a[b][h] = W::load4(w).v;
+            }
+    }
+    __device__ inline void load_rest(In& in, int s) const {
+        const int j = s * 32 + 4 * (lane & 7), i = s * 32 + a_col();
+        constexpr int N = 16 / sizeof(typename W::T);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) in.x[h][c] = j + c < k ? xr[h][j + c] : 0.0f;
+#pragma unroll
+        for (int b = 0; b < NR; ++b)
+#pragma unroll
+            for (int h = 0; h < CH; ++h) {
+                union {
+                    typename W::T t[N];
+                    lf4 v;
+                } w;
+#pragma unroll
+                for (int c = 0; c < N; ++c) w.t[c] = i + c < k ? A[at[b][h] + (uint32_t)(s * 32 + c)] : (typename W::T)0;
+                in.a[b][h] = w.v;
+            }
+    }
+    // 16 rows from the order of their loads to the operand's, eight values per lane.  The reads wait for the
+    // writes (one wave, LDS in order); the barriers keep the compiler from moving either.
+    __device__ inline void turn_rows128(lf4* lds, const lf4 (&in)[2], lf4 (&v)[2]) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) lds[(8 * h + (lane >> 3)) * 9 + (lane & 7)] = in[h];
+        __builtin_amdgcn_wave_barrier();
+        v[0] = lds[p * 9 + 2 * q];
+        v[1] = lds[p * 9 + 2 * q + 1];
+        __builtin_amdgcn_wave_barrier();
+    }
+    __device__ inline lf4 turn_rows64(lf4* lds, const lf4& in) const {
+        lds[(lane >> 2) * 5 + (lane & 3)] = in;
+        __builtin_amdgcn_wave_barrier();
+        const lf4 v = lds[p * 5 + q];
+        __builtin_amdgcn_wave_barrier();
+        return v;
+    }
+    __device__ inline void mul(const In& in, lf4 (&acc)[NR]) {
+        lf4 t[2];
+        turn_rows128(lx, in.x, t);
+        if constexpr (kLoraPieces<W> > 0) {
+            float v[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] = t[c >> 2][c & 3];
+            const float here = lora_most(v, 0.0f);
+            most = fmaxf(most, here);
+            float back = 1.0f, scale = 1.0f;
+            if constexpr (std::is_same<W, LoraF16>::value) scale = lora_scale_of(lora_column_most(here), back);
+            LoraWords P[kLoraPieces<W>];
+            lora_split(W{}, v, scale, P);
+#pragma unroll
+            for (int b = 0; b < NR; ++b) {
+                const LoraWords w = __builtin_bit_cast(LoraWords, turn_rows64(la, in.a[b][0]));
+                if constexpr (std::is_same<W, LoraF16>::value) {
+                    lf4 d = {0, 0, 0, 0};
+#pragma unroll
+                    for (int g = kLoraPieces<W> - 1; g >= 0; --g) d = lora_mfma(W{}, w, P[g], d);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[b][i] = __builtin_fmaf(d[i], back, acc[b][i]);
+                } else {
+#pragma unroll
+                    for (int g = kLoraPieces<W> - 1; g >= 0; --g) acc[b] = lora_mfma(W{}, w, P[g], acc[b]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < NR; ++b) {
+                lf4 w[2];
+                turn_rows128(la, in.a[b], w);
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[c >> 2][c & 3], t[c >> 2][c & 3], acc[b], 0, 0, 0);
+            }
+        }
+    }
+    // part as above
+    __device__ inline void run(float* part) {
+        const int wave = (int)threadIdx.x >> 6;
+        lf4 acc[NR];
+#pragma unroll
+        for (int b = 0; b < NR; ++b) acc[b] = lf4{0, 0, 0, 0};
+        In in[U];
+        for (int s = s0 + wave; s < steps; s += U * NW) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) load(in[u], min(s + u * NW, steps - 1));
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s + u * NW < steps) mul(in[u], acc);
+        }
+        const bool rest = rest_is(wave);
+        if (rest) {
+            load_rest(in[0], steps);
+            mul(in[0], acc);
+        }
+        float* mine = part + (size_t)wave * 16 * NR * kLoraPart;
+#pragma unroll
+        for (int b = 0; b < NR; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine[(16 * b + 4 * q + i) * kLoraPart + p] = acc[b][i];
+        if constexpr (kLoraPieces<W> > 0) {
+            if (__any(most == __builtin_inff())) plain(mine, lora_big_rows(most), wave, rest);
+        }
+    }
+    // k's rest belongs to the wave whose turn it is after the last whole step of all
+    __device__ inline bool rest_is(int wave) const {
+        return steps == k / 32 && k % 32 != 0 && (steps - s0) % NW == wave;
+    }
+    // rare: the tile's rows in `rows` with plain products, over the wave's own share of k
+    __device__ inline void plain(float* mine, unsigned rows, int wave, bool rest) const {
+        __builtin_amdgcn_wave_barrier();
+        for (int t = 0; t < 16; ++t) {
+            const uint64_t at_lo = (uint64_t)(uintptr_t)xr[t >> 3];     // lane 8 (t % 8) holds row t's address
+            const float* x = reinterpret_cast<const float*>(
+                (uintptr_t)((uint64_t)(uint32_t)__shfl((int)(uint32_t)at_lo, 8 * (t & 7)) |
+                            (uint64_t)(uint32_t)__shfl((int)(uint32_t)(at_lo >> 32), 8 * (t & 7)) << 32));
+            if (!((rows >> t) & 1u)) continue;
+            for (int r = 0; r < rank; ++r) {
+                float sum = 0.0f;
+                for (int s = s0 + wave; s < steps + (rest ? 1 : 0); s += NW) {
+                    const int i = s * 32 + (lane & 31);
+                    if (lane < 32 && i < k) sum = __builtin_fmaf(W::value(A[(size_t)r * k + i]), x[i], sum);
+                }
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+                if (lane == 0) mine[r * kLoraPart + t] = sum;
+            }
+        }
     }
 };
 
-// y = base + B S over columns c0 .. c1 of the tile, in steps of 32 columns per wave: D = B S^T, two products of 16
-// columns, so that a lane holds eight neighbouring columns (four of each) of row lane % 16.
+// y = base + S B^T over columns c0 .. c1 of the tile, in steps of 64 columns per wave: product j of four has the
+// columns o0 + 4 n + j, so that a lane holds four neighbouring columns (4 (lane % 16)) of each
+// of the rows 4 (lane / 16) .. +3, and a load or store covers 256 bytes of four rows.
 // The ranks of a lane's 4 NR values of a row of B and of S: groups of GW from 4 NR (lane / 16) on; a
 // group that reaches past the rank is moved back to the row's last GW (rows of fewer than four: the
 // last value again), so that loads stay inside the row.  A value counts if it is not one that an
 // earlier group has, and below the adapter's own rank; the others' weights become zeros by a
 // mask in registers (a NaN or an infinity past an adapter's own rank must not meet its zero in S).
+template <int NR>
+constexpr int kLoraGroupWidth = NR == 1 ? 4 : 8;
+// the rank of value j of a row's 16 NR (lane j / (4 NR)'s j % (4 NR)), and whether it counts
+template <int NR>
+__device__ inline int lora_value_at(int j, int rank) {
+    constexpr int GW = kLoraGroupWidth<NR>;
+    return min(j / GW * GW, max(0, rank - GW)) + j % GW;
+}
+template <int NR>
+__device__ inline bool lora_value_counts(int j, int rank, int rk) {
+    const int r = lora_value_at<NR>(j, rank);
+    return r >= j / kLoraGroupWidth<NR> * kLoraGroupWidth<NR> && r < rk;
+}
 template <typename W, int NR, int NW>
 struct LoraExpand {
-    static constexpr int GW = NR == 1 ? 4 : 8, NG = 4 * NR / GW;
+    static constexpr int GW = kLoraGroupWidth<NR>, NG = 4 * NR / GW;
     typedef typename std::conditional<NR == 1, typename W::V4, typename W::V8>::type V;
     struct In {
-        V w[2][NG];
-        lf4 y[2];
+        V w[4][NG];
+        lf4 y[4];
     };
-    const typename W::T* B;
-    const float* base;
-    float* dst;
+    const typename W::T* B;                                 // rows * rank is below 2^28
+    const uint8_t* base[4];                                 // of the lane's four rows; base[0] null: zeros
+    uint8_t* dst[4];
     int rank, rows, c1, p, q, at[NG];
-    bool live;
 
-    __device__ inline LoraExpand(const typename W::T* B_, int rank_, int rows_, const float* base_, float* dst_, bool live_,
-                                 int c1_)
-        : B(B_), base(base_), dst(dst_), rank(rank_), rows(rows_), c1(c1_), live(live_) {
+    // row: of the lane's place lane % 16 in the tile
+    __device__ inline LoraExpand(const LoraArgs& a, const typename W::T* B_, int row, int c1_)
+        : B(B_), rank(a.rank), rows(a.rows), c1(c1_) {
         const int lane = (int)threadIdx.x & 63;
         p = lane & 15;
         q = lane >> 4;
 #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = __shfl(row, 4 * q + i);
+            base[i] = a.base ? a.base + lora_at(r, a.n_ids, a.base_id, a.base_tok) : nullptr;
+            dst[i] = a.dst + lora_at(r, a.n_ids, a.dst_id, a.dst_tok);
+        }
+#pragma unroll
         for (int g = 0; g < NG; ++g) at[g] = min(4 * NR * q + GW * g, max(0, rank - GW));
     }
-    __device__ inline bool counts(int j, int rk) const {
+    // all bits of a value that counts, else none: by the signs, since conditions for every value fill the scalar registers
+    __device__ inline uint32_t counts(int j, int rk) const {
         const int r = at[j / GW] + j % GW;
-        return r >= 4 * NR * q + j / GW * GW && r < rk;
+        return ~(uint32_t)(((r - (4 * NR * q + j / GW * GW)) | (rk - 1 - r)) >> 31);
     }
     __device__ inline void load(In& in, int o0) const {
+        load_y(in, o0);
+        load_w(in, o0);
+    }
+    __device__ inline void load_w(In& in, int o0) const {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const typename W::T* row = B + (size_t)min(o0 + 8 * (p >> 2) + 4 * h + (p & 3), rows - 1) * rank;
+        for (int h = 0; h < 4; ++h) {
+            const typename W::T* row = B + (uint32_t)min(o0 + 4 * p + h, rows - 1) * (uint32_t)rank;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 if constexpr (NR == 1) {
@@ -514,167 +668,264 @@ struct LoraExpand {
                 }
             }
         }
-        const int o = o0 + 8 * q;
-        in.y[0] = lf4{0, 0, 0, 0};
-        in.y[1] = lf4{0, 0, 0, 0};
-        if (!base) return;
-        if (o + 8 <= c1) {
-            in.y[0] = *reinterpret_cast<const lf4u*>(base + o);
-            in.y[1] = *reinterpret_cast<const lf4u*>(base + o + 4);
-        } else {
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-                if (o + c < c1) in.y[c >> 2][c & 3] = base[o + c];
-        }
     }
-    __device__ inline void store(const lf4 (&y)[2], int o0) const {
-        const int o = o0 + 8 * q;
-        if (!live) return;
-        if (o + 8 <= c1) {
-            *reinterpret_cast<lf4u*>(dst + o) = y[0];
-            *reinterpret_cast<lf4u*>(dst + o + 4) = y[1];
-        } else {
+    __device__ inline void load_y(In& in, int o0) const {
+        const int o = o0 + 4 * p;
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                if (o + c < c1) dst[o + c] = y[c >> 2][c & 3];
-        }
-    }
-    // in: the first step's, loaded by the caller (ahead of the shrink); s: the lane's S, already scaled, zeros
-    // where a value does not count
-    template <bool WHOLE>
-    __device__ inline void run(In& in, int o0, const float (&s)[4 * NR], int rk) const {
-        uint32_t mask[4 * NR];                              // of single values (f32 products), or pairs
-        if constexpr (!WHOLE) {
+        for (int i = 0; i < 4; ++i) {
+            in.y[i] = lf4{0, 0, 0, 0};
+            if (!base[0]) continue;
+            const float* b = reinterpret_cast<const float*>(base[i]) + o;
+            if (o + 4 <= c1) {
+                in.y[i] = *reinterpret_cast<const lf4u*>(b);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4 * NR; ++j) {
-                if constexpr (kLoraPieces<W>)
-                    mask[j] = j % 2 ? 0 : (counts(j, rk) ? 0xFFFFu : 0u) | (counts(j + 1, rk) ? 0xFFFF0000u : 0u);
-                else
-                    mask[j] = counts(j, rk) ? 0xFFFFFFFFu : 0u;
-                asm volatile("" : "+v"(mask[j]));           // kept as a word, not as a condition
+                for (int c = 0; c < 4; ++c)
+                    if (o + c < c1) in.y[i][c] = b[c];
             }
         }
-        constexpr int NP = (NR + 1) / 2;                    // bf16 products of 32 ranks
-        LoraPieces P[kLoraPieces<W> ? NP : 1];
-        bool big = false, any_big = false;
-        if constexpr (kLoraPieces<W>) {
-            float most = 0.0f;
+    }
+    __device__ inline void store(const In& in, const lf4 (&d)[4], int o0, unsigned rows_in) const {
+        const int o = o0 + 4 * p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (!((rows_in >> (4 * q + i)) & 1u)) continue;
+            lf4 y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = in.y[i][j] + d[j][i];
+            float* b = reinterpret_cast<float*>(dst[i]) + o;
+            if (o + 4 <= c1) {
+                *reinterpret_cast<lf4u*>(b) = y;
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (o + c < c1) b[c] = y[c];
+            }
+        }
+    }
+    // rare: 64 columns of row t of the tile with plain products
+    __device__ inline void plain(const float (&s)[4 * NR], int rk, int o0, int t) const {
+        const int lane = (int)threadIdx.x & 63, o = o0 + lane;
+        float sum = 0.0f;
+        for (int r = 0; r < rk; ++r) {
+            float v = 0.0f;                                 // S's rank r, from the lane that counts it
+#pragma unroll
+            for (int j = 0; j < 4 * NR; ++j)
+                if (at[j / GW] + j % GW == r && counts(j, rk)) v = s[j];
+            const uint64_t who = __ballot(p == t && v != 0.0f);
+            v = who ? __shfl(v, __builtin_ctzll(who)) : 0.0f;
+            if (o < c1) sum = __builtin_fmaf(W::value(B[(uint32_t)o * (uint32_t)rank + r]), v, sum);
+        }
+        uint64_t to = 0, from = 0;                          // lane 16 (t / 4) holds the row's addresses
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i == (t & 3)) to = (uint64_t)(uintptr_t)dst[i], from = (uint64_t)(uintptr_t)base[i];
+        auto there = [&](uint64_t a) {
+            return (uintptr_t)((uint64_t)(uint32_t)__shfl((int)(uint32_t)a, 16 * (t >> 2)) |
+                               (uint64_t)(uint32_t)__shfl((int)(uint32_t)(a >> 32), 16 * (t >> 2)) << 32);
+        };
+        float* y = reinterpret_cast<float*>(there(to));
+        const float* b = reinterpret_cast<const float*>(there(from));
+        if (o < c1) y[o] = b ? b[o] + sum : sum;
+    }
+    // The wave's steps from o0 on.  s: the lane's S, already scaled, zeros where a value does not count; n: the
+    // tile's rows
+    __device__ inline void run(int o0, const float (&s)[4 * NR], int rk, int n) const {
+        unsigned rows_in = (1u << n) - 1u, alone = 0u;
+        if constexpr (kLoraPieces<W> > 0) {
+            const float most = lora_most(s, 0.0f);
+            if (__any(most == __builtin_inff())) alone = lora_big_rows(most) & rows_in;
+            rows_in &= ~alone;
+        }
+        constexpr int NP = (NR + 1) / 2, N = kLoraPieces<W>, M = N > 0 ? 2 : 1;   // products of 32 ranks, pieces, values of a mask
+        uint32_t mask[4 * NR / M];
+#pragma unroll
+        for (int j = 0; j < 4 * NR / M; ++j) {
+            if constexpr (M == 2) mask[j] = (counts(2 * j, rk) & 0xFFFFu) | (counts(2 * j + 1, rk) & 0xFFFF0000u);
+            else mask[j] = counts(j, rk);
+            asm volatile("" : "+v"(mask[j]));               // kept as a word
+        }
+        LoraWords P[NP][N > 0 ? N : 1];
+        float back[4] = {1.0f, 1.0f, 1.0f, 1.0f};           // of the lane's four rows
+        if constexpr (N > 0) {
+            float scale = 1.0f;
+            if constexpr (std::is_same<W, LoraF16>::value) {
+                float mine;
+                scale = lora_scale_of(lora_column_most(lora_most(s, 0.0f)), mine);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) back[i] = __shfl(mine, 4 * q + i);
+            }
 #pragma unroll
             for (int b = 0; b < NP; ++b) {
                 float v[8];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) v[c] = 8 * b + c < 4 * NR ? s[(8 * b + c) % (4 * NR)] : 0.0f;
-                most = lora_most(v, most);
-                P[b] = lora_split(v);
+                lora_split(W{}, v, scale, P[b]);
             }
-            any_big = __any(most == __builtin_inff());
-            if (any_big) big = lora_column_big(most);
         }
-        auto weight = [&](const V& v, int g, int c) {
-            const float w = W::get(v, c);
-            if constexpr (WHOLE) return w;
-            else if constexpr (kLoraPieces<W>)
-                return __uint_as_float(__float_as_uint(w) & (mask[(GW * g + c) & ~1] << (c & 1 ? 0 : 16)) & 0xFFFF0000u);
-            else return __uint_as_float(__float_as_uint(w) & mask[GW * g + c]);
-        };
-        auto f32_products = [&](const In& z, lf4 (&d)[2]) {
-#pragma unroll
-            for (int j = 0; j < 4 * NR; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    d[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(weight(z.w[h][j / GW], j / GW, j % GW), s[j], d[h], 0, 0, 0);
-        };
-        for (;;) {
-            const int next = o0 + 32 * NW;
-            In ahead;
-            if (next < c1) load(ahead, next);
-            lf4 d[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-            if constexpr (kLoraPieces<W>) {
+        for (; o0 < c1; o0 += 64 * NW) {
+            In in;
+            load(in, o0);
+            lf4 d[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+            if constexpr (N > 0) {
 #pragma unroll
                 for (int b = 0; b < NP; ++b)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        union {
-                            uint32_t u[4];
-                            lb8 v;
-                        } w;
+                    for (int h = 0; h < 4; ++h) {
+                        LoraWords w;
                         if constexpr (NR == 1) {
                             const uint2 r = __builtin_bit_cast(uint2, in.w[h][0]);
-                            w.u[0] = r.x, w.u[1] = r.y, w.u[2] = 0, w.u[3] = 0;
+                            w = LoraWords{{r.x, r.y, 0, 0}};
                         } else {
-                            w.v = __builtin_bit_cast(lb8, in.w[h][b]);
-                        }
-                        if constexpr (!WHOLE) {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if (8 * b + 2 * c < 4 * NR) w.u[c] &= mask[(8 * b + 2 * c) % (4 * NR)];
+                            w = __builtin_bit_cast(LoraWords, in.w[h][b]);
                         }
 #pragma unroll
-                        for (int g = 2; g >= 0; --g) d[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v, P[b].v[g], d[h], 0, 0, 0);
+                        for (int c = 0; c < 4; ++c)
+                            if (4 * b + c < 2 * NR) w.u[c] &= mask[(4 * b + c) % (4 * NR / M)];
+#pragma unroll
+                        for (int g = N - 1; g >= 0; --g) d[h] = lora_mfma(W{}, P[b][g], w, d[h]);
                     }
-                if (any_big) {
-                    lf4 again[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-                    f32_products(in, again);
+                if constexpr (std::is_same<W, LoraF16>::value) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < 4; ++h)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) d[h][i] = big ? again[h][i] : d[h][i];
+                        for (int i = 0; i < 4; ++i) d[h][i] *= back[i];
                 }
             } else {
-                f32_products(in, d);
+#pragma unroll
+                for (int j = 0; j < 4 * NR; ++j)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const float w = __uint_as_float(__float_as_uint(W::get(in.w[h][j / GW], j % GW)) & mask[j % (4 * NR / M)]);
+                        d[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[j], w, d[h], 0, 0, 0);
+                    }
             }
-            const lf4 y[2] = {in.y[0] + d[0], in.y[1] + d[1]};
-            store(y, o0);
-            if (next >= c1) return;
-            in = ahead;
-            o0 = next;
+            store(in, d, o0, rows_in);
+            if constexpr (N > 0) {
+                for (unsigned left = alone; left; left &= left - 1u) plain(s, rk, o0, __builtin_ctz(left));
+            }
         }
     }
 };
 
 // the lane's operand of S^T, of row lane % 16, times c; 0 where a value does not count
-template <typename W, int NR, int NW>
-__device__ inline void lora_sum_parts(const LoraExpand<W, NR, NW>& E, const float* part, int rk, float c, float (&s)[4 * NR]) {
-    constexpr int GW = LoraExpand<W, NR, NW>::GW;
+template <int NR, int NW, typename E_>
+__device__ inline void lora_sum_parts(const E_& E, const float* part, int rk, float c, float (&s)[4 * NR]) {
+    constexpr int GW = E_::GW;
 #pragma unroll
     for (int j = 0; j < 4 * NR; ++j) {
         const int r = E.at[j / GW] + j % GW;
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) v += part[((size_t)w * 16 * NR + r) * 16 + E.p];
-        s[j] = E.counts(j, rk) ? v * c : 0.0f;
+        for (int w = 0; w < NW; ++w) v += part[((size_t)w * 16 * NR + r) * kLoraPart + E.p];
+        s[j] = __uint_as_float(__float_as_uint(v * c) & E.counts(j, rk));
     }
 }
 
-// One tile and t.cols columns per workgroup.  grid (slots, column parts, windows).
-template <typename W, int NR, int NW, int U>
-__global__ __launch_bounds__(64 * NW) void k_lora_apply(LoraArgs a, LoraTiles t) {
-    __shared__ float part[NW * 16 * NR * 16];
-    __shared__ LoraFind<NW> find;
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    int key, n, row;
-    if (!lora_tile<NW>(a, t, find, key, n, row)) return;
-    const int c0 = (int)blockIdx.y * t.cols, c1 = min(a.rows, c0 + t.cols), o0 = c0 + 32 * wave;
+template <typename W>
+__device__ inline const typename W::T* lora_a(const LoraArgs& a, int key) {
+    return static_cast<const typename W::T*>(a.a) + (size_t)key * a.rank * a.k;
+}
+template <typename W>
+__device__ inline const typename W::T* lora_b(const LoraArgs& a, int key) {
+    return static_cast<const typename W::T*>(a.b) + (size_t)key * a.rows * a.rank;
+}
+
+// The shrink and the expand of a tile in one workgroup, for the calls at both ends (between them the two
+// kernels below).  Small ones, in one launch: a workgroup finds its tile by itself (FIND)
+// and shrinks it whole, also when several share its columns; up to U steps of loads at a time, which it
+// waits for.  Large ones, with tiles to fill the chip, take them from the lists, and hold OCC
+// waves per SIMD to cover the loads: 96 us where the two kernels take 108 (16,384 rows, rank 32,
+// 2048 x 2048).  grid (slots, column parts, windows).
+template <typename W, int NR, int NW, int U, int OCC, bool FIND>
+__global__ __launch_bounds__(64 * NW, OCC) void k_lora_apply(LoraArgs a, LoraTiles t) {
+    __shared__ float part[NW * 16 * NR * kLoraPart];
+    __shared__ lf4 turn[NW * (kLoraXLds + kLoraALds<W>)];
+    __shared__ typename std::conditional<FIND, LoraFind<NW>, int>::type find;
+    int key, n, row, pos;
+    if constexpr (FIND) {
+        if (!lora_tile<NW>(a, t, find, key, n, row)) return;
+    } else {
+        if (!lora_item(t, key, n, row, pos)) return;
+    }
+    const int c0 = (int)blockIdx.y * t.cols, c1 = min(a.rows, c0 + t.cols), o0 = c0 + 64 * ((int)threadIdx.x >> 6);
     if (key < 0) {
         lora_plain_rows(a, key, n, row, c0, c1);
         return;
     }
     const int rk = lora_rank(a, key);
     const float c = lora_scale(a, key);
-    typedef LoraExpand<W, NR, NW> Expand;
-    const Expand E(static_cast<const typename W::T*>(a.b) + (size_t)key * a.rows * a.rank, a.rank, a.rows,
-                   a.base ? reinterpret_cast<const float*>(a.base + lora_at(row, a.n_ids, a.base_id, a.base_tok)) : nullptr,
-                   reinterpret_cast<float*>(a.dst + lora_at(row, a.n_ids, a.dst_id, a.dst_tok)), (lane & 15) < n, c1);
-    typename Expand::In in;
-    if (o0 < c1) E.load(in, o0);
-    LoraShrink<W, NR, NW, U>(static_cast<const typename W::T*>(a.a) + (size_t)key * a.rank * a.k, lora_x(a, row), a.k, a.rank)
-        .run(part);
+    LoraShrink<W, NR, NW, U>(a, lora_a<W>(a, key), row, turn, 0, 1 << 28).run(part);
     __syncthreads();
     if (o0 >= c1) return;
+    const LoraExpand<W, NR, NW> E(a, lora_b<W>(a, key), row, c1);
     float s[4 * NR];
-    lora_sum_parts(E, part, rk, c, s);
-    if (rk == 16 * NR) E.template run<true>(in, o0, s, rk);
-    else E.template run<false>(in, o0, s, rk);
+    lora_sum_parts<NR, NW>(E, part, rk, c, s);
+    E.run(o0, s, rk, n);
+}
+
+// Larger calls: S = X A^T of a tile and one part of k per workgroup, to t.s, [k parts][position in order][16 NR]
+// in all, a tile of n rows as the expand reads it: [4 NR groups of four values][n rows][4] of every lane's values in
+// lora_value_at's order (zeros where one does not count), so that its loads are whole lines.  grid (slots, k parts, windows).
+template <typename W, int NR, int U, int OCC>
+__global__ __launch_bounds__(256, OCC) void k_lora_shrink(LoraArgs a, LoraTiles t) {
+    constexpr int NW = 4;
+    __shared__ float part[NW * 16 * NR * kLoraPart];
+    __shared__ lf4 turn[NW * (kLoraXLds + kLoraALds<W>)];
+    int key, n, row, pos;
+    if (!lora_item(t, key, n, row, pos) || key < 0) return;
+    const int s0 = (int)blockIdx.y * t.k_steps;
+    LoraShrink<W, NR, NW, U>(a, lora_a<W>(a, key), row, turn, s0, s0 + t.k_steps).run(part);
+    __syncthreads();
+    float* out = t.s + ((size_t)blockIdx.y * t.positions + pos) * (16 * NR);
+    const int rk = lora_rank(a, key);
+    for (int i = (int)threadIdx.x; i < 16 * 16 * NR; i += 256) {
+        const int j = i / 16, p = i % 16, r = lora_value_at<NR>(j, a.rank);     // value j of the 16 NR, row p
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) v += part[(w * 16 * NR + r) * kLoraPart + p];
+        if (p < n) out[((j >> 2) * n + p) * 4 + (j & 3)] = lora_value_counts<NR>(j, a.rank, rk) ? v : 0.0f;
+    }
+}
+
+// y = base + c S B^T of a tile and t.cols columns.  grid (slots, column parts, windows).
+template <typename W, int NR, int OCC>
+__global__ __launch_bounds__(256, OCC) void k_lora_expand(LoraArgs a, LoraTiles t) {
+    constexpr int NW = 4;
+    int key, n, row, pos;
+    if (!lora_item(t, key, n, row, pos)) return;
+    const int c0 = (int)blockIdx.y * t.cols, c1 = min(a.rows, c0 + t.cols), o0 = c0 + 64 * ((int)threadIdx.x >> 6);
+    if (key < 0) {
+        lora_plain_rows(a, key, n, row, c0, c1);
+        return;
+    }
+    if (o0 >= c1) return;
+    const int rk = lora_rank(a, key);
+    const float c = lora_scale(a, key);
+    typedef LoraExpand<W, NR, NW> Expand;
+    const Expand E(a, lora_b<W>(a, key), row, c1);
+    const float* in = t.s + (size_t)pos * (16 * NR) + (NR * E.q * n + min(E.p, n - 1)) * 4;
+    lf4 v[NR];
+#pragma unroll
+    for (int j = 0; j < NR; ++j) v[j] = lf4{0, 0, 0, 0};
+    for (int z = 0; z < t.k_parts; z += 4) {                // the parts in order, the loads of four at a time
+        lf4 l[4][NR];
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+            for (int j = 0; j < NR; ++j)
+                l[y][j] = *reinterpret_cast<const lf4*>(in + (size_t)min(z + y, t.k_parts - 1) * t.positions * (16 * NR) + j * n * 4);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+            if (z + y < t.k_parts) {
+#pragma unroll
+                for (int j = 0; j < NR; ++j) v[j] += l[y][j];
+            }
+    }
+    float s[4 * NR];
+#pragma unroll
+    for (int j = 0; j < 4 * NR; ++j) s[j] = v[j / 4][j % 4] * c;
+    E.run(o0, s, rk, n);
 }
 
 // one workgroup per row: s, u and dx
