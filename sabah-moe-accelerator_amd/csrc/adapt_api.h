@@ -215,6 +215,14 @@ static bool stride_ok(size_t s) { return s % 4 == 0; }
 constexpr int kLoraDirectRows = 256;
 constexpr int kLoraFusedTiles = 256;          // from here on a tile's shrink and expand in one workgroup
 constexpr int kLoraShrinkGroups = 1024, kLoraShrinkParts = 8, kLoraShrinkSteps = 8;
+// k of a shrink in parts while there are few tiles
+static void lora_k_parts(int k, int tiles, int& parts, int& steps) {
+    const int all = (k + 31) / 32;
+    parts = std::max(1, std::min({kLoraShrinkParts, kLoraShrinkGroups / tiles, all / kLoraShrinkSteps}));
+    steps = (all + parts - 1) / parts;
+    parts = (all + steps - 1) / steps;
+}
+
 struct LoraSpace {
     size_t order, items, n_items, s, bytes;
     int windows, slots, key_bits, k_parts, k_steps, rank16;
@@ -231,10 +239,8 @@ static LoraSpace lora_space(const sabah_lora_desc* L, int n_rows) {
         s.windows = 1;
         return s;
     }
-    const int steps = (L->k + 31) / 32, tiles = (n_rows + kLoraTile - 1) / kLoraTile;
-    const int parts = std::max(1, std::min({kLoraShrinkParts, kLoraShrinkGroups / tiles, steps / kLoraShrinkSteps}));
-    s.k_steps = (steps + parts - 1) / parts;
-    s.k_parts = (steps + s.k_steps - 1) / s.k_steps;
+    const int tiles = (n_rows + kLoraTile - 1) / kLoraTile;
+    lora_k_parts(L->k, tiles, s.k_parts, s.k_steps);
     const size_t positions = tiles < kLoraFusedTiles ? (size_t)s.windows * kLoraWindow : 0;
     s.items = align256((size_t)s.windows * kLoraWindow * 4);
     s.n_items = s.items + align256((size_t)s.windows * s.slots * 16);
@@ -244,9 +250,62 @@ static LoraSpace lora_space(const sabah_lora_desc* L, int n_rows) {
     return s;
 }
 
+// A backward call's: the tiles and runs, the parts of s and u, the transposed pairs, the pieces and offsets that
+// the weights' gradients read, and their partial sums.
+struct LoraBackSpace {
+    size_t order, items, n_items, runs, s, u, at, bt, ps, pu, ox, oy, part, bytes;
+    int windows, slots, key_bits, rank16, positions, s_parts, s_steps, u_parts, u_steps, tiles_a, tiles_b, splits;
+};
+constexpr int kLoraBackKeys = 1 << 15;        // a word per key and window
+constexpr int kLoraGradGroups = 1024;         // workgroups of the weights' gradients to aim at
+static LoraBackSpace lora_back_space(const sabah_lora_desc* L, int n_rows) {
+    LoraBackSpace s{};
+    const int keys = L->n_adapters * L->n_experts, span = std::min(n_rows, kLoraWindow);
+    s.windows = std::max(1, (n_rows + kLoraWindow - 1) / kLoraWindow);
+    s.slots = std::max(1, std::min(span, span / kLoraTile + std::min(keys + 2, span)));
+    s.rank16 = L->rank <= 16 ? 16 : L->rank <= 32 ? 32 : L->rank <= 64 ? 64 : 128;
+    while ((keys + 2) >> s.key_bits) ++s.key_bits;
+    s.positions = s.windows * kLoraWindow;
+    const int tiles = std::max(1, (n_rows + kLoraTile - 1) / kLoraTile);
+    lora_k_parts(L->k, 2 * tiles, s.s_parts, s.s_steps);
+    lora_k_parts(L->rows, 2 * tiles, s.u_parts, s.u_steps);
+    s.tiles_a = (L->k + 63) / 64;
+    s.tiles_b = (L->rows + 63) / 64;
+    s.splits = std::max(1, std::min({s.windows, 32, (int)(kLoraGradGroups / ((long long)keys * (s.tiles_a + s.tiles_b)))}));
+    const size_t esize = L->type == kTypeF32 ? 4 : 2, all = (size_t)s.windows * s.slots;
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at += align256(n);
+        return here;
+    };
+    s.order = take((size_t)s.positions * 4);
+    s.items = take(all * 16);
+    s.n_items = take((size_t)s.windows * 4);
+    s.runs = take((size_t)s.windows * keys * 4);
+    s.s = take((size_t)s.s_parts * s.positions * s.rank16 * 4);
+    s.u = take((size_t)s.u_parts * s.positions * s.rank16 * 4);
+    s.at = take((size_t)keys * L->rank * L->k * esize);
+    s.bt = take((size_t)keys * L->rank * L->rows * esize);
+    s.ps = take(all * 3 * s.rank16 * 32);
+    s.pu = take(all * 3 * s.rank16 * 32);
+    s.ox = take(all * 16 * 8);
+    s.oy = take(all * 16 * 8);
+    s.part = take(s.splits > 1 ? (size_t)s.splits * keys * (s.tiles_a + s.tiles_b) * s.rank16 * 64 * 4 : 0);
+    s.bytes = at;
+    return s;
+}
+
+static int check_lora_keys(const sabah_lora_desc* L) {
+    if ((long long)L->n_adapters * L->n_experts > kLoraBackKeys)
+        return fail("adapters backward: %d adapters of %d experts are more than %d pairs", L->n_adapters, L->n_experts,
+                    kLoraBackKeys);
+    return 0;
+}
+
 SABAH_API size_t sabah_lora_workspace(const sabah_lora_desc* lora, int n_ids, int n_tokens, int backward) {
-    if (check_lora("adapters", lora, n_ids, n_tokens)) return 0;
-    return backward ? align256((size_t)n_ids * n_tokens * lora->rank * 8) : lora_space(lora, n_ids * n_tokens).bytes;
+    if (check_lora("adapters", lora, n_ids, n_tokens) || (backward && check_lora_keys(lora))) return 0;
+    return backward ? lora_back_space(lora, n_ids * n_tokens).bytes : lora_space(lora, n_ids * n_tokens).bytes;
 }
 
 static LoraArgs lora_args(const sabah_lora_desc* L, const float* d_x, size_t x_id_stride, int x_rows,
@@ -300,7 +359,7 @@ static void launch_lora_apply_rank(const LoraArgs& a, const LoraTiles& t, int co
         return;
     }
     hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC>), dim3((unsigned)t.slots, (unsigned)t.k_parts, (unsigned)windows),
-                       dim3(256), 0, st, a, t);
+                       dim3(256), 0, st, a, t, a, t, windows);
     hipLaunchKernelGGL((k_lora_expand<W, NR, std::min(OCC, 3)>), grid, dim3(256), 0, st, a, t);
 }
 template <typename W>
@@ -353,7 +412,7 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
     if (sp.bytes) {
         uint8_t* ws = static_cast<uint8_t*>(d_workspace);
         const LoraGroup g{reinterpret_cast<int*>(ws + sp.order), reinterpret_cast<int4*>(ws + sp.items),
-                          reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, t.skip_none, sp.key_bits};
+                          reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, t.skip_none, sp.key_bits, nullptr};
         hipLaunchKernelGGL(k_lora_group, dim3((unsigned)sp.windows),
                            dim3((unsigned)std::min(kLoraWindow, (n_rows + 63) / 64 * 64)), 0, st, a, g);
         if (!ck(hipGetLastError(), "adapters grouping launch")) return -1;
@@ -378,6 +437,52 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
     return ck(hipGetLastError(), "adapters launch") ? 0 : -1;
 }
 
+struct LoraBack {
+    LoraBackSpace sp;
+    LoraArgs a, u, x;             // s = A x; u = c B^T dy; dx = A^T u
+    LoraGroup g;
+    LoraTiles ts, tu;
+    LoraTurn turn;
+    LoraJoin join;
+    LoraGrad w;
+    int grad_tiles;
+    hipStream_t st;
+};
+
+template <typename W, int NR, int U, int OCC, int GOCC>
+static int launch_lora_back_rank(const LoraBack& b) {
+    const LoraBackSpace& sp = b.sp;
+    const unsigned slots = (unsigned)sp.slots, windows = (unsigned)sp.windows, keys = (unsigned)b.w.keys;
+    hipLaunchKernelGGL(k_lora_group, dim3(windows), dim3((unsigned)std::max(64, std::min(kLoraWindow, (b.g.n_rows + 63) / 64 * 64))),
+                       0, b.st, b.a, b.g);
+    if (b.g.n_rows && (b.x.dst || b.grad_tiles)) {
+        hipLaunchKernelGGL(k_lora_transpose<typename W::T>, dim3((unsigned)(sp.tiles_a + sp.tiles_b), keys), dim3(256), 0, b.st, b.turn);
+        const bool s = b.grad_tiles > b.w.tiles_a;          // s is dB's alone
+        hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC>), dim3(slots, (unsigned)std::max(sp.s_parts, sp.u_parts), windows * (s ? 2u : 1u)),
+                           dim3(256), 0, b.st, b.u, b.tu, b.a, b.ts, (int)windows);
+    }
+    if (b.g.n_rows && b.x.dst) {
+        LoraTiles t = b.tu;
+        t.cols = 256;
+        hipLaunchKernelGGL((k_lora_expand<W, NR, std::min(OCC, 3)>), dim3(slots, (unsigned)((b.x.rows + 255) / 256), windows), dim3(256), 0,
+                           b.st, b.x, t);
+    }
+    if (b.grad_tiles) {
+        if (b.g.n_rows) hipLaunchKernelGGL(k_lora_join<NR>, dim3(slots, windows), dim3(256), 0, b.st, b.a, b.join);
+        hipLaunchKernelGGL((k_lora_grad<NR, GOCC>), dim3((unsigned)b.grad_tiles, keys, (unsigned)b.w.splits), dim3(256), 0, b.st, b.w);
+        if (b.w.splits > 1)
+            hipLaunchKernelGGL(k_lora_grad_sum<NR>, dim3((unsigned)b.grad_tiles, keys), dim3(256), 0, b.st, b.w);
+    }
+    return ck(hipGetLastError(), "adapters backward launch") ? 0 : -1;
+}
+template <typename W>
+static int launch_lora_back(const LoraBack& b) {
+    if (b.a.rank <= 16) return launch_lora_back_rank<W, 1, 2, 4, 3>(b);
+    if (b.a.rank <= 32) return launch_lora_back_rank<W, 2, 2, 4, 3>(b);
+    if (b.a.rank <= 64) return launch_lora_back_rank<W, 4, 1, 2, 2>(b);
+    return launch_lora_back_rank<W, 8, 1, 1, 1>(b);
+}
+
 SABAH_API int sabah_lora_backward(const sabah_lora_desc* lora, const float* d_x, size_t x_id_stride, int x_rows,
                                   size_t x_token_stride, const int32_t* d_adapters, const int32_t* d_ids,
                                   size_t ids_id_stride, size_t ids_token_stride, int n_ids, int n_tokens,
@@ -390,9 +495,11 @@ SABAH_API int sabah_lora_backward(const sabah_lora_desc* lora, const float* d_x,
     if (n_tokens && !d_dy) return fail("adapters backward: null pointer");
     if (!stride_ok(dy_id_stride) || !stride_ok(dy_token_stride) || !stride_ok(dx_id_stride) || !stride_ok(dx_token_stride))
         return fail("adapters backward: strides are in bytes and multiples of 4");
-    const size_t need = sabah_lora_workspace(lora, n_ids, n_tokens, 1);
-    if (need && (!d_workspace || workspace_bytes < need || (uintptr_t)d_workspace % 16))
-        return fail("adapters backward: the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", need,
+    if (check_lora_keys(lora)) return -1;
+    const int n_rows = n_ids * n_tokens, keys = lora->n_adapters * lora->n_experts;
+    const LoraBackSpace sp = lora_back_space(lora, n_rows);
+    if (!d_workspace || workspace_bytes < sp.bytes || (uintptr_t)d_workspace % 16)
+        return fail("adapters backward: the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", sp.bytes,
                     workspace_bytes);
     if (g_device < 0) return fail("sabah_rt_init has not been called");
     if (!check_sticky()) return -1;
@@ -403,23 +510,78 @@ SABAH_API int sabah_lora_backward(const sabah_lora_desc* lora, const float* d_x,
     a.dy = reinterpret_cast<const uint8_t*>(d_dy);
     a.dy_id = dy_id_stride;
     a.dy_tok = dy_token_stride;
-    a.dx = reinterpret_cast<uint8_t*>(d_dx);
-    a.dx_id = dx_id_stride;
-    a.dx_tok = dx_token_stride;
-    a.da = d_da;
-    a.db = d_db;
-    a.add_dx = add_dx != 0;
-    a.add_dw = add_dw != 0;
-    a.su = static_cast<float*>(d_workspace);
-    hipStream_t st = pick_stream(stream);
-    const dim3 grid((unsigned)(n_ids * n_tokens)), block(kLoraThreads);
-    if (n_tokens) switch (lora->type) {
-        case kTypeF32: hipLaunchKernelGGL(k_lora_back_rows<LoraF32>, grid, block, 0, st, a); break;
-        case kTypeF16: hipLaunchKernelGGL(k_lora_back_rows<LoraF16>, grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL(k_lora_back_rows<LoraBF16>, grid, block, 0, st, a); break;
-        }
-    if (d_da || d_db)
-        hipLaunchKernelGGL(k_lora_back_weights, dim3((unsigned)(lora->n_adapters * lora->n_experts), (unsigned)lora->rank),
-                           block, 0, st, a);
-    return ck(hipGetLastError(), "adapters backward launch") ? 0 : -1;
+    uint8_t* ws = static_cast<uint8_t*>(d_workspace);
+    LoraBack b{};
+    b.sp = sp;
+    b.st = pick_stream(stream);
+    b.a = a;
+    b.u = a;                                                // u: dy shrunk by B^T
+    b.u.x = a.dy;
+    b.u.x_id = dy_id_stride;
+    b.u.x_tok = dy_token_stride;
+    b.u.x_rows = n_ids;
+    b.u.k = lora->rows;
+    b.u.a = ws + sp.bt;
+    b.x = a;                                                // dx: u expanded by A^T
+    b.x.b = ws + sp.at;
+    b.x.rows = lora->k;
+    b.x.dst = reinterpret_cast<uint8_t*>(d_dx);
+    b.x.dst_id = dx_id_stride;
+    b.x.dst_tok = dx_token_stride;
+    b.x.base = add_dx ? b.x.dst : nullptr;
+    b.x.base_id = dx_id_stride;
+    b.x.base_tok = dx_token_stride;
+    const LoraGroup g{reinterpret_cast<int*>(ws + sp.order), reinterpret_cast<int4*>(ws + sp.items),
+                      reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, !d_dx || add_dx, sp.key_bits,
+                      reinterpret_cast<uint32_t*>(ws + sp.runs)};
+    b.g = g;
+    LoraTiles t{};
+    t.order = g.order;
+    t.items = g.items;
+    t.n_items = g.n_items;
+    t.n_rows = n_rows;
+    t.slots = sp.slots;
+    t.skip_none = g.skip_none;
+    t.key_bits = sp.key_bits;
+    t.positions = sp.positions;
+    b.ts = b.tu = t;
+    b.ts.s = reinterpret_cast<float*>(ws + sp.s);
+    b.ts.k_parts = sp.s_parts;
+    b.ts.k_steps = sp.s_steps;
+    b.tu.s = reinterpret_cast<float*>(ws + sp.u);
+    b.tu.k_parts = sp.u_parts;
+    b.tu.k_steps = sp.u_steps;
+    b.turn = LoraTurn{lora->a, lora->b, ws + sp.at, ws + sp.bt, g.runs, sp.windows, keys, lora->rank, lora->k, lora->rows,
+                      sp.tiles_a};
+    b.join = LoraJoin{b.ts, b.tu, reinterpret_cast<uint16_t*>(ws + sp.ps), reinterpret_cast<uint16_t*>(ws + sp.pu),
+                      reinterpret_cast<uint64_t*>(ws + sp.ox), reinterpret_cast<uint64_t*>(ws + sp.oy)};
+    LoraGrad& w = b.w;
+    w.runs = g.runs;
+    w.windows = sp.windows;
+    w.keys = keys;
+    w.slots = sp.slots;
+    w.splits = sp.splits;
+    w.rank = lora->rank;
+    w.tiles_a = d_da ? sp.tiles_a : 0;
+    w.p[0] = b.join.pu;
+    w.p[1] = b.join.ps;
+    w.off[0] = b.join.ox;
+    w.off[1] = b.join.oy;
+    w.src[0] = a.x;
+    w.src[1] = a.dy;
+    w.width[0] = lora->k;
+    w.width[1] = lora->rows;
+    w.out[0] = d_da;
+    w.out[1] = d_db;
+    w.part[0] = reinterpret_cast<float*>(ws + sp.part);
+    w.part[1] = w.part[0] + (size_t)sp.splits * keys * sp.tiles_a * sp.rank16 * 64;
+    w.scale = lora->scale;
+    w.n_experts = lora->n_experts;
+    w.add = add_dw != 0;
+    b.grad_tiles = w.tiles_a + (d_db ? sp.tiles_b : 0);
+    switch (lora->type) {
+    case kTypeF32: return launch_lora_back<LoraF32>(b);
+    case kTypeF16: return launch_lora_back<LoraF16>(b);
+    default: return launch_lora_back<LoraBF16>(b);
+    }
 }

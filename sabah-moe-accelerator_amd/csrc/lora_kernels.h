@@ -37,11 +37,6 @@ struct LoraArgs {
     // backward
     const uint8_t* dy;
     size_t dy_id, dy_tok;
-    uint8_t* dx;                  // or null
-    size_t dx_id, dx_tok;
-    float *da, *db;               // or null
-    int add_dx, add_dw;
-    float* su;                    // [rows of the call][2 rank]: s, u
     unsigned int* err;
 };
 
@@ -108,20 +103,6 @@ __device__ inline const float* lora_x(const LoraArgs& a, int row) {
     return reinterpret_cast<const float*>(a.x + (size_t)t * a.x_tok + (size_t)(i % a.x_rows) * a.x_id);
 }
 
-// s[r] = A[r] . x for r below rk, one wave per r at a time
-template <typename W>
-__device__ inline void lora_shrink(const typename W::T* A, const float* x, int k, int rk, float* s) {
-    const int v = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, nw = (int)blockDim.x >> 6;
-    for (int r = wave; r < rk; r += nw) {
-        float acc = 0.0f;
-        for (int i = v; i < k; i += 64) acc = __builtin_fmaf(W::value(A[(size_t)r * k + i]), x[i], acc);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) acc += __shfl_xor(acc, o);
-        if (v == 0) s[r] = acc;
-    }
-    __syncthreads();
-}
-
 // ---------------------------------------------------------------------------
 // Tiles: up to 16 rows of one key.  In small calls each workgroup finds its tile by itself
 // (lora_tile, a thread for every row of the call); above, k_lora_group sorts each window of 1,024
@@ -146,6 +127,7 @@ struct LoraGroup {
     int4* items;
     int* n_items;
     int n_rows, slots, skip_none, key_bits;
+    uint32_t* runs;               // or [windows][keys]: a key's rows in the window << 16 | its first tile's slot, 0 without any
 };
 
 // A row's word, (key + 2, row of the window); past the rows one above every key
@@ -208,7 +190,7 @@ __device__ inline uint32_t lora_sort(uint32_t c, int bits, LoraSort<NW>& f) {
 // In sorted order: every 16th row of a run of equal keys begins a tile.  The thread's tile, if it begins one
 // (its number of rows, else 0), and the tiles before it.
 template <int NW>
-__device__ inline int lora_leader(uint32_t c, LoraSort<NW>& f, int n_keys2, bool skip_none, int& slot) {
+__device__ inline int lora_leader(uint32_t c, LoraSort<NW>& f, int n_keys2, bool skip_none, int& slot, int* run = nullptr) {
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), nt = (int)blockDim.x;
     const uint32_t k2 = c >> 10;
     const uint64_t head = __ballot(tid == 0 || (f.c[max(tid - 1, 0)] >> 10) != k2);   // rows that begin a run
@@ -234,6 +216,15 @@ __device__ inline int lora_leader(uint32_t c, LoraSort<NW>& f, int n_keys2, bool
     __syncthreads();
     const uint32_t before = lora_row_scan(f.w[lane & 15].x);
     slot = __builtin_amdgcn_readlane((int)before, wave) - __popcll(m) + __popcll(m & ((1ull << lane) - 1ull));
+    if (run) {                                              // of the threads that begin one, the whole run's rows
+        int stop = after || next ? end : nt;
+        for (int v = wave + 2; v < NW && !after && !next; ++v)
+            if (f.m[v]) {
+                stop = 64 * v + __builtin_ctzll(f.m[v]);
+                break;
+            }
+        *run = leader && tid == start ? stop - tid : 0;
+    }
     return leader ? min(kLoraTile, end - tid) : 0;          // a head two waves on is more than 16 rows away
 }
 
@@ -242,8 +233,12 @@ __global__ __launch_bounds__(kLoraWindow) void k_lora_group(LoraArgs a, LoraGrou
     __shared__ LoraSort<kLoraWindow / 64> f;
     const int tid = (int)threadIdx.x, w = (int)blockIdx.x, n_keys2 = a.n_adapters * a.n_experts + 2;
     const uint32_t c = lora_sort(lora_word(a, w * kLoraWindow + tid, g.n_rows, tid), g.key_bits, f);
-    int slot;
-    const int n = lora_leader(c, f, n_keys2, g.skip_none, slot);
+    if (g.runs)
+        for (int i = tid; i < n_keys2 - 2; i += (int)blockDim.x) g.runs[(size_t)w * (n_keys2 - 2) + i] = 0u;
+    int slot, run;
+    const int n = lora_leader(c, f, n_keys2, g.skip_none, slot, &run);     // its barriers order the zeros before the runs
+    if (g.runs && run && (int)(c >> 10) >= 2)
+        g.runs[(size_t)w * (n_keys2 - 2) + (c >> 10) - 2] = (uint32_t)run << 16 | (uint32_t)slot;
     if (n) g.items[(size_t)w * g.slots + slot] = make_int4((int)(c >> 10) - 2, w * kLoraWindow + tid, n, 0);
     if (tid == (int)blockDim.x - 1) g.n_items[w] = slot + (n ? 1 : 0);
     if ((int)(c >> 10) < n_keys2) g.order[w * kLoraWindow + tid] = w * kLoraWindow + (int)(c & 1023u);
@@ -305,8 +300,7 @@ __device__ inline bool lora_tile(const LoraArgs& a, const LoraTiles& t, LoraFind
 }
 
 // The same from the lists of k_lora_group, with the tile's position in order
-__device__ inline bool lora_item(const LoraTiles& t, int& key, int& n, int& row, int& pos) {
-    const int w = (int)blockIdx.z;
+__device__ inline bool lora_item(const LoraTiles& t, int w, int& key, int& n, int& row, int& pos) {
     if ((int)blockIdx.x >= t.n_items[w]) return false;
     const int4 it = t.items[(size_t)w * t.slots + blockIdx.x];
     key = __builtin_amdgcn_readfirstlane(it.x);
@@ -846,7 +840,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void k_lora_apply(LoraArgs a, LoraTil
     if constexpr (FIND) {
         if (!lora_tile<NW>(a, t, find, key, n, row)) return;
     } else {
-        if (!lora_item(t, key, n, row, pos)) return;
+        if (!lora_item(t, (int)blockIdx.z, key, n, row, pos)) return;
     }
     const int c0 = (int)blockIdx.y * t.cols, c1 = min(a.rows, c0 + t.cols), o0 = c0 + 64 * ((int)threadIdx.x >> 6);
     if (key < 0) {
@@ -867,13 +861,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void k_lora_apply(LoraArgs a, LoraTil
 // Larger calls: S = X A^T of a tile and one part of k per workgroup, to t.s, [k parts][position in order][16 NR]
 // in all, a tile of n rows as the expand reads it: [4 NR groups of four values][n rows][4] of every lane's values in
 // lora_value_at's order (zeros where one does not count), so that its loads are whole lines.  grid (slots, k parts, windows).
-template <typename W, int NR, int U, int OCC>
-__global__ __launch_bounds__(256, OCC) void k_lora_shrink(LoraArgs a, LoraTiles t) {
+template <typename W, int NR, int U>
+__device__ inline void lora_shrink_part(const LoraArgs& a, const LoraTiles& t, int w, float* part, lf4* turn) {
     constexpr int NW = 4;
-    __shared__ float part[NW * 16 * NR * kLoraPart];
-    __shared__ lf4 turn[NW * (kLoraXLds + kLoraALds<W>)];
     int key, n, row, pos;
-    if (!lora_item(t, key, n, row, pos) || key < 0) return;
+    if ((int)blockIdx.y >= t.k_parts || !lora_item(t, w, key, n, row, pos) || key < 0) return;
     const int s0 = (int)blockIdx.y * t.k_steps;
     LoraShrink<W, NR, NW, U>(a, lora_a<W>(a, key), row, turn, s0, s0 + t.k_steps).run(part);
     __syncthreads();
@@ -883,9 +875,18 @@ __global__ __launch_bounds__(256, OCC) void k_lora_shrink(LoraArgs a, LoraTiles 
         const int j = i / 16, p = i % 16, r = lora_value_at<NR>(j, a.rank);     // value j of the 16 NR, row p
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) v += part[(w * 16 * NR + r) * kLoraPart + p];
+        for (int w4 = 0; w4 < NW; ++w4) v += part[(w4 * 16 * NR + r) * kLoraPart + p];
         if (p < n) out[((j >> 2) * n + p) * 4 + (j & 3)] = lora_value_counts<NR>(j, a.rank, rk) ? v : 0.0f;
     }
+}
+// Both sides' in one launch, the windows of the second after the first's (forward: windows of b none)
+template <typename W, int NR, int U, int OCC>
+__global__ __launch_bounds__(256, OCC) void k_lora_shrink(LoraArgs a, LoraTiles t, LoraArgs b, LoraTiles u, int windows) {
+    __shared__ float part[4 * 16 * NR * kLoraPart];
+    __shared__ lf4 turn[4 * (kLoraXLds + kLoraALds<W>)];
+    const int w = (int)blockIdx.z;
+    if (w < windows) lora_shrink_part<W, NR, U>(a, t, w, part, turn);
+    else lora_shrink_part<W, NR, U>(b, u, w - windows, part, turn);
 }
 
 // y = base + c S B^T of a tile and t.cols columns.  grid (slots, column parts, windows).
@@ -893,7 +894,7 @@ template <typename W, int NR, int OCC>
 __global__ __launch_bounds__(256, OCC) void k_lora_expand(LoraArgs a, LoraTiles t) {
     constexpr int NW = 4;
     int key, n, row, pos;
-    if (!lora_item(t, key, n, row, pos)) return;
+    if (!lora_item(t, (int)blockIdx.z, key, n, row, pos)) return;
     const int c0 = (int)blockIdx.y * t.cols, c1 = min(a.rows, c0 + t.cols), o0 = c0 + 64 * ((int)threadIdx.x >> 6);
     if (key < 0) {
         lora_plain_rows(a, key, n, row, c0, c1);
@@ -928,68 +929,249 @@ __global__ __launch_bounds__(256, OCC) void k_lora_expand(LoraArgs a, LoraTiles 
     E.run(o0, s, rk, n);
 }
 
-// one workgroup per row: s, u and dx
-template <typename W>
-__global__ __launch_bounds__(kLoraThreads) void k_lora_back_rows(LoraArgs a) {
-    __shared__ float s[kLoraMaxRank];
-    __shared__ float u[kLoraMaxRank];
-    const int row = (int)blockIdx.x, key = lora_key(a, row), tid = (int)threadIdx.x;
-    float* dx = a.dx ? reinterpret_cast<float*>(a.dx + lora_at(row, a.n_ids, a.dx_id, a.dx_tok)) : nullptr;
-    if (key < 0) {
-        if (key == kLoraBad && tid == 0) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrLora;
-        if (dx && (key == kLoraBad || !a.add_dx))
-            for (int i = tid; i < a.k; i += kLoraThreads) dx[i] = key == kLoraBad ? __builtin_nanf("") : 0.0f;
-        return;
-    }
-    const int rk = lora_rank(a, key), v = tid & 63, wave = tid >> 6;
-    const float c = lora_scale(a, key);
-    const float* dy = reinterpret_cast<const float*>(a.dy + lora_at(row, a.n_ids, a.dy_id, a.dy_tok));
-    const typename W::T* A = static_cast<const typename W::T*>(a.a) + (size_t)key * a.rank * a.k;
-    const typename W::T* B = static_cast<const typename W::T*>(a.b) + (size_t)key * a.rows * a.rank;
-    lora_shrink<W>(A, lora_x(a, row), a.k, rk, s);
-    for (int r = wave; r < rk; r += kLoraThreads / 64) {
-        float acc = 0.0f;
-        for (int o = v; o < a.rows; o += 64) acc = __builtin_fmaf(W::value(B[(size_t)o * a.rank + r]), dy[o], acc);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) acc += __shfl_xor(acc, o);
-        if (v == 0) u[r] = c * acc;
+// ---------------------------------------------------------------------------
+// Backward.  s = A x and u = c B^T dy of every row are shrinks (of x by A, of dy by B^T) and dx = A^T u is an
+// expand, on transposed copies of the pairs in use; dA = sum u x^T and dB = c sum dy s^T are sums over a key's rows.
+// ---------------------------------------------------------------------------
+
+// whether any window has rows of the key; the whole workgroup asks
+__device__ inline bool lora_key_used(const uint32_t* runs, int windows, int keys, int key) {
+    uint32_t any = 0;
+    for (int w = (int)threadIdx.x; w < windows; w += (int)blockDim.x) any |= runs[(size_t)w * keys + key];
+    return __syncthreads_or(any != 0u);
+}
+
+struct LoraTurn {
+    const void *a, *b;            // [keys][rank][k], [keys][rows][rank]
+    void *at, *bt;                // [keys][k][rank], [keys][rank][rows]
+    const uint32_t* runs;
+    int windows, keys, rank, k, rows, tiles_a;
+};
+// 64 columns of A, or rows of B, per workgroup, through LDS: both sides are read and written along their rows.
+// grid (64s of k, then of rows; keys)
+template <typename T>
+__global__ __launch_bounds__(256) void k_lora_transpose(LoraTurn a) {
+    __shared__ T s[64 * (kLoraMaxRank + 2)];
+    const int key = (int)blockIdx.y, rank = a.rank, pitch = rank + 2;
+    if (!lora_key_used(a.runs, a.windows, a.keys, key)) return;
+    const bool of_a = (int)blockIdx.x < a.tiles_a;
+    const int n = of_a ? a.k : a.rows, c0 = 64 * ((int)blockIdx.x - (of_a ? 0 : a.tiles_a)), m = min(64, n - c0);
+    const T* in = static_cast<const T*>(of_a ? a.a : a.b) + (size_t)key * rank * n;
+    T* out = static_cast<T*>(of_a ? a.at : a.bt) + (size_t)key * rank * n;
+    for (int i = (int)threadIdx.x; i < 64 * rank; i += 256) {
+        const int c = of_a ? i % 64 : i / rank, r = of_a ? i / 64 : i % rank;
+        if (c < m) s[c * pitch + r] = in[of_a ? (size_t)r * n + c0 + c : (size_t)(c0 + c) * rank + r];
     }
     __syncthreads();
-    for (int r = tid; r < a.rank; r += kLoraThreads) {
-        a.su[(size_t)row * 2 * a.rank + r] = r < rk ? s[r] : 0.0f;
-        a.su[((size_t)row * 2 + 1) * a.rank + r] = r < rk ? u[r] : 0.0f;
-    }
-    if (!dx) return;
-    for (int i = tid; i < a.k; i += kLoraThreads) {
-        float acc = 0.0f;
-        for (int r = 0; r < rk; ++r) acc = __builtin_fmaf(W::value(A[(size_t)r * a.k + i]), u[r], acc);
-        dx[i] = a.add_dx ? dx[i] + acc : acc;
+    for (int i = (int)threadIdx.x; i < 64 * rank; i += 256) {
+        const int c = of_a ? i / rank : i % 64, r = of_a ? i % rank : i / 64;
+        if (c < m) out[of_a ? (size_t)(c0 + c) * rank + r : (size_t)r * n + c0 + c] = s[c * pitch + r];
     }
 }
 
-// one workgroup per (key, r): dA[key][r] and dB[key][..][r], over the call's rows in order
-__global__ __launch_bounds__(kLoraThreads) void k_lora_back_weights(LoraArgs a) {
-    const int key = (int)blockIdx.x, r = (int)blockIdx.y, R = a.n_tokens * a.n_ids, tid = (int)threadIdx.x;
-    const float c = lora_scale(a, key);
-    float* da = a.da ? a.da + ((size_t)key * a.rank + r) * a.k : nullptr;
-    float* db = a.db ? a.db + (size_t)key * a.rows * a.rank + r : nullptr;
-    for (int i0 = 0; da && i0 < a.k; i0 += kLoraThreads) {
-        const int i = i0 + tid;
-        float acc = 0.0f;
-        for (int row = 0; row < R; ++row)
-            if (lora_key(a, row) == key && i < a.k)
-                acc = __builtin_fmaf(a.su[((size_t)row * 2 + 1) * a.rank + r], lora_x(a, row)[i], acc);
-        if (i < a.k) da[i] = a.add_dw ? da[i] + acc : acc;
+// The three bf16 pieces of a value (as lora_split's)
+__device__ inline void lora_split1(float x, uint16_t (&w)[3]) {
+#pragma unroll
+    for (int g = 0; g < 3; ++g) {
+        w[g] = (uint16_t)(__float_as_uint(x) >> 16);
+        x = x - __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
     }
-    for (int o0 = 0; db && o0 < a.rows; o0 += kLoraThreads) {
-        const int o = o0 + tid;
-        float acc = 0.0f;
-        for (int row = 0; row < R; ++row)
-            if (lora_key(a, row) == key && o < a.rows)
-                acc = __builtin_fmaf(
-                    a.su[(size_t)row * 2 * a.rank + r],
-                    reinterpret_cast<const float*>(a.dy + lora_at(row, a.n_ids, a.dy_id, a.dy_tok))[o], acc);
-        if (o < a.rows) db[(size_t)o * a.rank] = a.add_dw ? db[(size_t)o * a.rank] + c * acc : c * acc;
+}
+
+struct LoraJoin {
+    LoraTiles s, u;               // the parts of s and u
+    uint16_t *ps, *pu;            // [windows * slots][3 pieces][rank, in 16s][16 rows]
+    uint64_t *ox, *oy;            // [windows * slots][16]: byte offsets of the rows of x and dy
+};
+// Per tile: s and c u as the weights' gradients read them, in bf16 pieces, rows side by side, and zeros past the tile's
+// rows and the adapter's rank; and where its rows of x and dy are (past the last row, the last).
+// grid (slots, windows)
+template <int NR>
+__global__ __launch_bounds__(256) void k_lora_join(LoraArgs a, LoraJoin j) {
+    const int w = (int)blockIdx.y, tid = (int)threadIdx.x;
+    int key, n, row, pos;
+    if (!lora_item(j.s, w, key, n, row, pos) || key < 0) return;
+    const size_t slot = (size_t)w * j.s.slots + blockIdx.x;
+    if (tid < 16) {
+        const int t = row / a.n_ids, i = row - t * a.n_ids;
+        j.ox[slot * 16 + tid] = (uint64_t)t * a.x_tok + (uint64_t)(i % a.x_rows) * a.x_id;
+        j.oy[slot * 16 + tid] = (uint64_t)t * a.dy_tok + (uint64_t)i * a.dy_id;
+    }
+    const int rk = lora_rank(a, key);
+    const float c = lora_scale(a, key);
+    constexpr int GW = kLoraGroupWidth<NR>;
+    for (int i = tid; i < 16 * 16 * NR; i += 256) {
+        const int r = i / 16, p = i % 16, g = r / GW;
+        const int v = g * GW + r - min(g * GW, max(0, a.rank - GW));            // the value that counts rank r
+        float s = 0.0f, u = 0.0f;
+        if (p < n && r < rk) {
+            const size_t at = (size_t)pos * (16 * NR) + ((v >> 2) * n + p) * 4 + (v & 3);
+            for (int z = 0; z < j.s.k_parts; ++z) s += j.s.s[(size_t)z * j.s.positions * (16 * NR) + at];
+            for (int z = 0; z < j.u.k_parts; ++z) u += j.u.s[(size_t)z * j.u.positions * (16 * NR) + at];
+        }
+        uint16_t ps[3], pu[3];
+        lora_split1(s, ps);
+        lora_split1(u * c, pu);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            j.ps[(slot * 3 + q) * (256 * NR) + i] = ps[q];
+            j.pu[(slot * 3 + q) * (256 * NR) + i] = pu[q];
+        }
+    }
+}
+
+struct LoraGrad {
+    const uint32_t* runs;
+    int windows, keys, slots, splits, rank;
+    int tiles_a;                  // column tiles of dA; dB's follow
+    const uint16_t* p[2];         // pieces of u, of s
+    const uint64_t* off[2];       // offsets of x's rows, of dy's
+    const uint8_t* src[2];        // x, dy
+    int width[2];                 // k, rows
+    float* out[2];                // dA, dB
+    float* part[2];               // several splits: [splits][keys][tiles][16 NR][64]
+    const float* scale;
+    int n_experts, add;
+};
+
+// 16 ranks (rank block b) by 64 columns, summed in sum[16][64] of LDS, to the gradient.  dA [rank][k], dB [rows][rank].
+__device__ inline void lora_grad_store(const LoraGrad& g, int side, int key, int b, int c0, const float* sum) {
+    const int tid = (int)threadIdx.x, n = g.width[side];
+    float* out = g.out[side] + (size_t)key * g.rank * n;
+    const float c = side && g.scale ? g.scale[key / g.n_experts] : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int e = tid + 256 * i, r = side ? e & 15 : e >> 6, o = side ? e >> 4 : e & 63;
+        if (16 * b + r >= g.rank || c0 + o >= n) continue;
+        float* to = out + (side ? (size_t)(c0 + o) * g.rank + 16 * b + r : (size_t)(16 * b + r) * n + c0 + o);
+        const float v = sum[r * 64 + o] * c;
+        *to = g.add ? *to + v : v;
+    }
+}
+
+// dA or dB of one key and 64 columns: rank blocks of 16 by columns, summed over the key's tiles, two (32 rows) per
+// v_mfma_f32_16x16x32_bf16, which the waves share.  Both operands are f32 in three bf16 pieces; the six
+// products above 2^-24 of the whole are kept: 96 cycles where the f32 form takes 256.  Column 4 n + j
+// of x (dy) belongs to product j of four, so a lane loads four neighbours of eight rows, 256 bytes
+// a row.  splits > 1: a workgroup takes a range of the windows, and k_lora_grad_sum adds them up.
+// grid (column tiles, keys, splits)
+template <int NR, int OCC>
+__global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
+    __shared__ float sum[4][16 * 64];
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, p = lane & 15, q = lane >> 4;
+    const int side = (int)blockIdx.x < g.tiles_a ? 0 : 1, tile = (int)blockIdx.x - (side ? g.tiles_a : 0), c0 = 64 * tile;
+    const int key = (int)blockIdx.y, n = g.width[side], col = c0 + 4 * p;
+    const int per = (g.windows + g.splits - 1) / g.splits, w0 = (int)blockIdx.z * per, w1 = min(g.windows, w0 + per);
+    lf4 acc[NR][4];
+#pragma unroll
+    for (int b = 0; b < NR; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[b][j] = lf4{0, 0, 0, 0};
+    auto step = [&](size_t slot, bool two) {
+        const size_t mine = slot + (two && q > 1 ? 1 : 0);
+        const uint64_t* off = g.off[side] + mine * 16 + 8 * (q & 1);
+        lf4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float* row = reinterpret_cast<const float*>(g.src[side] + off[i]);
+            if (col + 4 <= n) {
+                x[i] = *reinterpret_cast<const lf4u*>(row + col);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[i][c] = col + c < n ? row[col + c] : 0.0f;
+            }
+        }
+        LoraWords X[4][3];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float v[8] = {x[0][j], x[1][j], x[2][j], x[3][j], x[4][j], x[5][j], x[6][j], x[7][j]};
+            lora_split(LoraBF16{}, v, 1.0f, X[j]);
+        }
+        const bool none = !two && q > 1;                    // a lone tile: the other 16 rows count nothing
+#pragma unroll
+        for (int b = 0; b < NR; ++b) {
+            LoraWords U[3];
+#pragma unroll
+            for (int z = 0; z < 3; ++z) {
+                U[z] = *reinterpret_cast<const LoraWords*>(g.p[side] + (mine * 3 + z) * (256 * NR) + (16 * b + p) * 16 + 8 * (q & 1));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) U[z].u[c] = none ? 0u : U[z].u[c];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int lo = 2; lo >= 0; --lo)             // the smallest products first
+#pragma unroll
+                    for (int z = 0; z <= lo; ++z) acc[b][j] = lora_mfma(LoraBF16{}, U[z], X[j][lo - z], acc[b][j]);
+        }
+    };
+    int turn = 0, any = 0;
+    for (int wb = w0; wb < w1; wb += 64) {
+        const uint32_t e = wb + lane < w1 ? g.runs[(size_t)(wb + lane) * g.keys + key] : 0u;
+        for (uint64_t m = __ballot(e != 0u); m; m &= m - 1ull) {
+            const int l = __builtin_ctzll(m);
+            const uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)e, l);
+            const int tiles = ((int)(r >> 16) + kLoraTile - 1) / kLoraTile;
+            const size_t first = (size_t)(wb + l) * g.slots + (r & 0xFFFFu);
+            any = 1;
+            for (int t = 0; t < tiles; t += 2, ++turn)
+                if ((turn & 3) == wave) step(first + t, t + 1 < tiles);
+        }
+    }
+    if (g.splits > 1 && !any) return;                       // k_lora_grad_sum skips it too
+    for (int b = 0; b < NR; ++b) {
+        if (g.splits == 1 && 16 * b >= g.rank) return;
+        __syncthreads();
+#pragma unroll
+        for (int bb = 0; bb < NR; ++bb)
+            if (bb == b) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<lf4*>(&sum[wave][(4 * q + i) * 64 + 4 * p]) = lf4{acc[bb][0][i], acc[bb][1][i], acc[bb][2][i], acc[bb][3][i]};
+            }
+        __syncthreads();
+        float* to = sum[0];
+        if (g.splits > 1) {
+            const int tiles = (n + 63) / 64;
+            to = g.part[side] + ((((size_t)blockIdx.z * g.keys + key) * tiles + tile) * NR + b) * (16 * 64);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = (int)threadIdx.x + 256 * i;
+            to[e] = ((sum[0][e] + sum[1][e]) + sum[2][e]) + sum[3][e];
+        }
+        if (g.splits == 1) {
+            __syncthreads();
+            lora_grad_store(g, side, key, b, c0, sum[0]);
+        }
+    }
+}
+
+// grid (column tiles, keys)
+template <int NR>
+__global__ __launch_bounds__(256) void k_lora_grad_sum(LoraGrad g) {
+    __shared__ float sum[16 * 64];
+    const int tid = (int)threadIdx.x;
+    const int side = (int)blockIdx.x < g.tiles_a ? 0 : 1, tile = (int)blockIdx.x - (side ? g.tiles_a : 0);
+    const int key = (int)blockIdx.y, tiles = (g.width[side] + 63) / 64, per = (g.windows + g.splits - 1) / g.splits;
+    uint64_t used = 0;                                      // splits with rows of the key
+    for (int z = 0; z < g.splits; ++z) {
+        uint32_t any = 0;
+        for (int w = z * per + tid; w < min(g.windows, (z + 1) * per); w += 256) any |= g.runs[(size_t)w * g.keys + key];
+        used |= (uint64_t)(__syncthreads_or(any != 0u) != 0) << z;
+    }
+    for (int b = 0; b < NR && 16 * b < g.rank; ++b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = tid + 256 * i;
+            float v = 0.0f;
+            for (int z = 0; z < g.splits; ++z)
+                if ((used >> z) & 1ull) v += g.part[side][((((size_t)z * g.keys + key) * tiles + tile) * NR + b) * (16 * 64) + e];
+            sum[e] = v;
+        }
+        __syncthreads();
+        lora_grad_store(g, side, key, b, 64 * tile, sum);
+        __syncthreads();
     }
 }
 
