@@ -250,14 +250,17 @@ static LoraSpace lora_space(const sabah_lora_desc* L, int n_rows) {
     return s;
 }
 
-// A backward call's: the tiles and runs, the parts of s and u, the transposed pairs, the pieces and offsets that
+// A backward call's: the tiles and runs, s and u, the transposed pairs, the pieces and offsets that
 // the weights' gradients read, and their partial sums.
 struct LoraBackSpace {
     size_t order, items, n_items, runs, s, u, at, bt, ps, pu, ox, oy, part, bytes;
-    int windows, slots, key_bits, rank16, positions, s_parts, s_steps, u_parts, u_steps, tiles_a, tiles_b, splits;
+    int windows, slots, key_bits, rank16, positions, tiles_a, tiles_b, splits;
 };
 constexpr int kLoraBackKeys = 1 << 15;        // a word per key and window
-constexpr int kLoraGradGroups = 1024;         // workgroups of the weights' gradients to aim at
+// Splits of the weights' gradients, over the windows: what one request sends is together, so without them the
+// longest request's key would be a few workgroups' work
+constexpr int kLoraGradSplits = 8;
+constexpr size_t kLoraGradBytes = (size_t)128 << 20;    // of partial sums at most
 static LoraBackSpace lora_back_space(const sabah_lora_desc* L, int n_rows) {
     LoraBackSpace s{};
     const int keys = L->n_adapters * L->n_experts, span = std::min(n_rows, kLoraWindow);
@@ -266,12 +269,10 @@ static LoraBackSpace lora_back_space(const sabah_lora_desc* L, int n_rows) {
     s.rank16 = L->rank <= 16 ? 16 : L->rank <= 32 ? 32 : L->rank <= 64 ? 64 : 128;
     while ((keys + 2) >> s.key_bits) ++s.key_bits;
     s.positions = s.windows * kLoraWindow;
-    const int tiles = std::max(1, (n_rows + kLoraTile - 1) / kLoraTile);
-    lora_k_parts(L->k, 2 * tiles, s.s_parts, s.s_steps);
-    lora_k_parts(L->rows, 2 * tiles, s.u_parts, s.u_steps);
     s.tiles_a = (L->k + 63) / 64;
     s.tiles_b = (L->rows + 63) / 64;
-    s.splits = std::max(1, std::min({s.windows, 32, (int)(kLoraGradGroups / ((long long)keys * (s.tiles_a + s.tiles_b)))}));
+    const size_t part = (size_t)keys * (s.tiles_a + s.tiles_b) * s.rank16 * 64 * 4;
+    s.splits = (int)std::max<size_t>(1, std::min<size_t>({(size_t)s.windows, (size_t)kLoraGradSplits, kLoraGradBytes / part}));
     const size_t esize = L->type == kTypeF32 ? 4 : 2, all = (size_t)s.windows * s.slots;
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -283,15 +284,15 @@ static LoraBackSpace lora_back_space(const sabah_lora_desc* L, int n_rows) {
     s.items = take(all * 16);
     s.n_items = take((size_t)s.windows * 4);
     s.runs = take((size_t)s.windows * keys * 4);
-    s.s = take((size_t)s.s_parts * s.positions * s.rank16 * 4);
-    s.u = take((size_t)s.u_parts * s.positions * s.rank16 * 4);
+    s.s = take((size_t)s.positions * s.rank16 * 4);
+    s.u = take((size_t)s.positions * s.rank16 * 4);
     s.at = take((size_t)keys * L->rank * L->k * esize);
     s.bt = take((size_t)keys * L->rank * L->rows * esize);
     s.ps = take(all * 3 * s.rank16 * 32);
     s.pu = take(all * 3 * s.rank16 * 32);
     s.ox = take(all * 16 * 8);
     s.oy = take(all * 16 * 8);
-    s.part = take(s.splits > 1 ? (size_t)s.splits * keys * (s.tiles_a + s.tiles_b) * s.rank16 * 64 * 4 : 0);
+    s.part = take(s.splits > 1 ? s.splits * part : 0);
     s.bytes = at;
     return s;
 }
@@ -443,7 +444,6 @@ struct LoraBack {
     LoraGroup g;
     LoraTiles ts, tu;
     LoraTurn turn;
-    LoraJoin join;
     LoraGrad w;
     int grad_tiles;
     hipStream_t st;
@@ -457,9 +457,7 @@ static int launch_lora_back_rank(const LoraBack& b) {
                        0, b.st, b.a, b.g);
     if (b.g.n_rows && (b.x.dst || b.grad_tiles)) {
         hipLaunchKernelGGL(k_lora_transpose<typename W::T>, dim3((unsigned)(sp.tiles_a + sp.tiles_b), keys), dim3(256), 0, b.st, b.turn);
-        const bool s = b.grad_tiles > b.w.tiles_a;          // s is dB's alone
-        hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC>), dim3(slots, (unsigned)std::max(sp.s_parts, sp.u_parts), windows * (s ? 2u : 1u)),
-                           dim3(256), 0, b.st, b.u, b.tu, b.a, b.ts, (int)windows);
+        hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC>), dim3(slots, 1u, windows * (b.grad_tiles ? 2u : 1u)), dim3(256), 0, b.st, b.u, b.tu, b.a, b.ts, (int)windows);
     }
     if (b.g.n_rows && b.x.dst) {
         LoraTiles t = b.tu;
@@ -468,10 +466,9 @@ static int launch_lora_back_rank(const LoraBack& b) {
                            b.st, b.x, t);
     }
     if (b.grad_tiles) {
-        if (b.g.n_rows) hipLaunchKernelGGL(k_lora_join<NR>, dim3(slots, windows), dim3(256), 0, b.st, b.a, b.join);
         hipLaunchKernelGGL((k_lora_grad<NR, GOCC>), dim3((unsigned)b.grad_tiles, keys, (unsigned)b.w.splits), dim3(256), 0, b.st, b.w);
         if (b.w.splits > 1)
-            hipLaunchKernelGGL(k_lora_grad_sum<NR>, dim3((unsigned)b.grad_tiles, keys), dim3(256), 0, b.st, b.w);
+            hipLaunchKernelGGL(k_lora_grad_sum<NR>, dim3((unsigned)b.grad_tiles, keys, (unsigned)((b.a.rank + 15) / 16)), dim3(256), 0, b.st, b.w);
     }
     return ck(hipGetLastError(), "adapters backward launch") ? 0 : -1;
 }
@@ -546,15 +543,18 @@ SABAH_API int sabah_lora_backward(const sabah_lora_desc* lora, const float* d_x,
     t.positions = sp.positions;
     b.ts = b.tu = t;
     b.ts.s = reinterpret_cast<float*>(ws + sp.s);
-    b.ts.k_parts = sp.s_parts;
-    b.ts.k_steps = sp.s_steps;
+    b.ts.k_parts = 1;                                       // whole: the epilogue writes the pieces
+    b.ts.k_steps = (lora->k + 31) / 32;
+    b.ts.pieces = reinterpret_cast<uint16_t*>(ws + sp.ps);
+    b.ts.off = reinterpret_cast<uint64_t*>(ws + sp.ox);
     b.tu.s = reinterpret_cast<float*>(ws + sp.u);
-    b.tu.k_parts = sp.u_parts;
-    b.tu.k_steps = sp.u_steps;
+    b.tu.k_parts = 1;
+    b.tu.k_steps = (lora->rows + 31) / 32;
+    b.tu.pieces = d_da || d_db ? reinterpret_cast<uint16_t*>(ws + sp.pu) : nullptr;
+    b.tu.off = reinterpret_cast<uint64_t*>(ws + sp.oy);
+    b.tu.scaled = 1;
     b.turn = LoraTurn{lora->a, lora->b, ws + sp.at, ws + sp.bt, g.runs, sp.windows, keys, lora->rank, lora->k, lora->rows,
                       sp.tiles_a};
-    b.join = LoraJoin{b.ts, b.tu, reinterpret_cast<uint16_t*>(ws + sp.ps), reinterpret_cast<uint16_t*>(ws + sp.pu),
-                      reinterpret_cast<uint64_t*>(ws + sp.ox), reinterpret_cast<uint64_t*>(ws + sp.oy)};
     LoraGrad& w = b.w;
     w.runs = g.runs;
     w.windows = sp.windows;
@@ -563,10 +563,10 @@ SABAH_API int sabah_lora_backward(const sabah_lora_desc* lora, const float* d_x,
     w.splits = sp.splits;
     w.rank = lora->rank;
     w.tiles_a = d_da ? sp.tiles_a : 0;
-    w.p[0] = b.join.pu;
-    w.p[1] = b.join.ps;
-    w.off[0] = b.join.ox;
-    w.off[1] = b.join.oy;
+    w.p[0] = reinterpret_cast<const uint16_t*>(ws + sp.pu);
+    w.p[1] = b.ts.pieces;
+    w.off[0] = b.ts.off;
+    w.off[1] = b.tu.off;
     w.src[0] = a.x;
     w.src[1] = a.dy;
     w.width[0] = lora->k;

@@ -120,6 +120,9 @@ struct LoraTiles {
     int cols;                     // columns of the output per workgroup
     float* s;                     // larger calls: [k_parts][positions][rank, in 16s]
     int k_parts, k_steps, positions;
+    uint16_t* pieces;             // backward, one k part: [windows * slots][3 pieces][rank, in 16s][16 rows] of s, or null
+    uint64_t* off;                // with pieces: [windows * slots][16], the rows' byte offsets in x
+    int scaled;                   // pieces of c s
 };
 
 struct LoraGroup {
@@ -402,6 +405,16 @@ __device__ inline float lora_column_most(float most) {
 }
 __device__ inline unsigned lora_big_rows(float most) {
     return (unsigned)(__ballot(lora_column_most(most) == __builtin_inff()) & 0xFFFFu);
+}
+
+// Two values' next bf16 piece, to nearest, packed, and their rests.  Three such pieces are within 2^-24 of a value, and so
+// are the six products that k_lora_grad keeps of two values' nine.
+__device__ inline uint32_t lora_split2(float (&v)[2]) {
+    typedef __bf16 lb2 __attribute__((ext_vector_type(2)));
+    const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_convertvector((lf2{v[0], v[1]}), lb2));
+    v[0] = v[0] - __uint_as_float(h << 16);
+    v[1] = v[1] - __uint_as_float(h & 0xFFFF0000u);
+    return h;
 }
 
 // S = X A^T of a tile: the waves share k in steps of 32, of which lane l's operands are the eight
@@ -878,6 +891,30 @@ __device__ inline void lora_shrink_part(const LoraArgs& a, const LoraTiles& t, i
         for (int w4 = 0; w4 < NW; ++w4) v += part[(w4 * 16 * NR + r) * kLoraPart + p];
         if (p < n) out[((j >> 2) * n + p) * 4 + (j & 3)] = lora_value_counts<NR>(j, a.rank, rk) ? v : 0.0f;
     }
+    if (!t.pieces) return;
+    // As the weights' gradients read it: in bf16 pieces, a rank's rows side by side, zeros past the tile's rows and the
+    // adapter's rank; and where the rows of x are (past the last row, the last)
+    const size_t slot = (size_t)w * t.slots + blockIdx.x;
+    if (threadIdx.x < 16) {
+        const int tok = row / a.n_ids;
+        t.off[slot * 16 + threadIdx.x] = (uint64_t)tok * a.x_tok + (uint64_t)((row - tok * a.n_ids) % a.x_rows) * a.x_id;
+    }
+    const float c = t.scaled ? lora_scale(a, key) : 1.0f;
+    for (int i = (int)threadIdx.x; i < 16 * 8 * NR; i += 256) {
+        const int r = i / 8, p = 2 * (i % 8);               // two rows at a time
+        float v[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (p + e < n && r < rk) {
+#pragma unroll
+                for (int w4 = 0; w4 < NW; ++w4) v[e] += part[(w4 * 16 * NR + r) * kLoraPart + p + e];
+                v[e] *= c;
+            }
+#pragma unroll
+        for (int z = 0; z < 3; ++z) {
+            reinterpret_cast<uint32_t*>(t.pieces)[(slot * 3 + z) * (128 * NR) + i] = lora_split2(v);
+        }
+    }
 }
 // Both sides' in one launch, the windows of the second after the first's (forward: windows of b none)
 template <typename W, int NR, int U, int OCC>
@@ -958,65 +995,24 @@ __global__ __launch_bounds__(256) void k_lora_transpose(LoraTurn a) {
     const int n = of_a ? a.k : a.rows, c0 = 64 * ((int)blockIdx.x - (of_a ? 0 : a.tiles_a)), m = min(64, n - c0);
     const T* in = static_cast<const T*>(of_a ? a.a : a.b) + (size_t)key * rank * n;
     T* out = static_cast<T*>(of_a ? a.at : a.bt) + (size_t)key * rank * n;
-    for (int i = (int)threadIdx.x; i < 64 * rank; i += 256) {
-        const int c = of_a ? i % 64 : i / rank, r = of_a ? i / 64 : i % rank;
-        if (c < m) s[c * pitch + r] = in[of_a ? (size_t)r * n + c0 + c : (size_t)(c0 + c) * rank + r];
+    constexpr int U = 8;                                    // loads at a time
+    for (int i0 = (int)threadIdx.x; i0 < 64 * rank; i0 += 256 * U) {
+        T v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = min(i0 + 256 * u, 64 * rank - 1), c = min(of_a ? i & 63 : i / rank, m - 1), r = of_a ? i >> 6 : i % rank;
+            v[u] = in[of_a ? (size_t)r * n + c0 + c : (size_t)(c0 + c) * rank + r];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 256 * u;
+            if (i < 64 * rank) s[(of_a ? i & 63 : i / rank) * pitch + (of_a ? i >> 6 : i % rank)] = v[u];
+        }
     }
     __syncthreads();
     for (int i = (int)threadIdx.x; i < 64 * rank; i += 256) {
-        const int c = of_a ? i / rank : i % 64, r = of_a ? i % rank : i / 64;
+        const int c = of_a ? i / rank : i & 63, r = of_a ? i % rank : i >> 6;
         if (c < m) out[of_a ? (size_t)(c0 + c) * rank + r : (size_t)r * n + c0 + c] = s[c * pitch + r];
-    }
-}
-
-// The three bf16 pieces of a value (as lora_split's)
-__device__ inline void lora_split1(float x, uint16_t (&w)[3]) {
-#pragma unroll
-    for (int g = 0; g < 3; ++g) {
-        w[g] = (uint16_t)(__float_as_uint(x) >> 16);
-        x = x - __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-    }
-}
-
-struct LoraJoin {
-    LoraTiles s, u;               // the parts of s and u
-    uint16_t *ps, *pu;            // [windows * slots][3 pieces][rank, in 16s][16 rows]
-    uint64_t *ox, *oy;            // [windows * slots][16]: byte offsets of the rows of x and dy
-};
-// Per tile: s and c u as the weights' gradients read them, in bf16 pieces, rows side by side, and zeros past the tile's
-// rows and the adapter's rank; and where its rows of x and dy are (past the last row, the last).
-// grid (slots, windows)
-template <int NR>
-__global__ __launch_bounds__(256) void k_lora_join(LoraArgs a, LoraJoin j) {
-    const int w = (int)blockIdx.y, tid = (int)threadIdx.x;
-    int key, n, row, pos;
-    if (!lora_item(j.s, w, key, n, row, pos) || key < 0) return;
-    const size_t slot = (size_t)w * j.s.slots + blockIdx.x;
-    if (tid < 16) {
-        const int t = row / a.n_ids, i = row - t * a.n_ids;
-        j.ox[slot * 16 + tid] = (uint64_t)t * a.x_tok + (uint64_t)(i % a.x_rows) * a.x_id;
-        j.oy[slot * 16 + tid] = (uint64_t)t * a.dy_tok + (uint64_t)i * a.dy_id;
-    }
-    const int rk = lora_rank(a, key);
-    const float c = lora_scale(a, key);
-    constexpr int GW = kLoraGroupWidth<NR>;
-    for (int i = tid; i < 16 * 16 * NR; i += 256) {
-        const int r = i / 16, p = i % 16, g = r / GW;
-        const int v = g * GW + r - min(g * GW, max(0, a.rank - GW));            // the value that counts rank r
-        float s = 0.0f, u = 0.0f;
-        if (p < n && r < rk) {
-            const size_t at = (size_t)pos * (16 * NR) + ((v >> 2) * n + p) * 4 + (v & 3);
-            for (int z = 0; z < j.s.k_parts; ++z) s += j.s.s[(size_t)z * j.s.positions * (16 * NR) + at];
-            for (int z = 0; z < j.u.k_parts; ++z) u += j.u.s[(size_t)z * j.u.positions * (16 * NR) + at];
-        }
-        uint16_t ps[3], pu[3];
-        lora_split1(s, ps);
-        lora_split1(u * c, pu);
-#pragma unroll
-        for (int q = 0; q < 3; ++q) {
-            j.ps[(slot * 3 + q) * (256 * NR) + i] = ps[q];
-            j.pu[(slot * 3 + q) * (256 * NR) + i] = pu[q];
-        }
     }
 }
 
@@ -1029,7 +1025,7 @@ struct LoraGrad {
     const uint8_t* src[2];        // x, dy
     int width[2];                 // k, rows
     float* out[2];                // dA, dB
-    float* part[2];               // several splits: [splits][keys][tiles][16 NR][64]
+    float* part[2];               // several splits: [splits][keys][tiles][16 NR][64]; window w is split w % splits'
     const float* scale;
     int n_experts, add;
 };
@@ -1049,28 +1045,69 @@ __device__ inline void lora_grad_store(const LoraGrad& g, int side, int key, int
     }
 }
 
+// The splits that have rows of the key, a bit each (at most 32); a wave asks
+__device__ inline uint32_t lora_grad_splits(const LoraGrad& g, int key) {
+    const int lane = (int)threadIdx.x & 63;
+    uint32_t used = 0;
+    for (int w = lane; w < g.windows; w += 64) used |= (g.runs[(size_t)w * g.keys + key] != 0u ? 1u : 0u) << (w % g.splits);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) used |= (uint32_t)__shfl_xor((int)used, o);
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)used);
+}
+
 // dA or dB of one key and 64 columns: rank blocks of 16 by columns, summed over the key's tiles, two (32 rows) per
 // v_mfma_f32_16x16x32_bf16, which the waves share.  Both operands are f32 in three bf16 pieces; the six
 // products above 2^-24 of the whole are kept: 96 cycles where the f32 form takes 256.  Column 4 n + j
 // of x (dy) belongs to product j of four, so a lane loads four neighbours of eight rows, 256 bytes
-// a row.  splits > 1: a workgroup takes a range of the windows, and k_lora_grad_sum adds them up.
+// a row; the next tiles' rows are loaded under the products.  splits > 1: a workgroup takes
+// the windows of its split, and if others have rows of the key too k_lora_grad_sum adds them up.
 // grid (column tiles, keys, splits)
 template <int NR, int OCC>
 __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
     __shared__ float sum[4][16 * 64];
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, p = lane & 15, q = lane >> 4;
+    const int lane = (int)threadIdx.x & 63, p = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int side = (int)blockIdx.x < g.tiles_a ? 0 : 1, tile = (int)blockIdx.x - (side ? g.tiles_a : 0), c0 = 64 * tile;
-    const int key = (int)blockIdx.y, n = g.width[side], col = c0 + 4 * p;
-    const int per = (g.windows + g.splits - 1) / g.splits, w0 = (int)blockIdx.z * per, w1 = min(g.windows, w0 + per);
+    const int key = (int)blockIdx.y, split = (int)blockIdx.z, n = g.width[side], col = c0 + 4 * p;
+    const uint32_t used = g.splits > 1 ? lora_grad_splits(g, key) : 1u;
+    if (!((used >> split) & 1u) && !(used == 0u && split == 0)) return;     // a key without rows: split 0 writes its zeros
     lf4 acc[NR][4];
 #pragma unroll
     for (int b = 0; b < NR; ++b)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[b][j] = lf4{0, 0, 0, 0};
-    auto step = [&](size_t slot, bool two) {
-        const size_t mine = slot + (two && q > 1 ? 1 : 0);
-        const uint64_t* off = g.off[side] + mine * 16 + 8 * (q & 1);
-        lf4 x[8];
+    // the key's tiles in pairs, every fourth this wave's: windows split, split + splits, ..., 64 at a time
+    int wb = split - 64 * g.splits, left = 0, turn = -1;
+    uint64_t some = 0;
+    uint32_t e = 0;
+    size_t at = 0;
+    auto advance = [&](size_t& slot, bool& two) {
+        for (;;) {
+            if (left > 0) {
+                slot = at;
+                two = left > 1;
+                at += 2;
+                left -= 2;
+                turn = (turn + 1) & 3;
+                if (turn == wave) return true;
+                continue;
+            }
+            while (some == 0) {
+                wb += 64 * g.splits;
+                if (wb >= g.windows) return false;
+                const int w = wb + lane * g.splits;
+                e = w < g.windows ? g.runs[(size_t)w * g.keys + key] : 0u;
+                some = __ballot(e != 0u);
+            }
+            const int l = __builtin_ctzll(some);
+            some &= some - 1ull;
+            const uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)e, l);
+            left = ((int)(r >> 16) + kLoraTile - 1) / kLoraTile;
+            at = (size_t)(wb + l * g.splits) * g.slots + (r & 0xFFFFu);
+        }
+    };
+    auto load = [&](lf4 (&x)[8], size_t slot, bool two) {
+        const uint64_t* off = g.off[side] + (slot + (two && q > 1 ? 1 : 0)) * 16 + 8 * (q & 1);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float* row = reinterpret_cast<const float*>(g.src[side] + off[i]);
@@ -1081,19 +1118,25 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
                 for (int c = 0; c < 4; ++c) x[i][c] = col + c < n ? row[col + c] : 0.0f;
             }
         }
+    };
+    auto mul = [&](const lf4 (&x)[8], size_t slot, bool two) {
         LoraWords X[4][3];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float v[8] = {x[0][j], x[1][j], x[2][j], x[3][j], x[4][j], x[5][j], x[6][j], x[7][j]};
-            lora_split(LoraBF16{}, v, 1.0f, X[j]);
-        }
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float v[2] = {x[2 * c][j], x[2 * c + 1][j]};
+#pragma unroll
+                for (int z = 0; z < 3; ++z) X[j][z].u[c] = lora_split2(v);
+            }
         const bool none = !two && q > 1;                    // a lone tile: the other 16 rows count nothing
+        const uint16_t* pieces = g.p[side] + (slot + (two && q > 1 ? 1 : 0)) * (768 * NR) + 16 * p + 8 * (q & 1);
 #pragma unroll
         for (int b = 0; b < NR; ++b) {
             LoraWords U[3];
 #pragma unroll
             for (int z = 0; z < 3; ++z) {
-                U[z] = *reinterpret_cast<const LoraWords*>(g.p[side] + (mine * 3 + z) * (256 * NR) + (16 * b + p) * 16 + 8 * (q & 1));
+                U[z] = *reinterpret_cast<const LoraWords*>(pieces + z * (256 * NR) + 256 * b);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) U[z].u[c] = none ? 0u : U[z].u[c];
             }
@@ -1105,22 +1148,24 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
                     for (int z = 0; z <= lo; ++z) acc[b][j] = lora_mfma(LoraBF16{}, U[z], X[j][lo - z], acc[b][j]);
         }
     };
-    int turn = 0, any = 0;
-    for (int wb = w0; wb < w1; wb += 64) {
-        const uint32_t e = wb + lane < w1 ? g.runs[(size_t)(wb + lane) * g.keys + key] : 0u;
-        for (uint64_t m = __ballot(e != 0u); m; m &= m - 1ull) {
-            const int l = __builtin_ctzll(m);
-            const uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)e, l);
-            const int tiles = ((int)(r >> 16) + kLoraTile - 1) / kLoraTile;
-            const size_t first = (size_t)(wb + l) * g.slots + (r & 0xFFFFu);
-            any = 1;
-            for (int t = 0; t < tiles; t += 2, ++turn)
-                if ((turn & 3) == wave) step(first + t, t + 1 < tiles);
-        }
+    lf4 x[8];
+    size_t slot = 0;
+    bool two = false, more = advance(slot, two);
+    if (more) load(x, slot, two);
+    while (more) {
+        lf4 y[8];
+        size_t slot2 = 0;
+        bool two2 = false;
+        more = advance(slot2, two2);
+        if (more) load(y, slot2, two2);
+        mul(x, slot, two);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = y[i];
+        slot = slot2;
+        two = two2;
     }
-    if (g.splits > 1 && !any) return;                       // k_lora_grad_sum skips it too
-    for (int b = 0; b < NR; ++b) {
-        if (g.splits == 1 && 16 * b >= g.rank) return;
+    const bool whole = (used & (used - 1u)) == 0u;          // no other split has rows
+    for (int b = 0; b < NR && 16 * b < g.rank; ++b) {
         __syncthreads();
 #pragma unroll
         for (int bb = 0; bb < NR; ++bb)
@@ -1131,48 +1176,33 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
             }
         __syncthreads();
         float* to = sum[0];
-        if (g.splits > 1) {
-            const int tiles = (n + 63) / 64;
-            to = g.part[side] + ((((size_t)blockIdx.z * g.keys + key) * tiles + tile) * NR + b) * (16 * 64);
-        }
+        if (!whole) to = g.part[side] + ((((size_t)split * g.keys + key) * ((n + 63) / 64) + tile) * NR + b) * (16 * 64);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int e = (int)threadIdx.x + 256 * i;
-            to[e] = ((sum[0][e] + sum[1][e]) + sum[2][e]) + sum[3][e];
+            const int o = (int)threadIdx.x + 256 * i;
+            to[o] = ((sum[0][o] + sum[1][o]) + sum[2][o]) + sum[3][o];
         }
-        if (g.splits == 1) {
+        if (whole) {
             __syncthreads();
             lora_grad_store(g, side, key, b, c0, sum[0]);
         }
     }
 }
 
-// grid (column tiles, keys)
+// grid (column tiles, keys, blocks of 16 ranks)
 template <int NR>
 __global__ __launch_bounds__(256) void k_lora_grad_sum(LoraGrad g) {
     __shared__ float sum[16 * 64];
-    const int tid = (int)threadIdx.x;
     const int side = (int)blockIdx.x < g.tiles_a ? 0 : 1, tile = (int)blockIdx.x - (side ? g.tiles_a : 0);
-    const int key = (int)blockIdx.y, tiles = (g.width[side] + 63) / 64, per = (g.windows + g.splits - 1) / g.splits;
-    uint64_t used = 0;                                      // splits with rows of the key
-    for (int z = 0; z < g.splits; ++z) {
-        uint32_t any = 0;
-        for (int w = z * per + tid; w < min(g.windows, (z + 1) * per); w += 256) any |= g.runs[(size_t)w * g.keys + key];
-        used |= (uint64_t)(__syncthreads_or(any != 0u) != 0) << z;
-    }
-    for (int b = 0; b < NR && 16 * b < g.rank; ++b) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int e = tid + 256 * i;
-            float v = 0.0f;
-            for (int z = 0; z < g.splits; ++z)
-                if ((used >> z) & 1ull) v += g.part[side][((((size_t)z * g.keys + key) * tiles + tile) * NR + b) * (16 * 64) + e];
-            sum[e] = v;
-        }
-        __syncthreads();
-        lora_grad_store(g, side, key, b, 64 * tile, sum);
-        __syncthreads();
-    }
+    const int key = (int)blockIdx.y, b = (int)blockIdx.z, tiles = (g.width[side] + 63) / 64;
+    const uint32_t used = lora_grad_splits(g, key);
+    if ((used & (used - 1u)) == 0u) return;                 // written by its only split
+    lf4 v = {0, 0, 0, 0};
+    for (uint32_t left = used; left; left &= left - 1u)
+        v += reinterpret_cast<const lf4*>(g.part[side] + ((((size_t)__builtin_ctz(left) * g.keys + key) * tiles + tile) * NR + b) * (16 * 64))[threadIdx.x];
+    reinterpret_cast<lf4*>(sum)[threadIdx.x] = v;
+    __syncthreads();
+    lora_grad_store(g, side, key, b, 64 * tile, sum);
 }
 
 }  // namespace sabah
