@@ -29,18 +29,19 @@ constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 // ---------------------------------------------------------------------------
 // balance loss, counts; the logits' gradient
 // ---------------------------------------------------------------------------
-constexpr int kBalanceChunkTokens = 16;      // tokens per workgroup of k_balance_rows, four per wave
-constexpr int kBalanceMaxChunks = 2048;      // workgroups at most: a larger batch has longer runs
+// Workgroups of k_balance_rows to aim at: enough to fill the chip, few enough that adding up their sums stays small
+constexpr int kBalanceGroups = 512;
 
+// a group's tokens in runs: multiples of four, one for each wave of a workgroup
 static void balance_plan(int n_tokens, int n_groups, int& chunks, int& chunk_len) {
     const int len = n_tokens / n_groups;
-    const int most = std::max(1, kBalanceMaxChunks / n_groups);
-    chunk_len = std::max(kBalanceChunkTokens, (len + most - 1) / most);
+    const int most = std::max(1, kBalanceGroups / n_groups);
+    chunk_len = std::max(4, ((len + most - 1) / most + 3) / 4 * 4);
     chunks = std::max(1, (len + chunk_len - 1) / chunk_len);
 }
 
 struct BalanceSpace {
-    size_t p, c, z, loss, ticket, bytes;
+    size_t p, c, z, loss, group, ticket, bytes;
 };
 static BalanceSpace balance_space(int n_tokens, int n_experts, int n_groups) {
     int chunks, len;
@@ -51,7 +52,8 @@ static BalanceSpace balance_space(int n_tokens, int n_experts, int n_groups) {
     s.c = s.p + align256(parts * n_experts * 4);
     s.z = s.c + align256(parts * n_experts * 4);
     s.loss = s.z + align256(parts * 8);
-    s.ticket = s.loss + align256((size_t)n_groups * ((n_experts + 63) / 64) * 8);
+    s.group = s.loss + align256((size_t)n_groups * ((n_experts + kBalanceCols - 1) / kBalanceCols) * 8);
+    s.ticket = s.group + align256((size_t)n_groups * 16);
     s.bytes = s.ticket + 256;
     return s;
 }
@@ -72,9 +74,9 @@ SABAH_API size_t sabah_moe_balance_workspace(int n_tokens, int n_experts, int n_
     return balance_space(n_tokens, n_experts, n_groups).bytes;
 }
 
-template <int PER, int W>
+template <int PER, int VEC, int W>
 static void launch_balance_rows(const BalanceArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_balance_rows<PER, W>), dim3((unsigned)a.chunks, (unsigned)a.n_groups), dim3(row_threads(W)),
+    hipLaunchKernelGGL((k_balance_rows<PER, VEC, W>), dim3((unsigned)a.chunks, (unsigned)a.n_groups), dim3(row_threads(W)),
                        (uint32_t)a.n_experts * 8, st, a);
 }
 
@@ -109,6 +111,7 @@ SABAH_API int sabah_moe_balance(const float* d_logits, size_t logits_stride, con
     a.part_c = reinterpret_cast<int*>(ws + sp.c);
     a.part_z = reinterpret_cast<float2*>(ws + sp.z);
     a.part_loss = reinterpret_cast<double*>(ws + sp.loss);
+    a.group = reinterpret_cast<double2*>(ws + sp.group);
     a.ticket = reinterpret_cast<unsigned*>(ws + sp.ticket);
     a.counts = d_counts;
     a.mean_p = d_mean_p;
@@ -116,22 +119,22 @@ SABAH_API int sabah_moe_balance(const float* d_logits, size_t logits_stride, con
     a.n_valid = d_n_valid;
     a.err = g_err_dev;
     hipStream_t st = pick_stream(stream);
-    if (n_experts <= 64) launch_balance_rows<1, 1>(a, st);
-    else if (n_experts <= 128) launch_balance_rows<2, 1>(a, st);
-    else if (n_experts <= 256) launch_balance_rows<4, 1>(a, st);
-    else if (n_experts <= 512) launch_balance_rows<8, 1>(a, st);
-    else if (n_experts <= 2048) launch_balance_rows<8, 4>(a, st);
-    else launch_balance_rows<8, 8>(a, st);
+    if (n_experts <= 64) launch_balance_rows<1, 1, 1>(a, st);
+    else if (n_experts <= 128) launch_balance_rows<2, 2, 1>(a, st);
+    else if (n_experts <= 256) launch_balance_rows<4, 4, 1>(a, st);
+    else if (n_experts <= 512) launch_balance_rows<8, 4, 1>(a, st);
+    else if (n_experts <= 2048) launch_balance_rows<8, 4, 4>(a, st);
+    else launch_balance_rows<8, 4, 8>(a, st);
     if (!ck(hipGetLastError(), "balance launch")) return -1;
-    hipLaunchKernelGGL(k_balance_sum, dim3((unsigned)((n_experts + 63) / 64), (unsigned)n_groups), dim3(kBalanceThreads),
-                       0, st, a);
+    hipLaunchKernelGGL(k_balance_sum, dim3((unsigned)((n_experts + kBalanceCols - 1) / kBalanceCols), (unsigned)n_groups),
+                       dim3(kBalanceSumThreads), 0, st, a);
     return ck(hipGetLastError(), "balance sum launch") ? 0 : -1;
 }
 
-template <int PER, int W>
+template <int PER, int VEC, int W>
 static void launch_route_backward(const RouteBackArgs& a, hipStream_t st) {
     constexpr int kSide = row_threads(W) / (64 * W);               // tokens of a workgroup
-    hipLaunchKernelGGL((k_route_backward<PER, W>), dim3((unsigned)((a.n_tokens + kSide - 1) / kSide)),
+    hipLaunchKernelGGL((k_route_backward<PER, VEC, W>), dim3((unsigned)((a.n_tokens + kSide - 1) / kSide)),
                        dim3(row_threads(W)), 0, st, a);
 }
 
@@ -177,12 +180,12 @@ SABAH_API int sabah_moe_route_backward(const float* d_logits, size_t logits_stri
     a.c_z = c_z;
     a.err = g_err_dev;
     hipStream_t st = pick_stream(stream);
-    if (n_experts <= 64) launch_route_backward<1, 1>(a, st);
-    else if (n_experts <= 128) launch_route_backward<2, 1>(a, st);
-    else if (n_experts <= 256) launch_route_backward<4, 1>(a, st);
-    else if (n_experts <= 512) launch_route_backward<8, 1>(a, st);
-    else if (n_experts <= 2048) launch_route_backward<8, 4>(a, st);
-    else launch_route_backward<8, 8>(a, st);
+    if (n_experts <= 64) launch_route_backward<1, 1, 1>(a, st);
+    else if (n_experts <= 128) launch_route_backward<2, 2, 1>(a, st);
+    else if (n_experts <= 256) launch_route_backward<4, 4, 1>(a, st);
+    else if (n_experts <= 512) launch_route_backward<8, 4, 1>(a, st);
+    else if (n_experts <= 2048) launch_route_backward<8, 4, 4>(a, st);
+    else launch_route_backward<8, 4, 8>(a, st);
     return ck(hipGetLastError(), "route backward launch") ? 0 : -1;
 }
 
@@ -215,12 +218,21 @@ static bool stride_ok(size_t s) { return s % 4 == 0; }
 constexpr int kLoraDirectRows = 256;
 constexpr int kLoraFusedTiles = 256;          // from here on a tile's shrink and expand in one workgroup
 constexpr int kLoraShrinkGroups = 1024, kLoraShrinkParts = 8, kLoraShrinkSteps = 8;
+constexpr int kLoraExpandGroups = 1024;
 // k of a shrink in parts while there are few tiles
 static void lora_k_parts(int k, int tiles, int& parts, int& steps) {
     const int all = (k + 31) / 32;
     parts = std::max(1, std::min({kLoraShrinkParts, kLoraShrinkGroups / tiles, all / kLoraShrinkSteps}));
     steps = (all + parts - 1) / parts;
     parts = (all + steps - 1) / steps;
+}
+
+// The expand's columns in parts of a step of 64 or more for each of its four waves, about kLoraExpandGroups workgroups
+static int lora_columns(int columns, int n_rows, int& cols) {
+    const int tiles = (n_rows + kLoraTile - 1) / kLoraTile;
+    const int parts = std::max(1, std::min((columns + 255) / 256, kLoraExpandGroups / tiles));
+    cols = ((columns + parts - 1) / parts + 63) / 64 * 64;
+    return (columns + cols - 1) / cols;
 }
 
 struct LoraSpace {
@@ -425,11 +437,15 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
         t.k_steps = sp.k_steps;
         t.positions = sp.windows * kLoraWindow;
     }
-    // columns per workgroup: a step of 64 for each wave of the expand; in small calls what fills the chip
-    int parts = t.s ? (lora->rows + 255) / 256 : 1;
-    if (!sp.bytes) parts = std::max(1, std::min((lora->rows + 63) / 64, 2 * g_num_cu / sp.slots));
-    t.cols = ((lora->rows + parts - 1) / parts + 63) / 64 * 64;
-    parts = (lora->rows + t.cols - 1) / t.cols;
+    int parts = 1;
+    t.cols = (lora->rows + 63) / 64 * 64;
+    if (t.s) {
+        parts = lora_columns(lora->rows, n_rows, t.cols);
+    } else if (!sp.bytes) {                                 // what fills the chip
+        parts = std::max(1, std::min((lora->rows + 63) / 64, 2 * g_num_cu / sp.slots));
+        t.cols = ((lora->rows + parts - 1) / parts + 63) / 64 * 64;
+        parts = (lora->rows + t.cols - 1) / t.cols;
+    }
     switch (lora->type) {
     case kTypeF32: launch_lora_apply<LoraF32>(a, t, parts, sp.windows, st); break;
     case kTypeF16: launch_lora_apply<LoraF16>(a, t, parts, sp.windows, st); break;
@@ -461,9 +477,8 @@ static int launch_lora_back_rank(const LoraBack& b) {
     }
     if (b.g.n_rows && b.x.dst) {
         LoraTiles t = b.tu;
-        t.cols = 256;
-        hipLaunchKernelGGL((k_lora_expand<W, NR, std::min(OCC, 3)>), dim3(slots, (unsigned)((b.x.rows + 255) / 256), windows), dim3(256), 0,
-                           b.st, b.x, t);
+        const int parts = lora_columns(b.x.rows, b.g.n_rows, t.cols);
+        hipLaunchKernelGGL((k_lora_expand<W, NR, std::min(OCC, 3)>), dim3(slots, (unsigned)parts, windows), dim3(256), 0, b.st, b.x, t);
     }
     if (b.grad_tiles) {
         hipLaunchKernelGGL((k_lora_grad<NR, GOCC>), dim3((unsigned)b.grad_tiles, keys, (unsigned)b.w.splits), dim3(256), 0, b.st, b.w);
@@ -475,8 +490,8 @@ static int launch_lora_back_rank(const LoraBack& b) {
 template <typename W>
 static int launch_lora_back(const LoraBack& b) {
     if (b.a.rank <= 16) return launch_lora_back_rank<W, 1, 2, 4, 3>(b);
-    if (b.a.rank <= 32) return launch_lora_back_rank<W, 2, 2, 4, 3>(b);
-    if (b.a.rank <= 64) return launch_lora_back_rank<W, 4, 1, 2, 2>(b);
+    if (b.a.rank <= 32) return launch_lora_back_rank<W, 2, 2, 4, 2>(b);
+    if (b.a.rank <= 64) return launch_lora_back_rank<W, 4, 2, 3, 2>(b);
     return launch_lora_back_rank<W, 8, 1, 1, 1>(b);
 }
 

@@ -19,9 +19,12 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace sabah {
 
-constexpr int kBalanceThreads = 256;          // of k_balance_sum, and where a row is one wave's or four's
+constexpr int kBalanceThreads = 256;          // where a row is one wave's or four's
+constexpr int kBalanceSumThreads = 1024, kBalanceCols = 16;   // of k_balance_sum, and its experts per workgroup
 constexpr int row_threads(int w) { return w > 4 ? 64 * w : kBalanceThreads; }
 constexpr unsigned kErrRouteId = 3u;          // sticky error word: a selected expert id out of range
 
@@ -36,6 +39,7 @@ struct BalanceArgs {
     int* part_c;                  // the same of counts
     float2* part_z;               // [n_groups * chunks] (valid tokens' number as int bits, sum of lse^2)
     double* part_loss;            // [n_groups * column blocks]
+    double2* group;               // [n_groups] (valid tokens, sum of lse^2)
     unsigned* ticket;
     int* counts;                  // [n_groups][n_experts]
     float* mean_p;                // [n_groups][n_experts]
@@ -44,13 +48,28 @@ struct BalanceArgs {
     unsigned int* err;
 };
 
-// A token's row is held by W waves: one up to 512 experts, else 4 or 8, the workgroup;
-// thread v of them has the experts v, v + 64 W, ....  Sums and maxima over the
-// row; tmp: W floats of LDS, used with W > 1, where the whole workgroup takes part.
+// A token's row is held by W waves: one up to 512 experts, else 4 or 8, the workgroup.  Thread v of them
+// has VEC neighbours of every 64 W VEC experts, PER in all.
+template <int VEC, int W>
+__device__ inline int row_expert(int v, int j) { return 64 * W * VEC * (j / VEC) + VEC * v + j % VEC; }
+
+// Sums and maxima over the row, the same bits in every lane: within 16 lanes by DPP, then across them
+// by lane swaps (shuffles through LDS took a token's three reductions from 0.1 to 0.6 us).
+// tmp: W floats of LDS, used with W > 1, where the whole workgroup takes part.
+template <int CTRL>
+__device__ inline float row_dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
 template <int W, typename F>
 __device__ inline float row_reduce(float v, float* tmp, F f) {
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) v = f(v, __shfl_xor(v, k));
+    v = f(v, row_dpp<0xB1>(v));                             // quad_perm [1,0,3,2]
+    v = f(v, row_dpp<0x4E>(v));                             // quad_perm [2,3,0,1]
+    v = f(v, row_dpp<0x141>(v));                            // row_half_mirror
+    v = f(v, row_dpp<0x140>(v));                            // row_mirror
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(h[0]), __uint_as_float(h[1]));
     if constexpr (W > 1) {
         __syncthreads();
         if ((threadIdx.x & 63u) == 0) tmp[threadIdx.x >> 6] = v;
@@ -70,43 +89,75 @@ __device__ inline float row_sum(float v, float* tmp) {
     return row_reduce<W>(v, tmp, [](float a, float b) { return a + b; });
 }
 
+// exp by the hardware's 2^x: the argument's product with log2 e is rounded, |x| 2^-24 of the result
+__device__ inline float row_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+
 // The softmax of a row: e becomes p.  Returns false for a row of minus infinities only.
 template <int PER, int W>
 __device__ inline bool row_softmax(float (&e)[PER], float& lse, float* tmp) {
-    float m = -__builtin_inff(), some = 0.0f;
+    float m = -__builtin_inff();
+    bool nan = false;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         m = fmaxf(m, e[j]);
-        some = e[j] == -__builtin_inff() ? some : 1.0f;    // a NaN counts: it is passed on, not hidden
+        nan |= e[j] != e[j];                                // passed on, not hidden
     }
-    if (row_max<W>(some, tmp) == 0.0f) return false;
+    if (nan) m = __builtin_inff();                          // every difference is then a NaN or an infinity: the row becomes NaN
     m = row_max<W>(m, tmp);
+    if (m == -__builtin_inff()) return false;
     float s = 0.0f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        e[j] = expf(e[j] - m);                              // 0 past the experts (row_load's minus infinities)
+        e[j] = row_exp(e[j] - m);                           // 0 past the experts (row_load's minus infinities)
         s += e[j];
     }
     s = row_sum<W>(s, tmp);
-    const float inv = 1.0f / s;
+    const float inv = m == __builtin_inff() ? __builtin_nanf("") : 1.0f / s;
 #pragma unroll
     for (int j = 0; j < PER; ++j) e[j] *= inv;
     lse = m + logf(s);
+    if (m == __builtin_inff()) lse = __builtin_nanf("");
     return true;
 }
 
-template <int PER, int W>
-__device__ inline void row_load(const uint8_t* row, int n_experts, int v, float (&e)[PER]) {
-    const float* l = reinterpret_cast<const float*>(row);
+typedef float rf4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef float rf2 __attribute__((ext_vector_type(2), aligned(4)));
+typedef int ri4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef int ri2 __attribute__((ext_vector_type(2), aligned(4)));
+
+// T: float or int, of one row; `past` beyond the experts
+template <int PER, int VEC, int W, typename T>
+__device__ inline void row_load(const void* row, int n_experts, int v, T past, T (&e)[PER]) {
+    typedef typename std::conditional<std::is_same<T, int>::value, ri4, rf4>::type T4;
+    typedef typename std::conditional<std::is_same<T, int>::value, ri2, rf2>::type T2;
+    const T* l = static_cast<const T*>(row);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) e[j] = v + 64 * W * j < n_experts ? l[v + 64 * W * j] : -__builtin_inff();
+    for (int j = 0; j < PER; j += VEC) {
+        const int i = row_expert<VEC, W>(v, j);
+        if (i + VEC <= n_experts) {
+            if constexpr (VEC == 4) {
+                const T4 w = *reinterpret_cast<const T4*>(l + i);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) e[j + c] = w[c];
+            } else if constexpr (VEC == 2) {
+                const T2 w = *reinterpret_cast<const T2*>(l + i);
+                e[j] = w[0], e[j + 1] = w[1];
+            } else {
+                e[j] = l[i];
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) e[j + c] = i + c < n_experts ? l[i + c] : past;
+        }
+    }
 }
 
 // dynamic LDS: n_experts floats, n_experts ints
-template <int PER, int W>
+template <int PER, int VEC, int W>
 __global__ __launch_bounds__(row_threads(W)) void k_balance_rows(BalanceArgs a) {
     extern __shared__ float blds[];
     constexpr int kThr = row_threads(W), kSide = kThr / (64 * W);   // kSide tokens side by side
+    constexpr int B = W == 1 ? 4 : 1;                       // and B of them loaded at a time
     __shared__ int s_n[kSide];
     __shared__ float s_z[kSide];
     __shared__ float s_tmp[W];
@@ -124,20 +175,31 @@ __global__ __launch_bounds__(row_threads(W)) void k_balance_rows(BalanceArgs a) 
     float z = 0.0f;
     int n = 0;
     const int end = min(a.group_len, (c + 1) * a.chunk_len);
-    for (int i = c * a.chunk_len + side; i < end; i += kSide) {
-        const size_t t = (size_t)g * a.group_len + i;
-        if (a.mask && !a.mask[t]) continue;                 // with W > 1 the same for the whole workgroup
-        float e[PER], lse;
-        row_load<PER, W>(a.logits + t * a.stride, E, v, e);
-        if (!row_softmax<PER, W>(e, lse, s_tmp)) continue;
+    for (int i0 = c * a.chunk_len + side; i0 < end; i0 += kSide * B) {
+        float e[B][PER];
+        int id[B];
+        bool live[B];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) acc[j] += e[j];
-        z += lse * lse;
-        ++n;
-        if (v < a.n_used) {
-            const int id = a.ids[t * a.n_used + v];
-            if (id >= 0 && id < E) atomicAdd(&s_c[id], 1);
-            else *reinterpret_cast<volatile unsigned int*>(a.err) = kErrRouteId;
+        for (int b = 0; b < B; ++b) {
+            const int i = min(i0 + kSide * b, end - 1);     // past the run: a token again, which counts nothing
+            const size_t t = (size_t)g * a.group_len + i;
+            live[b] = i0 + kSide * b < end && !(a.mask && !a.mask[t]);   // the same for all threads of the row
+            if (!live[b]) continue;
+            row_load<PER, VEC, W>(a.logits + t * a.stride, E, v, -__builtin_inff(), e[b]);
+            id[b] = v < a.n_used ? a.ids[t * a.n_used + v] : 0;
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            float lse;
+            if (!live[b] || !row_softmax<PER, W>(e[b], lse, s_tmp)) continue;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) acc[j] += e[b][j];
+            z += lse * lse;
+            ++n;
+            if (v < a.n_used) {
+                if (id[b] >= 0 && id[b] < E) atomicAdd(&s_c[id[b]], 1);
+                else *reinterpret_cast<volatile unsigned int*>(a.err) = kErrRouteId;
+            }
         }
     }
     if (v == 0) {
@@ -149,7 +211,7 @@ __global__ __launch_bounds__(row_threads(W)) void k_balance_rows(BalanceArgs a) 
         if (side == w) {
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                const int i = v + 64 * W * j;
+                const int i = row_expert<VEC, W>(v, j);
                 if (i < E) s_p[i] = w ? s_p[i] + acc[j] : acc[j];
             }
         }
@@ -167,82 +229,105 @@ __global__ __launch_bounds__(row_threads(W)) void k_balance_rows(BalanceArgs a) 
     }
 }
 
-// sum over the workgroup's threads, in a fixed order; every thread gets it
+// sum over a wave, in a fixed order; every lane gets it
 template <typename T>
-__device__ inline T block_sum(T v, T* tmp) {
+__device__ inline T wave_add(T v) {
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) v += __shfl_xor(v, k);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0) tmp[threadIdx.x >> 6] = v;
-    __syncthreads();
-    T s = tmp[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) s += tmp[w];
-    return s;
+    return v;
 }
 
-__global__ __launch_bounds__(kBalanceThreads) void k_balance_sum(BalanceArgs a) {
-    constexpr int kWaves = kBalanceThreads / 64;
-    __shared__ double s_d[kWaves][64];
-    __shared__ int s_c[kWaves][64];
-    __shared__ double s_t[kWaves];
-    __shared__ int s_i[kWaves];
-    __shared__ unsigned s_last;
-    const int tid = (int)threadIdx.x, v = tid & 63, wave = tid >> 6, E = a.n_experts;
-    const int g = (int)blockIdx.y, e = (int)blockIdx.x * 64 + v;
+// Thread (chunk row, expert): 64 rows of the chunks by 16 experts.  grid (16s of experts, groups)
+__global__ __launch_bounds__(kBalanceSumThreads) void k_balance_sum(BalanceArgs a) {
+    constexpr int kWaves = kBalanceSumThreads / 64, U = 8;
+    __shared__ double s_p[kWaves][kBalanceCols], s_z[kWaves];
+    __shared__ int s_c[kWaves][kBalanceCols], s_n[kWaves];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, E = a.n_experts;
+    const int g = (int)blockIdx.y, e = (int)blockIdx.x * kBalanceCols + (tid & 15), r0 = tid >> 4;
     const size_t p0 = (size_t)g * a.chunks;
-    int n = 0;
-    for (int c = tid; c < a.chunks; c += kBalanceThreads) n += __float_as_int(a.part_z[p0 + c].x);
-    n = block_sum(n, s_i);
-    double p = 0.0;
-    int cnt = 0;
-    if (e < E)
-        for (int c = wave; c < a.chunks; c += kWaves) {
-            p += (double)a.part_p[(p0 + c) * E + e];
-            cnt += a.part_c[(p0 + c) * E + e];
+    double p = 0.0, z = 0.0;
+    int cnt = 0, n = 0;
+    for (int c0 = r0; c0 < a.chunks; c0 += 64 * U) {        // U loads at a time
+        float x[U];
+        int k[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t at = (p0 + min(c0 + 64 * u, a.chunks - 1)) * E + min(e, E - 1);
+            x[u] = a.part_p[at];
+            k[u] = a.part_c[at];
         }
-    s_d[wave][v] = p;
-    s_c[wave][v] = cnt;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + 64 * u < a.chunks) {
+                p += (double)x[u];
+                cnt += k[u];
+            }
+    }
+    for (int c = tid; c < a.chunks; c += kBalanceSumThreads) {
+        const float2 pz = a.part_z[p0 + c];
+        n += __float_as_int(pz.x);
+        z += (double)pz.y;
+    }
+    p += __shfl_xor(p, 16);
+    p += __shfl_xor(p, 32);
+    cnt += __shfl_xor(cnt, 16);
+    cnt += __shfl_xor(cnt, 32);
+    n = wave_add(n);
+    z = wave_add(z);
+    if (lane < kBalanceCols) {
+        s_p[wave][lane] = p;
+        s_c[wave][lane] = cnt;
+    }
+    if (lane == 0) {
+        s_n[wave] = n;
+        s_z[wave] = z;
+    }
     __syncthreads();
+    if (wave != 0) return;
+    n = 0, z = 0.0, p = 0.0, cnt = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) n += s_n[w], z += s_z[w], p += s_p[w][lane & 15], cnt += s_c[w][lane & 15];
     double term = 0.0;
-    if (wave == 0 && e < E) {
-        for (int w = 1; w < kWaves; ++w) p += s_d[w][v], cnt += s_c[w][v];
+    if (lane < kBalanceCols && e < E) {
         const double mp = n > 0 ? p / (double)n : 0.0;
         a.counts[(size_t)g * E + e] = cnt;
         a.mean_p[(size_t)g * E + e] = (float)mp;
         if (n > 0) term = mp * (double)cnt / ((double)n * (double)a.n_used) * (double)E;
     }
-    const double sum = block_sum(term, s_t);
-    if (tid == 0) {
-        if (blockIdx.x == 0) a.n_valid[g] = n;
-        __hip_atomic_store(&a.part_loss[(size_t)g * gridDim.x + blockIdx.x], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (s_last != gridDim.x * gridDim.y - 1u) return;
-    // the last workgroup: every other's sums are in memory
-    double loss = 0.0, z = 0.0;
-    int total = 0, filled = 0;
-    for (int i = tid; i < (int)(gridDim.x * gridDim.y); i += kBalanceThreads)
-        loss += __hip_atomic_load(&a.part_loss[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int q = tid; q < a.n_groups; q += kBalanceThreads) {
-        int m = 0;
-        for (int c = 0; c < a.chunks; ++c) {
-            const float2 pz = a.part_z[(size_t)q * a.chunks + c];
-            m += __float_as_int(pz.x);
-            z += (double)pz.y;
+    term = wave_add(term);
+    // the last workgroup to come adds up the groups: what the others wrote for it they wrote past their caches
+    unsigned last = 0u;
+    if (lane == 0) {
+        if (blockIdx.x == 0) {
+            a.n_valid[g] = n;
+            __hip_atomic_store(&a.group[g].x, (double)n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(&a.group[g].y, z, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        total += m;
-        filled += m > 0;
+        __hip_atomic_store(&a.part_loss[(size_t)g * gridDim.x + blockIdx.x], term, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
     }
-    loss = block_sum(loss, s_t);
-    z = block_sum(z, s_t);
-    total = block_sum(total, s_i);
-    filled = block_sum(filled, s_i);
-    if (tid == 0) {
-        a.losses[0] = filled ? (float)(loss / (double)filled) : 0.0f;
-        a.losses[1] = total ? (float)(z / (double)total) : 0.0f;
-        a.n_valid[a.n_groups] = total;
-        a.n_valid[a.n_groups + 1] = filled;
+    last = (unsigned)__builtin_amdgcn_readfirstlane((int)last);
+    if (last != gridDim.x * gridDim.y - 1u) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    double loss = 0.0, total = 0.0, filled = 0.0;
+    z = 0.0;
+    for (int i = lane; i < (int)(gridDim.x * gridDim.y); i += 64)
+        loss += __hip_atomic_load(&a.part_loss[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int q = lane; q < a.n_groups; q += 64) {
+        const double m = __hip_atomic_load(&a.group[q].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        z += __hip_atomic_load(&a.group[q].y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        total += m;
+        filled += m > 0.0 ? 1.0 : 0.0;
+    }
+    loss = wave_add(loss);
+    z = wave_add(z);
+    total = wave_add(total);
+    filled = wave_add(filled);
+    if (lane == 0) {
+        a.losses[0] = filled > 0.0 ? (float)(loss / filled) : 0.0f;
+        a.losses[1] = total > 0.0 ? (float)(z / total) : 0.0f;
+        a.n_valid[a.n_groups] = (int)total;
+        a.n_valid[a.n_groups + 1] = (int)filled;
     }
 }
 
@@ -268,55 +353,64 @@ struct RouteBackArgs {
     unsigned int* err;
 };
 
-template <int PER, int W>
+// The selected experts' parts meet the row in LDS: a lane adds up the parts of its slot's expert in slot order
+// (an expert may be named twice), the expert's first slot stores the sum, and the row's lanes pick theirs up.
+template <int PER, int VEC, int W>
 __global__ __launch_bounds__(row_threads(W)) void k_route_backward(RouteBackArgs a) {
+    constexpr int kSide = row_threads(W) / (64 * W);
     __shared__ float s_tmp[W];
-    const int tid = (int)threadIdx.x, v = tid % (64 * W), E = a.n_experts;
-    const int t = (int)blockIdx.x * (row_threads(W) / (64 * W)) + tid / (64 * W);
+    __shared__ float s_add[kSide][64 * W * PER];
+    const int tid = (int)threadIdx.x, v = tid % (64 * W), side = tid / (64 * W), slot = tid & 63, E = a.n_experts;
+    const int t = (int)blockIdx.x * kSide + side;
     if (t >= a.n_tokens) return;                            // W = 1: whole waves leave, and no barrier follows
+    const uint8_t* row = a.logits + (size_t)t * a.stride;
     float* out = reinterpret_cast<float*>(a.dlogits + (size_t)t * a.dstride);
     float p[PER], d[PER], lse = 0.0f;
-    bool live = !(a.mask && !a.mask[t]);
-    if (live) {
-        row_load<PER, W>(a.logits + (size_t)t * a.stride, E, v, p);
+    int counts[PER], id = -1;
+    float w = 0.0f, l = -__builtin_inff(), n_g = 0.0f, n = 0.0f, filled = 0.0f;
+    bool live = !(a.mask && !a.mask[t]), bad = false;
+    if (live) {                                             // every load before the first result is needed
+        row_load<PER, VEC, W>(row, E, v, -__builtin_inff(), p);
+        if (a.dw && slot < a.n_used) {
+            id = a.ids[(size_t)t * a.n_used + slot];
+            w = a.dw[(size_t)t * a.n_used + slot];
+        }
+        if (a.counts) {
+            const int g = t / a.group_len;
+            row_load<PER, VEC, W>(a.counts + (size_t)g * E, E, v, 0, counts);
+            n_g = (float)a.n_valid[g], n = (float)a.n_valid[a.n_groups], filled = (float)a.n_valid[a.n_groups + 1];
+        }
+        if (a.dw && slot < a.n_used) {
+            bad = id < 0 || id >= E;
+            if (bad) {
+                *reinterpret_cast<volatile unsigned int*>(a.err) = kErrRouteId;
+                w = __builtin_nanf("");                     // the row becomes NaN
+                id = -1;
+            } else {
+                l = reinterpret_cast<const float*>(row)[id];
+            }
+        }
         live = row_softmax<PER, W>(p, lse, s_tmp);
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) d[j] = 0.0f;
     if (live && a.counts) {
-        const int g = t / a.group_len;
-        const float n_g = (float)a.n_valid[g], n = (float)a.n_valid[a.n_groups], filled = (float)a.n_valid[a.n_groups + 1];
         const float cb = a.c_balance * (float)E / (n_g * filled), fs = 1.0f / (n_g * (float)a.n_used);
         const float cz = 2.0f * a.c_z * lse / n;
         float dot = 0.0f;
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (v + 64 * W * j < E) {
-                d[j] = (float)a.counts[(size_t)g * E + v + 64 * W * j] * fs;
-                dot += d[j] * p[j];
-            }
+        for (int j = 0; j < PER; ++j) {
+            d[j] = (float)counts[j] * fs;
+            dot += d[j] * p[j];
+        }
         dot = row_sum<W>(dot, s_tmp);
 #pragma unroll
         for (int j = 0; j < PER; ++j) d[j] = p[j] * (cb * (d[j] - dot) + cz);
     }
     if (live && a.dw) {
-        int id = -1;
-        float w = 0.0f, l = -__builtin_inff();
-        const int slot = v & 63;                            // every wave of the row holds the slots
-        if (slot < a.n_used) {
-            id = a.ids[(size_t)t * a.n_used + slot];
-            w = a.dw[(size_t)t * a.n_used + slot];
-            if (id < 0 || id >= E) {
-                *reinterpret_cast<volatile unsigned int*>(a.err) = kErrRouteId;
-                id = -1;
-                w = __builtin_nanf("");                     // the row becomes NaN
-            } else {
-                l = reinterpret_cast<const float*>(a.logits + (size_t)t * a.stride)[id];
-            }
-        }
-        // the selected experts' shares, lane j with slot j
+        // the selected experts' shares, lane j with slot j (every wave of the row holds the slots)
         const float m = a.norm_w ? row_max<1>(l, s_tmp) : lse;
-        float q = slot < a.n_used && l > -__builtin_inff() ? expf(l - m) : 0.0f;
+        float q = slot < a.n_used && l > -__builtin_inff() ? row_exp(l - m) : 0.0f;
         if (l != l) q = l;
         if (a.norm_w) {
             const float s = row_sum<1>(q, s_tmp);
@@ -328,17 +422,38 @@ __global__ __launch_bounds__(row_threads(W)) void k_route_backward(RouteBackArgs
 #pragma unroll
             for (int j = 0; j < PER; ++j) d[j] -= a.w_scale * p[j] * dot;
         }
-        for (int k = 0; k < a.n_used; ++k) {                // in slot order: an expert named twice gets both
-            const int ik = __builtin_amdgcn_readlane(id, k);
+        float sum = 0.0f;
+        bool first = id >= 0;
+        for (int k = 0; k < a.n_used; ++k) {
+            const bool same = __builtin_amdgcn_readlane(id, k) == id;
             const float ak = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(add), k));
-#pragma unroll
-            for (int j = 0; j < PER; ++j)
-                if (v + 64 * W * j == ik) d[j] += ak;
+            sum += same ? ak : 0.0f;
+            first = first && !(same && k < slot);
         }
+        float* mine = s_add[side];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) mine[row_expert<VEC, W>(v, j)] = 0.0f;
+        if constexpr (W > 1) __syncthreads();
+        __builtin_amdgcn_wave_barrier();
+        if (first && tid % (64 * W) < 64) mine[id] = sum;
+        if constexpr (W > 1) __syncthreads();
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < PER; ++j) d[j] += mine[row_expert<VEC, W>(v, j)];
     }
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-        if (v + 64 * W * j < E) out[v + 64 * W * j] = d[j];
+    for (int j = 0; j < PER; j += VEC) {
+        const int i = row_expert<VEC, W>(v, j);
+        if (i + VEC <= E) {
+            if constexpr (VEC == 4) *reinterpret_cast<rf4*>(out + i) = rf4{d[j], d[j + 1], d[j + 2], d[j + 3]};
+            else if constexpr (VEC == 2) *reinterpret_cast<rf2*>(out + i) = rf2{d[j], d[j + 1]};
+            else out[i] = d[j];
+        } else {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c)
+                if (i + c < E) out[i + c] = d[j + c];
+        }
+    }
 }
 
 }  // namespace sabah

@@ -425,7 +425,7 @@ __device__ inline uint32_t lora_split2(float (&v)[2]) {
 constexpr int kLoraPart = 17;                 // floats of part per rank
 constexpr int kLoraXLds = 16 * 9;             // of a wave: 16 rows of 128 bytes, 144 apart: no bank conflicts either way
 template <typename W>
-constexpr int kLoraALds = sizeof(typename W::T) == 4 ? 16 * 9 : 16 * 5;   // rows of 128 or 64 bytes
+constexpr int kLoraALds = sizeof(typename W::T) == 4 ? 16 * 9 : 16 * 4;   // rows of 128 bytes, or of 64 with their quarters exchanged
 template <typename W, int NR, int NW, int U>
 struct LoraShrink {
     static constexpr int CH = sizeof(typename W::T) / 2;    // loads of 16 bytes for 16 rows of A
@@ -500,9 +500,9 @@ struct LoraShrink {
         __builtin_amdgcn_wave_barrier();
     }
     __device__ inline lf4 turn_rows64(lf4* lds, const lf4& in) const {
-        lds[(lane >> 2) * 5 + (lane & 3)] = in;
+        lds[(lane & ~3) + ((lane & 3) ^ ((lane >> 3) & 3))] = in;           // row lane / 4
         __builtin_amdgcn_wave_barrier();
-        const lf4 v = lds[p * 5 + q];
+        const lf4 v = lds[4 * p + (q ^ ((p >> 1) & 3))];
         __builtin_amdgcn_wave_barrier();
         return v;
     }
@@ -519,19 +519,26 @@ struct LoraShrink {
             if constexpr (std::is_same<W, LoraF16>::value) scale = lora_scale_of(lora_column_most(here), back);
             LoraWords P[kLoraPieces<W>];
             lora_split(W{}, v, scale, P);
+            LoraWords w[NR];
 #pragma unroll
-            for (int b = 0; b < NR; ++b) {
-                const LoraWords w = __builtin_bit_cast(LoraWords, turn_rows64(la, in.a[b][0]));
-                if constexpr (std::is_same<W, LoraF16>::value) {
-                    lf4 d = {0, 0, 0, 0};
+            for (int b = 0; b < NR; ++b) w[b] = __builtin_bit_cast(LoraWords, turn_rows64(la, in.a[b][0]));
+            if constexpr (std::is_same<W, LoraF16>::value) {
+                lf4 d[NR];
 #pragma unroll
-                    for (int g = kLoraPieces<W> - 1; g >= 0; --g) d = lora_mfma(W{}, w, P[g], d);
+                for (int b = 0; b < NR; ++b) d[b] = lf4{0, 0, 0, 0};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[b][i] = __builtin_fmaf(d[i], back, acc[b][i]);
-                } else {
+                for (int g = kLoraPieces<W> - 1; g >= 0; --g)
 #pragma unroll
-                    for (int g = kLoraPieces<W> - 1; g >= 0; --g) acc[b] = lora_mfma(W{}, w, P[g], acc[b]);
-                }
+                    for (int b = 0; b < NR; ++b) d[b] = lora_mfma(W{}, w[b], P[g], d[b]);
+#pragma unroll
+                for (int b = 0; b < NR; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[b][i] = __builtin_fmaf(d[b][i], back, acc[b][i]);
+            } else {
+#pragma unroll
+                for (int g = kLoraPieces<W> - 1; g >= 0; --g)
+#pragma unroll
+                    for (int b = 0; b < NR; ++b) acc[b] = lora_mfma(W{}, w[b], P[g], acc[b]);
             }
         } else {
 #pragma unroll
@@ -776,22 +783,25 @@ struct LoraExpand {
             lf4 d[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
             if constexpr (N > 0) {
 #pragma unroll
-                for (int b = 0; b < NP; ++b)
+                for (int b = 0; b < NP; ++b) {
+                    LoraWords w[4];
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
-                        LoraWords w;
                         if constexpr (NR == 1) {
                             const uint2 r = __builtin_bit_cast(uint2, in.w[h][0]);
-                            w = LoraWords{{r.x, r.y, 0, 0}};
+                            w[h] = LoraWords{{r.x, r.y, 0, 0}};
                         } else {
-                            w = __builtin_bit_cast(LoraWords, in.w[h][b]);
+                            w[h] = __builtin_bit_cast(LoraWords, in.w[h][b]);
                         }
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
-                            if (4 * b + c < 2 * NR) w.u[c] &= mask[(4 * b + c) % (4 * NR / M)];
-#pragma unroll
-                        for (int g = N - 1; g >= 0; --g) d[h] = lora_mfma(W{}, P[b][g], w, d[h]);
+                            if (4 * b + c < 2 * NR) w[h].u[c] &= mask[(4 * b + c) % (4 * NR / M)];
                     }
+#pragma unroll
+                    for (int g = N - 1; g >= 0; --g)
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) d[h] = lora_mfma(W{}, P[b][g], w[h], d[h]);
+                }
                 if constexpr (std::is_same<W, LoraF16>::value) {
 #pragma unroll
                     for (int h = 0; h < 4; ++h)
@@ -995,23 +1005,27 @@ __global__ __launch_bounds__(256) void k_lora_transpose(LoraTurn a) {
     const int n = of_a ? a.k : a.rows, c0 = 64 * ((int)blockIdx.x - (of_a ? 0 : a.tiles_a)), m = min(64, n - c0);
     const T* in = static_cast<const T*>(of_a ? a.a : a.b) + (size_t)key * rank * n;
     T* out = static_cast<T*>(of_a ? a.at : a.bt) + (size_t)key * rank * n;
+    // i / rank for i below 64 * rank, exactly: the reciprocal is too large by less than 2^-20, i below 2^13
+    const uint32_t inv = ((1u << 20) + rank - 1) / rank;
+    auto over = [&](int i) { return (int)(((uint32_t)i * inv) >> 20); };
     constexpr int U = 8;                                    // loads at a time
     for (int i0 = (int)threadIdx.x; i0 < 64 * rank; i0 += 256 * U) {
         T v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = min(i0 + 256 * u, 64 * rank - 1), c = min(of_a ? i & 63 : i / rank, m - 1), r = of_a ? i >> 6 : i % rank;
+            const int i = min(i0 + 256 * u, 64 * rank - 1), j = over(i), c = min(of_a ? i & 63 : j, m - 1), r = of_a ? i >> 6 : i - j * rank;
             v[u] = in[of_a ? (size_t)r * n + c0 + c : (size_t)(c0 + c) * rank + r];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + 256 * u;
-            if (i < 64 * rank) s[(of_a ? i & 63 : i / rank) * pitch + (of_a ? i >> 6 : i % rank)] = v[u];
+            const int i = i0 + 256 * u, j = over(min(i, 64 * rank - 1));
+            if (i < 64 * rank) s[(of_a ? i & 63 : j) * pitch + (of_a ? i >> 6 : i - j * rank)] = v[u];
         }
     }
     __syncthreads();
+#pragma unroll 4
     for (int i = (int)threadIdx.x; i < 64 * rank; i += 256) {
-        const int c = of_a ? i / rank : i & 63, r = of_a ? i % rank : i >> 6;
+        const int j = over(i), c = of_a ? j : i & 63, r = of_a ? i - j * rank : i >> 6;
         if (c < m) out[of_a ? (size_t)(c0 + c) * rank + r : (size_t)r * n + c0 + c] = s[c * pitch + r];
     }
 }
@@ -1045,14 +1059,19 @@ __device__ inline void lora_grad_store(const LoraGrad& g, int side, int key, int
     }
 }
 
-// The splits that have rows of the key, a bit each (at most 32); a wave asks
-__device__ inline uint32_t lora_grad_splits(const LoraGrad& g, int key) {
+// The splits that have rows of the key, a bit each (at most 32); a wave asks.  first: the lane's run of the first 64 windows
+__device__ inline uint32_t lora_grad_splits(const LoraGrad& g, int key, uint32_t& first) {
     const int lane = (int)threadIdx.x & 63;
     uint32_t used = 0;
-    for (int w = lane; w < g.windows; w += 64) used |= (g.runs[(size_t)w * g.keys + key] != 0u ? 1u : 0u) << (w % g.splits);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) used |= (uint32_t)__shfl_xor((int)used, o);
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)used);
+    first = 0;
+    for (int w = lane; w < g.windows; w += 64) {
+        const uint32_t r = g.runs[(size_t)w * g.keys + key];
+        if (w == lane) first = r;
+        used |= (r != 0u ? 1u : 0u) << (w % g.splits);
+    }
+    uint32_t all = 0;
+    for (int z = 0; z < g.splits; ++z) all |= (__ballot((used >> z) & 1u) ? 1u : 0u) << z;
+    return all;
 }
 
 // dA or dB of one key and 64 columns: rank blocks of 16 by columns, summed over the key's tiles, two (32 rows) per
@@ -1064,22 +1083,24 @@ __device__ inline uint32_t lora_grad_splits(const LoraGrad& g, int key) {
 // grid (column tiles, keys, splits)
 template <int NR, int OCC>
 __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
-    __shared__ float sum[4][16 * 64];
+    constexpr int RB = NR < 4 ? NR : 4;                     // rank blocks summed at a time
+    __shared__ float sum[4][RB * 16 * 64];
     const int lane = (int)threadIdx.x & 63, p = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int side = (int)blockIdx.x < g.tiles_a ? 0 : 1, tile = (int)blockIdx.x - (side ? g.tiles_a : 0), c0 = 64 * tile;
     const int key = (int)blockIdx.y, split = (int)blockIdx.z, n = g.width[side], col = c0 + 4 * p;
-    const uint32_t used = g.splits > 1 ? lora_grad_splits(g, key) : 1u;
+    uint32_t e;
+    const uint32_t used = lora_grad_splits(g, key, e);
     if (!((used >> split) & 1u) && !(used == 0u && split == 0)) return;     // a key without rows: split 0 writes its zeros
     lf4 acc[NR][4];
 #pragma unroll
     for (int b = 0; b < NR; ++b)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[b][j] = lf4{0, 0, 0, 0};
-    // the key's tiles in pairs, every fourth this wave's: windows split, split + splits, ..., 64 at a time
-    int wb = split - 64 * g.splits, left = 0, turn = -1;
-    uint64_t some = 0;
-    uint32_t e = 0;
+    // the key's tiles in pairs, every fourth this wave's, 64 windows at a time
+    auto own = [&](int w) { return w < g.windows && w % g.splits == split; };
+    int wb = 0, left = 0, turn = -1;
+    uint64_t some = __ballot(e != 0u && own(lane));
     size_t at = 0;
     auto advance = [&](size_t& slot, bool& two) {
         for (;;) {
@@ -1093,21 +1114,25 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
                 continue;
             }
             while (some == 0) {
-                wb += 64 * g.splits;
+                wb += 64;
                 if (wb >= g.windows) return false;
-                const int w = wb + lane * g.splits;
-                e = w < g.windows ? g.runs[(size_t)w * g.keys + key] : 0u;
+                e = own(wb + lane) ? g.runs[(size_t)(wb + lane) * g.keys + key] : 0u;
                 some = __ballot(e != 0u);
             }
             const int l = __builtin_ctzll(some);
             some &= some - 1ull;
             const uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)e, l);
             left = ((int)(r >> 16) + kLoraTile - 1) / kLoraTile;
-            at = (size_t)(wb + l * g.splits) * g.slots + (r & 0xFFFFu);
+            at = (size_t)(wb + l) * g.slots + (r & 0xFFFFu);
         }
     };
-    auto load = [&](lf4 (&x)[8], size_t slot, bool two) {
-        const uint64_t* off = g.off[side] + (slot + (two && q > 1 ? 1 : 0)) * 16 + 8 * (q & 1);
+    auto tile_of = [&](size_t slot, bool two) { return slot + (two && q > 1 ? 1 : 0); };
+    auto load_off = [&](uint64_t (&off)[8], size_t slot, bool two) {
+        const uint64_t* o = g.off[side] + tile_of(slot, two) * 16 + 8 * (q & 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) off[i] = o[i];
+    };
+    auto load_x = [&](lf4 (&x)[8], const uint64_t (&off)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float* row = reinterpret_cast<const float*>(g.src[side] + off[i]);
@@ -1119,7 +1144,25 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
             }
         }
     };
-    auto mul = [&](const lf4 (&x)[8], size_t slot, bool two) {
+    lf4 x[8];
+    uint64_t off[8];
+    size_t slot = 0, slot2 = 0;
+    bool two = false, two2 = false, more = advance(slot, two);
+    if (more) {
+        load_off(off, slot, two);
+        load_x(x, off);
+    }
+    while (more) {
+        // this step's pieces and the next one's offsets; x to pieces; the next x, under the products
+        more = advance(slot2, two2);
+        const uint16_t* pieces = g.p[side] + tile_of(slot, two) * (768 * NR) + 16 * p + 8 * (q & 1);
+        constexpr int UB = NR < 4 ? NR : 4;
+        LoraWords U[UB][3];
+#pragma unroll
+        for (int b = 0; b < UB; ++b)
+#pragma unroll
+            for (int z = 0; z < 3; ++z) U[b][z] = *reinterpret_cast<const LoraWords*>(pieces + z * (256 * NR) + 256 * b);
+        if (more) load_off(off, slot2, two2);
         LoraWords X[4][3];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -1129,62 +1172,53 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
 #pragma unroll
                 for (int z = 0; z < 3; ++z) X[j][z].u[c] = lora_split2(v);
             }
-        const bool none = !two && q > 1;                    // a lone tile: the other 16 rows count nothing
-        const uint16_t* pieces = g.p[side] + (slot + (two && q > 1 ? 1 : 0)) * (768 * NR) + 16 * p + 8 * (q & 1);
+        if (more) load_x(x, off);
+        const uint32_t keep = !two && q > 1 ? 0u : 0xFFFFFFFFu;     // a lone tile: the other 16 rows count nothing
 #pragma unroll
         for (int b = 0; b < NR; ++b) {
-            LoraWords U[3];
+            LoraWords V[3];
 #pragma unroll
             for (int z = 0; z < 3; ++z) {
-                U[z] = *reinterpret_cast<const LoraWords*>(pieces + z * (256 * NR) + 256 * b);
+                V[z] = U[b % UB][z];
+                if (b + UB < NR) U[b % UB][z] = *reinterpret_cast<const LoraWords*>(pieces + z * (256 * NR) + 256 * (b + UB));
 #pragma unroll
-                for (int c = 0; c < 4; ++c) U[z].u[c] = none ? 0u : U[z].u[c];
+                for (int c = 0; c < 4; ++c) V[z].u[c] &= keep;
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int lo = 2; lo >= 0; --lo)                 // the smallest products first; four sums in turn
 #pragma unroll
-                for (int lo = 2; lo >= 0; --lo)             // the smallest products first
+                for (int z = 0; z <= lo; ++z)
 #pragma unroll
-                    for (int z = 0; z <= lo; ++z) acc[b][j] = lora_mfma(LoraBF16{}, U[z], X[j][lo - z], acc[b][j]);
+                    for (int j = 0; j < 4; ++j) acc[b][j] = lora_mfma(LoraBF16{}, V[z], X[j][lo - z], acc[b][j]);
         }
-    };
-    lf4 x[8];
-    size_t slot = 0;
-    bool two = false, more = advance(slot, two);
-    if (more) load(x, slot, two);
-    while (more) {
-        lf4 y[8];
-        size_t slot2 = 0;
-        bool two2 = false;
-        more = advance(slot2, two2);
-        if (more) load(y, slot2, two2);
-        mul(x, slot, two);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = y[i];
         slot = slot2;
         two = two2;
     }
     const bool whole = (used & (used - 1u)) == 0u;          // no other split has rows
-    for (int b = 0; b < NR && 16 * b < g.rank; ++b) {
+#pragma unroll
+    for (int b0 = 0; b0 < NR; b0 += RB) {
+        if (16 * b0 >= g.rank) break;
+        if (b0) __syncthreads();
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<lf4*>(&sum[wave][b * 1024 + (4 * q + i) * 64 + 4 * p]) =
+                    lf4{acc[b0 + b][0][i], acc[b0 + b][1][i], acc[b0 + b][2][i], acc[b0 + b][3][i]};
         __syncthreads();
+        lf4* to = reinterpret_cast<lf4*>(sum[0]);
+        if (!whole) to = reinterpret_cast<lf4*>(g.part[side] + ((((size_t)split * g.keys + key) * ((n + 63) / 64) + tile) * NR + b0) * (16 * 64));
 #pragma unroll
-        for (int bb = 0; bb < NR; ++bb)
-            if (bb == b) {
+        for (int b = 0; b < RB; ++b) {
+            const int o = (int)threadIdx.x + 256 * b;
+            lf4 v = reinterpret_cast<const lf4*>(sum[0])[o];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<lf4*>(&sum[wave][(4 * q + i) * 64 + 4 * p]) = lf4{acc[bb][0][i], acc[bb][1][i], acc[bb][2][i], acc[bb][3][i]};
-            }
-        __syncthreads();
-        float* to = sum[0];
-        if (!whole) to = g.part[side] + ((((size_t)split * g.keys + key) * ((n + 63) / 64) + tile) * NR + b) * (16 * 64);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int o = (int)threadIdx.x + 256 * i;
-            to[o] = ((sum[0][o] + sum[1][o]) + sum[2][o]) + sum[3][o];
+            for (int w = 1; w < 4; ++w) v += reinterpret_cast<const lf4*>(sum[w])[o];
+            to[o] = v;
         }
         if (whole) {
             __syncthreads();
-            lora_grad_store(g, side, key, b, c0, sum[0]);
+            for (int b = 0; b < RB && 16 * (b0 + b) < g.rank; ++b) lora_grad_store(g, side, key, b0 + b, c0, sum[0] + 1024 * b);
         }
     }
 }
@@ -1195,7 +1229,8 @@ __global__ __launch_bounds__(256) void k_lora_grad_sum(LoraGrad g) {
     __shared__ float sum[16 * 64];
     const int side = (int)blockIdx.x < g.tiles_a ? 0 : 1, tile = (int)blockIdx.x - (side ? g.tiles_a : 0);
     const int key = (int)blockIdx.y, b = (int)blockIdx.z, tiles = (g.width[side] + 63) / 64;
-    const uint32_t used = lora_grad_splits(g, key);
+    uint32_t e;
+    const uint32_t used = lora_grad_splits(g, key, e);
     if ((used & (used - 1u)) == 0u) return;                 // written by its only split
     lf4 v = {0, 0, 0, 0};
     for (uint32_t left = used; left; left &= left - 1u)
