@@ -89,13 +89,19 @@ __device__ inline float row_sum(float v, float* tmp) {
     return row_reduce<W>(v, tmp, [](float a, float b) { return a + b; });
 }
 
-// exp by the hardware's 2^x: the argument's product with log2 e is rounded, |x| 2^-24 of the result
-__device__ inline float row_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+// exp(x) as 2^(x log2 e), with the rest that the product's rounding and log2 e's own leave out as a factor 1 + rest ln 2
+__device__ inline float row_exp(float x) {
+    constexpr float kLog2e = 1.44269502162933349609375f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147182f;
+    const float t = x * kLog2e, rest = __builtin_fmaf(x, kLog2eRest, __builtin_fmaf(x, kLog2e, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return t > -126.0f && t < 126.0f ? __builtin_fmaf(e, rest * kLn2, e) : e;   // past them e is 0 or infinite, and x may be
+}
 
-// The softmax of a row: e becomes p.  Returns false for a row of minus infinities only.
+// The softmax of a row: e becomes p; m, inv: the row's largest logit, and p is exp(l - m) inv.  Returns false for a row of
+// minus infinities only.
 template <int PER, int W>
-__device__ inline bool row_softmax(float (&e)[PER], float& lse, float* tmp) {
-    float m = -__builtin_inff();
+__device__ inline bool row_softmax(float (&e)[PER], float& m, float& inv, float& lse, float* tmp) {
+    m = -__builtin_inff();
     bool nan = false;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -112,7 +118,7 @@ __device__ inline bool row_softmax(float (&e)[PER], float& lse, float* tmp) {
         s += e[j];
     }
     s = row_sum<W>(s, tmp);
-    const float inv = m == __builtin_inff() ? __builtin_nanf("") : 1.0f / s;
+    inv = m == __builtin_inff() ? __builtin_nanf("") : 1.0f / s;
 #pragma unroll
     for (int j = 0; j < PER; ++j) e[j] *= inv;
     lse = m + logf(s);
@@ -190,8 +196,8 @@ __global__ __launch_bounds__(row_threads(W)) void k_balance_rows(BalanceArgs a) 
         }
 #pragma unroll
         for (int b = 0; b < B; ++b) {
-            float lse;
-            if (!live[b] || !row_softmax<PER, W>(e[b], lse, s_tmp)) continue;
+            float m, inv, lse;
+            if (!live[b] || !row_softmax<PER, W>(e[b], m, inv, lse, s_tmp)) continue;
 #pragma unroll
             for (int j = 0; j < PER; ++j) acc[j] += e[b][j];
             z += lse * lse;
@@ -365,7 +371,7 @@ __global__ __launch_bounds__(row_threads(W)) void k_route_backward(RouteBackArgs
     if (t >= a.n_tokens) return;                            // W = 1: whole waves leave, and no barrier follows
     const uint8_t* row = a.logits + (size_t)t * a.stride;
     float* out = reinterpret_cast<float*>(a.dlogits + (size_t)t * a.dstride);
-    float p[PER], d[PER], lse = 0.0f;
+    float p[PER], d[PER], top = 0.0f, inv = 0.0f, lse = 0.0f;
     int counts[PER], id = -1;
     float w = 0.0f, l = -__builtin_inff(), n_g = 0.0f, n = 0.0f, filled = 0.0f;
     bool live = !(a.mask && !a.mask[t]), bad = false;
@@ -390,7 +396,7 @@ __global__ __launch_bounds__(row_threads(W)) void k_route_backward(RouteBackArgs
                 l = reinterpret_cast<const float*>(row)[id];
             }
         }
-        live = row_softmax<PER, W>(p, lse, s_tmp);
+        live = row_softmax<PER, W>(p, top, inv, lse, s_tmp);
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) d[j] = 0.0f;
@@ -409,9 +415,10 @@ __global__ __launch_bounds__(row_threads(W)) void k_route_backward(RouteBackArgs
     }
     if (live && a.dw) {
         // the selected experts' shares, lane j with slot j (every wave of the row holds the slots)
-        const float m = a.norm_w ? row_max<1>(l, s_tmp) : lse;
+        const float m = a.norm_w ? row_max<1>(l, s_tmp) : top;
         float q = slot < a.n_used && l > -__builtin_inff() ? row_exp(l - m) : 0.0f;
         if (l != l) q = l;
+        if (!a.norm_w) q *= inv;
         if (a.norm_w) {
             const float s = row_sum<1>(q, s_tmp);
             q = s > 0.0f || s != s ? q / s : 0.0f;

@@ -62,6 +62,7 @@ class MoEExecutor:
         self.bank = bank
         self.shared = shared
         self.device = bank.device
+        self._index = bank.storage.get_device()
         self.d_model = bank.d_model
         self.ff = bank.d_ff
         self.max_used = max_used
@@ -145,38 +146,46 @@ class MoEExecutor:
         return out
 
     # ---- adapters beside a projection --------------------------------------------
+    # These calls too wait for what Python does before the launch: shapes and strides are read once, and devices
+    # compared as numbers.
     def _lora_rows(self, lora: LoraBank, x: torch.Tensor, adapters: torch.Tensor, ids: torch.Tensor | None,
                    y: torch.Tensor | None):
         """The checks that the two calls share; (tokens, slots, C arguments of x, adapters and ids).
         y: a tensor with the output's shape [T, rows] or [T, n_ids, rows], if there is one."""
-        T = adapters.shape[0]
-        slots = ids.shape[1] if ids is not None else y.shape[1] if y is not None and y.dim() == 3 else 1
-        xs, xr = x.stride(), x.shape[1] if x.dim() == 3 else 1
-        if (x.dtype != torch.float32 or x.shape[-1] != lora.k or (xs[-1] != 1 and T) or x.shape[0] != T or xr not in (1, slots)
-                or adapters.dtype != torch.int32 or not adapters.is_contiguous() or x.dim() not in (2, 3)):
-            raise ValueError("adapters: x %s %s for %d values, adapters %s %s"
-                             % (tuple(x.shape), x.dtype, lora.k, tuple(adapters.shape), adapters.dtype))
-        if x.device != self.device or adapters.device != self.device or lora.a.device != self.device:
-            raise ValueError("adapters: the tensors are not on %s" % self.device)
-        if ids is None:
+        shape, xs, dev = x.shape, x.stride(), self._index
+        T, k = shape[0], lora.k
+        if len(shape) == 3:
+            xr, xi = shape[1], xs[1] * 4
+        else:
+            xr, xi = 1, 0
+        if ids is not None:
+            slots, ns = ids.shape[1], ids.stride()
+            if ids.dtype is not torch.int32 or ids.shape[0] != T or ids.get_device() != dev:
+                raise ValueError("adapters: ids %s %s for %d tokens" % (tuple(ids.shape), ids.dtype, T))
+            ids_args = ids.data_ptr(), ns[1] * 4, ns[0] * 4
+        else:
+            slots = y.shape[1] if y is not None and len(y.shape) == 3 else 1
             if lora.n_experts != 1:
                 raise ValueError("adapters of %d experts need ids" % lora.n_experts)
-            return T, slots, (x.data_ptr(), xs[1] * 4 if x.dim() == 3 else 0, xr, xs[0] * 4, adapters.data_ptr(),
-                              None, 0, 0, slots, T)
-        if ids.dtype != torch.int32 or ids.shape[0] != T or ids.device != self.device:
-            raise ValueError("adapters: ids %s %s for %d tokens" % (tuple(ids.shape), ids.dtype, T))
-        ns = ids.stride()
-        return T, slots, (x.data_ptr(), xs[1] * 4 if x.dim() == 3 else 0, xr, xs[0] * 4, adapters.data_ptr(),
-                          ids.data_ptr(), ns[1] * 4, ns[0] * 4, slots, T)
+            ids_args = None, 0, 0
+        if (x.dtype is not torch.float32 or shape[-1] != k or (xs[-1] != 1 and T) or (xr != 1 and xr != slots)
+                or len(shape) > 3 or adapters.dtype is not torch.int32 or adapters.shape != (T,)
+                or not adapters.is_contiguous()):
+            raise ValueError("adapters: x %s %s for %d values, adapters %s %s"
+                             % (tuple(shape), x.dtype, k, tuple(adapters.shape), adapters.dtype))
+        if x.get_device() != dev or adapters.get_device() != dev or lora.index != dev:
+            raise ValueError("adapters: the tensors are not on %s" % self.device)
+        return T, slots, (x.data_ptr(), xi, xr, xs[0] * 4, adapters.data_ptr(), *ids_args, slots, T)
 
     def _lora_y(self, what: str, y: torch.Tensor, T: int, slots: int, width: int):
         """(address, slot stride, token stride) of rows [T, width] or [T, slots, width] f32."""
-        s = y.stride()
-        if (y.dtype != torch.float32 or (s[-1] != 1 and T) or y.device != self.device
-                or tuple(y.shape) not in ((T, slots, width),) + (((T, width),) if slots == 1 else ())):
+        shape, s = y.shape, y.stride()
+        three = len(shape) == 3
+        if (y.dtype is not torch.float32 or (s[-1] != 1 and T) or y.get_device() != self._index
+                or shape != ((T, slots, width) if three or slots != 1 else (T, width))):
             raise ValueError("adapters: %s is %s %s, expected f32 [%d, %d, %d] with contiguous rows on %s"
-                             % (what, tuple(y.shape), y.dtype, T, slots, width, self.device))
-        return y.data_ptr(), s[1] * 4 if y.dim() == 3 else 0, s[0] * 4
+                             % (what, tuple(shape), y.dtype, T, slots, width, self.device))
+        return (y.data_ptr(), s[1] * 4, s[0] * 4) if three else (y.data_ptr(), 0, s[0] * 4)
 
     def lora_apply(self, lora: LoraBank, x: torch.Tensor, adapters: torch.Tensor, base: torch.Tensor | None = None,
                    ids: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -189,11 +198,13 @@ class MoEExecutor:
             out = (torch.empty_like(base) if base is not None else
                    torch.empty((T, lora.rows) if x.dim() == 2 and ids is None else (T, slots, lora.rows),
                                dtype=torch.float32, device=self.device))
-        b = self._lora_y("base", base, T, slots, lora.rows) if base is not None else (None, 0, 0)
-        n = rt.lib().sabah_lora_workspace(lora.ref, slots, T, 0)
-        ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
-        rc = rt.lib().sabah_lora_apply(lora.ref, *rows, *b, *self._lora_y("out", out, T, slots, lora.rows),
-                                       ws.data_ptr() if n else None, n, _stream(self.device))
+        y = self._lora_y("out", out, T, slots, lora.rows)
+        b = y if base is out else self._lora_y("base", base, T, slots, lora.rows) if base is not None else (None, 0, 0)
+        lib = rt.lib()
+        ws, n = None, lora.space(lib, slots, T)
+        if n:
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        rc = lib.sabah_lora_apply(lora.ref, *rows, *b, *y, ws.data_ptr() if n else None, n, _stream(self.device))
         if rc:
             rt.check(rc, "lora_apply")
         return out
@@ -220,7 +231,7 @@ class MoEExecutor:
                     raise ValueError("lora_backward: a weight gradient is %s %s, expected contiguous f32 %s"
                                      % (tuple(g.shape), g.dtype, tuple(w.shape)))
         d = self._lora_y("dx", dx, T, slots, lora.k) if need_dx else (None, 0, 0)
-        n = rt.lib().sabah_lora_workspace(lora.ref, slots, T, 1)
+        n = lora.space(rt.lib(), slots, T, 1)
         ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
         rc = rt.lib().sabah_lora_backward(lora.ref, *rows, *self._lora_y("dy", dy, T, slots, lora.rows), *d,
                                           int(add_dx), da.data_ptr() if need_dw else None,
@@ -258,12 +269,13 @@ class MoEExecutor:
 
     def _router_rows(self, logits: torch.Tensor, ids: torch.Tensor, mask: torch.Tensor | None, n_groups: int):
         T, E = logits.shape
-        if (logits.dtype != torch.float32 or (logits.stride(1) != 1 and T) or logits.device != self.device
-                or ids.dtype != torch.int32 or ids.shape[0] != T or not ids.is_contiguous() or ids.device != self.device):
+        dev = self._index
+        if (logits.dtype is not torch.float32 or (logits.stride(1) != 1 and T) or logits.get_device() != dev
+                or ids.dtype is not torch.int32 or ids.shape[0] != T or not ids.is_contiguous() or ids.get_device() != dev):
             raise ValueError("router: logits %s %s, ids %s %s" % (tuple(logits.shape), logits.dtype, tuple(ids.shape),
                                                                  ids.dtype))
         if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.numel() != T
-                                 or not mask.is_contiguous() or mask.device != self.device):
+                                 or not mask.is_contiguous() or mask.get_device() != dev):
             raise ValueError("router: mask %s %s for %d tokens" % (tuple(mask.shape), mask.dtype, T))
         return T, E, ids.shape[1]
 
@@ -279,9 +291,12 @@ class MoEExecutor:
         T, E, k = self._router_rows(logits, ids, mask, n_groups)
         if out.n_experts != E:
             raise ValueError("balance: %d experts, out has %d" % (E, out.n_experts))
-        n = rt.lib().sabah_moe_balance_workspace(T, E, n_groups)
+        lib = rt.lib()
+        n = lib.sabah_moe_balance_workspace(T, E, n_groups)
+        if not n:
+            rt.check(-1, "moe_balance")
         ws = torch.empty(n, dtype=torch.uint8, device=self.device)
-        rc = rt.lib().sabah_moe_balance(logits.data_ptr(), logits.stride(0) * 4 if T > 1 else E * 4, ids.data_ptr(),
+        rc = lib.sabah_moe_balance(logits.data_ptr(), logits.stride(0) * 4 if T > 1 else E * 4, ids.data_ptr(),
                                         mask.data_ptr() if mask is not None else None, T, E, k, n_groups,
                                         out.counts.data_ptr(), out.mean_p.data_ptr(), out.losses.data_ptr(),
                                         out.n_valid.data_ptr(), ws.data_ptr(), n, _stream(self.device))
@@ -300,12 +315,13 @@ class MoEExecutor:
         T, E, k = self._router_rows(logits, ids, mask, n_groups)
         if balance is not None and balance.n_experts != E:
             raise ValueError("route_backward: %d experts, balance has %d" % (E, balance.n_experts))
-        if dw is not None and (dw.dtype != torch.float32 or dw.shape != ids.shape or not dw.is_contiguous()
-                               or dw.device != self.device):
+        if dw is not None and (dw.dtype is not torch.float32 or dw.shape != ids.shape or not dw.is_contiguous()
+                               or dw.get_device() != self._index):
             raise ValueError("route_backward: dw %s %s, ids %s" % (tuple(dw.shape), dw.dtype, tuple(ids.shape)))
         if out is None:
             out = torch.empty((T, E), dtype=torch.float32, device=self.device)
-        elif out.dtype != torch.float32 or out.shape != logits.shape or out.stride(1) != 1 or out.device != self.device:
+        elif (out.dtype is not torch.float32 or out.shape != logits.shape or out.stride(1) != 1
+              or out.get_device() != self._index):
             raise ValueError("route_backward: out %s %s" % (tuple(out.shape), out.dtype))
         rc = rt.lib().sabah_moe_route_backward(
             logits.data_ptr(), logits.stride(0) * 4 if T > 1 else E * 4, ids.data_ptr(), mask.data_ptr() if mask is not None else None,

@@ -46,6 +46,18 @@ class LoraBank:
         self.desc = rt.LoraDesc(self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), self.ranks.data_ptr(),
                                 TYPES[dtype], n_adapters, n_experts, rank, k, rows)
         self.ref = ctypes.byref(self.desc)
+        self.index = self.a.get_device()
+        self._space = {}
+
+    def space(self, lib, slots: int, tokens: int, backward: int = 0) -> int:
+        """sabah_lora_workspace of a call, asked once for each size."""
+        key = (slots, tokens, backward)
+        n = self._space.get(key)
+        if n is None:
+            if len(self._space) > 4096:
+                self._space.clear()
+            n = self._space[key] = lib.sabah_lora_workspace(self.ref, slots, tokens, backward)
+        return n
 
     def load(self, adapter: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
         """One adapter: a [r, k] and b [rows, r], or [n_experts, r, k] and [n_experts, rows, r],
