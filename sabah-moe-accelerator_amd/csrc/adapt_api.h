@@ -192,6 +192,9 @@ SABAH_API int sabah_moe_route_backward(const float* d_logits, size_t logits_stri
 // ---------------------------------------------------------------------------
 // adapters
 // ---------------------------------------------------------------------------
+template <int NR, int H>
+constexpr int kLoraExpandOcc = NR * H <= 2 ? 3 : NR <= 4 ? 2 : 1;   // waves per SIMD that the registers are kept to
+
 // type codes of adapter weights (ggml's F32, F16 and BF16)
 constexpr int kLoraMaxKeys = 1 << 21;         // (adapter, expert) pairs: a key and its row sort as one 32-bit word
 constexpr int kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 30;
@@ -216,7 +219,7 @@ static bool stride_ok(size_t s) { return s % 4 == 0; }
 // one tile per 16 rows and one more per key; the shrink's k in parts of at least eight steps
 // of 32 while there are few tiles, so that the launch fills the chip.
 constexpr int kLoraDirectRows = 256;
-constexpr int kLoraFusedTiles = 256;          // from here on a tile's shrink and expand in one workgroup
+constexpr int kLoraFusedRows = 4096;          // from here on a tile's shrink and expand in one workgroup
 constexpr int kLoraShrinkGroups = 1024, kLoraShrinkParts = 8, kLoraShrinkSteps = 8;
 constexpr int kLoraExpandGroups = 1024;
 // k of a shrink in parts while there are few tiles
@@ -237,23 +240,23 @@ static int lora_columns(int columns, int n_rows, int& cols) {
 
 struct LoraSpace {
     size_t order, items, n_items, s, bytes;
-    int windows, slots, key_bits, k_parts, k_steps, rank16;
+    int windows, slots, key_bits, k_parts, k_steps, rank16, tile;
 };
 static LoraSpace lora_space(const sabah_lora_desc* L, int n_rows) {
     LoraSpace s{};
     const int keys = L->n_adapters * L->n_experts + 2;      // without an adapter, and with a bad id
     const int span = std::min(n_rows, kLoraWindow);
     s.windows = (n_rows + kLoraWindow - 1) / kLoraWindow;
-    s.slots = std::min(span, span / kLoraTile + std::min(keys, span));
+    s.tile = n_rows > kLoraDirectRows && L->rank > 32 ? 32 : kLoraTile;
+    s.slots = std::min(span, span / s.tile + std::min(keys, span));
     s.rank16 = L->rank <= 16 ? 16 : L->rank <= 32 ? 32 : L->rank <= 64 ? 64 : 128;
     while (keys >> s.key_bits) ++s.key_bits;                // the word past the rows has key + 2 == keys
     if (n_rows <= kLoraDirectRows) {
         s.windows = 1;
         return s;
     }
-    const int tiles = (n_rows + kLoraTile - 1) / kLoraTile;
-    lora_k_parts(L->k, tiles, s.k_parts, s.k_steps);
-    const size_t positions = tiles < kLoraFusedTiles ? (size_t)s.windows * kLoraWindow : 0;
+    lora_k_parts(L->k, (n_rows + s.tile - 1) / s.tile, s.k_parts, s.k_steps);
+    const size_t positions = n_rows < kLoraFusedRows ? (size_t)s.windows * kLoraWindow : 0;
     s.items = align256((size_t)s.windows * kLoraWindow * 4);
     s.n_items = s.items + align256((size_t)s.windows * s.slots * 16);
     s.s = s.n_items + align256((size_t)s.windows * 4);
@@ -277,7 +280,7 @@ static LoraBackSpace lora_back_space(const sabah_lora_desc* L, int n_rows) {
     LoraBackSpace s{};
     const int keys = L->n_adapters * L->n_experts, span = std::min(n_rows, kLoraWindow);
     s.windows = std::max(1, (n_rows + kLoraWindow - 1) / kLoraWindow);
-    s.slots = std::max(1, std::min(span, span / kLoraTile + std::min(keys + 2, span)));
+    s.slots = std::max(1, std::min(span, span / 32 + std::min(keys + 2, span)));
     s.rank16 = L->rank <= 16 ? 16 : L->rank <= 32 ? 32 : L->rank <= 64 ? 64 : 128;
     while ((keys + 2) >> s.key_bits) ++s.key_bits;
     s.positions = s.windows * kLoraWindow;
@@ -300,10 +303,10 @@ static LoraBackSpace lora_back_space(const sabah_lora_desc* L, int n_rows) {
     s.u = take((size_t)s.positions * s.rank16 * 4);
     s.at = take((size_t)keys * L->rank * L->k * esize);
     s.bt = take((size_t)keys * L->rank * L->rows * esize);
-    s.ps = take(all * 3 * s.rank16 * 32);
-    s.pu = take(all * 3 * s.rank16 * 32);
-    s.ox = take(all * 16 * 8);
-    s.oy = take(all * 16 * 8);
+    s.ps = take(all * 3 * s.rank16 * 64);
+    s.pu = take(all * 3 * s.rank16 * 64);
+    s.ox = take(all * 32 * 8);
+    s.oy = take(all * 32 * 8);
     s.part = take(s.splits > 1 ? s.splits * part : 0);
     s.bytes = at;
     return s;
@@ -360,27 +363,27 @@ static int check_lora_rows(const char* what, const sabah_lora_desc* L, const flo
     return 0;
 }
 
-template <typename W, int NR, int NW, int US, int U, int OCC>
+template <typename W, int NR, int NW, int US, int U, int OCC, int H>
 static void launch_lora_apply_rank(const LoraArgs& a, const LoraTiles& t, int column_parts, int windows, hipStream_t st) {
     const dim3 grid((unsigned)t.slots, (unsigned)column_parts, (unsigned)windows);
     if (!t.order) {
-        hipLaunchKernelGGL((k_lora_apply<W, NR, NW, US, 1, true>), grid, dim3(64 * NW), 0, st, a, t);
+        hipLaunchKernelGGL((k_lora_apply<W, NR, NW, US, 1, 1, true>), grid, dim3(64 * NW), 0, st, a, t);
         return;
     }
     if (!t.s) {
-        hipLaunchKernelGGL((k_lora_apply<W, NR, 4, U, OCC, false>), grid, dim3(256), 0, st, a, t);
+        hipLaunchKernelGGL((k_lora_apply<W, NR, 4, U, OCC, H, false>), grid, dim3(256), 0, st, a, t);
         return;
     }
-    hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC>), dim3((unsigned)t.slots, (unsigned)t.k_parts, (unsigned)windows),
+    hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC, H>), dim3((unsigned)t.slots, (unsigned)t.k_parts, (unsigned)windows),
                        dim3(256), 0, st, a, t, a, t, windows);
-    hipLaunchKernelGGL((k_lora_expand<W, NR, std::min(OCC, 3)>), grid, dim3(256), 0, st, a, t);
+    hipLaunchKernelGGL((k_lora_expand<W, NR, kLoraExpandOcc<NR, H>, H>), grid, dim3(256), 0, st, a, t);
 }
 template <typename W>
 static void launch_lora_apply(const LoraArgs& a, const LoraTiles& t, int column_parts, int windows, hipStream_t st) {
-    if (a.rank <= 16) launch_lora_apply_rank<W, 1, 8, 4, 2, 4>(a, t, column_parts, windows, st);
-    else if (a.rank <= 32) launch_lora_apply_rank<W, 2, 8, 4, 2, 4>(a, t, column_parts, windows, st);
-    else if (a.rank <= 64) launch_lora_apply_rank<W, 4, 4, 2, 1, 2>(a, t, column_parts, windows, st);
-    else launch_lora_apply_rank<W, 8, 4, 1, 1, 1>(a, t, column_parts, windows, st);
+    if (a.rank <= 16) launch_lora_apply_rank<W, 1, 8, 4, 2, 4, 1>(a, t, column_parts, windows, st);
+    else if (a.rank <= 32) launch_lora_apply_rank<W, 2, 8, 4, 2, 4, 1>(a, t, column_parts, windows, st);
+    else if (a.rank <= 64) launch_lora_apply_rank<W, 4, 4, 2, 1, 2, 2>(a, t, column_parts, windows, st);
+    else launch_lora_apply_rank<W, 8, 4, 1, 1, 1, 2>(a, t, column_parts, windows, st);
 }
 
 SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, size_t x_id_stride, int x_rows,
@@ -425,7 +428,7 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
     if (sp.bytes) {
         uint8_t* ws = static_cast<uint8_t*>(d_workspace);
         const LoraGroup g{reinterpret_cast<int*>(ws + sp.order), reinterpret_cast<int4*>(ws + sp.items),
-                          reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, t.skip_none, sp.key_bits, nullptr};
+                          reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, t.skip_none, sp.key_bits, sp.tile, nullptr};
         hipLaunchKernelGGL(k_lora_group, dim3((unsigned)sp.windows),
                            dim3((unsigned)std::min(kLoraWindow, (n_rows + 63) / 64 * 64)), 0, st, a, g);
         if (!ck(hipGetLastError(), "adapters grouping launch")) return -1;
@@ -473,12 +476,12 @@ static int launch_lora_back_rank(const LoraBack& b) {
                        0, b.st, b.a, b.g);
     if (b.g.n_rows && (b.x.dst || b.grad_tiles)) {
         hipLaunchKernelGGL(k_lora_transpose<typename W::T>, dim3((unsigned)(sp.tiles_a + sp.tiles_b), keys), dim3(256), 0, b.st, b.turn);
-        hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC>), dim3(slots, 1u, windows * (b.grad_tiles ? 2u : 1u)), dim3(256), 0, b.st, b.u, b.tu, b.a, b.ts, (int)windows);
+        hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC, 2>), dim3(slots, 1u, windows * (b.grad_tiles ? 2u : 1u)), dim3(256), 0, b.st, b.u, b.tu, b.a, b.ts, (int)windows);
     }
     if (b.g.n_rows && b.x.dst) {
         LoraTiles t = b.tu;
         const int parts = lora_columns(b.x.rows, b.g.n_rows, t.cols);
-        hipLaunchKernelGGL((k_lora_expand<W, NR, std::min(OCC, 3)>), dim3(slots, (unsigned)parts, windows), dim3(256), 0, b.st, b.x, t);
+        hipLaunchKernelGGL((k_lora_expand<W, NR, kLoraExpandOcc<NR, 2>, 2>), dim3(slots, (unsigned)parts, windows), dim3(256), 0, b.st, b.x, t);
     }
     if (b.grad_tiles) {
         hipLaunchKernelGGL((k_lora_grad<NR, GOCC>), dim3((unsigned)b.grad_tiles, keys, (unsigned)b.w.splits), dim3(256), 0, b.st, b.w);
@@ -489,9 +492,9 @@ static int launch_lora_back_rank(const LoraBack& b) {
 }
 template <typename W>
 static int launch_lora_back(const LoraBack& b) {
-    if (b.a.rank <= 16) return launch_lora_back_rank<W, 1, 2, 4, 3>(b);
-    if (b.a.rank <= 32) return launch_lora_back_rank<W, 2, 2, 4, 2>(b);
-    if (b.a.rank <= 64) return launch_lora_back_rank<W, 4, 2, 3, 2>(b);
+    if (b.a.rank <= 16) return launch_lora_back_rank<W, 1, 2, 3, 3>(b);
+    if (b.a.rank <= 32) return launch_lora_back_rank<W, 2, 2, 3, 2>(b);
+    if (b.a.rank <= 64) return launch_lora_back_rank<W, 4, 1, 2, 2>(b);
     return launch_lora_back_rank<W, 8, 1, 1, 1>(b);
 }
 
@@ -544,7 +547,7 @@ SABAH_API int sabah_lora_backward(const sabah_lora_desc* lora, const float* d_x,
     b.x.base_id = dx_id_stride;
     b.x.base_tok = dx_token_stride;
     const LoraGroup g{reinterpret_cast<int*>(ws + sp.order), reinterpret_cast<int4*>(ws + sp.items),
-                      reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, !d_dx || add_dx, sp.key_bits,
+                      reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, !d_dx || add_dx, sp.key_bits, 32,
                       reinterpret_cast<uint32_t*>(ws + sp.runs)};
     b.g = g;
     LoraTiles t{};

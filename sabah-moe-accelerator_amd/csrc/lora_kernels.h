@@ -108,6 +108,8 @@ __device__ inline const float* lora_x(const LoraArgs& a, int row) {
 // (lora_tile, a thread for every row of the call); above, k_lora_group sorts each window of 1,024
 // rows by key and lists its tiles.
 // ---------------------------------------------------------------------------
+// A tile of the lists is one or two sixteens of rows (LoraGroup::tile), which share the reads of A and B: of
+// rank 64 these come from L2 at 16 rows a tile as fast as it gives (10.8 TB/s), while x and y take half the time.
 constexpr int kLoraTile = 16;
 constexpr int kLoraWindow = 1024;
 
@@ -120,8 +122,8 @@ struct LoraTiles {
     int cols;                     // columns of the output per workgroup
     float* s;                     // larger calls: [k_parts][positions][rank, in 16s]
     int k_parts, k_steps, positions;
-    uint16_t* pieces;             // backward, one k part: [windows * slots][3 pieces][rank, in 16s][16 rows] of s, or null
-    uint64_t* off;                // with pieces: [windows * slots][16], the rows' byte offsets in x
+    uint16_t* pieces;             // backward, one k part: [windows * slots][3 pieces][rank, in 16s][32 rows] of s, or null
+    uint64_t* off;                // with pieces: [windows * slots][32], the rows' byte offsets in x
     int scaled;                   // pieces of c s
 };
 
@@ -129,7 +131,7 @@ struct LoraGroup {
     int* order;
     int4* items;
     int* n_items;
-    int n_rows, slots, skip_none, key_bits;
+    int n_rows, slots, skip_none, key_bits, tile;
     uint32_t* runs;               // or [windows][keys]: a key's rows in the window << 16 | its first tile's slot, 0 without any
 };
 
@@ -190,10 +192,10 @@ __device__ inline uint32_t lora_sort(uint32_t c, int bits, LoraSort<NW>& f) {
     return c;
 }
 
-// In sorted order: every 16th row of a run of equal keys begins a tile.  The thread's tile, if it begins one
+// In sorted order: every 16th (or tile-th) row of a run of equal keys begins a tile.  The thread's tile, if it begins one
 // (its number of rows, else 0), and the tiles before it.
 template <int NW>
-__device__ inline int lora_leader(uint32_t c, LoraSort<NW>& f, int n_keys2, bool skip_none, int& slot, int* run = nullptr) {
+__device__ inline int lora_leader(uint32_t c, LoraSort<NW>& f, int n_keys2, bool skip_none, int& slot, int tile = kLoraTile, int* run = nullptr) {
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), nt = (int)blockDim.x;
     const uint32_t k2 = c >> 10;
     const uint64_t head = __ballot(tid == 0 || (f.c[max(tid - 1, 0)] >> 10) != k2);   // rows that begin a run
@@ -212,7 +214,7 @@ __device__ inline int lora_leader(uint32_t c, LoraSort<NW>& f, int n_keys2, bool
     for (int v = 0; v < NW; ++v) start = max(start, v < wave ? __builtin_amdgcn_readlane((int)last, v) : 0);
     if (upto) start = 64 * wave + 63 - __builtin_clzll(upto);
     const int end = after ? 64 * wave + __builtin_ctzll(after) : next ? 64 * wave + 64 + __builtin_ctzll(next) : nt;
-    const bool leader = (int)k2 < n_keys2 && ((tid - start) & (kLoraTile - 1)) == 0 && !(skip_none && (int)k2 == kLoraNone + 2);
+    const bool leader = (int)k2 < n_keys2 && ((tid - start) & (tile - 1)) == 0 && !(skip_none && (int)k2 == kLoraNone + 2);
     const uint64_t m = __ballot(leader);
     __syncthreads();
     if (lane == 0) f.w[wave].x = (uint32_t)__popcll(m);
@@ -228,7 +230,7 @@ __device__ inline int lora_leader(uint32_t c, LoraSort<NW>& f, int n_keys2, bool
             }
         *run = leader && tid == start ? stop - tid : 0;
     }
-    return leader ? min(kLoraTile, end - tid) : 0;          // a head two waves on is more than 16 rows away
+    return leader ? min(tile, end - tid) : 0;               // a head two waves on is more than a tile away
 }
 
 // One window per workgroup, a row per thread.  Without atomics: the same rows give the same tiles.
@@ -239,7 +241,7 @@ __global__ __launch_bounds__(kLoraWindow) void k_lora_group(LoraArgs a, LoraGrou
     if (g.runs)
         for (int i = tid; i < n_keys2 - 2; i += (int)blockDim.x) g.runs[(size_t)w * (n_keys2 - 2) + i] = 0u;
     int slot, run;
-    const int n = lora_leader(c, f, n_keys2, g.skip_none, slot, &run);     // its barriers order the zeros before the runs
+    const int n = lora_leader(c, f, n_keys2, g.skip_none, slot, g.tile, &run);     // its barriers order the zeros before the runs
     if (g.runs && run && (int)(c >> 10) >= 2)
         g.runs[(size_t)w * (n_keys2 - 2) + (c >> 10) - 2] = (uint32_t)run << 16 | (uint32_t)slot;
     if (n) g.items[(size_t)w * g.slots + slot] = make_int4((int)(c >> 10) - 2, w * kLoraWindow + tid, n, 0);
@@ -257,7 +259,8 @@ struct LoraFind {
 // The workgroup's tile: its key and number of rows, and the row of the lane's place
 // lane % 16 in it (the last one's again past the number).  False: no tile is left for it.
 template <int NW>
-__device__ inline bool lora_tile(const LoraArgs& a, const LoraTiles& t, LoraFind<NW>& f, int& key, int& n, int& row) {
+__device__ inline bool lora_tile(const LoraArgs& a, const LoraTiles& t, LoraFind<NW>& f, int& key, int& n, int (&rows)[1]) {
+    int& row = rows[0];
     const int tid = (int)threadIdx.x, p = tid & (kLoraTile - 1);
     if (t.n_rows == 1) {
         row = 0;
@@ -302,21 +305,24 @@ __device__ inline bool lora_tile(const LoraArgs& a, const LoraTiles& t, LoraFind
     return true;
 }
 
-// The same from the lists of k_lora_group, with the tile's position in order
-__device__ inline bool lora_item(const LoraTiles& t, int w, int& key, int& n, int& row, int& pos) {
+// The same from the lists of k_lora_group, with the tile's position in order; row[h]: of place 16 h + lane % 16
+template <int H>
+__device__ inline bool lora_item(const LoraTiles& t, int w, int& key, int& n, int (&row)[H], int& pos) {
     if ((int)blockIdx.x >= t.n_items[w]) return false;
     const int4 it = t.items[(size_t)w * t.slots + blockIdx.x];
     key = __builtin_amdgcn_readfirstlane(it.x);
     pos = __builtin_amdgcn_readfirstlane(it.y);
     n = __builtin_amdgcn_readfirstlane(it.z);
-    row = t.order[pos + min((int)threadIdx.x & (kLoraTile - 1), n - 1)];
+#pragma unroll
+    for (int h = 0; h < H; ++h) row[h] = t.order[pos + min(16 * h + ((int)threadIdx.x & 15), n - 1)];
     return true;
 }
 
 // columns c0 .. c1 of a tile whose rows have no adapter (a copy of base, or zeros) or a bad id (NaN)
-__device__ inline void lora_plain_rows(const LoraArgs& a, int key, int n, int row, int c0, int c1) {
+template <int H>
+__device__ inline void lora_plain_rows(const LoraArgs& a, int key, int n, const int (&row)[H], int c0, int c1) {
     for (int p = 0; p < n; ++p) {
-        const int r = __shfl(row, p);
+        const int r = __shfl(H == 1 || p < 16 ? row[0] : row[H - 1], p & 15);
         float* dst = reinterpret_cast<float*>(a.dst + lora_at(r, a.n_ids, a.dst_id, a.dst_tok));
         const float* base =
             a.base ? reinterpret_cast<const float*>(a.base + lora_at(r, a.n_ids, a.base_id, a.base_tok)) : nullptr;
@@ -426,29 +432,34 @@ constexpr int kLoraPart = 17;                 // floats of part per rank
 constexpr int kLoraXLds = 16 * 9;             // of a wave: 16 rows of 128 bytes, 144 apart: no bank conflicts either way
 template <typename W>
 constexpr int kLoraALds = sizeof(typename W::T) == 4 ? 16 * 9 : 16 * 4;   // rows of 128 bytes, or of 64 with their quarters exchanged
-template <typename W, int NR, int NW, int U>
+template <typename W, int NR, int NW, int U, int H>
 struct LoraShrink {
     static constexpr int CH = sizeof(typename W::T) / 2;    // loads of 16 bytes for 16 rows of A
     struct In {
-        lf4 x[2], a[NR][CH];
+        lf4 x[H][2], a[NR][CH];
     };
     const typename W::T* A;
-    const float* xr[2];
+    const float* xr[H][2];
     uint32_t at[NR][CH];                                    // elements; rank * k is below 2^28
     lf4 *lx, *la;                                           // the wave's
     int k, s0, steps, p, q, lane, rank;                     // whole steps s0 .. steps, and k's rest if steps is the last
-    float most = 0.0f;
+    bool second;                                            // the tile has more than 16 rows
+    float most[H];
+    lf4 acc[H][NR];
 
-    // row: of the lane's place lane % 16 in the tile; lds: NW * (kLoraXLds + kLoraALds<W>); of k the steps from s0 on, below s1
-    __device__ inline LoraShrink(const LoraArgs& a, const typename W::T* A_, int row, lf4* lds, int s0_, int s1)
-        : A(A_), k(a.k), s0(s0_), steps(min(s1, a.k / 32)), rank(a.rank) {
+    // row: of the lane's places lane % 16 in the tile of n rows; lds: NW * (kLoraXLds + kLoraALds<W>); of k the steps from s0
+    // on, below s1
+    __device__ inline LoraShrink(const LoraArgs& a, const typename W::T* A_, const int (&row)[H], int n, lf4* lds, int s0_, int s1)
+        : A(A_), k(a.k), s0(s0_), steps(min(s1, a.k / 32)), rank(a.rank), second(H > 1 && n > 16) {
         lane = (int)threadIdx.x & 63;
         p = lane & 15;
         q = lane >> 4;
         lx = lds + ((int)threadIdx.x >> 6) * (kLoraXLds + kLoraALds<W>);
         la = lx + kLoraXLds;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) xr[h] = lora_x(a, __shfl(row, 8 * h + (lane >> 3)));
+        for (int t = 0; t < H; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) xr[t][h] = lora_x(a, __shfl(row[t], 8 * h + (lane >> 3)));
 #pragma unroll
         for (int b = 0; b < NR; ++b)
 #pragma unroll
@@ -459,7 +470,11 @@ struct LoraShrink {
     __device__ inline int a_col() const { return CH == 1 ? 8 * (lane & 3) : 4 * (lane & 7); }
     __device__ inline void load(In& in, int s) const {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) in.x[h] = *reinterpret_cast<const lf4u*>(xr[h] + s * 32 + 4 * (lane & 7));
+        for (int t = 0; t < H; ++t)
+            if (t == 0 || second) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) in.x[t][h] = *reinterpret_cast<const lf4u*>(xr[t][h] + s * 32 + 4 * (lane & 7));
+            }
 #pragma unroll
         for (int b = 0; b < NR; ++b)
 #pragma unroll
@@ -473,9 +488,13 @@ struct LoraShrink {
         const int j = s * 32 + 4 * (lane & 7), i = s * 32 + a_col();
         constexpr int N = 16 / sizeof(typename W::T);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int t = 0; t < H; ++t)
+            if (t == 0 || second) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) in.x[h][c] = j + c < k ? xr[h][j + c] : 0.0f;
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) in.x[t][h][c] = j + c < k ? xr[t][h][j + c] : 0.0f;
+            }
 #pragma unroll
         for (int b = 0; b < NR; ++b)
 #pragma unroll
@@ -506,101 +525,127 @@ struct LoraShrink {
         __builtin_amdgcn_wave_barrier();
         return v;
     }
-    __device__ inline void mul(const In& in, lf4 (&acc)[NR]) {
-        lf4 t[2];
-        turn_rows128(lx, in.x, t);
+    __device__ inline void mul(const In& in) {
         if constexpr (kLoraPieces<W> > 0) {
-            float v[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) v[c] = t[c >> 2][c & 3];
-            const float here = lora_most(v, 0.0f);
-            most = fmaxf(most, here);
-            float back = 1.0f, scale = 1.0f;
-            if constexpr (std::is_same<W, LoraF16>::value) scale = lora_scale_of(lora_column_most(here), back);
-            LoraWords P[kLoraPieces<W>];
-            lora_split(W{}, v, scale, P);
             LoraWords w[NR];
 #pragma unroll
             for (int b = 0; b < NR; ++b) w[b] = __builtin_bit_cast(LoraWords, turn_rows64(la, in.a[b][0]));
-            if constexpr (std::is_same<W, LoraF16>::value) {
-                lf4 d[NR];
 #pragma unroll
-                for (int b = 0; b < NR; ++b) d[b] = lf4{0, 0, 0, 0};
+            for (int t = 0; t < H; ++t) {
+                if (t > 0 && !second) continue;
+                lf4 x[2];
+                turn_rows128(lx, in.x[t], x);
+                float v[8];
 #pragma unroll
-                for (int g = kLoraPieces<W> - 1; g >= 0; --g)
+                for (int c = 0; c < 8; ++c) v[c] = x[c >> 2][c & 3];
+                const float here = lora_most(v, 0.0f);
+                most[t] = fmaxf(most[t], here);
+                float back = 1.0f, scale = 1.0f;
+                if constexpr (std::is_same<W, LoraF16>::value) scale = lora_scale_of(lora_column_most(here), back);
+                LoraWords P[kLoraPieces<W>];
+                lora_split(W{}, v, scale, P);
+                if constexpr (std::is_same<W, LoraF16>::value) {
+                    lf4 d[NR];
 #pragma unroll
-                    for (int b = 0; b < NR; ++b) d[b] = lora_mfma(W{}, w[b], P[g], d[b]);
+                    for (int b = 0; b < NR; ++b) d[b] = lf4{0, 0, 0, 0};
 #pragma unroll
-                for (int b = 0; b < NR; ++b)
+                    for (int g = kLoraPieces<W> - 1; g >= 0; --g)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[b][i] = __builtin_fmaf(d[b][i], back, acc[b][i]);
-            } else {
+                        for (int b = 0; b < NR; ++b) d[b] = lora_mfma(W{}, w[b], P[g], d[b]);
 #pragma unroll
-                for (int g = kLoraPieces<W> - 1; g >= 0; --g)
+                    for (int b = 0; b < NR; ++b)
 #pragma unroll
-                    for (int b = 0; b < NR; ++b) acc[b] = lora_mfma(W{}, w[b], P[g], acc[b]);
+                        for (int i = 0; i < 4; ++i) acc[t][b][i] = __builtin_fmaf(d[b][i], back, acc[t][b][i]);
+                } else {
+#pragma unroll
+                    for (int g = kLoraPieces<W> - 1; g >= 0; --g)
+#pragma unroll
+                        for (int b = 0; b < NR; ++b) acc[t][b] = lora_mfma(W{}, w[b], P[g], acc[t][b]);
+                }
             }
         } else {
+            lf4 x[H][2];
+#pragma unroll
+            for (int t = 0; t < H; ++t)
+                if (t == 0 || second) turn_rows128(lx, in.x[t], x[t]);
 #pragma unroll
             for (int b = 0; b < NR; ++b) {
                 lf4 w[2];
                 turn_rows128(la, in.a[b], w);
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[c >> 2][c & 3], t[c >> 2][c & 3], acc[b], 0, 0, 0);
+                for (int t = 0; t < H; ++t) {
+                    if (t > 0 && !second) continue;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        acc[t][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[c >> 2][c & 3], x[t][c >> 2][c & 3], acc[t][b], 0, 0, 0);
+                }
             }
         }
     }
-    // part as above
-    __device__ inline void run(float* part) {
+    __device__ inline void run() {
         const int wave = (int)threadIdx.x >> 6;
-        lf4 acc[NR];
 #pragma unroll
-        for (int b = 0; b < NR; ++b) acc[b] = lf4{0, 0, 0, 0};
+        for (int t = 0; t < H; ++t) {
+            most[t] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NR; ++b) acc[t][b] = lf4{0, 0, 0, 0};
+        }
         In in[U];
         for (int s = s0 + wave; s < steps; s += U * NW) {
 #pragma unroll
             for (int u = 0; u < U; ++u) load(in[u], min(s + u * NW, steps - 1));
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (s + u * NW < steps) mul(in[u], acc);
+                if (s + u * NW < steps) mul(in[u]);
         }
-        const bool rest = rest_is(wave);
-        if (rest) {
+        if (rest_is(wave)) {
             load_rest(in[0], steps);
-            mul(in[0], acc);
+            mul(in[0]);
         }
+    }
+    // part as above, of sixteen t of the tile
+    __device__ inline void give(float* part, int t) const {
+        const int wave = (int)threadIdx.x >> 6;
         float* mine = part + (size_t)wave * 16 * NR * kLoraPart;
+        float big = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NR; ++b)
+        for (int h = 0; h < H; ++h) {
+            if (h != t) continue;
+            big = most[h];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mine[(16 * b + 4 * q + i) * kLoraPart + p] = acc[b][i];
+            for (int b = 0; b < NR; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mine[(16 * b + 4 * q + i) * kLoraPart + p] = acc[h][b][i];
+        }
         if constexpr (kLoraPieces<W> > 0) {
-            if (__any(most == __builtin_inff())) plain(mine, lora_big_rows(most), wave, rest);
+            if (__any(big == __builtin_inff())) plain(mine, lora_big_rows(big), t, wave);
         }
     }
     // k's rest belongs to the wave whose turn it is after the last whole step of all
     __device__ inline bool rest_is(int wave) const {
         return steps == k / 32 && k % 32 != 0 && (steps - s0) % NW == wave;
     }
-    // rare: the tile's rows in `rows` with plain products, over the wave's own share of k
-    __device__ inline void plain(float* mine, unsigned rows, int wave, bool rest) const {
+    // rare: rows of sixteen t with plain products, over the wave's own share of k
+    __device__ inline void plain(float* mine, unsigned rows, int t, int wave) const {
         __builtin_amdgcn_wave_barrier();
-        for (int t = 0; t < 16; ++t) {
-            const uint64_t at_lo = (uint64_t)(uintptr_t)xr[t >> 3];     // lane 8 (t % 8) holds row t's address
+        for (int i = 0; i < 16; ++i) {
+            uint64_t at = 0;                                // lane 8 (i % 8) holds row i's address
+#pragma unroll
+            for (int h = 0; h < 2 * H; ++h)
+                if (h == 2 * t + (i >> 3)) at = (uint64_t)(uintptr_t)xr[h >> 1][h & 1];
             const float* x = reinterpret_cast<const float*>(
-                (uintptr_t)((uint64_t)(uint32_t)__shfl((int)(uint32_t)at_lo, 8 * (t & 7)) |
-                            (uint64_t)(uint32_t)__shfl((int)(uint32_t)(at_lo >> 32), 8 * (t & 7)) << 32));
-            if (!((rows >> t) & 1u)) continue;
+                (uintptr_t)((uint64_t)(uint32_t)__shfl((int)(uint32_t)at, 8 * (i & 7)) |
+                            (uint64_t)(uint32_t)__shfl((int)(uint32_t)(at >> 32), 8 * (i & 7)) << 32));
+            if (!((rows >> i) & 1u)) continue;
             for (int r = 0; r < rank; ++r) {
                 float sum = 0.0f;
-                for (int s = s0 + wave; s < steps + (rest ? 1 : 0); s += NW) {
-                    const int i = s * 32 + (lane & 31);
-                    if (lane < 32 && i < k) sum = __builtin_fmaf(W::value(A[(size_t)r * k + i]), x[i], sum);
+                for (int s = s0 + wave; s < steps + (rest_is(wave) ? 1 : 0); s += NW) {
+                    const int c = s * 32 + (lane & 31);
+                    if (lane < 32 && c < k) sum = __builtin_fmaf(W::value(A[(size_t)r * k + c]), x[c], sum);
                 }
 #pragma unroll
                 for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
-                if (lane == 0) mine[r * kLoraPart + t] = sum;
+                if (lane == 0) mine[r * kLoraPart + i] = sum;
             }
         }
     }
@@ -627,31 +672,30 @@ __device__ inline bool lora_value_counts(int j, int rank, int rk) {
     const int r = lora_value_at<NR>(j, rank);
     return r >= j / kLoraGroupWidth<NR> * kLoraGroupWidth<NR> && r < rk;
 }
-template <typename W, int NR, int NW>
+template <typename W, int NR, int NW, int H, bool STREAM>
 struct LoraExpand {
     static constexpr int GW = kLoraGroupWidth<NR>, NG = 4 * NR / GW;
     typedef typename std::conditional<NR == 1, typename W::V4, typename W::V8>::type V;
-    struct In {
-        V w[4][NG];
-        lf4 y[4];
-    };
     const typename W::T* B;                                 // rows * rank is below 2^28
-    const uint8_t* base[4];                                 // of the lane's four rows; base[0] null: zeros
-    uint8_t* dst[4];
-    int rank, rows, c1, p, q, at[NG];
+    const uint8_t* base[H][4];                              // of the lane's four rows of each sixteen; null: zeros
+    uint8_t* dst[H][4];
+    int rank, rows, c1, n, p, q, at[NG];
+    bool based;
 
-    // row: of the lane's place lane % 16 in the tile
-    __device__ inline LoraExpand(const LoraArgs& a, const typename W::T* B_, int row, int c1_)
-        : B(B_), rank(a.rank), rows(a.rows), c1(c1_) {
+    // row: of the lane's places lane % 16 in the tile of n rows
+    __device__ inline LoraExpand(const LoraArgs& a, const typename W::T* B_, const int (&row)[H], int n_, int c1_)
+        : B(B_), rank(a.rank), rows(a.rows), c1(c1_), n(n_), based(a.base != nullptr) {
         const int lane = (int)threadIdx.x & 63;
         p = lane & 15;
         q = lane >> 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = __shfl(row, 4 * q + i);
-            base[i] = a.base ? a.base + lora_at(r, a.n_ids, a.base_id, a.base_tok) : nullptr;
-            dst[i] = a.dst + lora_at(r, a.n_ids, a.dst_id, a.dst_tok);
-        }
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = __shfl(row[h], 4 * q + i);
+                base[h][i] = a.base ? a.base + lora_at(r, a.n_ids, a.base_id, a.base_tok) : nullptr;
+                dst[h][i] = a.dst + lora_at(r, a.n_ids, a.dst_id, a.dst_tok);
+            }
 #pragma unroll
         for (int g = 0; g < NG; ++g) at[g] = min(4 * NR * q + GW * g, max(0, rank - GW));
     }
@@ -660,11 +704,7 @@ struct LoraExpand {
         const int r = at[j / GW] + j % GW;
         return ~(uint32_t)(((r - (4 * NR * q + j / GW * GW)) | (rk - 1 - r)) >> 31);
     }
-    __device__ inline void load(In& in, int o0) const {
-        load_y(in, o0);
-        load_w(in, o0);
-    }
-    __device__ inline void load_w(In& in, int o0) const {
+    __device__ inline void load_w(V (&w)[4][NG], int o0) const {
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
             const typename W::T* row = B + (uint32_t)min(o0 + 4 * p + h, rows - 1) * (uint32_t)rank;
@@ -673,43 +713,46 @@ struct LoraExpand {
                 if constexpr (NR == 1) {
                     if (rank < 4) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) W::set(in.w[h][g], c, row[min(c, rank - 1)]);
+                        for (int c = 0; c < 4; ++c) W::set(w[h][g], c, row[min(c, rank - 1)]);
                     } else {
-                        in.w[h][g] = W::load4(row + at[g]);
+                        w[h][g] = W::load4(row + at[g]);
                     }
                 } else {
-                    in.w[h][g] = W::load8(row + at[g]);
+                    w[h][g] = W::load8(row + at[g]);
                 }
             }
         }
     }
-    __device__ inline void load_y(In& in, int o0) const {
+    __device__ inline void load_y(lf4 (&y)[4], int t, int o0) const {
         const int o = o0 + 4 * p;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            in.y[i] = lf4{0, 0, 0, 0};
-            if (!base[0]) continue;
-            const float* b = reinterpret_cast<const float*>(base[i]) + o;
+            y[i] = lf4{0, 0, 0, 0};
+            if (!based) continue;
+            const float* b = reinterpret_cast<const float*>(base[t][i]) + o;
             if (o + 4 <= c1) {
-                in.y[i] = *reinterpret_cast<const lf4u*>(b);
+                y[i] = *reinterpret_cast<const lf4u*>(b);
             } else {
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    if (o + c < c1) in.y[i][c] = b[c];
+                    if (o + c < c1) y[i][c] = b[c];
             }
         }
     }
-    __device__ inline void store(const In& in, const lf4 (&d)[4], int o0, unsigned rows_in) const {
+    // Streamed past the caches in large calls: their output does not fit there, and A and B, which the other tiles read again,
+    // stay (16,384 rows at rank 32: 82 us against 97)
+    __device__ inline void store(const lf4 (&in)[4], const lf4 (&d)[4], int t, int o0, unsigned rows_in) const {
         const int o = o0 + 4 * p;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (!((rows_in >> (4 * q + i)) & 1u)) continue;
             lf4 y;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = in.y[i][j] + d[j][i];
-            float* b = reinterpret_cast<float*>(dst[i]) + o;
+            for (int j = 0; j < 4; ++j) y[j] = in[i][j] + d[j][i];
+            float* b = reinterpret_cast<float*>(dst[t][i]) + o;
             if (o + 4 <= c1) {
-                *reinterpret_cast<lf4u*>(b) = y;
+                if constexpr (STREAM) __builtin_nontemporal_store(y, reinterpret_cast<lf4u*>(b));
+                else *reinterpret_cast<lf4u*>(b) = y;
             } else {
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
@@ -717,8 +760,8 @@ struct LoraExpand {
             }
         }
     }
-    // rare: 64 columns of row t of the tile with plain products
-    __device__ inline void plain(const float (&s)[4 * NR], int rk, int o0, int t) const {
+    // rare: 64 columns of row t of sixteen x of the tile with plain products
+    __device__ inline void plain(const float (&s)[4 * NR], int rk, int o0, int x, int t) const {
         const int lane = (int)threadIdx.x & 63, o = o0 + lane;
         float sum = 0.0f;
         for (int r = 0; r < rk; ++r) {
@@ -733,7 +776,7 @@ struct LoraExpand {
         uint64_t to = 0, from = 0;                          // lane 16 (t / 4) holds the row's addresses
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i == (t & 3)) to = (uint64_t)(uintptr_t)dst[i], from = (uint64_t)(uintptr_t)base[i];
+            if (i == (t & 3)) to = (uint64_t)(uintptr_t)dst[x][i], from = (uint64_t)(uintptr_t)base[x][i];
         auto there = [&](uint64_t a) {
             return (uintptr_t)((uint64_t)(uint32_t)__shfl((int)(uint32_t)a, 16 * (t >> 2)) |
                                (uint64_t)(uint32_t)__shfl((int)(uint32_t)(a >> 32), 16 * (t >> 2)) << 32);
@@ -742,15 +785,8 @@ struct LoraExpand {
         const float* b = reinterpret_cast<const float*>(there(from));
         if (o < c1) y[o] = b ? b[o] + sum : sum;
     }
-    // The wave's steps from o0 on.  s: the lane's S, already scaled, zeros where a value does not count; n: the
-    // tile's rows
-    __device__ inline void run(int o0, const float (&s)[4 * NR], int rk, int n) const {
-        unsigned rows_in = (1u << n) - 1u, alone = 0u;
-        if constexpr (kLoraPieces<W> > 0) {
-            const float most = lora_most(s, 0.0f);
-            if (__any(most == __builtin_inff())) alone = lora_big_rows(most) & rows_in;
-            rows_in &= ~alone;
-        }
+    // The wave's steps from o0 on.  s: the lane's S, already scaled, zeros where a value does not count
+    __device__ inline void run(int o0, const float (&s)[H][4 * NR], int rk) const {
         constexpr int NP = (NR + 1) / 2, N = kLoraPieces<W>, M = N > 0 ? 2 : 1;   // products of 32 ranks, pieces, values of a mask
         uint32_t mask[4 * NR / M];
 #pragma unroll
@@ -759,67 +795,89 @@ struct LoraExpand {
             else mask[j] = counts(j, rk);
             asm volatile("" : "+v"(mask[j]));               // kept as a word
         }
-        LoraWords P[NP][N > 0 ? N : 1];
-        float back[4] = {1.0f, 1.0f, 1.0f, 1.0f};           // of the lane's four rows
-        if constexpr (N > 0) {
-            float scale = 1.0f;
-            if constexpr (std::is_same<W, LoraF16>::value) {
-                float mine;
-                scale = lora_scale_of(lora_column_most(lora_most(s, 0.0f)), mine);
+        unsigned rows_in[H], alone[H];                      // the rows to be written here, and those with an infinity in s
+        LoraWords P[H][NP][N > 0 ? N : 1];
+        float back[H][4];                                   // of the lane's four rows
 #pragma unroll
-                for (int i = 0; i < 4; ++i) back[i] = __shfl(mine, 4 * q + i);
-            }
+        for (int t = 0; t < H; ++t) {
+            rows_in[t] = (unsigned)((1u << max(0, min(16, n - 16 * t))) - 1u);
+            alone[t] = 0u;
 #pragma unroll
-            for (int b = 0; b < NP; ++b) {
-                float v[8];
+            for (int i = 0; i < 4; ++i) back[t][i] = 1.0f;
+            if constexpr (N > 0) {
+                const float most = lora_most(s[t], 0.0f);
+                if (__any(most == __builtin_inff())) alone[t] = lora_big_rows(most) & rows_in[t];
+                rows_in[t] &= ~alone[t];
+                float scale = 1.0f;
+                if constexpr (std::is_same<W, LoraF16>::value) {
+                    float mine;
+                    scale = lora_scale_of(lora_column_most(most), mine);
 #pragma unroll
-                for (int c = 0; c < 8; ++c) v[c] = 8 * b + c < 4 * NR ? s[(8 * b + c) % (4 * NR)] : 0.0f;
-                lora_split(W{}, v, scale, P[b]);
+                    for (int i = 0; i < 4; ++i) back[t][i] = __shfl(mine, 4 * q + i);
+                }
+#pragma unroll
+                for (int b = 0; b < NP; ++b) {
+                    float v[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) v[c] = 8 * b + c < 4 * NR ? s[t][(8 * b + c) % (4 * NR)] : 0.0f;
+                    lora_split(W{}, v, scale, P[t][b]);
+                }
             }
         }
         for (; o0 < c1; o0 += 64 * NW) {
-            In in;
-            load(in, o0);
-            lf4 d[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+            V w[4][NG];
+            lf4 y[H][4];
+#pragma unroll
+            for (int t = 0; t < H; ++t)
+                if (t == 0 || n > 16 * t) load_y(y[t], t, o0);
+            load_w(w, o0);
+            LoraWords ww[NP][4];                            // 16-bit weights: the operands
             if constexpr (N > 0) {
 #pragma unroll
-                for (int b = 0; b < NP; ++b) {
-                    LoraWords w[4];
+                for (int b = 0; b < NP; ++b)
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         if constexpr (NR == 1) {
-                            const uint2 r = __builtin_bit_cast(uint2, in.w[h][0]);
-                            w[h] = LoraWords{{r.x, r.y, 0, 0}};
+                            const uint2 r = __builtin_bit_cast(uint2, w[h][0]);
+                            ww[b][h] = LoraWords{{r.x, r.y, 0, 0}};
                         } else {
-                            w[h] = __builtin_bit_cast(LoraWords, in.w[h][b]);
+                            ww[b][h] = __builtin_bit_cast(LoraWords, w[h][b]);
                         }
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
-                            if (4 * b + c < 2 * NR) w[h].u[c] &= mask[(4 * b + c) % (4 * NR / M)];
-                    }
-#pragma unroll
-                    for (int g = N - 1; g >= 0; --g)
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) d[h] = lora_mfma(W{}, P[b][g], w[h], d[h]);
-                }
-                if constexpr (std::is_same<W, LoraF16>::value) {
-#pragma unroll
-                    for (int h = 0; h < 4; ++h)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) d[h][i] *= back[i];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4 * NR; ++j)
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        const float w = __uint_as_float(__float_as_uint(W::get(in.w[h][j / GW], j % GW)) & mask[j % (4 * NR / M)]);
-                        d[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[j], w, d[h], 0, 0, 0);
+                            if (4 * b + c < 2 * NR) ww[b][h].u[c] &= mask[(4 * b + c) % (4 * NR / M)];
                     }
             }
-            store(in, d, o0, rows_in);
-            if constexpr (N > 0) {
-                for (unsigned left = alone; left; left &= left - 1u) plain(s, rk, o0, __builtin_ctz(left));
+#pragma unroll
+            for (int t = 0; t < H; ++t) {
+                if (t > 0 && n <= 16 * t) continue;
+                lf4 d[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+                if constexpr (N > 0) {
+#pragma unroll
+                    for (int b = 0; b < NP; ++b)
+#pragma unroll
+                        for (int g = N - 1; g >= 0; --g)
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) d[h] = lora_mfma(W{}, P[t][b][g], ww[b][h], d[h]);
+                    if constexpr (std::is_same<W, LoraF16>::value) {
+#pragma unroll
+                        for (int h = 0; h < 4; ++h)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) d[h][i] *= back[t][i];
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4 * NR; ++j)
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const float v = __uint_as_float(__float_as_uint(W::get(w[h][j / GW], j % GW)) & mask[j % (4 * NR / M)]);
+                            d[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[t][j], v, d[h], 0, 0, 0);
+                        }
+                }
+                store(y[t], d, t, o0, rows_in[t]);
+                if constexpr (N > 0) {
+                    for (unsigned left = alone[t]; left; left &= left - 1u) plain(s[t], rk, o0, t, __builtin_ctz(left));
+                }
             }
         }
     }
@@ -854,12 +912,12 @@ __device__ inline const typename W::T* lora_b(const LoraArgs& a, int key) {
 // waits for.  Large ones, with tiles to fill the chip, take them from the lists, and hold OCC
 // waves per SIMD to cover the loads: 96 us where the two kernels take 108 (16,384 rows, rank 32,
 // 2048 x 2048).  grid (slots, column parts, windows).
-template <typename W, int NR, int NW, int U, int OCC, bool FIND>
+template <typename W, int NR, int NW, int U, int OCC, int H, bool FIND>
 __global__ __launch_bounds__(64 * NW, OCC) void k_lora_apply(LoraArgs a, LoraTiles t) {
     __shared__ float part[NW * 16 * NR * kLoraPart];
     __shared__ lf4 turn[NW * (kLoraXLds + kLoraALds<W>)];
     __shared__ typename std::conditional<FIND, LoraFind<NW>, int>::type find;
-    int key, n, row, pos;
+    int key, n, row[H], pos;
     if constexpr (FIND) {
         if (!lora_tile<NW>(a, t, find, key, n, row)) return;
     } else {
@@ -872,75 +930,87 @@ __global__ __launch_bounds__(64 * NW, OCC) void k_lora_apply(LoraArgs a, LoraTil
     }
     const int rk = lora_rank(a, key);
     const float c = lora_scale(a, key);
-    LoraShrink<W, NR, NW, U>(a, lora_a<W>(a, key), row, turn, 0, 1 << 28).run(part);
-    __syncthreads();
-    if (o0 >= c1) return;
-    const LoraExpand<W, NR, NW> E(a, lora_b<W>(a, key), row, c1);
-    float s[4 * NR];
-    lora_sum_parts<NR, NW>(E, part, rk, c, s);
-    E.run(o0, s, rk, n);
+    LoraShrink<W, NR, NW, U, H> S(a, lora_a<W>(a, key), row, n, turn, 0, 1 << 28);
+    S.run();
+    const LoraExpand<W, NR, NW, H, !FIND> E(a, lora_b<W>(a, key), row, n, c1);
+    float s[H][4 * NR];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        if (h) __syncthreads();
+        S.give(part, h);
+        __syncthreads();
+        lora_sum_parts<NR, NW>(E, part, rk, c, s[h]);
+    }
+    E.run(o0, s, rk);
 }
 
 // Larger calls: S = X A^T of a tile and one part of k per workgroup, to t.s, [k parts][position in order][16 NR]
 // in all, a tile of n rows as the expand reads it: [4 NR groups of four values][n rows][4] of every lane's values in
 // lora_value_at's order (zeros where one does not count), so that its loads are whole lines.  grid (slots, k parts, windows).
-template <typename W, int NR, int U>
+template <typename W, int NR, int U, int H>
 __device__ inline void lora_shrink_part(const LoraArgs& a, const LoraTiles& t, int w, float* part, lf4* turn) {
     constexpr int NW = 4;
-    int key, n, row, pos;
+    int key, n, row[H], pos;
     if ((int)blockIdx.y >= t.k_parts || !lora_item(t, w, key, n, row, pos) || key < 0) return;
-    const int s0 = (int)blockIdx.y * t.k_steps;
-    LoraShrink<W, NR, NW, U>(a, lora_a<W>(a, key), row, turn, s0, s0 + t.k_steps).run(part);
-    __syncthreads();
+    const int s0 = (int)blockIdx.y * t.k_steps, rk = lora_rank(a, key);
+    LoraShrink<W, NR, NW, U, H> S(a, lora_a<W>(a, key), row, n, turn, s0, s0 + t.k_steps);
+    S.run();
     float* out = t.s + ((size_t)blockIdx.y * t.positions + pos) * (16 * NR);
-    const int rk = lora_rank(a, key);
-    for (int i = (int)threadIdx.x; i < 16 * 16 * NR; i += 256) {
-        const int j = i / 16, p = i % 16, r = lora_value_at<NR>(j, a.rank);     // value j of the 16 NR, row p
-        float v = 0.0f;
-#pragma unroll
-        for (int w4 = 0; w4 < NW; ++w4) v += part[(w4 * 16 * NR + r) * kLoraPart + p];
-        if (p < n) out[((j >> 2) * n + p) * 4 + (j & 3)] = lora_value_counts<NR>(j, a.rank, rk) ? v : 0.0f;
-    }
-    if (!t.pieces) return;
-    // As the weights' gradients read it: in bf16 pieces, a rank's rows side by side, zeros past the tile's rows and the
-    // adapter's rank; and where the rows of x are (past the last row, the last)
     const size_t slot = (size_t)w * t.slots + blockIdx.x;
-    if (threadIdx.x < 16) {
-        const int tok = row / a.n_ids;
-        t.off[slot * 16 + threadIdx.x] = (uint64_t)tok * a.x_tok + (uint64_t)((row - tok * a.n_ids) % a.x_rows) * a.x_id;
-    }
     const float c = t.scaled ? lora_scale(a, key) : 1.0f;
-    for (int i = (int)threadIdx.x; i < 16 * 8 * NR; i += 256) {
-        const int r = i / 8, p = 2 * (i % 8);               // two rows at a time
-        float v[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-            if (p + e < n && r < rk) {
+    for (int h = 0; h < H; ++h) {
+        if (h) __syncthreads();
+        S.give(part, h);
+        __syncthreads();
+        const int m = n - 16 * h;                           // rows of this sixteen: part holds the last one's again past them
+        if (m > 0)
+            for (int i = (int)threadIdx.x; i < 16 * 16 * NR; i += 256) {
+                const int j = i / 16, p = i % 16, r = lora_value_at<NR>(j, a.rank);     // value j of the 16 NR, row p
+                float v = 0.0f;
 #pragma unroll
-                for (int w4 = 0; w4 < NW; ++w4) v[e] += part[(w4 * 16 * NR + r) * kLoraPart + p + e];
-                v[e] *= c;
+                for (int w4 = 0; w4 < NW; ++w4) v += part[(w4 * 16 * NR + r) * kLoraPart + p];
+                if (p < m) out[((j >> 2) * n + 16 * h + p) * 4 + (j & 3)] = lora_value_counts<NR>(j, a.rank, rk) ? v : 0.0f;
             }
+        if (!t.pieces) continue;
+        // As the weights' gradients read it: in bf16 pieces, a rank's rows side by side, zeros past the tile's rows and the
+        // adapter's rank; and where the rows of x are (past the last row, the last)
+        if (threadIdx.x < 16) {
+            const int tok = row[h] / a.n_ids;
+            t.off[slot * (16 * H) + 16 * h + threadIdx.x] =
+                (uint64_t)tok * a.x_tok + (uint64_t)((row[h] - tok * a.n_ids) % a.x_rows) * a.x_id;
+        }
+        for (int i = (int)threadIdx.x; i < 16 * 8 * NR; i += 256) {
+            const int r = i / 8, p = 2 * (i % 8);           // two rows at a time
+            float v[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int z = 0; z < 3; ++z) {
-            reinterpret_cast<uint32_t*>(t.pieces)[(slot * 3 + z) * (128 * NR) + i] = lora_split2(v);
+            for (int e = 0; e < 2; ++e)
+                if (p + e < m && r < rk) {
+#pragma unroll
+                    for (int w4 = 0; w4 < NW; ++w4) v[e] += part[(w4 * 16 * NR + r) * kLoraPart + p + e];
+                    v[e] *= c;
+                }
+#pragma unroll
+            for (int z = 0; z < 3; ++z)
+                reinterpret_cast<uint32_t*>(t.pieces)[((slot * 3 + z) * (16 * NR) + r) * (8 * H) + 8 * h + i % 8] = lora_split2(v);
         }
     }
 }
 // Both sides' in one launch, the windows of the second after the first's (forward: windows of b none)
-template <typename W, int NR, int U, int OCC>
+template <typename W, int NR, int U, int OCC, int H>
 __global__ __launch_bounds__(256, OCC) void k_lora_shrink(LoraArgs a, LoraTiles t, LoraArgs b, LoraTiles u, int windows) {
     __shared__ float part[4 * 16 * NR * kLoraPart];
     __shared__ lf4 turn[4 * (kLoraXLds + kLoraALds<W>)];
     const int w = (int)blockIdx.z;
-    if (w < windows) lora_shrink_part<W, NR, U>(a, t, w, part, turn);
-    else lora_shrink_part<W, NR, U>(b, u, w - windows, part, turn);
+    if (w < windows) lora_shrink_part<W, NR, U, H>(a, t, w, part, turn);
+    else lora_shrink_part<W, NR, U, H>(b, u, w - windows, part, turn);
 }
 
 // y = base + c S B^T of a tile and t.cols columns.  grid (slots, column parts, windows).
-template <typename W, int NR, int OCC>
+template <typename W, int NR, int OCC, int H>
 __global__ __launch_bounds__(256, OCC) void k_lora_expand(LoraArgs a, LoraTiles t) {
     constexpr int NW = 4;
-    int key, n, row, pos;
+    int key, n, row[H], pos;
     if (!lora_item(t, (int)blockIdx.z, key, n, row, pos)) return;
     const int c0 = (int)blockIdx.y * t.cols, c1 = min(a.rows, c0 + t.cols), o0 = c0 + 64 * ((int)threadIdx.x >> 6);
     if (key < 0) {
@@ -950,30 +1020,35 @@ __global__ __launch_bounds__(256, OCC) void k_lora_expand(LoraArgs a, LoraTiles 
     if (o0 >= c1) return;
     const int rk = lora_rank(a, key);
     const float c = lora_scale(a, key);
-    typedef LoraExpand<W, NR, NW> Expand;
-    const Expand E(a, lora_b<W>(a, key), row, c1);
-    const float* in = t.s + (size_t)pos * (16 * NR) + (NR * E.q * n + min(E.p, n - 1)) * 4;
-    lf4 v[NR];
+    const LoraExpand<W, NR, NW, H, true> E(a, lora_b<W>(a, key), row, n, c1);
+    float s[H][4 * NR];
 #pragma unroll
-    for (int j = 0; j < NR; ++j) v[j] = lf4{0, 0, 0, 0};
-    for (int z = 0; z < t.k_parts; z += 4) {                // the parts in order, the loads of four at a time
-        lf4 l[4][NR];
+    for (int h = 0; h < H; ++h) {
+        const float* in = t.s + (size_t)pos * (16 * NR) + (NR * E.q * n + min(16 * h + E.p, n - 1)) * 4;
+        lf4 v[NR];
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
+        for (int j = 0; j < NR; ++j) v[j] = lf4{0, 0, 0, 0};
+        constexpr int Z = NR == 8 ? 1 : 4;                  // the parts in order, the loads of Z at a time
+        for (int z = 0; z < t.k_parts; z += Z) {
+            lf4 l[Z][NR];
 #pragma unroll
-            for (int j = 0; j < NR; ++j)
-                l[y][j] = *reinterpret_cast<const lf4*>(in + (size_t)min(z + y, t.k_parts - 1) * t.positions * (16 * NR) + j * n * 4);
+            for (int y = 0; y < Z; ++y) {
+                if (z + y >= t.k_parts) continue;
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-            if (z + y < t.k_parts) {
-#pragma unroll
-                for (int j = 0; j < NR; ++j) v[j] += l[y][j];
+                for (int j = 0; j < NR; ++j)
+                    l[y][j] = *reinterpret_cast<const lf4*>(in + (size_t)(z + y) * t.positions * (16 * NR) + j * n * 4);
             }
-    }
-    float s[4 * NR];
 #pragma unroll
-    for (int j = 0; j < 4 * NR; ++j) s[j] = v[j / 4][j % 4] * c;
-    E.run(o0, s, rk, n);
+            for (int y = 0; y < Z; ++y)
+                if (z + y < t.k_parts) {
+#pragma unroll
+                    for (int j = 0; j < NR; ++j) v[j] += l[y][j];
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < 4 * NR; ++j) s[h][j] = v[j / 4][j % 4] * c;
+    }
+    E.run(o0, s, rk);
 }
 
 // ---------------------------------------------------------------------------
@@ -1034,7 +1109,7 @@ struct LoraGrad {
     const uint32_t* runs;
     int windows, keys, slots, splits, rank;
     int tiles_a;                  // column tiles of dA; dB's follow
-    const uint16_t* p[2];         // pieces of u, of s
+    const uint16_t* p[2];         // pieces of u, of s (tiles of 32 rows)
     const uint64_t* off[2];       // offsets of x's rows, of dy's
     const uint8_t* src[2];        // x, dy
     int width[2];                 // k, rows
@@ -1074,8 +1149,8 @@ __device__ inline uint32_t lora_grad_splits(const LoraGrad& g, int key, uint32_t
     return all;
 }
 
-// dA or dB of one key and 64 columns: rank blocks of 16 by columns, summed over the key's tiles, two (32 rows) per
-// v_mfma_f32_16x16x32_bf16, which the waves share.  Both operands are f32 in three bf16 pieces; the six
+// dA or dB of one key and 64 columns: rank blocks of 16 by columns, summed over the key's tiles, 32 rows and one
+// v_mfma_f32_16x16x32_bf16 each, which the waves share.  Both operands are f32 in three bf16 pieces; the six
 // products above 2^-24 of the whole are kept: 96 cycles where the f32 form takes 256.  Column 4 n + j
 // of x (dy) belongs to product j of four, so a lane loads four neighbours of eight rows, 256 bytes
 // a row; the next tiles' rows are loaded under the products.  splits > 1: a workgroup takes
@@ -1097,18 +1172,16 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
     for (int b = 0; b < NR; ++b)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[b][j] = lf4{0, 0, 0, 0};
-    // the key's tiles in pairs, every fourth this wave's, 64 windows at a time
+    // the key's tiles, every fourth this wave's, 64 windows at a time
     auto own = [&](int w) { return w < g.windows && w % g.splits == split; };
     int wb = 0, left = 0, turn = -1;
     uint64_t some = __ballot(e != 0u && own(lane));
     size_t at = 0;
-    auto advance = [&](size_t& slot, bool& two) {
+    auto advance = [&](size_t& slot) {
         for (;;) {
             if (left > 0) {
-                slot = at;
-                two = left > 1;
-                at += 2;
-                left -= 2;
+                slot = at++;
+                --left;
                 turn = (turn + 1) & 3;
                 if (turn == wave) return true;
                 continue;
@@ -1122,13 +1195,12 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
             const int l = __builtin_ctzll(some);
             some &= some - 1ull;
             const uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)e, l);
-            left = ((int)(r >> 16) + kLoraTile - 1) / kLoraTile;
+            left = ((int)(r >> 16) + 31) / 32;
             at = (size_t)(wb + l) * g.slots + (r & 0xFFFFu);
         }
     };
-    auto tile_of = [&](size_t slot, bool two) { return slot + (two && q > 1 ? 1 : 0); };
-    auto load_off = [&](uint64_t (&off)[8], size_t slot, bool two) {
-        const uint64_t* o = g.off[side] + tile_of(slot, two) * 16 + 8 * (q & 1);
+    auto load_off = [&](uint64_t (&off)[8], size_t slot) {
+        const uint64_t* o = g.off[side] + slot * 32 + 8 * q;
 #pragma unroll
         for (int i = 0; i < 8; ++i) off[i] = o[i];
     };
@@ -1147,22 +1219,22 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
     lf4 x[8];
     uint64_t off[8];
     size_t slot = 0, slot2 = 0;
-    bool two = false, two2 = false, more = advance(slot, two);
+    bool more = advance(slot);
     if (more) {
-        load_off(off, slot, two);
+        load_off(off, slot);
         load_x(x, off);
     }
     while (more) {
         // this step's pieces and the next one's offsets; x to pieces; the next x, under the products
-        more = advance(slot2, two2);
-        const uint16_t* pieces = g.p[side] + tile_of(slot, two) * (768 * NR) + 16 * p + 8 * (q & 1);
+        more = advance(slot2);
+        const uint16_t* pieces = g.p[side] + slot * (1536 * NR) + 32 * p + 8 * q;
         constexpr int UB = NR < 4 ? NR : 4;
         LoraWords U[UB][3];
 #pragma unroll
         for (int b = 0; b < UB; ++b)
 #pragma unroll
-            for (int z = 0; z < 3; ++z) U[b][z] = *reinterpret_cast<const LoraWords*>(pieces + z * (256 * NR) + 256 * b);
-        if (more) load_off(off, slot2, two2);
+            for (int z = 0; z < 3; ++z) U[b][z] = *reinterpret_cast<const LoraWords*>(pieces + z * (512 * NR) + 512 * b);
+        if (more) load_off(off, slot2);
         LoraWords X[4][3];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -1173,16 +1245,13 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
                 for (int z = 0; z < 3; ++z) X[j][z].u[c] = lora_split2(v);
             }
         if (more) load_x(x, off);
-        const uint32_t keep = !two && q > 1 ? 0u : 0xFFFFFFFFu;     // a lone tile: the other 16 rows count nothing
 #pragma unroll
         for (int b = 0; b < NR; ++b) {
             LoraWords V[3];
 #pragma unroll
             for (int z = 0; z < 3; ++z) {
                 V[z] = U[b % UB][z];
-                if (b + UB < NR) U[b % UB][z] = *reinterpret_cast<const LoraWords*>(pieces + z * (256 * NR) + 256 * (b + UB));
-#pragma unroll
-                for (int c = 0; c < 4; ++c) V[z].u[c] &= keep;
+                if (b + UB < NR) U[b % UB][z] = *reinterpret_cast<const LoraWords*>(pieces + z * (512 * NR) + 512 * (b + UB));
             }
 #pragma unroll
             for (int lo = 2; lo >= 0; --lo)                 // the smallest products first; four sums in turn
@@ -1192,7 +1261,6 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
                     for (int j = 0; j < 4; ++j) acc[b][j] = lora_mfma(LoraBF16{}, V[z], X[j][lo - z], acc[b][j]);
         }
         slot = slot2;
-        two = two2;
     }
     const bool whole = (used & (used - 1u)) == 0u;          // no other split has rows
 #pragma unroll
