@@ -231,8 +231,7 @@ static void lora_k_parts(int k, int tiles, int& parts, int& steps) {
 }
 
 // The expand's columns in parts of a step of 64 or more for each of its four waves, about kLoraExpandGroups workgroups
-static int lora_columns(int columns, int n_rows, int& cols) {
-    const int tiles = (n_rows + kLoraTile - 1) / kLoraTile;
+static int lora_columns(int columns, int tiles, int& cols) {
     const int parts = std::max(1, std::min((columns + 255) / 256, kLoraExpandGroups / tiles));
     cols = ((columns + parts - 1) / parts + 63) / 64 * 64;
     return (columns + cols - 1) / cols;
@@ -271,6 +270,11 @@ struct LoraBackSpace {
     size_t order, items, n_items, runs, s, u, at, bt, ps, pu, ox, oy, part, bytes;
     int windows, slots, key_bits, rank16, positions, tiles_a, tiles_b, splits;
 };
+// Rows up to which a workgroup of the backward's shrinks takes half a tile, with eight waves.  A CU reads its tile's rows
+// and A at little more than 64 bytes a cycle, so few tiles are shared out; many read A half as often as wholes.  us at 512 /
+// 1,024 / 2,048 rows, k 2048, halves against wholes: f32 to 768 at rank 16 8.1 / 8.9 / 11.7 against 13.3 / 14.2 / 15.6,
+// bf16 to 2048 at rank 64 11.3 / 11.9 / 18.6 against 21.4 / 22.0 / 22.5
+constexpr int kLoraHalfRows = 2048;
 constexpr int kLoraBackKeys = 1 << 15;        // a word per key and window
 // Splits of the weights' gradients, over the windows: what one request sends is together, so without them the
 // longest request's key would be a few workgroups' work
@@ -374,7 +378,7 @@ static void launch_lora_apply_rank(const LoraArgs& a, const LoraTiles& t, int co
         hipLaunchKernelGGL((k_lora_apply<W, NR, 4, U, OCC, H, false>), grid, dim3(256), 0, st, a, t);
         return;
     }
-    hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC, H>), dim3((unsigned)t.slots, (unsigned)t.k_parts, (unsigned)windows),
+    hipLaunchKernelGGL((k_lora_shrink<W, NR, 4, U, OCC, H, false>), dim3((unsigned)t.slots, (unsigned)t.k_parts, (unsigned)windows),
                        dim3(256), 0, st, a, t, a, t, windows);
     hipLaunchKernelGGL((k_lora_expand<W, NR, kLoraExpandOcc<NR, H>, H>), grid, dim3(256), 0, st, a, t);
 }
@@ -443,7 +447,7 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
     int parts = 1;
     t.cols = (lora->rows + 63) / 64 * 64;
     if (t.s) {
-        parts = lora_columns(lora->rows, n_rows, t.cols);
+        parts = lora_columns(lora->rows, (n_rows + sp.tile - 1) / sp.tile, t.cols);
     } else if (!sp.bytes) {                                 // what fills the chip
         parts = std::max(1, std::min((lora->rows + 63) / 64, 2 * g_num_cu / sp.slots));
         t.cols = ((lora->rows + parts - 1) / parts + 63) / 64 * 64;
@@ -476,11 +480,15 @@ static int launch_lora_back_rank(const LoraBack& b) {
                        0, b.st, b.a, b.g);
     if (b.g.n_rows && (b.x.dst || b.grad_tiles)) {
         hipLaunchKernelGGL(k_lora_transpose<typename W::T>, dim3((unsigned)(sp.tiles_a + sp.tiles_b), keys), dim3(256), 0, b.st, b.turn);
-        hipLaunchKernelGGL((k_lora_shrink<W, NR, U, OCC, 2>), dim3(slots, 1u, windows * (b.grad_tiles ? 2u : 1u)), dim3(256), 0, b.st, b.u, b.tu, b.a, b.ts, (int)windows);
+        const unsigned sides = windows * (b.grad_tiles ? 2u : 1u);
+        if (b.g.n_rows <= kLoraHalfRows)
+            hipLaunchKernelGGL((k_lora_shrink<W, NR, 8, U, 1, 1, true>), dim3(slots, 2u, sides), dim3(512), 0, b.st, b.u, b.tu, b.a, b.ts, (int)windows);
+        else
+            hipLaunchKernelGGL((k_lora_shrink<W, NR, 4, U, OCC, 2, false>), dim3(slots, 1u, sides), dim3(256), 0, b.st, b.u, b.tu, b.a, b.ts, (int)windows);
     }
     if (b.g.n_rows && b.x.dst) {
         LoraTiles t = b.tu;
-        const int parts = lora_columns(b.x.rows, b.g.n_rows, t.cols);
+        const int parts = lora_columns(b.x.rows, (b.g.n_rows + 31) / 32, t.cols);
         hipLaunchKernelGGL((k_lora_expand<W, NR, kLoraExpandOcc<NR, 2>, 2>), dim3(slots, (unsigned)parts, windows), dim3(256), 0, b.st, b.x, t);
     }
     if (b.grad_tiles) {

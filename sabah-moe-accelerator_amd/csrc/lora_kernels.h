@@ -305,16 +305,16 @@ __device__ inline bool lora_tile(const LoraArgs& a, const LoraTiles& t, LoraFind
     return true;
 }
 
-// The same from the lists of k_lora_group, with the tile's position in order; row[h]: of place 16 h + lane % 16
+// The same from the lists of k_lora_group, with the tile's position in order; row[h]: of place h0 + 16 h + lane % 16
 template <int H>
-__device__ inline bool lora_item(const LoraTiles& t, int w, int& key, int& n, int (&row)[H], int& pos) {
+__device__ inline bool lora_item(const LoraTiles& t, int w, int& key, int& n, int (&row)[H], int& pos, int h0 = 0) {
     if ((int)blockIdx.x >= t.n_items[w]) return false;
     const int4 it = t.items[(size_t)w * t.slots + blockIdx.x];
     key = __builtin_amdgcn_readfirstlane(it.x);
     pos = __builtin_amdgcn_readfirstlane(it.y);
     n = __builtin_amdgcn_readfirstlane(it.z);
 #pragma unroll
-    for (int h = 0; h < H; ++h) row[h] = t.order[pos + min(16 * h + ((int)threadIdx.x & 15), n - 1)];
+    for (int h = 0; h < H; ++h) row[h] = t.order[pos + min(h0 + 16 * h + ((int)threadIdx.x & 15), n - 1)];
     return true;
 }
 
@@ -947,15 +947,16 @@ __global__ __launch_bounds__(64 * NW, OCC) void k_lora_apply(LoraArgs a, LoraTil
 // Larger calls: S = X A^T of a tile and one part of k per workgroup, to t.s, [k parts][position in order][16 NR]
 // in all, a tile of n rows as the expand reads it: [4 NR groups of four values][n rows][4] of every lane's values in
 // lora_value_at's order (zeros where one does not count), so that its loads are whole lines.  grid (slots, k parts, windows).
-template <typename W, int NR, int U, int H>
+template <typename W, int NR, int NW, int U, int H, bool HALF>
 __device__ inline void lora_shrink_part(const LoraArgs& a, const LoraTiles& t, int w, float* part, lf4* turn) {
-    constexpr int NW = 4;
     int key, n, row[H], pos;
-    if ((int)blockIdx.y >= t.k_parts || !lora_item(t, w, key, n, row, pos) || key < 0) return;
-    const int s0 = (int)blockIdx.y * t.k_steps, rk = lora_rank(a, key);
+    const int part_k = HALF ? 0 : (int)blockIdx.y, h0 = HALF ? 16 * (int)blockIdx.y : 0;
+    if (part_k >= t.k_parts || !lora_item(t, w, key, n, row, pos, h0) || key < 0) return;
+    const int s0 = part_k * t.k_steps, rk = lora_rank(a, key);
+    constexpr int ROWS = HALF ? 32 : 16 * H;                // of the tile
     LoraShrink<W, NR, NW, U, H> S(a, lora_a<W>(a, key), row, n, turn, s0, s0 + t.k_steps);
     S.run();
-    float* out = t.s + ((size_t)blockIdx.y * t.positions + pos) * (16 * NR);
+    float* out = t.s + ((size_t)part_k * t.positions + pos) * (16 * NR);
     const size_t slot = (size_t)w * t.slots + blockIdx.x;
     const float c = t.scaled ? lora_scale(a, key) : 1.0f;
 #pragma unroll
@@ -963,24 +964,24 @@ __device__ inline void lora_shrink_part(const LoraArgs& a, const LoraTiles& t, i
         if (h) __syncthreads();
         S.give(part, h);
         __syncthreads();
-        const int m = n - 16 * h;                           // rows of this sixteen: part holds the last one's again past them
+        const int g = h0 + 16 * h, m = n - g;                // rows of this sixteen: part holds the last one's again past them
         if (m > 0)
-            for (int i = (int)threadIdx.x; i < 16 * 16 * NR; i += 256) {
+            for (int i = (int)threadIdx.x; i < 16 * 16 * NR; i += 64 * NW) {
                 const int j = i / 16, p = i % 16, r = lora_value_at<NR>(j, a.rank);     // value j of the 16 NR, row p
                 float v = 0.0f;
 #pragma unroll
                 for (int w4 = 0; w4 < NW; ++w4) v += part[(w4 * 16 * NR + r) * kLoraPart + p];
-                if (p < m) out[((j >> 2) * n + 16 * h + p) * 4 + (j & 3)] = lora_value_counts<NR>(j, a.rank, rk) ? v : 0.0f;
+                if (p < m) out[((j >> 2) * n + g + p) * 4 + (j & 3)] = lora_value_counts<NR>(j, a.rank, rk) ? v : 0.0f;
             }
         if (!t.pieces) continue;
         // As the weights' gradients read it: in bf16 pieces, a rank's rows side by side, zeros past the tile's rows and the
         // adapter's rank; and where the rows of x are (past the last row, the last)
         if (threadIdx.x < 16) {
             const int tok = row[h] / a.n_ids;
-            t.off[slot * (16 * H) + 16 * h + threadIdx.x] =
+            t.off[slot * ROWS + g + threadIdx.x] =
                 (uint64_t)tok * a.x_tok + (uint64_t)((row[h] - tok * a.n_ids) % a.x_rows) * a.x_id;
         }
-        for (int i = (int)threadIdx.x; i < 16 * 8 * NR; i += 256) {
+        for (int i = (int)threadIdx.x; i < 16 * 8 * NR; i += 64 * NW) {
             const int r = i / 8, p = 2 * (i % 8);           // two rows at a time
             float v[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -992,18 +993,18 @@ __device__ inline void lora_shrink_part(const LoraArgs& a, const LoraTiles& t, i
                 }
 #pragma unroll
             for (int z = 0; z < 3; ++z)
-                reinterpret_cast<uint32_t*>(t.pieces)[((slot * 3 + z) * (16 * NR) + r) * (8 * H) + 8 * h + i % 8] = lora_split2(v);
+                reinterpret_cast<uint32_t*>(t.pieces)[((slot * 3 + z) * (16 * NR) + r) * (ROWS / 2) + g / 2 + i % 8] = lora_split2(v);
         }
     }
 }
 // Both sides' in one launch, the windows of the second after the first's (forward: windows of b none)
-template <typename W, int NR, int U, int OCC, int H>
-__global__ __launch_bounds__(256, OCC) void k_lora_shrink(LoraArgs a, LoraTiles t, LoraArgs b, LoraTiles u, int windows) {
-    __shared__ float part[4 * 16 * NR * kLoraPart];
-    __shared__ lf4 turn[4 * (kLoraXLds + kLoraALds<W>)];
+template <typename W, int NR, int NW, int U, int OCC, int H, bool HALF>
+__global__ __launch_bounds__(64 * NW, OCC) void k_lora_shrink(LoraArgs a, LoraTiles t, LoraArgs b, LoraTiles u, int windows) {
+    __shared__ float part[NW * 16 * NR * kLoraPart];
+    __shared__ lf4 turn[NW * (kLoraXLds + kLoraALds<W>)];
     const int w = (int)blockIdx.z;
-    if (w < windows) lora_shrink_part<W, NR, U, H>(a, t, w, part, turn);
-    else lora_shrink_part<W, NR, U, H>(b, u, w - windows, part, turn);
+    if (w < windows) lora_shrink_part<W, NR, NW, U, H, HALF>(a, t, w, part, turn);
+    else lora_shrink_part<W, NR, NW, U, H, HALF>(b, u, w - windows, part, turn);
 }
 
 // y = base + c S B^T of a tile and t.cols columns.  grid (slots, column parts, windows).
