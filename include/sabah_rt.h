@@ -312,7 +312,7 @@ int sabah_moe_balance(const float *d_logits, size_t logits_stride, const int32_t
  * counts are constants of the gradient; both may be NULL when c_balance and c_z are 0).
  * Every row of d_dlogits is written: zeros for a masked token, whose inputs are not
  * read, and for a row of minus infinities only.  An expert named twice by a token gets both parts.
- * An id out of range makes its token's row NaN and fails the next call. */
+ * An id out of range makes its token's row NaN and fails the next call.  d_dlogits overlaps no input. */
 int sabah_moe_route_backward(const float *d_logits, size_t logits_stride, const int32_t *d_ids, const uint8_t *d_mask,
                              int n_tokens, int n_experts, int n_used, int norm_w, float w_scale, const float *d_dw,
                              const int32_t *d_counts, const int32_t *d_n_valid, int n_groups, float c_balance, float c_z,
@@ -320,8 +320,8 @@ int sabah_moe_route_backward(const float *d_logits, size_t logits_stride, const 
 
 /* Low-rank adapters of a projection, one (A, B) pair for each (adapter, expert); a
  * dense projection has one expert.  type: ggml's code of A and B, F32 0, F16 1 or
- * BF16 30.  rank <= 128, n_adapters * n_experts <= 2^21, rank * k and rank * rows <= 2^28; an adapter of a lower rank says so in ranks (the
- * values past it are not used) or pads A and B with zeros. */
+ * BF16 30.  rank <= 128, n_adapters * n_experts <= 2^21, rank * k and rank * rows <= 2^28; an adapter of a lower
+ * rank says so in ranks (the values past it are not used) or pads A and B with zeros. */
 typedef struct sabah_lora_desc {
     const void *a;            /* device [n_adapters][n_experts][rank][k] */
     const void *b;            /* device [n_adapters][n_experts][rows][rank] */
@@ -337,8 +337,8 @@ typedef struct sabah_lora_desc {
  *   n_experts == 1)
  * with x, ids and dst addressed as in sabah_rt_mul_mat_id_v2, whose dst is the base
  * (base may be dst itself, with the same strides: rows without an adapter are then not touched;
- * NULL: zeros).  All strides are bytes and multiples of 4; x and dst must not overlap; at most 2^24
- * rows.  Sums are f32.  An adapter or expert id out of range makes its row NaN and fails
+ * NULL: zeros).  All strides are bytes and multiples of 4 (0: one row for all, of inputs); x and dst must not
+ * overlap, and of dst each row is its own; at most 2^24 rows.  Sums are f32.  An adapter or expert id out of range makes its row NaN and fails
  * the next call. */
 size_t sabah_lora_workspace(const sabah_lora_desc *lora, int n_ids, int n_tokens, int backward);
 int sabah_lora_apply(const sabah_lora_desc *lora, const float *d_x, size_t x_id_stride, int x_rows,
@@ -353,8 +353,11 @@ int sabah_lora_apply(const sabah_lora_desc *lora, const float *d_x, size_t x_id_
  *                    zeros for a row without an adapter; added to dx with add_dx
  *   d_da, d_db     f32 in the layouts of A and B, written for every adapter and expert (zeros where no
  *                  row uses the pair and past an adapter's own rank); added to them with add_dw
- * Each of d_dx, d_da and d_db may be NULL.  A row with an id out of range gives no part of d_da and
- * d_db, its dx is NaN, and the next call fails. */
+ * Each of d_dx, d_da and d_db may be NULL; they overlap neither each other nor an input.
+ * n_adapters * n_experts <= 2^15.  A row with an id out of range gives no part of d_da and d_db, its dx is NaN,
+ * and the next call fails.  A value of x or dy that is not finite, or at least 3.39e38 (what rounds to infinity in
+ * bf16), leaves its pair's d_da and d_db not finite within the adapter's rank (NaN, also where
+ * the sums would give an infinity), and no other pair's. */
 int sabah_lora_backward(const sabah_lora_desc *lora, const float *d_x, size_t x_id_stride, int x_rows,
                         size_t x_token_stride, const int32_t *d_adapters, const int32_t *d_ids, size_t ids_id_stride,
                         size_t ids_token_stride, int n_ids, int n_tokens, const float *d_dy, size_t dy_id_stride,

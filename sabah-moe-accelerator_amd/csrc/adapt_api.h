@@ -411,6 +411,7 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
         return fail("adapters: the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", sp.bytes,
                     workspace_bytes);
     if (g_device < 0) return fail("sabah_rt_init has not been called");
+    if (n_tokens && d_dst == d_x) return fail("adapters: dst would overwrite x");
     if (!check_sticky()) return -1;
     if (n_tokens == 0) return 0;
     OnDevice dev;
@@ -525,6 +526,7 @@ SABAH_API int sabah_lora_backward(const sabah_lora_desc* lora, const float* d_x,
         return fail("adapters backward: the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", sp.bytes,
                     workspace_bytes);
     if (g_device < 0) return fail("sabah_rt_init has not been called");
+    if (n_tokens && d_dx && (d_dx == d_x || d_dx == d_dy)) return fail("adapters backward: dx would overwrite x or dy");
     if (!check_sticky()) return -1;
     OnDevice dev;
     if (!dev.ok) return -1;
@@ -602,6 +604,7 @@ SABAH_API int sabah_lora_backward(const sabah_lora_desc* lora, const float* d_x,
     w.part[0] = reinterpret_cast<float*>(ws + sp.part);
     w.part[1] = w.part[0] + (size_t)sp.splits * keys * sp.tiles_a * sp.rank16 * 64;
     w.scale = lora->scale;
+    w.ranks = lora->ranks;
     w.n_experts = lora->n_experts;
     w.add = add_dw != 0;
     b.grad_tiles = w.tiles_a + (d_db ? sp.tiles_b : 0);

@@ -1117,20 +1117,23 @@ struct LoraGrad {
     float* out[2];                // dA, dB
     float* part[2];               // several splits: [splits][keys][tiles][16 NR][64]; window w is split w % splits'
     const float* scale;
+    const int32_t* ranks;
     int n_experts, add;
 };
 
 // 16 ranks (rank block b) by 64 columns, summed in sum[16][64] of LDS, to the gradient.  dA [rank][k], dB [rows][rank].
+// Past the adapter's own rank the pieces are zeros, but 0 times an infinity of x or dy is not.
 __device__ inline void lora_grad_store(const LoraGrad& g, int side, int key, int b, int c0, const float* sum) {
     const int tid = (int)threadIdx.x, n = g.width[side];
     float* out = g.out[side] + (size_t)key * g.rank * n;
     const float c = side && g.scale ? g.scale[key / g.n_experts] : 1.0f;
+    const int rk = g.ranks ? g.ranks[key / g.n_experts] : g.rank;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int e = tid + 256 * i, r = side ? e & 15 : e >> 6, o = side ? e >> 4 : e & 63;
         if (16 * b + r >= g.rank || c0 + o >= n) continue;
         float* to = out + (side ? (size_t)(c0 + o) * g.rank + 16 * b + r : (size_t)(16 * b + r) * n + c0 + o);
-        const float v = sum[r * 64 + o] * c;
+        const float v = 16 * b + r < rk ? sum[r * 64 + o] * c : 0.0f;
         *to = g.add ? *to + v : v;
     }
 }

@@ -125,6 +125,10 @@ class MoEExecutor:
         b = self.bank
         T, n_ids = ids.shape
         rows, k, qt = b.rows[role], b.cols[role], b.layer_qtype(layer, role)
+        if lora is not None and (adapters is None or lora.n_experts not in (1, b.n_experts)
+                                 or (lora.k, lora.rows) != (k, rows)):
+            raise ValueError("adapters of %d experts, %d -> %d, beside a bank of %d, %d -> %d"
+                             % (lora.n_experts, lora.k, lora.rows, b.n_experts, k, rows))
         if out is None:
             out = torch.empty((T, n_ids, rows), dtype=torch.float32, device=self.device)
         src = b.base_ptr(layer, role) if source is None else source
@@ -140,8 +144,6 @@ class MoEExecutor:
         if rc:
             rt.check(rc, "MUL_MAT_ID")
         if lora is not None:
-            if lora.n_experts not in (1, b.n_experts):
-                raise ValueError("adapters of %d experts beside a bank of %d" % (lora.n_experts, b.n_experts))
             self.lora_apply(lora, x, adapters, out, ids=ids if lora.n_experts > 1 else None, out=out)
         return out
 
