@@ -215,11 +215,16 @@ static int check_lora(const char* what, const sabah_lora_desc* L, int n_ids, int
 
 static bool stride_ok(size_t s) { return s % 4 == 0; }
 
-// A call of at most kLoraDirectRows rows is one launch (k_lora_apply).  Above: per window of rows at most
-// one tile per 16 rows and one more per key; the shrink's k in parts of at least eight steps
-// of 32 while there are few tiles, so that the launch fills the chip.
+// Forward.  A call of at most kLoraDirectRows rows is one launch (k_lora_apply): at 256 rows of 64 adapters (k 2048, rows
+// 512, rank 16) 16.2 us, where the three launches of a larger call take 20.2 (15.6 and 16.4 at 128, 14.9 and 15.8 at 64).
+// Above, each window of rows has at most one tile per 16 rows and one more per key.  With kLoraFusedTiles of them, two
+// for every CU, a workgroup shrinks and expands its tile (one launch after the lists); with fewer two launches share out k and the
+// columns.  us of the one launch against the two, 2048 x 2048, rank 32, 8 adapters: 44.8 and 36.0 at 4,096 rows (328 tiles),
+// 56.2 and 59.0 at 8,192 (656), 95.3 and 103.5 at 16,384; of 512 experts' pairs 14.7 and 17.0 at 640 rows, 21.0 and 30.9 at 5,120.
 constexpr int kLoraDirectRows = 256;
-constexpr int kLoraFusedRows = 4096;          // from here on a tile's shrink and expand in one workgroup
+constexpr int kLoraFusedTiles = 512;
+// The two launches: k in parts of at least eight steps of 32, up to about 1,024 workgroups (1,999 rows of k 2048 at rank 64: the
+// shrink 12.4 us in eight parts, 25.8 whole; the expand, which adds them up, 11.2 and 8.4)
 constexpr int kLoraShrinkGroups = 1024, kLoraShrinkParts = 8, kLoraShrinkSteps = 8;
 constexpr int kLoraExpandGroups = 1024;
 // k of a shrink in parts while there are few tiles
@@ -239,23 +244,22 @@ static int lora_columns(int columns, int tiles, int& cols) {
 
 struct LoraSpace {
     size_t order, items, n_items, s, bytes;
-    int windows, slots, key_bits, k_parts, k_steps, rank16, tile;
+    int windows, slots, key_bits, k_parts, k_steps, rank16;
 };
 static LoraSpace lora_space(const sabah_lora_desc* L, int n_rows) {
     LoraSpace s{};
     const int keys = L->n_adapters * L->n_experts + 2;      // without an adapter, and with a bad id
     const int span = std::min(n_rows, kLoraWindow);
     s.windows = (n_rows + kLoraWindow - 1) / kLoraWindow;
-    s.tile = n_rows > kLoraDirectRows && L->rank > 32 ? 32 : kLoraTile;
-    s.slots = std::min(span, span / s.tile + std::min(keys, span));
+    s.slots = std::min(span, span / kLoraTile + std::min(keys, span));
     s.rank16 = L->rank <= 16 ? 16 : L->rank <= 32 ? 32 : L->rank <= 64 ? 64 : 128;
     while (keys >> s.key_bits) ++s.key_bits;                // the word past the rows has key + 2 == keys
     if (n_rows <= kLoraDirectRows) {
         s.windows = 1;
         return s;
     }
-    lora_k_parts(L->k, (n_rows + s.tile - 1) / s.tile, s.k_parts, s.k_steps);
-    const size_t positions = n_rows < kLoraFusedRows ? (size_t)s.windows * kLoraWindow : 0;
+    lora_k_parts(L->k, (n_rows + kLoraTile - 1) / kLoraTile, s.k_parts, s.k_steps);
+    const size_t positions = (long long)s.windows * s.slots < kLoraFusedTiles ? (size_t)s.windows * kLoraWindow : 0;
     s.items = align256((size_t)s.windows * kLoraWindow * 4);
     s.n_items = s.items + align256((size_t)s.windows * s.slots * 16);
     s.s = s.n_items + align256((size_t)s.windows * 4);
@@ -367,27 +371,27 @@ static int check_lora_rows(const char* what, const sabah_lora_desc* L, const flo
     return 0;
 }
 
-template <typename W, int NR, int NW, int US, int U, int OCC, int H>
+template <typename W, int NR, int NW, int US, int U, int OCC>
 static void launch_lora_apply_rank(const LoraArgs& a, const LoraTiles& t, int column_parts, int windows, hipStream_t st) {
     const dim3 grid((unsigned)t.slots, (unsigned)column_parts, (unsigned)windows);
     if (!t.order) {
-        hipLaunchKernelGGL((k_lora_apply<W, NR, NW, US, 1, 1, true>), grid, dim3(64 * NW), 0, st, a, t);
+        hipLaunchKernelGGL((k_lora_apply<W, NR, NW, US, 1, true>), grid, dim3(64 * NW), 0, st, a, t);
         return;
     }
     if (!t.s) {
-        hipLaunchKernelGGL((k_lora_apply<W, NR, 4, U, OCC, H, false>), grid, dim3(256), 0, st, a, t);
+        hipLaunchKernelGGL((k_lora_apply<W, NR, 4, U, OCC, false>), grid, dim3(256), 0, st, a, t);
         return;
     }
-    hipLaunchKernelGGL((k_lora_shrink<W, NR, 4, U, OCC, H, false>), dim3((unsigned)t.slots, (unsigned)t.k_parts, (unsigned)windows),
+    hipLaunchKernelGGL((k_lora_shrink<W, NR, 4, U, OCC, 1, false>), dim3((unsigned)t.slots, (unsigned)t.k_parts, (unsigned)windows),
                        dim3(256), 0, st, a, t, a, t, windows);
-    hipLaunchKernelGGL((k_lora_expand<W, NR, kLoraExpandOcc<NR, H>, H>), grid, dim3(256), 0, st, a, t);
+    hipLaunchKernelGGL((k_lora_expand<W, NR, kLoraExpandOcc<NR, 1>, 1>), grid, dim3(256), 0, st, a, t);
 }
 template <typename W>
 static void launch_lora_apply(const LoraArgs& a, const LoraTiles& t, int column_parts, int windows, hipStream_t st) {
-    if (a.rank <= 16) launch_lora_apply_rank<W, 1, 8, 4, 2, 4, 1>(a, t, column_parts, windows, st);
-    else if (a.rank <= 32) launch_lora_apply_rank<W, 2, 8, 4, 2, 4, 1>(a, t, column_parts, windows, st);
-    else if (a.rank <= 64) launch_lora_apply_rank<W, 4, 4, 2, 1, 2, 2>(a, t, column_parts, windows, st);
-    else launch_lora_apply_rank<W, 8, 4, 1, 1, 1, 2>(a, t, column_parts, windows, st);
+    if (a.rank <= 16) launch_lora_apply_rank<W, 1, 8, 4, 2, 4>(a, t, column_parts, windows, st);
+    else if (a.rank <= 32) launch_lora_apply_rank<W, 2, 8, 4, 2, 4>(a, t, column_parts, windows, st);
+    else if (a.rank <= 64) launch_lora_apply_rank<W, 4, 4, 2, 2, 2>(a, t, column_parts, windows, st);
+    else launch_lora_apply_rank<W, 8, 4, 1, 1, sizeof(typename W::T) == 4 ? 1 : 2>(a, t, column_parts, windows, st);
 }
 
 SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, size_t x_id_stride, int x_rows,
@@ -433,7 +437,7 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
     if (sp.bytes) {
         uint8_t* ws = static_cast<uint8_t*>(d_workspace);
         const LoraGroup g{reinterpret_cast<int*>(ws + sp.order), reinterpret_cast<int4*>(ws + sp.items),
-                          reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, t.skip_none, sp.key_bits, sp.tile, nullptr};
+                          reinterpret_cast<int*>(ws + sp.n_items), n_rows, sp.slots, t.skip_none, sp.key_bits, kLoraTile, nullptr};
         hipLaunchKernelGGL(k_lora_group, dim3((unsigned)sp.windows),
                            dim3((unsigned)std::min(kLoraWindow, (n_rows + 63) / 64 * 64)), 0, st, a, g);
         if (!ck(hipGetLastError(), "adapters grouping launch")) return -1;
@@ -448,7 +452,7 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
     int parts = 1;
     t.cols = (lora->rows + 63) / 64 * 64;
     if (t.s) {
-        parts = lora_columns(lora->rows, (n_rows + sp.tile - 1) / sp.tile, t.cols);
+        parts = lora_columns(lora->rows, (n_rows + kLoraTile - 1) / kLoraTile, t.cols);
     } else if (!sp.bytes) {                                 // what fills the chip
         parts = std::max(1, std::min((lora->rows + 63) / 64, 2 * g_num_cu / sp.slots));
         t.cols = ((lora->rows + parts - 1) / parts + 63) / 64 * 64;

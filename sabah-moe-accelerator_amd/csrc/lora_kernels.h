@@ -5,7 +5,6 @@
 //   backward   u = scale B^T dy_r;  dx_r (+)= A^T u;  dA (+)= u x_r^T;  dB (+)= scale dy_r s^T
 // Sums are f32; weights of f16 and bf16 are widened exactly.
 #pragma once
-#include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -14,7 +13,6 @@
 
 namespace sabah {
 
-constexpr int kLoraThreads = 256;
 constexpr int kLoraMaxRank = 128;
 constexpr unsigned kErrLora = 4u;             // sticky error word: an adapter or expert id out of range
 constexpr int kLoraNone = -1, kLoraBad = -2;  // keys of a row without an adapter, and of one with a bad id
@@ -108,8 +106,9 @@ __device__ inline const float* lora_x(const LoraArgs& a, int row) {
 // (lora_tile, a thread for every row of the call); above, k_lora_group sorts each window of 1,024
 // rows by key and lists its tiles.
 // ---------------------------------------------------------------------------
-// A tile of the lists is one or two sixteens of rows (LoraGroup::tile), which share the reads of A and B: of
-// rank 64 these come from L2 at 16 rows a tile as fast as it gives (10.8 TB/s), while x and y take half the time.
+// A tile of the lists is one sixteen of rows forward, two backward (LoraGroup::tile).  Two share the reads of A and B, which
+// pays where the weights' gradients take whole tiles of 32 anyway; forward, half as many workgroups cost more: 1,999
+// rows at rank 64 21.7 us in sixteens, 23.6 in twos; at rank 128 33 and 45; 16,384 rows at rank 64 96 and 93, at 128 154 and 162.
 constexpr int kLoraTile = 16;
 constexpr int kLoraWindow = 1024;
 
@@ -740,7 +739,7 @@ struct LoraExpand {
         }
     }
     // Streamed past the caches in large calls: their output does not fit there, and A and B, which the other tiles read again,
-    // stay (16,384 rows at rank 32: 82 us against 97)
+    // stay (16,384 rows at rank 32: 95 us against 99, and 82 against 97 where x and base come from the last-level cache)
     __device__ inline void store(const lf4 (&in)[4], const lf4 (&d)[4], int t, int o0, unsigned rows_in) const {
         const int o = o0 + 4 * p;
 #pragma unroll
@@ -910,14 +909,14 @@ __device__ inline const typename W::T* lora_b(const LoraArgs& a, int key) {
 // kernels below).  Small ones, in one launch: a workgroup finds its tile by itself (FIND)
 // and shrinks it whole, also when several share its columns; up to U steps of loads at a time, which it
 // waits for.  Large ones, with tiles to fill the chip, take them from the lists, and hold OCC
-// waves per SIMD to cover the loads: 96 us where the two kernels take 108 (16,384 rows, rank 32,
-// 2048 x 2048).  grid (slots, column parts, windows).
-template <typename W, int NR, int NW, int U, int OCC, int H, bool FIND>
+// waves per SIMD to cover the loads.  Bound by HBM there: 16,384 rows, 2048 x 2048, rank 32, 402 MB in 95 us (4.2 TB/s; a
+// large copy reaches 4.7).  One token: 7.7 us, waits on one load after another.  grid (slots, column parts, windows).
+template <typename W, int NR, int NW, int U, int OCC, bool FIND>
 __global__ __launch_bounds__(64 * NW, OCC) void k_lora_apply(LoraArgs a, LoraTiles t) {
     __shared__ float part[NW * 16 * NR * kLoraPart];
     __shared__ lf4 turn[NW * (kLoraXLds + kLoraALds<W>)];
     __shared__ typename std::conditional<FIND, LoraFind<NW>, int>::type find;
-    int key, n, row[H], pos;
+    int key, n, row[1], pos;
     if constexpr (FIND) {
         if (!lora_tile<NW>(a, t, find, key, n, row)) return;
     } else {
@@ -930,17 +929,13 @@ __global__ __launch_bounds__(64 * NW, OCC) void k_lora_apply(LoraArgs a, LoraTil
     }
     const int rk = lora_rank(a, key);
     const float c = lora_scale(a, key);
-    LoraShrink<W, NR, NW, U, H> S(a, lora_a<W>(a, key), row, n, turn, 0, 1 << 28);
+    LoraShrink<W, NR, NW, U, 1> S(a, lora_a<W>(a, key), row, n, turn, 0, 1 << 28);
     S.run();
-    const LoraExpand<W, NR, NW, H, !FIND> E(a, lora_b<W>(a, key), row, n, c1);
-    float s[H][4 * NR];
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-        if (h) __syncthreads();
-        S.give(part, h);
-        __syncthreads();
-        lora_sum_parts<NR, NW>(E, part, rk, c, s[h]);
-    }
+    const LoraExpand<W, NR, NW, 1, !FIND> E(a, lora_b<W>(a, key), row, n, c1);
+    float s[1][4 * NR];
+    S.give(part, 0);
+    __syncthreads();
+    lora_sum_parts<NR, NW>(E, part, rk, c, s[0]);
     E.run(o0, s, rk);
 }
 

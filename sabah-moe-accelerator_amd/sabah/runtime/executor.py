@@ -291,17 +291,18 @@ class MoEExecutor:
             out = RouterBalance(logits.shape[1], n_groups, device=self.device)
         n_groups = out.n_groups
         T, E, k = self._router_rows(logits, ids, mask, n_groups)
-        if out.n_experts != E:
-            raise ValueError("balance: %d experts, out has %d" % (E, out.n_experts))
+        if out.n_experts != E or out.counts.get_device() != self._index:
+            raise ValueError("balance: %d experts on %s, out has %d on %s"
+                             % (E, self.device, out.n_experts, out.counts.device))
         lib = rt.lib()
         n = lib.sabah_moe_balance_workspace(T, E, n_groups)
         if not n:
             rt.check(-1, "moe_balance")
         ws = torch.empty(n, dtype=torch.uint8, device=self.device)
         rc = lib.sabah_moe_balance(logits.data_ptr(), logits.stride(0) * 4 if T > 1 else E * 4, ids.data_ptr(),
-                                        mask.data_ptr() if mask is not None else None, T, E, k, n_groups,
-                                        out.counts.data_ptr(), out.mean_p.data_ptr(), out.losses.data_ptr(),
-                                        out.n_valid.data_ptr(), ws.data_ptr(), n, _stream(self.device))
+                                   mask.data_ptr() if mask is not None else None, T, E, k, n_groups,
+                                   out.counts.data_ptr(), out.mean_p.data_ptr(), out.losses.data_ptr(),
+                                   out.n_valid.data_ptr(), ws.data_ptr(), n, _stream(self.device))
         if rc:
             rt.check(rc, "moe_balance")
         return out
@@ -315,8 +316,9 @@ class MoEExecutor:
         c_z * losses[1] of `balance`, which balance() computed with the same mask."""
         n_groups = balance.n_groups if balance is not None else 1
         T, E, k = self._router_rows(logits, ids, mask, n_groups)
-        if balance is not None and balance.n_experts != E:
-            raise ValueError("route_backward: %d experts, balance has %d" % (E, balance.n_experts))
+        if balance is not None and (balance.n_experts != E or balance.counts.get_device() != self._index):
+            raise ValueError("route_backward: %d experts on %s, balance has %d on %s"
+                             % (E, self.device, balance.n_experts, balance.counts.device))
         if dw is not None and (dw.dtype is not torch.float32 or dw.shape != ids.shape or not dw.is_contiguous()
                                or dw.get_device() != self._index):
             raise ValueError("route_backward: dw %s %s, ids %s" % (tuple(dw.shape), dw.dtype, tuple(ids.shape)))
@@ -326,8 +328,8 @@ class MoEExecutor:
               or out.get_device() != self._index):
             raise ValueError("route_backward: out %s %s" % (tuple(out.shape), out.dtype))
         rc = rt.lib().sabah_moe_route_backward(
-            logits.data_ptr(), logits.stride(0) * 4 if T > 1 else E * 4, ids.data_ptr(), mask.data_ptr() if mask is not None else None,
-            T, E, k, int(norm_w), w_scale, dw.data_ptr() if dw is not None else None,
+            logits.data_ptr(), logits.stride(0) * 4 if T > 1 else E * 4, ids.data_ptr(),
+            mask.data_ptr() if mask is not None else None, T, E, k, int(norm_w), w_scale, dw.data_ptr() if dw is not None else None,
             balance.counts.data_ptr() if balance is not None else None,
             balance.n_valid.data_ptr() if balance is not None else None, n_groups, c_balance, c_z,
             out.data_ptr(), out.stride(0) * 4 if T > 1 else E * 4, _stream(self.device))
