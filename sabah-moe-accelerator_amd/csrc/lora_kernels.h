@@ -83,8 +83,8 @@ struct LoraBF16 : Lora16<LoraBF16> {
 // the row's key: adapter * n_experts + expert, kLoraNone or kLoraBad
 __device__ inline int lora_key(const LoraArgs& a, int row) {
     const int t = row / a.n_ids, i = row - t * a.n_ids, ad = a.adapters[t];
-    if (ad == -1) return kLoraNone;
     const int e = a.ids ? *reinterpret_cast<const int32_t*>(a.ids + (size_t)t * a.ids_tok + (size_t)i * a.ids_id) : 0;
+    if (ad == -1) return kLoraNone;
     if (ad < 0 || ad >= a.n_adapters || e < 0 || e >= a.n_experts) return kLoraBad;
     return ad * a.n_experts + e;
 }
