@@ -290,3 +290,34 @@ def test_calls_refuse_what_would_overwrite_their_inputs(ex, hip_rt):
     with pytest.raises(ValueError):
         ex.mul_mat_id(0, "gate", torch.zeros(2, 1, 256, device=DEV), torch.zeros(2, 1, dtype=torch.int32, device=DEV),
                       lora=c.lora)
+
+
+def test_the_losses_of_another_device_are_refused(ex):
+    from sabah.runtime.executor import RouterBalance
+    logits, ids = torch.zeros(4, 16, device=DEV), torch.zeros(4, 2, dtype=torch.int32, device=DEV)
+    away = RouterBalance(16, 1, device="cpu")
+    with pytest.raises(ValueError):
+        ex.balance(logits, ids, out=away)
+    with pytest.raises(ValueError):
+        ex.route_backward(logits, ids, None, away, 1.0, 1.0)
+
+
+def test_the_current_stream_orders_the_calls(ex):
+    """On a stream of its own, behind work that fills the inputs there, a call reads what that work wrote."""
+    c = Case(12, 300, 256, 128, 16, 3, BF16, adapters="runs")
+    want, bound = c.forward()
+    x = torch.zeros_like(c.d_x)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        busy = torch.randn(2048, 2048, device=DEV)
+        for _ in range(4):
+            busy = busy @ busy * 1e-3
+        x.copy_(c.d_x + busy[0, 0].nan_to_num(0, 0, 0) * 0)
+        got = ex.lora_apply(c.lora, x, c.d_ad, c.d_base)
+        dx, da, db = ex.lora_backward(c.lora, x, c.d_ad, c.d_dy)
+    s.synchronize()
+    close(got, want, bound, "forward")
+    wants, bounds = c.backward()
+    for g, w, b, what in zip((dx, da, db), wants, bounds, ("dx", "da", "db")):
+        close(g, w, b, what)
