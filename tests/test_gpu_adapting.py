@@ -321,3 +321,50 @@ def test_the_current_stream_orders_the_calls(ex):
     wants, bounds = c.backward()
     for g, w, b, what in zip((dx, da, db), wants, bounds, ("dx", "da", "db")):
         close(g, w, b, what)
+
+
+@pytest.mark.parametrize("T", [5, 300, 2100, 5000])
+@pytest.mark.parametrize("fill", [0, 255])
+def test_the_workspace_may_hold_anything_and_each_gradient_may_be_left_out(ex, hip_rt, T, fill):
+    """The calls of the C interface with a workspace full of zeros, or of ones (NaN, -1), and with
+    one output at a time: the executor's bits."""
+    lib = hip_rt.lib()
+    c = Case(T, T, 72, 40, 20, 5, BF16, adapters="each")
+    y = ex.lora_apply(c.lora, c.d_x, c.d_ad, c.d_base)
+    dx, da, db = ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy)
+    _, slots, rows = ex._lora_rows(c.lora, c.d_x, c.d_ad, None, c.d_base)
+    stream = torch.cuda.current_stream().cuda_stream
+    n = c.lora.space(lib, slots, T)
+    ws = torch.full((max(n, 16),), fill, dtype=torch.uint8, device=DEV)
+    got = torch.full_like(y, 3.0)
+    rc = lib.sabah_lora_apply(c.lora.ref, *rows, *ex._lora_y("base", c.d_base, T, 1, 40),
+                              *ex._lora_y("out", got, T, 1, 40), ws.data_ptr(), n, stream)
+    hip_rt.check(rc, "apply")
+    assert torch.equal(got, y)
+    n = c.lora.space(lib, slots, T, 1)
+    for which in range(3):
+        ws = torch.full((n,), fill, dtype=torch.uint8, device=DEV)
+        outs = [torch.full_like(g, 3.0) if i == which else None for i, g in enumerate((dx, da, db))]
+        d = ex._lora_y("dx", outs[0], T, 1, 72) if which == 0 else (None, 0, 0)
+        rc = lib.sabah_lora_backward(c.lora.ref, *rows, *ex._lora_y("dy", c.d_dy, T, 1, 40), *d, 0,
+                                     outs[1].data_ptr() if which == 1 else None,
+                                     outs[2].data_ptr() if which == 2 else None, 0, ws.data_ptr(), n, stream)
+        hip_rt.check(rc, "backward")
+        assert torch.equal(outs[which], (dx, da, db)[which]), which
+
+
+@pytest.mark.parametrize("T,E,groups", [(3, 8, 1), (96, 300, 8), (4000, 512, 4)])
+def test_the_losses_workspace_may_hold_anything(ex, hip_rt, T, E, groups):
+    lib = hip_rt.lib()
+    logits = torch.randn(T, E, generator=torch.Generator(device=DEV).manual_seed(T), device=DEV)
+    ids, _ = ex.route(logits, 4)
+    want = ex.balance(logits, ids, n_groups=groups)
+    n = lib.sabah_moe_balance_workspace(T, E, groups)
+    for fill in (0, 255):
+        ws = torch.full((n,), fill, dtype=torch.uint8, device=DEV)
+        got = [torch.full_like(t, 7) for t in (want.counts, want.mean_p, want.losses, want.n_valid)]
+        rc = lib.sabah_moe_balance(logits.data_ptr(), E * 4, ids.data_ptr(), None, T, E, 4, groups,
+                                   *(t.data_ptr() for t in got), ws.data_ptr(), n,
+                                   torch.cuda.current_stream().cuda_stream)
+        hip_rt.check(rc, "balance")
+        assert all(torch.equal(a, b) for a, b in zip(got, (want.counts, want.mean_p, want.losses, want.n_valid)))
