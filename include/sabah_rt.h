@@ -311,8 +311,9 @@ int sabah_moe_balance(const float *d_logits, size_t logits_stride, const int32_t
  * losses[1] (with sabah_moe_balance's d_counts and d_n_valid for the same mask and groups; the
  * counts are constants of the gradient; both may be NULL when c_balance and c_z are 0).
  * Every row of d_dlogits is written: zeros for a masked token, whose inputs are not
- * read, and for a row of minus infinities only.  An expert named twice by a token gets both parts.
- * An id out of range makes its token's row NaN and fails the next call.  d_dlogits overlaps no input. */
+ * read, and for a row of minus infinities only, whatever its ids (sabah_moe_route has no expert for it and
+ * writes -1).  An expert named twice by a token gets both parts.  Any other id out of range
+ * makes its token's row NaN and fails the next call.  d_dlogits overlaps no input. */
 int sabah_moe_route_backward(const float *d_logits, size_t logits_stride, const int32_t *d_ids, const uint8_t *d_mask,
                              int n_tokens, int n_experts, int n_used, int norm_w, float w_scale, const float *d_dw,
                              const int32_t *d_counts, const int32_t *d_n_valid, int n_groups, float c_balance, float c_z,

@@ -389,7 +389,6 @@ __global__ __launch_bounds__(row_threads(W)) void k_route_backward(RouteBackArgs
         if (a.dw && slot < a.n_used) {
             bad = id < 0 || id >= E;
             if (bad) {
-                *reinterpret_cast<volatile unsigned int*>(a.err) = kErrRouteId;
                 w = __builtin_nanf("");                     // the row becomes NaN
                 id = -1;
             } else {
@@ -397,6 +396,8 @@ __global__ __launch_bounds__(row_threads(W)) void k_route_backward(RouteBackArgs
             }
         }
         live = row_softmax<PER, W>(p, top, inv, lse, s_tmp);
+        // k_route has no expert for a row of minus infinities and names -1: no error, its token counts as masked
+        if (live && bad) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrRouteId;
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) d[j] = 0.0f;

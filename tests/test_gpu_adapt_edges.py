@@ -1,0 +1,44 @@
+"""Adapters and the router's losses where types and sizes end: wide ranges within a row, infinite
+weights, rows of infinities, high ranks, long batches (needs an MI355X).  Against the
+64-bit forms of adapt_refs.py within their counted roundings."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import adapt_refs as ref
+from test_gpu_balance import T as to_dev, batch
+from test_gpu_lora import BF16, DEV, F16, F32, Case, close, hip_ok
+
+pytestmark = pytest.mark.gpu
+
+TYPES = pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+
+
+@pytest.fixture(scope="module")
+def ex(hip_rt):
+    from sabah.runtime.bank import ExpertBank
+    from sabah.runtime.executor import MoEExecutor
+    return MoEExecutor(ExpertBank(1, 8, 256, 256, {"gate": 21, "up": 21, "down": 21}, device="cuda:0"))
+
+
+@pytest.mark.parametrize("E,k", [(60, 6), (512, 10), (700, 8)])
+@pytest.mark.parametrize("norm_w", [True, False])
+def test_the_routes_own_ids_of_a_row_without_experts_raise_nothing(ex, E, k, norm_w):
+    """route() has no expert for a row of minus infinities and says -1.  Such a token counts as masked: its
+    gradient is zeros, and the next call goes through."""
+    logits, _, _, dw = batch(E, 21, E, k)
+    logits[3], logits[20] = -np.inf, -np.inf
+    d_l = to_dev(logits)
+    ids, _ = ex.route(d_l, k, norm_w)
+    b = ex.balance(d_l, ids, n_groups=3)
+    got = ex.route_backward(d_l, ids, to_dev(dw), b, 0.7, 0.3, norm_w=norm_w)
+    torch.cuda.synchronize()
+    hip_ok()
+    host = ids.cpu().numpy()
+    _, _, _, n_valid, valid, _, _ = ref.router_losses(logits.astype(np.float64), host, None, 3)
+    assert not valid[3] and not valid[20] and np.array_equal(b.n_valid.cpu().numpy(), n_valid)
+    want, bound = ref.router_gradient(logits.astype(np.float64), host, valid, 3, dw.astype(np.float64), norm_w, 1.0, 0.7, 0.3)
+    close(got, want, bound, "dlogits")
+    assert not got[3].any() and not got[20].any()
