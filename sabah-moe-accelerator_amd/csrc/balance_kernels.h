@@ -122,7 +122,7 @@ __device__ inline bool row_softmax(float (&e)[PER], float& m, float& inv, float&
 #pragma unroll
     for (int j = 0; j < PER; ++j) e[j] *= inv;
     lse = m + logf(s);
-    if (m == __builtin_inff()) lse = __builtin_nanf("");
+    if (m == __builtin_inff()) lse = row_max<W>(nan ? 1.0f : 0.0f, tmp) > 0.0f ? __builtin_nanf("") : m;   // m: an infinite logit
     return true;
 }
 

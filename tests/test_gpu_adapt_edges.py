@@ -42,3 +42,18 @@ def test_the_routes_own_ids_of_a_row_without_experts_raise_nothing(ex, E, k, nor
     want, bound = ref.router_gradient(logits.astype(np.float64), host, valid, 3, dw.astype(np.float64), norm_w, 1.0, 0.7, 0.3)
     close(got, want, bound, "dlogits")
     assert not got[3].any() and not got[20].any()
+
+
+@pytest.mark.parametrize("E", [24, 512, 700])
+def test_an_infinite_logit_has_an_infinite_log_sum(ex, E):
+    """lse of a row with an infinity is infinite, of one with a NaN a NaN; neither has probabilities."""
+    logits, ids, _, dw = batch(E, 12, E, 4)
+    logits[5, 7] = np.inf
+    b = ex.balance(to_dev(logits), to_dev(ids))
+    assert b.losses[1].item() == float("inf") and b.losses[0].isnan() and b.mean_p.isnan().all()
+    got = ex.route_backward(to_dev(logits), to_dev(ids), to_dev(dw), b, 0.0, 0.3)
+    assert got[5].isnan().all()
+    logits[6, 3] = np.nan
+    assert ex.balance(to_dev(logits), to_dev(ids)).losses.isnan().all()
+    logits[6] = np.inf
+    assert ex.balance(to_dev(logits), to_dev(ids)).losses[1].item() == float("inf")
