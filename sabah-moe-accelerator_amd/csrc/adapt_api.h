@@ -134,7 +134,10 @@ SABAH_API int sabah_moe_balance(const float* d_logits, size_t logits_stride, con
 template <int PER, int VEC, int W>
 static void launch_route_backward(const RouteBackArgs& a, hipStream_t st) {
     constexpr int kSide = row_threads(W) / (64 * W);               // tokens of a workgroup
-    hipLaunchKernelGGL((k_route_backward<PER, VEC, W>), dim3((unsigned)((a.n_tokens + kSide - 1) / kSide)),
+    // a launch takes fewer than 2^32 threads along x, and 2^24 tokens of a workgroup each are more
+    constexpr unsigned kMost = 1u << 20;
+    const unsigned groups = (unsigned)((a.n_tokens + kSide - 1) / kSide);
+    hipLaunchKernelGGL((k_route_backward<PER, VEC, W>), dim3(std::min(groups, kMost), (groups + kMost - 1) / kMost),
                        dim3(row_threads(W)), 0, st, a);
 }
 

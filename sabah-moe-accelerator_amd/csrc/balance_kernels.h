@@ -367,7 +367,7 @@ __global__ __launch_bounds__(row_threads(W)) void k_route_backward(RouteBackArgs
     __shared__ float s_tmp[W];
     __shared__ float s_add[kSide][64 * W * PER];
     const int tid = (int)threadIdx.x, v = tid % (64 * W), side = tid / (64 * W), slot = tid & 63, E = a.n_experts;
-    const int t = (int)blockIdx.x * kSide + side;
+    const int t = ((int)blockIdx.y * (int)gridDim.x + (int)blockIdx.x) * kSide + side;
     if (t >= a.n_tokens) return;                            // W = 1: whole waves leave, and no barrier follows
     const uint8_t* row = a.logits + (size_t)t * a.stride;
     float* out = reinterpret_cast<float*>(a.dlogits + (size_t)t * a.dstride);

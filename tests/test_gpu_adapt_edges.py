@@ -57,3 +57,21 @@ def test_an_infinite_logit_has_an_infinite_log_sum(ex, E):
     assert ex.balance(to_dev(logits), to_dev(ids)).losses.isnan().all()
     logits[6] = np.inf
     assert ex.balance(to_dev(logits), to_dev(ids)).losses[1].item() == float("inf")
+
+
+def test_the_gradient_of_as_many_tokens_as_a_call_takes(ex):
+    """2^24 tokens of 513 experts: all but a few at both ends and between are masked."""
+    n, E, k = 1 << 24, 513, 4
+    at = [0, 1, 4095, (1 << 20) - 1, 1 << 20, (1 << 23) + 5, n - 2, n - 1]
+    logits, ids, _, dw = batch(1, len(at), E, k)
+    d_l = torch.empty(n, E, device=DEV)
+    d_i, d_w = torch.zeros(n, k, dtype=torch.int32, device=DEV), torch.zeros(n, k, device=DEV)
+    mask = torch.zeros(n, dtype=torch.bool, device=DEV)
+    d_l[at], d_i[at], d_w[at], mask[at] = to_dev(logits), to_dev(ids), to_dev(dw), True
+    out = torch.full((n, E), 5.0, device=DEV)
+    got = ex.route_backward(d_l, d_i, d_w, mask=mask, out=out)
+    want, bound = ref.router_gradient(logits.astype(np.float64), ids, np.ones(len(at), bool), 1, dw.astype(np.float64),
+                                      True, 1.0, 0, 0)
+    close(got[at], want, bound, "dlogits")
+    got[at] = 0
+    assert not any(bool(part.any()) for part in got.split(1 << 21))
