@@ -10,7 +10,8 @@
 // A row of minus infinities only has no distribution: its token counts as masked.
 //
 // k_balance_rows: one wave per token at a time (a workgroup above 512 experts), a workgroup per run of a group's tokens;
-//   the sums of p stay in registers (f32) and the counts in LDS; one partial per workgroup.
+//   the sums of p stay in registers (f32 for 64 tokens at a time, those sums in 64 bits: the 8,192 tokens that a lane
+//   of a long batch has would be off by 1e-4 in f32) and the counts in LDS; one partial per workgroup.
 // k_balance_sum:  the partials of 16 experts per workgroup, in a fixed order (no
 //   float atomics: the same inputs give the same bits); the last workgroup adds up the losses.
 // k_route_backward: the same split; the row stays in registers between the softmax
@@ -164,6 +165,7 @@ __global__ __launch_bounds__(row_threads(W)) void k_balance_rows(BalanceArgs a) 
     extern __shared__ float blds[];
     constexpr int kThr = row_threads(W), kSide = kThr / (64 * W);   // kSide tokens side by side
     constexpr int B = W == 1 ? 4 : 1;                       // and B of them loaded at a time
+    constexpr int kRun = 64;                                // terms summed in f32; such sums meet in 64 bits
     __shared__ int s_n[kSide];
     __shared__ float s_z[kSide];
     __shared__ float s_tmp[W];
@@ -176,10 +178,11 @@ __global__ __launch_bounds__(row_threads(W)) void k_balance_rows(BalanceArgs a) 
     for (int i = tid; i < E; i += kThr) s_c[i] = 0;
     __syncthreads();
     float acc[PER];
+    double sum[PER], z_sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < PER; ++j) acc[j] = 0.0f, sum[j] = 0.0;
     float z = 0.0f;
-    int n = 0;
+    int n = 0, left = kRun / B;
     const int end = min(a.group_len, (c + 1) * a.chunk_len);
     for (int i0 = c * a.chunk_len + side; i0 < end; i0 += kSide * B) {
         float e[B][PER];
@@ -207,10 +210,18 @@ __global__ __launch_bounds__(row_threads(W)) void k_balance_rows(BalanceArgs a) 
                 else *reinterpret_cast<volatile unsigned int*>(a.err) = kErrRouteId;
             }
         }
+        if (--left == 0) {
+            left = kRun / B;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) sum[j] += (double)acc[j], acc[j] = 0.0f;
+            z_sum += (double)z, z = 0.0f;
+        }
     }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) acc[j] = (float)(sum[j] + (double)acc[j]);
     if (v == 0) {
         s_n[side] = n;
-        s_z[side] = z;
+        s_z[side] = (float)(z_sum + (double)z);
     }
     // the sums of the tokens side by side, in their order
     for (int w = 0; w < kSide; ++w) {

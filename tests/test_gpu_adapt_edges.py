@@ -59,6 +59,24 @@ def test_an_infinite_logit_has_an_infinite_log_sum(ex, E):
     assert ex.balance(to_dev(logits), to_dev(ids)).losses[1].item() == float("inf")
 
 
+@pytest.mark.parametrize("n,E,groups", [(1 << 24, 8, 1), (1 << 21, 516, 1), (1 << 22, 40, 64)])
+def test_the_means_of_long_batches(ex, n, E, groups):
+    """The same row in every token: each rounding of a long sum goes the same way.  Its mean is p and the
+    z loss lse^2, within the roundings of p and lse, runs of 64 terms, the sides' and the result's."""
+    row = torch.linspace(-1.0, 1.3, E, device=DEV)
+    logits = row.expand(n, E).contiguous()
+    ids = torch.arange(2, dtype=torch.int32, device=DEV).expand(n, 2).contiguous()
+    b = ex.balance(logits, ids, n_groups=groups)
+    l64 = row.double()
+    p, lse = torch.softmax(l64, 0), torch.logsumexp(l64, 0)
+    # exp's argument and exp, the sum of E terms, the reciprocal and product; 64 terms; four sides; the result
+    rel = ref.U * (2.3 + E + 12 + 64 + 4 + 4)
+    assert ((b.mean_p.double() - p).abs() <= rel * p).all()
+    want = lse * lse
+    assert abs(b.losses[1].double() - want) <= ref.U * (2 * (abs(lse) * 2 + E + 8) * abs(lse) + 76 * want)
+    assert (b.counts[:, :2] == n // groups).all() and not b.counts[:, 2:].any()
+
+
 def test_the_gradient_of_as_many_tokens_as_a_call_takes(ex):
     """2^24 tokens of 513 experts: all but a few at both ends and between are masked."""
     n, E, k = 1 << 24, 513, 4
