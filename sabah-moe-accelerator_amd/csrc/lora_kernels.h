@@ -336,8 +336,11 @@ __device__ inline void lora_plain_rows(const LoraArgs& a, int key, int n, const 
 //   bf16 weights   the f32 operand in three bf16 pieces that add up to it exactly (each keeps the next 8 of
 //                  its 24 bits), three v_mfma_f32_16x16x32_bf16: 48 cycles, the same products
 //   f16 weights    two f16 pieces of 11 bits, rounded to nearest, of the operand scaled by a power of two that
-//                  brings its row's largest of these values to 2^14 .. 2^15: what is left out is below
-//                  2^-24 of a value, or 2^-39 of the largest.  32 cycles, and a product with the scale
+//                  brings its row's largest of these values to 2^14 .. 2^15: what is left out is at most
+//                  2^-23 of a value.  32 cycles, and a product with the scale.  Below 2^-16 of the largest that no
+//                  longer holds (f16's exponents end; and the instruction aligns its products to the largest's even where that
+//                  one's weight is 0): the shrink takes such values as bf16 products, of both pieces that an
+//                  f16 weight has there, and the expand does their rows with plain products
 // Sums are f32.  An infinity has no pieces (its rest is inf - inf): a wave that meets one does the rows
 // that have it again with plain products.
 // ---------------------------------------------------------------------------
@@ -375,10 +378,14 @@ __device__ inline void lora_split(LoraBF16, const float (&x)[8], float, LoraWord
         }
     }
 }
-__device__ inline void lora_split(LoraF16, const float (&x)[8], float scale, LoraWords (&w)[2]) {
+// Returns whether some value is small: not 0, and below 2^-2 (2^-16 of the largest)
+__device__ inline bool lora_split(LoraF16, const float (&x)[8], float scale, LoraWords (&w)[2]) {
+    uint32_t least = 0xFFFFFFFFu;                           // of the magnitudes' words times two less one: a 0 is the largest
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         lf2 r = {x[2 * c] * scale, x[2 * c + 1] * scale};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) least = min(least, 2u * __float_as_uint(r[e]) - 1u);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const lh2 h = __builtin_convertvector(r, lh2);
@@ -387,6 +394,46 @@ __device__ inline void lora_split(LoraF16, const float (&x)[8], float scale, Lor
             r[1] = r[1] - (float)h[1];
         }
     }
+    return least < 2u * 0x3E800000u - 1u;
+}
+// The small values in the three bf16 pieces of an f32 operand, zeros for the others, and zeros in their f16 pieces:
+// a row's sum is the same whichever rows are beside it
+__device__ inline void lora_small(const float (&x)[8], float scale, LoraWords (&h)[2], LoraWords (&w)[3]) {
+    float r[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        const float v = x[c] * scale;
+        const bool small = __builtin_fabsf(v) < 0.25f;
+        r[c] = small ? v : 0.0f;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+            if (small) h[g].u[c / 2] &= c & 1 ? 0xFFFFu : 0xFFFF0000u;
+    }
+    lora_split(LoraBF16{}, r, 1.0f, w);
+}
+// f16 weights in two bf16 pieces (8 of their 11 bits, and 3)
+__device__ inline void lora_bf16_of(const LoraWords& h, LoraWords (&w)[2]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const lh2 v = __builtin_bit_cast(lh2, h.u[c]);
+        float r[2] = {(float)v[0], (float)v[1]};
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            w[g].u[c] = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302u);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) r[e] = r[e] - __uint_as_float(__float_as_uint(r[e]) & 0xFFFF0000u);
+        }
+    }
+}
+// d + weights times small values
+__device__ inline lf4 lora_add_small(const LoraWords& h, const LoraWords (&r)[3], lf4 d) {
+    LoraWords w[2];
+    lora_bf16_of(h, w);
+#pragma unroll
+    for (int g = 2; g >= 0; --g)
+#pragma unroll
+        for (int z = 1; z >= 0; --z) d = lora_mfma(LoraBF16{}, w[z], r[g], d);
+    return d;
 }
 // The power of two that brings `most` to 2^14 .. 2^15 (at most 2^126), and its inverse
 __device__ inline float lora_scale_of(float most, float& back) {
@@ -407,6 +454,11 @@ __device__ inline float lora_column_most(float most) {
     const uint32_t n = max(h[0], h[1]);                                     // magnitudes order as words
     const auto r = __builtin_amdgcn_permlane16_swap(n, n, false, false);
     return __uint_as_float(max(r[0], r[1]));
+}
+// the rows (columns) that lanes of a ballot hold
+__device__ inline unsigned lora_rows_of(uint64_t lanes) {
+    lanes |= lanes >> 32;
+    return (unsigned)(lanes | lanes >> 16) & 0xFFFFu;
 }
 __device__ inline unsigned lora_big_rows(float most) {
     return (unsigned)(__ballot(lora_column_most(most) == __builtin_inff()) & 0xFFFFu);
@@ -542,11 +594,17 @@ struct LoraShrink {
                 float back = 1.0f, scale = 1.0f;
                 if constexpr (std::is_same<W, LoraF16>::value) scale = lora_scale_of(lora_column_most(here), back);
                 LoraWords P[kLoraPieces<W>];
-                lora_split(W{}, v, scale, P);
                 if constexpr (std::is_same<W, LoraF16>::value) {
+                    const bool some = lora_split(W{}, v, scale, P);
                     lf4 d[NR];
 #pragma unroll
                     for (int b = 0; b < NR; ++b) d[b] = lf4{0, 0, 0, 0};
+                    if (__any(some)) {                      // about one step in a hundred of normally distributed values
+                        LoraWords R[3];
+                        lora_small(v, scale, P, R);
+#pragma unroll
+                        for (int b = 0; b < NR; ++b) d[b] = lora_add_small(w[b], R, d[b]);
+                    }
 #pragma unroll
                     for (int g = kLoraPieces<W> - 1; g >= 0; --g)
 #pragma unroll
@@ -556,6 +614,7 @@ struct LoraShrink {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[t][b][i] = __builtin_fmaf(d[b][i], back, acc[t][b][i]);
                 } else {
+                    lora_split(W{}, v, scale, P);
 #pragma unroll
                     for (int g = kLoraPieces<W> - 1; g >= 0; --g)
 #pragma unroll
@@ -794,7 +853,8 @@ struct LoraExpand {
             else mask[j] = counts(j, rk);
             asm volatile("" : "+v"(mask[j]));               // kept as a word
         }
-        unsigned rows_in[H], alone[H];                      // the rows to be written here, and those with an infinity in s
+        // the rows to be written here, and those with an infinity in s, or with values too small for f16 pieces
+        unsigned rows_in[H], alone[H];
         LoraWords P[H][NP][N > 0 ? N : 1];
         float back[H][4];                                   // of the lane's four rows
 #pragma unroll
@@ -805,9 +865,9 @@ struct LoraExpand {
             for (int i = 0; i < 4; ++i) back[t][i] = 1.0f;
             if constexpr (N > 0) {
                 const float most = lora_most(s[t], 0.0f);
-                if (__any(most == __builtin_inff())) alone[t] = lora_big_rows(most) & rows_in[t];
-                rows_in[t] &= ~alone[t];
+                if (__any(most == __builtin_inff())) alone[t] = lora_big_rows(most);
                 float scale = 1.0f;
+                bool some = false;
                 if constexpr (std::is_same<W, LoraF16>::value) {
                     float mine;
                     scale = lora_scale_of(lora_column_most(most), mine);
@@ -819,8 +879,12 @@ struct LoraExpand {
                     float v[8];
 #pragma unroll
                     for (int c = 0; c < 8; ++c) v[c] = 8 * b + c < 4 * NR ? s[t][(8 * b + c) % (4 * NR)] : 0.0f;
-                    lora_split(W{}, v, scale, P[t][b]);
+                    if constexpr (std::is_same<W, LoraF16>::value) some |= lora_split(W{}, v, scale, P[t][b]);
+                    else lora_split(W{}, v, scale, P[t][b]);
                 }
+                if (__any(some)) alone[t] |= lora_rows_of(__ballot(some));
+                alone[t] &= rows_in[t];
+                rows_in[t] &= ~alone[t];
             }
         }
         for (; o0 < c1; o0 += 64 * NW) {

@@ -23,6 +23,11 @@ def ex(hip_rt):
     return MoEExecutor(ExpertBank(1, 8, 256, 256, {"gate": 21, "up": 21, "down": 21}, device="cuda:0"))
 
 
+def all_close(got, want, bound):
+    for g, w, b, what in zip(got, want, bound, ("dx", "da", "db")):
+        close(g, w, b, what)
+
+
 @pytest.mark.parametrize("E,k", [(60, 6), (512, 10), (700, 8)])
 @pytest.mark.parametrize("norm_w", [True, False])
 def test_the_routes_own_ids_of_a_row_without_experts_raise_nothing(ex, E, k, norm_w):
@@ -57,6 +62,45 @@ def test_an_infinite_logit_has_an_infinite_log_sum(ex, E):
     assert ex.balance(to_dev(logits), to_dev(ids)).losses.isnan().all()
     logits[6] = np.inf
     assert ex.balance(to_dev(logits), to_dev(ids)).losses[1].item() == float("inf")
+
+
+@TYPES
+@pytest.mark.parametrize("T,rank", [(5, 8), (40, 24), (200, 40), (600, 64), (600, 100), (4500, 20)])
+@pytest.mark.parametrize("size", [3e5, 1e8, 1e12])
+def test_a_large_value_that_no_weight_meets(ex, T, rank, size, dtype):
+    """One value of some rows is up to 1e12 times the others and its weights are zeros, or it makes an s
+    (u) that large whose weights are zeros: what the others give is right to f32 all the same, and
+    rows without such values keep their bits."""
+    c = Case(T + rank, T, 100, 44, rank, 2, dtype, adapters=[t % 2 for t in range(T)])
+    clean = ex.lora_apply(c.lora, c.d_x, c.d_ad, c.d_base)
+    c.lora.a[:, :, :, 5] = 0
+    c.lora.a[:, :, 2, 70] = 100.0
+    c.lora.a[:, :, :2, 70] = 0
+    c.lora.a[:, :, 3:, 70] = 0
+    c.lora.b[:, :, :, 2] = 0
+    clean = ex.lora_apply(c.lora, c.d_x, c.d_ad, c.d_base)
+    wide = np.arange(T) % 3 == 0
+    c.x[wide, :, 5] = size
+    c.x[wide, :, 70] = size / 100
+    c.d_x.copy_(torch.from_numpy(c.x))
+    want, bound = c.forward()
+    got = ex.lora_apply(c.lora, c.d_x, c.d_ad, c.d_base)
+    close(got, want, bound, "forward")
+    same = torch.from_numpy(~wide).to(DEV)
+    assert torch.equal(got[same], clean[same])
+    # the same backward: dy's value 3 meets zeros of B but at rank 1, whose row of A is zeros
+    c.lora.b[:, :, 3, :] = 0
+    c.lora.b[:, :, 3, 1] = 1.0
+    c.lora.b[:, :, 9, :] = 0
+    c.lora.a[:, :, 1, :] = 0
+    clean = ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy)[0]
+    c.dy[wide, :, 3] = size
+    c.dy[wide, :, 9] = -size
+    c.d_dy.copy_(torch.from_numpy(c.dy))
+    want, bound = c.backward()
+    got = ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy)
+    all_close(got, want, bound)
+    assert torch.equal(got[0][same], clean[same])
 
 
 @pytest.mark.parametrize("n,E,groups", [(1 << 24, 8, 1), (1 << 21, 516, 1), (1 << 22, 40, 64)])
