@@ -337,10 +337,13 @@ __device__ inline void lora_plain_rows(const LoraArgs& a, int key, int n, const 
 //                  its 24 bits), three v_mfma_f32_16x16x32_bf16: 48 cycles, the same products
 //   f16 weights    two f16 pieces of 11 bits, rounded to nearest, of the operand scaled by a power of two that
 //                  brings its row's largest of these values to 2^14 .. 2^15: what is left out is at most
-//                  2^-23 of a value.  32 cycles, and a product with the scale.  Below 2^-16 of the largest that no
-//                  longer holds (f16's exponents end; and the instruction aligns its products to the largest's even where that
-//                  one's weight is 0): the shrink takes such values as bf16 products, of both pieces that an
-//                  f16 weight has there, and the expand does their rows with plain products
+//                  2^-23 of a value.  32 cycles, and a product with the scale.  Below 2^-2 f16's exponents end: at
+//                  2^-4, 2^-18 of the largest, up to 2^-21 is left out, and below that all may be (the instruction also
+//                  aligns its products to the largest's, even where that one's weight is 0).  Rows with
+//                  values below 2^-4 take the f32 form, about one step of 16 rows in four hundred of normally distributed
+//                  values (with 2^-2 for the line, one in a hundred, 1,999 rows at rank 64 took 30.5 us, with 2^-4 29.4;
+//                  28.4 without any).  Which they are goes by the row alone: its sums are the same whichever
+//                  rows are beside it
 // Sums are f32.  An infinity has no pieces (its rest is inf - inf): a wave that meets one does the rows
 // that have it again with plain products.
 // ---------------------------------------------------------------------------
@@ -378,7 +381,7 @@ __device__ inline void lora_split(LoraBF16, const float (&x)[8], float, LoraWord
         }
     }
 }
-// Returns whether some value is small: not 0, and below 2^-2 (2^-16 of the largest)
+// Returns whether some value is small: not 0, and below 2^-4
 __device__ inline bool lora_split(LoraF16, const float (&x)[8], float scale, LoraWords (&w)[2]) {
     uint32_t least = 0xFFFFFFFFu;                           // of the magnitudes' words times two less one: a 0 is the largest
 #pragma unroll
@@ -394,46 +397,12 @@ __device__ inline bool lora_split(LoraF16, const float (&x)[8], float scale, Lor
             r[1] = r[1] - (float)h[1];
         }
     }
-    return least < 2u * 0x3E800000u - 1u;
+    return least < 2u * 0x3D800000u - 1u;
 }
-// The small values in the three bf16 pieces of an f32 operand, zeros for the others, and zeros in their f16 pieces:
-// a row's sum is the same whichever rows are beside it
-__device__ inline void lora_small(const float (&x)[8], float scale, LoraWords (&h)[2], LoraWords (&w)[3]) {
-    float r[8];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        const float v = x[c] * scale;
-        const bool small = __builtin_fabsf(v) < 0.25f;
-        r[c] = small ? v : 0.0f;
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-            if (small) h[g].u[c / 2] &= c & 1 ? 0xFFFFu : 0xFFFF0000u;
-    }
-    lora_split(LoraBF16{}, r, 1.0f, w);
-}
-// f16 weights in two bf16 pieces (8 of their 11 bits, and 3)
-__device__ inline void lora_bf16_of(const LoraWords& h, LoraWords (&w)[2]) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const lh2 v = __builtin_bit_cast(lh2, h.u[c]);
-        float r[2] = {(float)v[0], (float)v[1]};
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            w[g].u[c] = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302u);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) r[e] = r[e] - __uint_as_float(__float_as_uint(r[e]) & 0xFFFF0000u);
-        }
-    }
-}
-// d + weights times small values
-__device__ inline lf4 lora_add_small(const LoraWords& h, const LoraWords (&r)[3], lf4 d) {
-    LoraWords w[2];
-    lora_bf16_of(h, w);
-#pragma unroll
-    for (int g = 2; g >= 0; --g)
-#pragma unroll
-        for (int z = 1; z >= 0; --z) d = lora_mfma(LoraBF16{}, w[z], r[g], d);
-    return d;
+// value c of eight 16-bit ones
+template <typename W>
+__device__ inline float lora_value(const LoraWords& w, int c) {
+    return W::value((uint16_t)(c & 1 ? w.u[c / 2] >> 16 : w.u[c / 2] & 0xFFFFu));
 }
 // The power of two that brings `most` to 2^14 .. 2^15 (at most 2^126), and its inverse
 __device__ inline float lora_scale_of(float most, float& back) {
@@ -599,16 +568,26 @@ struct LoraShrink {
                     lf4 d[NR];
 #pragma unroll
                     for (int b = 0; b < NR; ++b) d[b] = lf4{0, 0, 0, 0};
-                    if (__any(some)) {                      // about one step in a hundred of normally distributed values
-                        LoraWords R[3];
-                        lora_small(v, scale, P, R);
-#pragma unroll
-                        for (int b = 0; b < NR; ++b) d[b] = lora_add_small(w[b], R, d[b]);
-                    }
 #pragma unroll
                     for (int g = kLoraPieces<W> - 1; g >= 0; --g)
 #pragma unroll
                         for (int b = 0; b < NR; ++b) d[b] = lora_mfma(W{}, w[b], P[g], d[b]);
+                    if (__builtin_expect(__any(some), 0)) {
+                        __builtin_amdgcn_wave_barrier();
+                        const bool mine = (lora_rows_of(__ballot(some)) >> p) & 1u;
+                        if (mine) back = 1.0f;
+                        const lf4 y[2] = {lx[p * 9 + 2 * q], lx[p * 9 + 2 * q + 1]};    // x again, not kept until here
+#pragma unroll
+                        for (int b = 0; b < NR; ++b) {
+                            lf4 e = {0, 0, 0, 0};
+#pragma unroll
+                            for (int c = 0; c < 8; ++c)
+                                e = __builtin_amdgcn_mfma_f32_16x16x4f32(lora_value<W>(w[b], c), y[c >> 2][c & 3], e, 0, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) d[b][i] = mine ? e[i] : d[b][i];
+                        }
+                        __builtin_amdgcn_wave_barrier();
+                    }
 #pragma unroll
                     for (int b = 0; b < NR; ++b)
 #pragma unroll
@@ -818,31 +797,6 @@ struct LoraExpand {
             }
         }
     }
-    // rare: 64 columns of row t of sixteen x of the tile with plain products
-    __device__ inline void plain(const float (&s)[4 * NR], int rk, int o0, int x, int t) const {
-        const int lane = (int)threadIdx.x & 63, o = o0 + lane;
-        float sum = 0.0f;
-        for (int r = 0; r < rk; ++r) {
-            float v = 0.0f;                                 // S's rank r, from the lane that counts it
-#pragma unroll
-            for (int j = 0; j < 4 * NR; ++j)
-                if (at[j / GW] + j % GW == r && counts(j, rk)) v = s[j];
-            const uint64_t who = __ballot(p == t && v != 0.0f);
-            v = who ? __shfl(v, __builtin_ctzll(who)) : 0.0f;
-            if (o < c1) sum = __builtin_fmaf(W::value(B[(uint32_t)o * (uint32_t)rank + r]), v, sum);
-        }
-        uint64_t to = 0, from = 0;                          // lane 16 (t / 4) holds the row's addresses
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i == (t & 3)) to = (uint64_t)(uintptr_t)dst[x][i], from = (uint64_t)(uintptr_t)base[x][i];
-        auto there = [&](uint64_t a) {
-            return (uintptr_t)((uint64_t)(uint32_t)__shfl((int)(uint32_t)a, 16 * (t >> 2)) |
-                               (uint64_t)(uint32_t)__shfl((int)(uint32_t)(a >> 32), 16 * (t >> 2)) << 32);
-        };
-        float* y = reinterpret_cast<float*>(there(to));
-        const float* b = reinterpret_cast<const float*>(there(from));
-        if (o < c1) y[o] = b ? b[o] + sum : sum;
-    }
     // The wave's steps from o0 on.  s: the lane's S, already scaled, zeros where a value does not count
     __device__ inline void run(int o0, const float (&s)[H][4 * NR], int rk) const {
         constexpr int NP = (NR + 1) / 2, N = kLoraPieces<W>, M = N > 0 ? 2 : 1;   // products of 32 ranks, pieces, values of a mask
@@ -853,7 +807,7 @@ struct LoraExpand {
             else mask[j] = counts(j, rk);
             asm volatile("" : "+v"(mask[j]));               // kept as a word
         }
-        // the rows to be written here, and those with an infinity in s, or with values too small for f16 pieces
+        // the rows to be written here, and those with an infinity in s, or with values too small for its f16 pieces
         unsigned rows_in[H], alone[H];
         LoraWords P[H][NP][N > 0 ? N : 1];
         float back[H][4];                                   // of the lane's four rows
@@ -939,7 +893,15 @@ struct LoraExpand {
                 }
                 store(y[t], d, t, o0, rows_in[t]);
                 if constexpr (N > 0) {
-                    for (unsigned left = alone[t]; left; left &= left - 1u) plain(s[t], rk, o0, t, __builtin_ctz(left));
+                    if (__builtin_expect(alone[t], 0)) {     // rare: those rows in the f32 form
+                        lf4 e[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+                        for (int j = 0; j < 4 * NR; ++j)
+#pragma unroll
+                            for (int h = 0; h < 4; ++h)
+                                e[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[t][j], lora_value<W>(ww[j / 8][h], j % 8), e[h], 0, 0, 0);
+                        store(y[t], e, t, o0, alone[t]);
+                    }
                 }
             }
         }
