@@ -357,8 +357,8 @@ int sabah_lora_apply(const sabah_lora_desc *lora, const float *d_x, size_t x_id_
  * Each of d_dx, d_da and d_db may be NULL; they overlap neither each other nor an input.
  * n_adapters * n_experts <= 2^15.  A row with an id out of range gives no part of d_da and d_db, its dx is NaN,
  * and the next call fails.  A value of x or dy that is not finite, or at least 3.39e38 (what rounds to infinity in
- * bf16), leaves its pair's d_da and d_db not finite within the adapter's rank (NaN, also where
- * the sums would give an infinity), and no other pair's. */
+ * bf16), or an infinite one of A or B, leaves its pair's d_da or d_db not finite within the adapter's rank (NaN, also
+ * where the sums would give an infinity), and no other pair's; dx is what the sums give. */
 int sabah_lora_backward(const sabah_lora_desc *lora, const float *d_x, size_t x_id_stride, int x_rows,
                         size_t x_token_stride, const int32_t *d_adapters, const int32_t *d_ids, size_t ids_id_stride,
                         size_t ids_token_stride, int n_ids, int n_tokens, const float *d_dy, size_t dy_id_stride,

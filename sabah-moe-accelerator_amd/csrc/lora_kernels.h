@@ -341,11 +341,11 @@ __device__ inline void lora_plain_rows(const LoraArgs& a, int key, int n, const 
 //                  2^-4, 2^-18 of the largest, up to 2^-21 is left out, and below that all may be (the instruction also
 //                  aligns its products to the largest's, even where that one's weight is 0).  Rows with
 //                  values below 2^-4 take the f32 form, about one step of 16 rows in four hundred of normally distributed
-//                  values (with 2^-2 for the line, one in a hundred, 1,999 rows at rank 64 took 30.5 us, with 2^-4 29.4;
-//                  28.4 without any).  Which they are goes by the row alone: its sums are the same whichever
+//                  values (with 2^-2 for the line, one in a hundred, 1,999 rows at rank 64 took 30.5 us, with 2^-4 28.9;
+//                  28.3 without any).  Which they are goes by the row alone: its sums are the same whichever
 //                  rows are beside it
-// Sums are f32.  An infinity has no pieces (its rest is inf - inf): a wave that meets one does the rows
-// that have it again with plain products.
+// Sums are f32.  An infinity has no pieces (its rest is inf - inf), and one of the weights meets pieces that are 0: sums that
+// come out as NaN are done again in the f32 form.
 // ---------------------------------------------------------------------------
 typedef __bf16 lb8 __attribute__((ext_vector_type(8)));
 typedef _Float16 lh2 __attribute__((ext_vector_type(2)));
@@ -429,9 +429,6 @@ __device__ inline unsigned lora_rows_of(uint64_t lanes) {
     lanes |= lanes >> 32;
     return (unsigned)(lanes | lanes >> 16) & 0xFFFFu;
 }
-__device__ inline unsigned lora_big_rows(float most) {
-    return (unsigned)(__ballot(lora_column_most(most) == __builtin_inff()) & 0xFFFFu);
-}
 
 // Two values' next bf16 piece, to nearest, packed, and their rests.  Three such pieces are within 2^-24 of a value, and so
 // are the six products that k_lora_grad keeps of two values' nine.
@@ -464,7 +461,6 @@ struct LoraShrink {
     lf4 *lx, *la;                                           // the wave's
     int k, s0, steps, p, q, lane, rank;                     // whole steps s0 .. steps, and k's rest if steps is the last
     bool second;                                            // the tile has more than 16 rows
-    float most[H];
     lf4 acc[H][NR];
 
     // row: of the lane's places lane % 16 in the tile of n rows; lds: NW * (kLoraXLds + kLoraALds<W>); of k the steps from s0
@@ -558,10 +554,8 @@ struct LoraShrink {
                 float v[8];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) v[c] = x[c >> 2][c & 3];
-                const float here = lora_most(v, 0.0f);
-                most[t] = fmaxf(most[t], here);
                 float back = 1.0f, scale = 1.0f;
-                if constexpr (std::is_same<W, LoraF16>::value) scale = lora_scale_of(lora_column_most(here), back);
+                if constexpr (std::is_same<W, LoraF16>::value) scale = lora_scale_of(lora_column_most(lora_most(v, 0.0f)), back);
                 LoraWords P[kLoraPieces<W>];
                 if constexpr (std::is_same<W, LoraF16>::value) {
                     const bool some = lora_split(W{}, v, scale, P);
@@ -619,14 +613,13 @@ struct LoraShrink {
             }
         }
     }
-    __device__ inline void run() {
+    // rk: the adapter's own rank
+    __device__ inline void run(int rk) {
         const int wave = (int)threadIdx.x >> 6;
 #pragma unroll
-        for (int t = 0; t < H; ++t) {
-            most[t] = 0.0f;
+        for (int t = 0; t < H; ++t)
 #pragma unroll
             for (int b = 0; b < NR; ++b) acc[t][b] = lf4{0, 0, 0, 0};
-        }
         In in[U];
         for (int s = s0 + wave; s < steps; s += U * NW) {
 #pragma unroll
@@ -639,52 +632,76 @@ struct LoraShrink {
             load_rest(in[0], steps);
             mul(in[0]);
         }
+        if constexpr (kLoraPieces<W> > 0) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int t = 0; t < H; ++t)
+#pragma unroll
+                for (int b = 0; b < NR; ++b) most = max(most, largest(acc[t][b], 16 * b, rk));
+            if (__builtin_expect(__any(most > kInfinity), 0)) again(wave, rk);
+        }
+    }
+    // rare: the sums that are NaN once more in the f32 form, sixteen ranks of sixteen rows at a time (in few registers): always
+    // the first ones, and the others move up
+    __device__ inline void again(int wave, int rk) {
+        constexpr int N = 8;
+        const int end = steps + (rest_is(wave) ? 1 : 0);
+#pragma unroll 1
+        for (int j = 0; j < H * NR; ++j) {
+            const bool bad = __any(largest(acc[0][0], 16 * (j % NR), rk) > kInfinity);
+            const float* row[2] = {j < NR ? xr[0][0] : xr[H - 1][0], j < NR ? xr[0][1] : xr[H - 1][1]};
+            const typename W::T* w0 = A + (uint32_t)min(16 * (j % NR) + a_row(0), rank - 1) * (uint32_t)k;
+            lf4 sum = {0, 0, 0, 0};
+            for (int s = s0 + wave; bad && s < end; s += NW) {
+                const int c0 = s * 32 + 4 * (lane & 7), i0 = s * 32 + a_col();
+                lf4 in[2], x[2];
+                union {
+                    typename W::T t[N];
+                    lf4 v;
+                } a;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) in[h][c] = c0 + c < k ? row[h][c0 + c] : 0.0f;
+#pragma unroll
+                for (int c = 0; c < N; ++c) a.t[c] = i0 + c < k ? w0[i0 + c] : (typename W::T)0;
+                turn_rows128(lx, in, x);
+                const LoraWords w = __builtin_bit_cast(LoraWords, turn_rows64(la, a.v));
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    sum = __builtin_amdgcn_mfma_f32_16x16x4f32(lora_value<W>(w, c), x[c >> 2][c & 3], sum, 0, 0, 0);
+            }
+            lf4 done;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) done[i] = bad && acc[0][0][i] != acc[0][0][i] ? sum[i] : acc[0][0][i];
+#pragma unroll
+            for (int b = 0; b < H * NR; ++b) acc[b / NR][b % NR] = b + 1 < H * NR ? acc[(b + 1) / NR % H][(b + 1) % NR] : done;
+        }
+    }
+    // the largest magnitude's word, times two, of sums below the adapter's own rank; above kInfinity it is a NaN
+    static constexpr uint32_t kInfinity = 0xFF000000u;
+    __device__ inline uint32_t largest(const lf4& sums, int r0, int rk) const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = max(m, (2u * __float_as_uint(sums[i])) & (uint32_t)((r0 + 4 * q + i - rk) >> 31));
+        return m;
     }
     // part as above, of sixteen t of the tile
     __device__ inline void give(float* part, int t) const {
         const int wave = (int)threadIdx.x >> 6;
         float* mine = part + (size_t)wave * 16 * NR * kLoraPart;
-        float big = 0.0f;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             if (h != t) continue;
-            big = most[h];
 #pragma unroll
             for (int b = 0; b < NR; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mine[(16 * b + 4 * q + i) * kLoraPart + p] = acc[h][b][i];
         }
-        if constexpr (kLoraPieces<W> > 0) {
-            if (__any(big == __builtin_inff())) plain(mine, lora_big_rows(big), t, wave);
-        }
     }
     // k's rest belongs to the wave whose turn it is after the last whole step of all
     __device__ inline bool rest_is(int wave) const {
         return steps == k / 32 && k % 32 != 0 && (steps - s0) % NW == wave;
-    }
-    // rare: rows of sixteen t with plain products, over the wave's own share of k
-    __device__ inline void plain(float* mine, unsigned rows, int t, int wave) const {
-        __builtin_amdgcn_wave_barrier();
-        for (int i = 0; i < 16; ++i) {
-            uint64_t at = 0;                                // lane 8 (i % 8) holds row i's address
-#pragma unroll
-            for (int h = 0; h < 2 * H; ++h)
-                if (h == 2 * t + (i >> 3)) at = (uint64_t)(uintptr_t)xr[h >> 1][h & 1];
-            const float* x = reinterpret_cast<const float*>(
-                (uintptr_t)((uint64_t)(uint32_t)__shfl((int)(uint32_t)at, 8 * (i & 7)) |
-                            (uint64_t)(uint32_t)__shfl((int)(uint32_t)(at >> 32), 8 * (i & 7)) << 32));
-            if (!((rows >> i) & 1u)) continue;
-            for (int r = 0; r < rank; ++r) {
-                float sum = 0.0f;
-                for (int s = s0 + wave; s < steps + (rest_is(wave) ? 1 : 0); s += NW) {
-                    const int c = s * 32 + (lane & 31);
-                    if (lane < 32 && c < k) sum = __builtin_fmaf(W::value(A[(size_t)r * k + c]), x[c], sum);
-                }
-#pragma unroll
-                for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
-                if (lane == 0) mine[r * kLoraPart + i] = sum;
-            }
-        }
     }
 };
 
@@ -807,7 +824,7 @@ struct LoraExpand {
             else mask[j] = counts(j, rk);
             asm volatile("" : "+v"(mask[j]));               // kept as a word
         }
-        // the rows to be written here, and those with an infinity in s, or with values too small for its f16 pieces
+        // the rows to be written, and of them those with values too small for f16 pieces
         unsigned rows_in[H], alone[H];
         LoraWords P[H][NP][N > 0 ? N : 1];
         float back[H][4];                                   // of the lane's four rows
@@ -819,7 +836,6 @@ struct LoraExpand {
             for (int i = 0; i < 4; ++i) back[t][i] = 1.0f;
             if constexpr (N > 0) {
                 const float most = lora_most(s[t], 0.0f);
-                if (__any(most == __builtin_inff())) alone[t] = lora_big_rows(most);
                 float scale = 1.0f;
                 bool some = false;
                 if constexpr (std::is_same<W, LoraF16>::value) {
@@ -836,9 +852,7 @@ struct LoraExpand {
                     if constexpr (std::is_same<W, LoraF16>::value) some |= lora_split(W{}, v, scale, P[t][b]);
                     else lora_split(W{}, v, scale, P[t][b]);
                 }
-                if (__any(some)) alone[t] |= lora_rows_of(__ballot(some));
-                alone[t] &= rows_in[t];
-                rows_in[t] &= ~alone[t];
+                if (__any(some)) alone[t] = lora_rows_of(__ballot(some)) & rows_in[t];
             }
         }
         for (; o0 < c1; o0 += 64 * NW) {
@@ -891,16 +905,35 @@ struct LoraExpand {
                             d[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[t][j], v, d[h], 0, 0, 0);
                         }
                 }
-                store(y[t], d, t, o0, rows_in[t]);
+                unsigned apart = 0u;                        // rare: rows in the f32 form
                 if constexpr (N > 0) {
-                    if (__builtin_expect(alone[t], 0)) {     // rare: those rows in the f32 form
+                    apart = alone[t];
+                    bool nan[4], any = false;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        nan[i] = __builtin_isunordered(d[0][i], d[1][i]) || __builtin_isunordered(d[2][i], d[3][i]);
+                        any |= nan[i];
+                    }
+                    if (__builtin_expect(__any(any), 0)) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint64_t m = __ballot(nan[i]);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) apart |= ((m >> (16 * r)) & 0xFFFFu ? 1u : 0u) << (4 * r + i);
+                        }
+                        apart &= rows_in[t];
+                    }
+                }
+                store(y[t], d, t, o0, rows_in[t] & ~apart);
+                if constexpr (N > 0) {
+                    if (__builtin_expect(apart != 0u, 0)) {
                         lf4 e[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
                         for (int j = 0; j < 4 * NR; ++j)
 #pragma unroll
                             for (int h = 0; h < 4; ++h)
                                 e[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[t][j], lora_value<W>(ww[j / 8][h], j % 8), e[h], 0, 0, 0);
-                        store(y[t], e, t, o0, alone[t]);
+                        store(y[t], e, t, o0, apart);
                     }
                 }
             }
@@ -956,7 +989,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void k_lora_apply(LoraArgs a, LoraTil
     const int rk = lora_rank(a, key);
     const float c = lora_scale(a, key);
     LoraShrink<W, NR, NW, U, 1> S(a, lora_a<W>(a, key), row, n, turn, 0, 1 << 28);
-    S.run();
+    S.run(rk);
     const LoraExpand<W, NR, NW, 1, !FIND> E(a, lora_b<W>(a, key), row, n, c1);
     float s[1][4 * NR];
     S.give(part, 0);
@@ -976,7 +1009,7 @@ __device__ inline void lora_shrink_part(const LoraArgs& a, const LoraTiles& t, i
     const int s0 = part_k * t.k_steps, rk = lora_rank(a, key);
     constexpr int ROWS = HALF ? 32 : 16 * H;                // of the tile
     LoraShrink<W, NR, NW, U, H> S(a, lora_a<W>(a, key), row, n, turn, s0, s0 + t.k_steps);
-    S.run();
+    S.run(rk);
     float* out = t.s + ((size_t)part_k * t.positions + pos) * (16 * NR);
     const size_t slot = (size_t)w * t.slots + blockIdx.x;
     const float c = t.scaled ? lora_scale(a, key) : 1.0f;

@@ -103,6 +103,60 @@ def test_a_large_value_that_no_weight_meets(ex, T, rank, size, dtype):
     assert torch.equal(got[0][same], clean[same])
 
 
+def by_sums(w, v):
+    """w [.., n, m] and v [.., m]: the sums over m in the definition's arithmetic, infinities and NaN included."""
+    with np.errstate(invalid="ignore", over="ignore"):
+        return (w * v[..., None, :]).sum(axis=-1)
+
+
+def same_places(got, want, what):
+    """Where the definition gives an infinity or a NaN, the call gives the same."""
+    got = got.double().cpu().numpy().reshape(want.shape)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), what
+    at = np.isinf(want)
+    assert np.array_equal(np.isinf(got), at) and np.array_equal(got[at], want[at]), what
+
+
+@TYPES
+@pytest.mark.parametrize("T,rank", [(1, 6), (6, 6), (150, 20), (600, 40), (600, 128), (4500, 16)])
+@pytest.mark.parametrize("where", ["a", "b", "both"])
+def test_infinite_weights_give_what_the_sums_give(ex, T, rank, where, dtype):
+    """Infinities in one adapter's A or B, beside values of few bits, of many, and zeros; rows of the other
+    adapter keep their bits."""
+    c = Case(T + rank, T, 70, 72, rank, 2, dtype, adapters=[t % 2 for t in range(T)])
+    c.x[:, 0, 5] = np.array([1.0, -0.5, 0.3, -1.7, 0.0, 3.0])[np.arange(T) // 2 % 6]
+    c.dy[:, 0, 7] = np.array([1.0, -0.5, 0.3, -1.7, 2.0, 0.0])[np.arange(T) // 2 % 6]
+    c.d_x.copy_(torch.from_numpy(c.x))
+    c.d_dy.copy_(torch.from_numpy(c.dy))
+    clean = ex.lora_apply(c.lora, c.d_x, c.d_ad, c.d_base), *ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy)
+    inf = float("inf")
+    if where != "b":
+        c.lora.a[0, 0, 2, 5] = inf
+    if where != "a":
+        c.lora.b[0, 0, 7, 3], c.lora.b[0, 0, 70, 1] = -inf, inf
+    a, b, scale, _ = c.weights()
+    A, B, s = a[c.ad, 0], b[c.ad, 0], scale[c.ad][:, None]
+    with np.errstate(invalid="ignore"):
+        y = by_sums(B, s * by_sums(A, c.x[:, 0].astype(np.float64))) + c.base[:, 0]
+        dx = by_sums(A.transpose(0, 2, 1), s * by_sums(B.transpose(0, 2, 1), c.dy[:, 0].astype(np.float64)))
+    out = c.d_base.clone()
+    got = ex.lora_apply(c.lora, c.d_x, c.d_ad, c.d_base), *ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy)
+    same_places(got[0], y, "forward")
+    same_places(got[1], dx, "dx")
+    ex.lora_apply(c.lora, c.d_x, c.d_ad, out, out=out)
+    same_places(out, y, "in place")
+    c.lora.a[0], c.lora.b[0] = c.lora.a[0].nan_to_num(0, 0, 0), c.lora.b[0].nan_to_num(0, 0, 0)
+    want, bound = c.forward()
+    finite = np.isfinite(y)
+    assert np.all((np.abs(got[0].double().cpu().numpy()[:, 0] - want[:, 0]) <= bound[:, 0])[finite])
+    want, bound = c.backward()
+    finite = np.isfinite(dx)
+    assert np.all((np.abs(got[1].double().cpu().numpy().reshape(T, -1) - want[0][:, 0]) <= bound[0][:, 0])[finite])
+    if T > 1:
+        assert torch.equal(got[0][1::2], clean[0][1::2]) and torch.equal(got[1][1::2], clean[1][1::2])
+        assert torch.equal(got[2][1], clean[2][1]) and torch.equal(got[3][1], clean[3][1])
+
+
 @pytest.mark.parametrize("n,E,groups", [(1 << 24, 8, 1), (1 << 21, 516, 1), (1 << 22, 40, 64)])
 def test_the_means_of_long_batches(ex, n, E, groups):
     """The same row in every token: each rounding of a long sum goes the same way.  Its mean is p and the
