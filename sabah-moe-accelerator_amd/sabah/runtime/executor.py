@@ -155,15 +155,18 @@ class MoEExecutor:
         """The checks that the two calls share; (tokens, slots, C arguments of x, adapters and ids).
         y: a tensor with the output's shape [T, rows] or [T, n_ids, rows], if there is one."""
         shape, xs, dev = x.shape, x.stride(), self._index
-        T, k = shape[0], lora.k
         if len(shape) == 3:
             xr, xi = shape[1], xs[1] * 4
-        else:
+        elif len(shape) == 2:
             xr, xi = 1, 0
+        else:
+            raise ValueError("adapters: x %s, expected [T, %d] or [T, x_rows, %d]" % (tuple(shape), lora.k, lora.k))
+        T, k = shape[0], lora.k
         if ids is not None:
-            slots, ns = ids.shape[1], ids.stride()
-            if ids.dtype is not torch.int32 or ids.shape[0] != T or ids.get_device() != dev:
+            ns = ids.stride()
+            if ids.dtype is not torch.int32 or len(ns) != 2 or ids.shape[0] != T or ids.get_device() != dev:
                 raise ValueError("adapters: ids %s %s for %d tokens" % (tuple(ids.shape), ids.dtype, T))
+            slots = ids.shape[1]
             ids_args = ids.data_ptr(), ns[1] * 4, ns[0] * 4
         else:
             slots = y.shape[1] if y is not None and len(y.shape) == 3 else 1
@@ -171,7 +174,7 @@ class MoEExecutor:
                 raise ValueError("adapters of %d experts need ids" % lora.n_experts)
             ids_args = None, 0, 0
         if (x.dtype is not torch.float32 or shape[-1] != k or (xs[-1] != 1 and T) or (xr != 1 and xr != slots)
-                or len(shape) > 3 or adapters.dtype is not torch.int32 or adapters.shape != (T,)
+                or adapters.dtype is not torch.int32 or adapters.shape != (T,)
                 or not adapters.is_contiguous()):
             raise ValueError("adapters: x %s %s for %d values, adapters %s %s"
                              % (tuple(shape), x.dtype, k, tuple(adapters.shape), adapters.dtype))
@@ -183,8 +186,8 @@ class MoEExecutor:
         """(address, slot stride, token stride) of rows [T, width] or [T, slots, width] f32."""
         shape, s = y.shape, y.stride()
         three = len(shape) == 3
-        if (y.dtype is not torch.float32 or (s[-1] != 1 and T) or y.get_device() != self._index
-                or shape != ((T, slots, width) if three or slots != 1 else (T, width))):
+        if (y.dtype is not torch.float32 or shape != ((T, slots, width) if three or slots != 1 else (T, width))
+                or (s[-1] != 1 and T) or y.get_device() != self._index):
             raise ValueError("adapters: %s is %s %s, expected f32 [%d, %d, %d] with contiguous rows on %s"
                              % (what, tuple(shape), y.dtype, T, slots, width, self.device))
         return (y.data_ptr(), s[1] * 4, s[0] * 4) if three else (y.data_ptr(), 0, s[0] * 4)
@@ -270,12 +273,13 @@ class MoEExecutor:
         return ids, w
 
     def _router_rows(self, logits: torch.Tensor, ids: torch.Tensor, mask: torch.Tensor | None, n_groups: int):
-        T, E = logits.shape
         dev = self._index
-        if (logits.dtype is not torch.float32 or (logits.stride(1) != 1 and T) or logits.get_device() != dev
-                or ids.dtype is not torch.int32 or ids.shape[0] != T or not ids.is_contiguous() or ids.get_device() != dev):
+        if (logits.dim() != 2 or ids.dim() != 2 or logits.dtype is not torch.float32
+                or (logits.stride(1) != 1 and logits.shape[0]) or logits.get_device() != dev or ids.dtype is not torch.int32
+                or ids.shape[0] != logits.shape[0] or not ids.is_contiguous() or ids.get_device() != dev):
             raise ValueError("router: logits %s %s, ids %s %s" % (tuple(logits.shape), logits.dtype, tuple(ids.shape),
                                                                  ids.dtype))
+        T, E = logits.shape
         if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.numel() != T
                                  or not mask.is_contiguous() or mask.get_device() != dev):
             raise ValueError("router: mask %s %s for %d tokens" % (tuple(mask.shape), mask.dtype, T))
@@ -287,10 +291,10 @@ class MoEExecutor:
         (sabah_moe_balance) from logits [T, n_experts] f32 and route()'s ids [T, n_used]
         over the tokens where mask [T] (bool or uint8) holds, in n_groups groups of equal length
         (`out` brings its own number)."""
-        if out is None:
-            out = RouterBalance(logits.shape[1], n_groups, device=self.device)
-        n_groups = out.n_groups
         T, E, k = self._router_rows(logits, ids, mask, n_groups)
+        if out is None:
+            out = RouterBalance(E, n_groups, device=self.device)
+        n_groups = out.n_groups
         if out.n_experts != E or out.counts.get_device() != self._index:
             raise ValueError("balance: %d experts on %s, out has %d on %s"
                              % (E, self.device, out.n_experts, out.counts.device))
