@@ -232,7 +232,7 @@ class MoEExecutor:
             da = torch.empty(lora.a.shape, dtype=torch.float32, device=self.device) if da is None else da
             db = torch.empty(lora.b.shape, dtype=torch.float32, device=self.device) if db is None else db
             for g, w in ((da, lora.a), (db, lora.b)):
-                if g.shape != w.shape or g.dtype != torch.float32 or not g.is_contiguous() or g.device != self.device:
+                if g.shape != w.shape or g.dtype != torch.float32 or not g.is_contiguous() or g.get_device() != self._index:
                     raise ValueError("lora_backward: a weight gradient is %s %s, expected contiguous f32 %s"
                                      % (tuple(g.shape), g.dtype, tuple(w.shape)))
         d = self._lora_y("dx", dx, T, slots, lora.k) if need_dx else (None, 0, 0)

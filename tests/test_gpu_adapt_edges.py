@@ -157,6 +157,17 @@ def test_infinite_weights_give_what_the_sums_give(ex, T, rank, where, dtype):
         assert torch.equal(got[2][1], clean[2][1]) and torch.equal(got[3][1], clean[3][1])
 
 
+def test_a_bank_on_the_current_device_without_a_number(hip_rt):
+    """device="cuda" names the device that its tensors call cuda:0."""
+    from sabah.runtime.bank import ExpertBank
+    from sabah.runtime.executor import MoEExecutor
+    ex = MoEExecutor(ExpertBank(1, 8, 256, 256, {"gate": 21, "up": 21, "down": 21}, device="cuda"))
+    c = Case(4, 30, 64, 48, 8, 2, BF16)
+    da, db = torch.zeros(c.lora.a.shape, device=DEV), torch.zeros(c.lora.b.shape, device=DEV)
+    all_close(ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy, da=da, db=db, add_dw=True), *c.backward())
+    assert da.any() and db.any()
+
+
 @pytest.mark.parametrize("n,E,groups", [(1 << 24, 8, 1), (1 << 21, 516, 1), (1 << 22, 40, 64)])
 def test_the_means_of_long_batches(ex, n, E, groups):
     """The same row in every token: each rounding of a long sum goes the same way.  Its mean is p and the
