@@ -410,7 +410,8 @@ SABAH_API int sabah_lora_apply(const sabah_lora_desc* lora, const float* d_x, si
     if (!stride_ok(base_id_stride) || !stride_ok(base_token_stride) || !stride_ok(dst_id_stride) ||
         !stride_ok(dst_token_stride))
         return fail("adapters: strides are in bytes and multiples of 4");
-    if (d_base == d_dst && (base_id_stride != dst_id_stride || base_token_stride != dst_token_stride))
+    // a stride that no row is reached by may be anything
+    if (d_base == d_dst && ((n_ids > 1 && base_id_stride != dst_id_stride) || (n_tokens > 1 && base_token_stride != dst_token_stride)))
         return fail("adapters: base in place of dst needs dst's strides");
     const int n_rows = n_ids * n_tokens;
     const LoraSpace sp = lora_space(lora, n_rows);

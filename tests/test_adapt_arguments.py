@@ -3,6 +3,8 @@ must refuse, or must not, seen before the device is touched (no GPU)."""
 import pytest
 import torch
 
+from test_adapt_refusals import P, apply, desc
+
 
 @pytest.fixture
 def ex():
@@ -42,3 +44,15 @@ def test_router_tensors_have_two_dimensions(ex):
         with pytest.raises(ValueError, match="router"):
             ex._router_rows(logits, ids, None, 1)
     assert ex._router_rows(torch.zeros(6, 8), i32(6, 2), None, 1) == (6, 8, 2)
+
+
+def test_in_place_where_a_stride_is_never_used():
+    """Base and dst are the same rows whatever the slots' stride of one slot, or the tokens' of one token:
+    the next check (a missing workspace) is what refuses these calls."""
+    from sabah.runtime import rt
+    L = rt.lib()
+    many = dict(ws=None, nws=0, base=P)
+    assert apply(L, desc(), T=5000, bi=0, di=192, bt=192, dt=192, **many) == -1 and "workspace" in rt.last_error()
+    assert apply(L, desc(), T=1, n=5000, bi=192, di=192, bt=0, dt=192 * 5000, **many) == -1 and "workspace" in rt.last_error()
+    assert apply(L, desc(), T=5000, bi=0, di=0, bt=96, dt=192, **many) == -1 and "in place" in rt.last_error()
+    assert apply(L, desc(), T=1, n=5000, bi=96, di=192, bt=0, dt=0, **many) == -1 and "in place" in rt.last_error()

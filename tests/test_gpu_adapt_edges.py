@@ -202,3 +202,16 @@ def test_the_gradient_of_as_many_tokens_as_a_call_takes(ex):
     close(got[at], want, bound, "dlogits")
     got[at] = 0
     assert not any(bool(part.any()) for part in got.split(1 << 21))
+
+
+@pytest.mark.parametrize("T", [1, 5, 300])
+def test_in_place_through_views_of_other_shapes(ex, T):
+    """The same rows as [T, rows] and as [T, 1, rows], or one token with any token stride."""
+    c = Case(T, T, 64, 48, 8, 2, BF16, adapters="each")
+    want = ex.lora_apply(c.lora, c.d_x, c.d_ad, c.d_base)
+    rows = c.d_base.clone()
+    assert ex.lora_apply(c.lora, c.d_x, c.d_ad, rows[:, 0], out=rows) is rows
+    assert torch.equal(rows, want)
+    one = c.d_base[:1].clone()
+    ex.lora_apply(c.lora, c.d_x[:1], c.d_ad[:1], one.as_strided((1, 1, 48), (4096, 48, 1)), out=one)
+    assert torch.equal(one, want[:1])
