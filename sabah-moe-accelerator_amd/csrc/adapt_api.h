@@ -229,6 +229,9 @@ constexpr int kLoraFusedTiles = 512;
 // The two launches: k in parts of at least eight steps of 32, up to about 1,024 workgroups (1,999 rows of k 2048 at rank 64: the
 // shrink 12.4 us in eight parts, 25.8 whole; the expand, which adds them up, 11.2 and 8.4)
 constexpr int kLoraShrinkGroups = 1024, kLoraShrinkParts = 8, kLoraShrinkSteps = 8;
+// Of a k of at least parts * kLoraShrinkSteps steps, the last part has at least kLoraShrinkSteps + 2 - parts.  It has to have two:
+// LoraShrink gives k's rest to the part whose whole steps end there, which two would be if the last were that rest alone.
+static_assert(kLoraShrinkSteps >= kLoraShrinkParts, "a last part of k's rest alone would be summed twice");
 constexpr int kLoraExpandGroups = 1024;
 // k of a shrink in parts while there are few tiles
 static void lora_k_parts(int k, int tiles, int& parts, int& steps) {
