@@ -157,6 +157,60 @@ def test_infinite_weights_give_what_the_sums_give(ex, T, rank, where, dtype):
         assert torch.equal(got[2][1], clean[2][1]) and torch.equal(got[3][1], clean[3][1])
 
 
+@TYPES
+@pytest.mark.parametrize("T,rank", [(6, 16), (150, 40), (600, 113), (1300, 16), (4500, 24)])
+def test_rows_of_nan_and_infinity_of_every_type(ex, T, rank, dtype):
+    """A NaN, infinities of both signs and a row with both touch no other row, forward and backward; what
+    they give is what the sums give."""
+    c = Case(T + rank, T, 70, 40, rank, 2, dtype, adapters=[t % 2 for t in range(T)])
+    clean = ex.lora_apply(c.lora, c.d_x, c.d_ad, c.d_base), ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy)[0]
+    inf = np.inf
+    c.x[1, 0, 5], c.x[2, 0, 69], c.x[4, 0, 1] = np.nan, inf, -inf
+    c.x[5, 0, 3], c.x[5, 0, 66] = inf, np.nan
+    c.dy[0, 0, 5], c.dy[2, 0, 39], c.dy[4, 0, 1] = np.nan, -inf, inf
+    a, b, scale, _ = c.weights()
+    A, B, s = a[c.ad, 0], b[c.ad, 0], scale[c.ad][:, None]
+    with np.errstate(invalid="ignore"):
+        y = by_sums(B, s * by_sums(A, c.x[:, 0].astype(np.float64))) + c.base[:, 0]
+        dx = by_sums(A.transpose(0, 2, 1), s * by_sums(B.transpose(0, 2, 1), c.dy[:, 0].astype(np.float64)))
+    x, dy = torch.from_numpy(c.x).to(DEV), torch.from_numpy(c.dy).to(DEV)
+    got = ex.lora_apply(c.lora, x, c.d_ad, c.d_base), ex.lora_backward(c.lora, x, c.d_ad, dy, need_dw=False)[0]
+    same_places(got[0], y, "forward")
+    same_places(got[1], dx, "dx")
+    rest = torch.ones(T, dtype=torch.bool, device=DEV)
+    rest[[1, 2, 4, 5]] = False
+    assert torch.equal(got[0][rest], clean[0][rest])
+    rest = torch.ones(T, dtype=torch.bool, device=DEV)
+    rest[[0, 2, 4]] = False
+    assert torch.equal(got[1][rest], clean[1][rest])
+
+
+@pytest.mark.parametrize("T,k,rows,rank", [(63, 72, 40, 113), (300, 40, 36, 113), (2100, 36, 24, 113), (200, 100, 36, 64),
+                                           (256, 40, 130, 128), (90, 65, 70, 33), (2049, 20, 12, 128)])
+def test_high_ranks_kept_in_f32(ex, T, k, rows, rank):
+    c = Case(T + rank, T, k, rows, rank, 3, F32, adapters="runs")
+    want, bound = c.forward()
+    close(ex.lora_apply(c.lora, c.d_x, c.d_ad, c.d_base), want, bound, "forward")
+    all_close(ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy), *c.backward())
+    hip_ok()
+
+
+@TYPES
+@pytest.mark.parametrize("T,rank", [(3, 24), (200, 40), (600, 24), (600, 128), (4500, 24)])
+def test_values_past_an_adapters_own_rank_count_nowhere(ex, T, rank, dtype):
+    """NaN and infinities past the own ranks of half of the adapters, in calls of every size."""
+    c = Case(T, T, 68, 36, rank, 4, dtype, adapters="each", ranks=[rank, 7, 0, 300])
+    for n, r in ((1, 7), (2, 0)):
+        c.lora.a[n, :, r:] = float("nan")
+        c.lora.b[n, :, :, r:] = float("inf")
+    a, b, scale, ranks = c.weights()
+    a, b = np.nan_to_num(a, nan=0, posinf=0), np.nan_to_num(b, nan=0, posinf=0)
+    want, bound = ref.lora_forward(c.x.astype(np.float64), c.ad, None, a, b, scale, ranks, c.base.astype(np.float64))
+    close(ex.lora_apply(c.lora, c.d_x, c.d_ad, c.d_base), want, bound, "forward")
+    all_close(ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy),
+              *ref.lora_backward(c.x.astype(np.float64), c.ad, None, a, b, scale, ranks, c.dy.astype(np.float64)))
+
+
 def test_a_bank_on_the_current_device_without_a_number(hip_rt):
     """device="cuda" names the device that its tensors call cuda:0."""
     from sabah.runtime.bank import ExpertBank
