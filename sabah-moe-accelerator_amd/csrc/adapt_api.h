@@ -219,7 +219,8 @@ static int check_lora(const char* what, const sabah_lora_desc* L, int n_ids, int
 static bool stride_ok(size_t s) { return s % 4 == 0; }
 
 // Forward.  A call of at most kLoraDirectRows rows is one launch (k_lora_apply): at 256 rows of 64 adapters (k 2048, rows
-// 512, rank 16) 16.2 us, where the three launches of a larger call take 20.2 (15.6 and 16.4 at 128, 14.9 and 15.8 at 64).
+// 512, rank 16, the one shape timed) 16.2 us, where the three launches of a larger call take 20.2 (15.6 and 16.4 at 128, 14.9
+// and 15.8 at 64).
 // Above, each window of rows has at most one tile per 16 rows and one more per key.  With kLoraFusedTiles of them, two
 // for every CU, a workgroup shrinks and expands its tile (one launch after the lists); with fewer two launches share out k and the
 // columns.  us of the one launch against the two, 2048 x 2048, rank 32, 8 adapters: 44.8 and 36.0 at 4,096 rows (328 tiles),
@@ -283,7 +284,8 @@ struct LoraBackSpace {
 // Rows up to which a workgroup of the backward's shrinks takes half a tile, with eight waves.  A CU reads its tile's rows
 // and A at little more than 64 bytes a cycle, so few tiles are shared out; many read A half as often as wholes.  us at 512 /
 // 1,024 / 2,048 rows, k 2048, halves against wholes: f32 to 768 at rank 16 8.1 / 8.9 / 11.7 against 13.3 / 14.2 / 15.6,
-// bf16 to 2048 at rank 64 11.3 / 11.9 / 18.6 against 21.4 / 22.0 / 22.5
+// bf16 to 2048 at rank 64 11.3 / 11.9 / 18.6 against 21.4 / 22.0 / 22.5.  At 8,192 the latter takes 55 - 65 in halves, 52 in
+// wholes: the crossing lies between, where nothing was timed
 constexpr int kLoraHalfRows = 2048;
 constexpr int kLoraBackKeys = 1 << 15;        // a word per key and window
 // Splits of the weights' gradients, over the windows: what one request sends is together, so without them the

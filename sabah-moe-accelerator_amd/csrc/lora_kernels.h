@@ -969,7 +969,8 @@ __device__ inline const typename W::T* lora_b(const LoraArgs& a, int key) {
 // and shrinks it whole, also when several share its columns; up to U steps of loads at a time, which it
 // waits for.  Large ones, with tiles to fill the chip, take them from the lists, and hold OCC
 // waves per SIMD to cover the loads.  Bound by HBM there: 16,384 rows, 2048 x 2048, rank 32, 402 MB in 95 us (4.2 TB/s; a
-// large copy reaches 4.7).  One token: 7.7 us, waits on one load after another.  grid (slots, column parts, windows).
+// large copy reaches 4.7).  One token: 7.5 us, of which the smallest launch takes 3.6; loads of B and base under the shrink
+// made it no shorter.  grid (slots, column parts, windows).
 template <typename W, int NR, int NW, int U, int OCC, bool FIND>
 __global__ __launch_bounds__(64 * NW, OCC) void k_lora_apply(LoraArgs a, LoraTiles t) {
     __shared__ float part[NW * 16 * NR * kLoraPart];
