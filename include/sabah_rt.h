@@ -353,7 +353,8 @@ int sabah_lora_apply(const sabah_lora_desc *lora, const float *d_x, size_t x_id_
  *                    x has one row per token (the caller adds the slots up);
  *                    zeros for a row without an adapter; added to dx with add_dx
  *   d_da, d_db     f32 in the layouts of A and B, written for every adapter and expert (zeros where no
- *                  row uses the pair and past an adapter's own rank); added to them with add_dw
+ *                  row uses the pair and past an adapter's own rank); added to them with add_dw, which
+ *                  leaves those alone
  * Each of d_dx, d_da and d_db may be NULL; they overlap neither each other nor an input.
  * n_adapters * n_experts <= 2^15.  A row with an id out of range gives no part of d_da and d_db, its dx is NaN,
  * and the next call fails.  A value of x or dy that is not finite, or at least 3.39e38 (what rounds to infinity in

@@ -1188,8 +1188,10 @@ __device__ inline void lora_grad_store(const LoraGrad& g, int side, int key, int
         const int e = tid + 256 * i, r = side ? e & 15 : e >> 6, o = side ? e >> 4 : e & 63;
         if (16 * b + r >= g.rank || c0 + o >= n) continue;
         float* to = out + (side ? (size_t)(c0 + o) * g.rank + 16 * b + r : (size_t)(16 * b + r) * n + c0 + o);
-        const float v = 16 * b + r < rk ? sum[r * 64 + o] * c : 0.0f;
-        *to = g.add ? *to + v : v;
+        const bool in = 16 * b + r < rk;
+        const float v = in ? sum[r * 64 + o] * c : 0.0f;
+        if (!g.add) *to = v;
+        else if (in) *to = *to + v;
     }
 }
 
@@ -1225,7 +1227,8 @@ __global__ __launch_bounds__(256, OCC) void k_lora_grad(LoraGrad g) {
     const int key = (int)blockIdx.y, split = (int)blockIdx.z, n = g.width[side], col = c0 + 4 * p;
     uint32_t e;
     const uint32_t used = lora_grad_splits(g, key, e);
-    if (!((used >> split) & 1u) && !(used == 0u && split == 0)) return;     // a key without rows: split 0 writes its zeros
+    // a key without rows: split 0 writes its zeros, but where they would be added (another call may be adding to that pair)
+    if (!((used >> split) & 1u) && !(used == 0u && split == 0 && !g.add)) return;
     lf4 acc[NR][4];
 #pragma unroll
     for (int b = 0; b < NR; ++b)

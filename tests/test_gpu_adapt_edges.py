@@ -269,3 +269,17 @@ def test_in_place_through_views_of_other_shapes(ex, T):
     one = c.d_base[:1].clone()
     ex.lora_apply(c.lora, c.d_x[:1], c.d_ad[:1], one.as_strided((1, 1, 48), (4096, 48, 1)), out=one)
     assert torch.equal(one, want[:1])
+
+
+@pytest.mark.parametrize("T", [4, 90, 2600])
+def test_accumulated_gradients_touch_only_pairs_with_rows(ex, T):
+    """With add_dw, pairs that no row uses and what lies past an adapter's own rank keep their bits (a zero its
+    sign), so that calls at the same time may add to different adapters of one gradient."""
+    c = Case(T, T, 72, 40, 20, 5, BF16, adapters=[(0, 3, -1, 3)[t % 4] for t in range(T)], ranks=[20, 20, 20, 7, 20])
+    _, a, b = ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy, need_dx=False)
+    da, db = torch.full_like(a, -0.0), torch.full_like(b, -0.0)
+    ex.lora_backward(c.lora, c.d_x, c.d_ad, c.d_dy, da=da, db=db, add_dw=True, need_dx=False)
+    assert torch.equal(da, a) and torch.equal(db, b)
+    for n in (1, 2, 4):
+        assert da[n].signbit().all() and db[n].signbit().all()
+    assert da[3, 0, 7:].signbit().all() and db[3, 0, :, 7:].signbit().all()
