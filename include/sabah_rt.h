@@ -366,6 +366,112 @@ int sabah_lora_backward(const sabah_lora_desc *lora, const float *d_x, size_t x_
                         size_t dy_token_stride, float *d_dx, size_t dx_id_stride, size_t dx_token_stride, int add_dx,
                         float *d_da, float *d_db, int add_dw, void *d_workspace, size_t workspace_bytes, void *stream);
 
+/* ---- training a block's own weights ---------------------------------------- */
+
+/* No reference counterpart, like the adapters, whose rules on scratch, captures, streams, devices and
+ * equal bits hold here too.  type: F32 0, F16 1 or BF16 30, of the activations (and an expert's
+ * weights); other tensors are f32 where nothing else is said. */
+
+/* The norms around a block: after it, with the block's gate and the scale of its branch on the residual
+ * stream, and before the next one.  With n(v; w) = v / sqrt(mean(v^2) + eps) * w for each row of `width` values:
+ *   out[t] = x[t] + scale * sigmoid(gate[t]) * n(y[t]; w_after)   (w_after NULL: y itself; gate NULL: 1)
+ *   h[t]   = n(out[t]; w_before), of out as it is stored          (w_before NULL: no h)
+ * y NULL: only h, of x.  Rows are strides (bytes) apart; out may be x itself.  width <= 8192, n_tokens <= 2^24. */
+typedef struct sabah_norm_desc {
+    const float *w_after, *w_before;       /* device [width], or NULL */
+    int type, width;
+    float eps, scale;
+} sabah_norm_desc;
+int sabah_block_norm(const sabah_norm_desc *norm, const void *d_x, size_t x_stride, const void *d_y, size_t y_stride,
+                     const float *d_gate, int n_tokens, void *d_out, size_t out_stride, void *d_h, size_t h_stride,
+                     void *stream);
+
+/* The gradients of sabah_block_norm, for dout (the gradient of out, NULL: zeros) and dh (that of h): dx
+ * (may be dout itself; without w_before dx is dout, and d_dx is not used), dy (NULL: y is left out, as in a call without it), dgate,
+ * dw_after and dw_before, written or with add_dw added to.  d_out is sabah_block_norm's out (x where that had no y). */
+size_t sabah_block_norm_workspace(int width, int n_tokens);
+int sabah_block_norm_backward(const sabah_norm_desc *norm, const void *d_out, size_t out_stride, const void *d_y,
+                              size_t y_stride, const float *d_gate, int n_tokens, const void *d_dout, size_t dout_stride,
+                              const void *d_dh, size_t dh_stride, void *d_dx, size_t dx_stride, void *d_dy, size_t dy_stride,
+                              float *d_dgate, float *d_dw_after, float *d_dw_before, int add_dw, void *d_workspace,
+                              size_t workspace_bytes, void *stream);
+
+/* The (token, slot) rows of ids [n_tokens][n_ids] (int32, strides in bytes) grouped by expert, in token order within
+ * one, in the caller's buffer of sabah_expert_groups_bytes (16-byte aligned device memory): made once for all products over
+ * the same ids, forward and backward.  Id -1 is a row without an expert; another id outside
+ * [0, n_experts) makes its row NaN and fails the next call.  n_experts <= 4096, at most 2^24 rows. */
+size_t sabah_expert_groups_bytes(int n_ids, int n_tokens, int n_experts);
+int sabah_expert_group(const int32_t *d_ids, size_t ids_id_stride, size_t ids_token_stride, int n_ids, int n_tokens,
+                       int n_experts, void *d_groups, size_t groups_bytes, void *stream);
+
+/* Experts kept in a float type: one matrix of a projection for each. */
+typedef struct sabah_expert_desc {
+    const void *w;                         /* device [n_experts][rows][k] */
+    int type, n_experts, k, rows;          /* k, rows <= 2^20 */
+} sabah_expert_desc;
+
+/* y[t][i] = W[ids[t][i]] x[t][i % x_rows] for the ids that d_groups was made from, with the same n_ids,
+ * n_tokens and n_experts (a kernel that is given other groups writes nothing, and the next call fails); zeros for a
+ * row without an expert.  x and y have the experts' type; strides are bytes, of inputs 0 too.  Sums are f32. */
+int sabah_expert_mul(const sabah_expert_desc *experts, const void *d_x, size_t x_id_stride, int x_rows, size_t x_token_stride,
+                     const void *d_groups, size_t groups_bytes, int n_ids, int n_tokens, void *d_y, size_t y_id_stride,
+                     size_t y_token_stride, void *stream);
+
+/* The gradients of sabah_expert_mul for dy[t][i]: dx[t][i] = W^T dy[t][i], one row per (token, slot) in
+ * the experts' type (zeros without an expert, NaN for a bad id), and d_dw f32 [n_experts][rows][k], written for every
+ * expert (zeros without rows), or with add_dw added to (experts without rows are left alone).  Either may be NULL. */
+int sabah_expert_mul_backward(const sabah_expert_desc *experts, const void *d_x, size_t x_id_stride, int x_rows,
+                              size_t x_token_stride, const void *d_groups, size_t groups_bytes, int n_ids, int n_tokens,
+                              const void *d_dy, size_t dy_id_stride, size_t dy_token_stride, void *d_dx, size_t dx_id_stride,
+                              size_t dx_token_stride, float *d_dw, int add_dw, void *stream);
+
+/* An AdamW step over many tensors at once.  For every value
+ *   g = c * grad;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+ *   p = p (1 - lr decay) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+ * with c = grad_scale, times min(1, max_norm / (norm + 1e-6)) where the norm of all gradients (times grad_scale) is wanted.
+ * A step whose norm is infinite or NaN changes nothing but the norm.  Tensors of 16 bits may have a master copy
+ * in f32, which is then what the step reads and writes; the tensor is its rounded copy. */
+typedef struct sabah_adamw_tensor {
+    void *p;                               /* n values of p_type */
+    const void *g;                         /* the gradient, n values of g_type */
+    float *master;                         /* or NULL */
+    double decay;                          /* weight decay */
+    long long n;
+    int p_type, g_type;                    /* F32 0, F16 1, BF16 30 */
+} sabah_adamw_tensor;
+
+/* The tensors' table for the device, written to host memory: the caller copies it to 16-byte aligned device
+ * memory and makes it again when a tensor moves.  n_values: length of the flat moments, in which each tensor begins at a
+ * multiple of 256.  A weight that shares memory with another tensor is refused. */
+size_t sabah_adamw_table_bytes(const sabah_adamw_tensor *tensors, int n_tensors, long long *n_values);
+int sabah_adamw_table(const sabah_adamw_tensor *tensors, int n_tensors, void *table, size_t table_bytes);
+
+/* Moments of 32 bits are f32 m and v of n_values, zeros before the first step.  Moments of 8 bits are a byte for
+ * each value and an f32 scale, the largest value, for each 256: m = sign * (code / 127)^2 * scale (int8), v = (code / 255)^4 *
+ * scale (uint8), zeros before the first step; a step reads them as those values and stores the nearest codes (no v above 0
+ * as 0), a block with a NaN as NaN. */
+typedef struct sabah_adamw_desc {
+    const void *table;                     /* device copy of the table */
+    size_t table_bytes;
+    int n_tensors, bits;                   /* 32 or 8 */
+    void *m, *v;                           /* device, 16-byte aligned */
+    float *m_scale, *v_scale;              /* bits 8: device [n_values / 256] */
+    double lr, beta1, beta2, eps, grad_scale, max_norm;
+    const float *d_lr;                     /* device, or NULL: lr; for captured steps */
+    long long *step;                       /* device: steps made, 0 before the first; counted here */
+    float *norm;                           /* device [1]: the gradients' norm, NULL: not wanted and not clipped */
+    void *workspace;
+    size_t workspace_bytes;
+} sabah_adamw_desc;
+size_t sabah_adamw_workspace(void);
+int sabah_adamw_step(const sabah_adamw_desc *adamw, void *stream);
+
+/* Moments of 8 bits as the values they stand for, and values as moments of 8 bits (n_values: whole blocks). */
+int sabah_adamw_moments_read(const void *m_code, const void *v_code, const float *m_scale, const float *v_scale,
+                             long long n_values, float *m, float *v, void *stream);
+int sabah_adamw_moments_write(const float *m, const float *v, long long n_values, void *m_code, void *v_code, float *m_scale,
+                              float *v_scale, void *stream);
+
 /* How sabah_rt_mul_mat_id_v2 runs calls over many tokens.  No reference
  * counterpart: the reference's kernel re-reads an expert per (token, slot)
  * (sabah_rt.cu:2791-2839).  Grouped, the (token, slot) pairs are grouped by

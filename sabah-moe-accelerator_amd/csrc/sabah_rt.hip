@@ -19,13 +19,16 @@
 #include <unordered_set>
 #include <vector>
 
+#include "adamw_kernels.h"
 #include "balance_kernels.h"
 #include "dense_kernels.h"
+#include "expert_kernels.h"
 #include "grouped_rows.h"
 #include "host_decode.h"
 #include "layer_kernels.h"
 #include "lora_kernels.h"
 #include "mmid_kernels.h"
+#include "norm_kernels.h"
 #include "prefill_kernels.h"
 #include "route_kernels.h"
 #include "synth_kernels.h"
@@ -355,6 +358,8 @@ bool check_sticky() {
     } else if (w == kErrLora) {
         fail("an earlier adapters call read an adapter id outside [-1, n_adapters) or an expert id outside "
              "[0, n_experts); its row was set to NaN");
+    } else if (w == kErrExpertGroups) {
+        fail("an earlier expert product was given groups that sabah_expert_group had not made for its shape; nothing was written");
     } else {
         fail("an earlier expert kernel read an expert id outside [0, n_experts); "
              "its slot outputs were set to NaN");
@@ -2457,3 +2462,4 @@ SABAH_API int sabah_synth_weights(void* d_dst, int qt, long long n_rows, int k, 
 }
 
 #include "adapt_api.h"
+#include "train_api.h"

@@ -26,7 +26,9 @@ import torch
 
 from . import rt
 from .bank import ROLES, DenseExpert, ExpertBank
+from .experts import FloatExperts, RowGroups
 from .lora import LoraBank
+from .norm import BlockNorm
 
 
 # A small call is bound by what Python does before the launch, so the hot
@@ -245,6 +247,180 @@ class MoEExecutor:
         if rc:
             rt.check(rc, "lora_backward")
         return dx if need_dx else None, da if need_dw else None, db if need_dw else None
+
+    # ---- a block's own weights in training ------------------------------------------
+    def _norm_rows(self, what: str, norm: BlockNorm, t: torch.Tensor | None, like: torch.Tensor):
+        """(address, row stride) of activations [T, width] in like's type, or (None, 0)."""
+        if t is None:
+            return None, 0
+        if (t.dtype is not like.dtype or t.shape != like.shape or t.get_device() != self._index
+                or (t.stride(1) != 1 and t.shape[0] and norm.width > 1)):
+            raise ValueError("block_norm: %s is %s %s, expected %s [%d, %d] with contiguous rows on %s"
+                             % (what, tuple(t.shape), t.dtype, like.dtype, like.shape[0], norm.width, self.device))
+        return t.data_ptr(), t.stride(0) * t.element_size() if t.shape[0] > 1 else norm.width * t.element_size()
+
+    def _norm_check(self, norm: BlockNorm, x: torch.Tensor, y, gate: torch.Tensor | None) -> int:
+        if x.dim() != 2 or x.shape[1] != norm.width or norm.device.index not in (None, self._index):
+            raise ValueError("block_norm: x %s beside a norm of width %d on %s" % (tuple(x.shape), norm.width, norm.device))
+        if y is None and (gate is not None or norm.w_before is None):
+            raise ValueError("block_norm: a gate, or no norm before the next block, needs y")
+        if gate is not None and (gate.dtype is not torch.float32 or gate.shape != (x.shape[0],) or not gate.is_contiguous()
+                                 or gate.get_device() != self._index):
+            raise ValueError("block_norm: gate %s %s for %d tokens" % (tuple(gate.shape), gate.dtype, x.shape[0]))
+        return x.shape[0]
+
+    def block_norm(self, norm: BlockNorm, x: torch.Tensor, y: torch.Tensor | None = None,
+                   gate: torch.Tensor | None = None, out: torch.Tensor | None = None, h: torch.Tensor | None = None):
+        """(out, h): the residual stream x [T, width] after a block whose output is y, and what the next block reads
+        (sabah_block_norm): out = x + scale * sigmoid(gate) * n(y; w_after), h = n(out; w_before).  gate [T] f32:
+        logits, None: 1.  y None: only h, of x.  `out` may be x itself.  None for what the call does not have."""
+        T = self._norm_check(norm, x, y, gate)
+        xs = self._norm_rows("x", norm, x, x)
+        if y is not None and out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=self.device)
+        if norm.w_before is not None and h is None:
+            h = torch.empty(x.shape, dtype=x.dtype, device=self.device)
+        if y is None:
+            out = None
+        if norm.w_before is None:
+            h = None
+        rc = rt.lib().sabah_block_norm(norm.ref(x.dtype, y is not None), *xs, *self._norm_rows("y", norm, y, x),
+                                       gate.data_ptr() if gate is not None else None, T, *self._norm_rows("out", norm, out, x),
+                                       *self._norm_rows("h", norm, h, x), _stream(self.device))
+        if rc:
+            rt.check(rc, "block_norm")
+        return out, h
+
+    def block_norm_backward(self, norm: BlockNorm, out: torch.Tensor, y: torch.Tensor | None = None,
+                            gate: torch.Tensor | None = None, dout: torch.Tensor | None = None,
+                            dh: torch.Tensor | None = None, dx: torch.Tensor | None = None, dy: torch.Tensor | None = None,
+                            dw_after: torch.Tensor | None = None, dw_before: torch.Tensor | None = None,
+                            add_dw: bool = False):
+        """(dx, dy, dgate, dw_after, dw_before) of block_norm (sabah_block_norm_backward) from its out (x where it had no
+        y), y, gate, and the gradients dout of out (None: zeros) and dh of h; None for what the norm does not have.  Without a norm
+        before the next block dx is dout.  `dx` may be dout itself; add_dw adds to the dw given."""
+        T = self._norm_check(norm, out, y, gate)
+        before, after = norm.w_before is not None, y is not None and norm.w_after is not None
+        if (dh is None) == before or (dout is None and not before):
+            raise ValueError("block_norm_backward: dh goes with a norm before the next block, dout with none")
+        if add_dw and ((after and dw_after is None) or (before and dw_before is None)):
+            raise ValueError("block_norm_backward: add_dw needs dw_after and dw_before")
+        rows = [self._norm_rows(n, norm, t, out) for n, t in (("out", out), ("y", y), ("dout", dout), ("dh", dh))]
+        if not before:
+            dx = None
+        elif dx is None:
+            dx = torch.empty(out.shape, dtype=out.dtype, device=self.device)
+        if y is None:
+            dy = None
+        elif dy is None:
+            dy = torch.empty(out.shape, dtype=out.dtype, device=self.device)
+        dgate = torch.empty(T, dtype=torch.float32, device=self.device) if gate is not None else None
+        dw = []
+        for has, w in ((after, dw_after), (before, dw_before)):
+            if not has:
+                w = None
+            elif w is None:
+                w = torch.empty(norm.width, dtype=torch.float32, device=self.device)
+            elif w.dtype is not torch.float32 or w.shape != (norm.width,) or not w.is_contiguous() or w.get_device() != self._index:
+                raise ValueError("block_norm_backward: a weight gradient is %s %s, expected contiguous f32 [%d]"
+                                 % (tuple(w.shape), w.dtype, norm.width))
+            dw.append(w)
+        lib = rt.lib()
+        n = lib.sabah_block_norm_workspace(norm.width, T)
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        rc = lib.sabah_block_norm_backward(
+            norm.ref(out.dtype, y is not None), *rows[0], *rows[1], gate.data_ptr() if gate is not None else None, T, *rows[2],
+            *rows[3], *self._norm_rows("dx", norm, dx, out), *self._norm_rows("dy", norm, dy, out),
+            dgate.data_ptr() if gate is not None else None, dw[0].data_ptr() if after else None,
+            dw[1].data_ptr() if before else None, int(add_dw), ws.data_ptr(), n, _stream(self.device))
+        if rc:
+            rt.check(rc, "block_norm_backward")
+        return dx if before else dout, dy, dgate, dw[0], dw[1]
+
+    def group_rows(self, ids: torch.Tensor, n_experts: int | None = None, out: RowGroups | None = None) -> RowGroups:
+        """The (token, slot) rows of ids [T, n_ids] i32 (-1: no expert) grouped by expert (sabah_expert_group), for
+        every product over the same ids.  n_experts: the bank's when not given; `out` brings its own."""
+        if ids.dtype is not torch.int32 or ids.dim() != 2 or ids.get_device() != self._index:
+            raise ValueError("group_rows: ids %s %s on %s" % (tuple(ids.shape), ids.dtype, ids.device))
+        T, n_ids = ids.shape
+        if out is None:
+            out = RowGroups(T, n_ids, self.bank.n_experts if n_experts is None else n_experts, device=self.device)
+        elif (out.n_tokens, out.n_ids) != (T, n_ids) or out.index != self._index or n_experts not in (None, out.n_experts):
+            raise ValueError("group_rows: ids %s, out is for [%d, %d]" % (tuple(ids.shape), out.n_tokens, out.n_ids))
+        s = ids.stride()
+        rc = rt.lib().sabah_expert_group(ids.data_ptr(), s[1] * 4, s[0] * 4, n_ids, T, out.n_experts, out.buffer.data_ptr(),
+                                         out.bytes, _stream(self.device))
+        if rc:
+            rt.check(rc, "group_rows")
+        return out
+
+    def _expert_x(self, experts: FloatExperts, x: torch.Tensor, groups: RowGroups):
+        """The checks that the two calls share; C arguments of x and the groups."""
+        shape, xs, es = x.shape, x.stride(), x.element_size()
+        if len(shape) == 3:
+            xr, xi = shape[1], xs[1] * es
+        elif len(shape) == 2:
+            xr, xi = 1, 0
+        else:
+            xr = 0
+        if (not xr or x.dtype is not experts.dtype or shape[0] != groups.n_tokens or shape[-1] != experts.k
+                or (xs[-1] != 1 and shape[0] and experts.k > 1) or (xr != 1 and xr != groups.n_ids)):
+            raise ValueError("experts: x %s %s for %s %d -> %d, groups of [%d, %d]"
+                             % (tuple(shape), x.dtype, experts.dtype, experts.k, experts.rows, groups.n_tokens, groups.n_ids))
+        if groups.n_experts != experts.n_experts:
+            raise ValueError("experts: groups of %d experts for %d" % (groups.n_experts, experts.n_experts))
+        if x.get_device() != self._index or experts.index != self._index or groups.index != self._index:
+            raise ValueError("experts: the tensors are not on %s" % self.device)
+        return (experts.ref, x.data_ptr(), xi, xr, xs[0] * es, groups.buffer.data_ptr(), groups.bytes, groups.n_ids,
+                groups.n_tokens)
+
+    def _expert_y(self, what: str, experts: FloatExperts, y: torch.Tensor, groups: RowGroups, width: int):
+        """(address, slot stride, token stride) of rows [T, n_ids, width] in the experts' type."""
+        if (y.dtype is not experts.dtype or y.shape != (groups.n_tokens, groups.n_ids, width) or y.get_device() != self._index
+                or (y.stride(2) != 1 and y.shape[0] and width > 1)):
+            raise ValueError("experts: %s is %s %s, expected %s [%d, %d, %d] with contiguous rows on %s"
+                             % (what, tuple(y.shape), y.dtype, experts.dtype, groups.n_tokens, groups.n_ids, width, self.device))
+        s, es = y.stride(), y.element_size()
+        return y.data_ptr(), s[1] * es, s[0] * es
+
+    def expert_mul(self, experts: FloatExperts, x: torch.Tensor, groups: RowGroups,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+        """y [T, n_ids, rows] = W[ids[t][i]] x[t][i] for the ids that `groups` was made from (sabah_expert_mul): x
+        [T, k] or [T, x_rows, k] (x_rows = 1 or n_ids) in the experts' type; zeros where the id is -1."""
+        args = self._expert_x(experts, x, groups)
+        if out is None:
+            out = torch.empty((groups.n_tokens, groups.n_ids, experts.rows), dtype=experts.dtype, device=self.device)
+        rc = rt.lib().sabah_expert_mul(*args, *self._expert_y("out", experts, out, groups, experts.rows), _stream(self.device))
+        if rc:
+            rt.check(rc, "expert_mul")
+        return out
+
+    def expert_mul_backward(self, experts: FloatExperts, x: torch.Tensor, groups: RowGroups, dy: torch.Tensor,
+                            dx: torch.Tensor | None = None, dw: torch.Tensor | None = None, add_dw: bool = False,
+                            need_dx: bool = True, need_dw: bool = True):
+        """The gradients (dx, dw) of expert_mul for dy, the gradient of its result (sabah_expert_mul_backward): dx
+        [T, n_ids, k] in the experts' type, a row for each slot, dw [n_experts, rows, k] f32, written or with add_dw added to;
+        None for what need_dx / need_dw leave out."""
+        args = self._expert_x(experts, x, groups)
+        if add_dw and dw is None:
+            raise ValueError("expert_mul_backward: add_dw needs dw")
+        d = None, 0, 0
+        if need_dx:
+            if dx is None:
+                dx = torch.empty((groups.n_tokens, groups.n_ids, experts.k), dtype=experts.dtype, device=self.device)
+            d = self._expert_y("dx", experts, dx, groups, experts.k)
+        if need_dw:
+            if dw is None:
+                dw = torch.empty(experts.w.shape, dtype=torch.float32, device=self.device)
+            elif (dw.dtype is not torch.float32 or dw.shape != experts.w.shape or not dw.is_contiguous()
+                  or dw.get_device() != self._index):
+                raise ValueError("expert_mul_backward: dw is %s %s, expected contiguous f32 %s"
+                                 % (tuple(dw.shape), dw.dtype, tuple(experts.w.shape)))
+        rc = rt.lib().sabah_expert_mul_backward(*args, *self._expert_y("dy", experts, dy, groups, experts.rows), *d,
+                                                dw.data_ptr() if need_dw else None, int(add_dw), _stream(self.device))
+        if rc:
+            rt.check(rc, "expert_mul_backward")
+        return dx if need_dx else None, dw if need_dw else None
 
     # ---- fused layer / chain --------------------------------------------------
     def run_layer(self, layer: int, x: torch.Tensor, ids: torch.Tensor, w: torch.Tensor,

@@ -64,6 +64,32 @@ class LoraDesc(ctypes.Structure):
                 ("n_adapters", c_i), ("n_experts", c_i), ("rank", c_i), ("k", c_i), ("rows", c_i)]
 
 
+class NormDesc(ctypes.Structure):
+    """sabah_norm_desc (include/sabah_rt.h)."""
+    _fields_ = [("w_after", c_vp), ("w_before", c_vp), ("type", c_i), ("width", c_i), ("eps", ctypes.c_float),
+                ("scale", ctypes.c_float)]
+
+
+class ExpertDesc(ctypes.Structure):
+    """sabah_expert_desc (include/sabah_rt.h)."""
+    _fields_ = [("w", c_vp), ("type", c_i), ("n_experts", c_i), ("k", c_i), ("rows", c_i)]
+
+
+class AdamWTensor(ctypes.Structure):
+    """sabah_adamw_tensor (include/sabah_rt.h)."""
+    _fields_ = [("p", c_vp), ("g", c_vp), ("master", c_vp), ("decay", ctypes.c_double), ("n", ctypes.c_longlong),
+                ("p_type", c_i), ("g_type", c_i)]
+
+
+class AdamWDesc(ctypes.Structure):
+    """sabah_adamw_desc (include/sabah_rt.h)."""
+    _fields_ = [("table", c_vp), ("table_bytes", c_sz), ("n_tensors", c_i), ("bits", c_i), ("m", c_vp), ("v", c_vp),
+                ("m_scale", c_vp), ("v_scale", c_vp), ("lr", ctypes.c_double), ("beta1", ctypes.c_double),
+                ("beta2", ctypes.c_double), ("eps", ctypes.c_double), ("grad_scale", ctypes.c_double),
+                ("max_norm", ctypes.c_double), ("d_lr", c_vp), ("step", c_vp), ("norm", c_vp), ("workspace", c_vp),
+                ("workspace_bytes", c_sz)]
+
+
 # every symbol include/sabah_rt.h declares, with its ctypes signature
 SIGNATURES = {
     "sabah_rt_init": ([c_i], c_i),
@@ -98,6 +124,22 @@ SIGNATURES = {
                           c_vp, c_sz, c_sz, c_vp, c_sz, c_sz, c_vp, c_sz, c_vp], c_i),
     "sabah_lora_backward": ([ctypes.POINTER(LoraDesc), c_vp, c_sz, c_i, c_sz, c_vp, c_vp, c_sz, c_sz, c_i, c_i,
                              c_vp, c_sz, c_sz, c_vp, c_sz, c_sz, c_i, c_vp, c_vp, c_i, c_vp, c_sz, c_vp], c_i),
+    "sabah_block_norm": ([ctypes.POINTER(NormDesc), c_vp, c_sz, c_vp, c_sz, c_vp, c_i, c_vp, c_sz, c_vp, c_sz, c_vp], c_i),
+    "sabah_block_norm_workspace": ([c_i, c_i], c_sz),
+    "sabah_block_norm_backward": ([ctypes.POINTER(NormDesc), c_vp, c_sz, c_vp, c_sz, c_vp, c_i, c_vp, c_sz, c_vp, c_sz,
+                                   c_vp, c_sz, c_vp, c_sz, c_vp, c_vp, c_vp, c_i, c_vp, c_sz, c_vp], c_i),
+    "sabah_expert_groups_bytes": ([c_i, c_i, c_i], c_sz),
+    "sabah_expert_group": ([c_vp, c_sz, c_sz, c_i, c_i, c_i, c_vp, c_sz, c_vp], c_i),
+    "sabah_expert_mul": ([ctypes.POINTER(ExpertDesc), c_vp, c_sz, c_i, c_sz, c_vp, c_sz, c_i, c_i, c_vp, c_sz, c_sz,
+                          c_vp], c_i),
+    "sabah_expert_mul_backward": ([ctypes.POINTER(ExpertDesc), c_vp, c_sz, c_i, c_sz, c_vp, c_sz, c_i, c_i, c_vp, c_sz,
+                                   c_sz, c_vp, c_sz, c_sz, c_vp, c_i, c_vp], c_i),
+    "sabah_adamw_table_bytes": ([ctypes.POINTER(AdamWTensor), c_i, ctypes.POINTER(ctypes.c_longlong)], c_sz),
+    "sabah_adamw_table": ([ctypes.POINTER(AdamWTensor), c_i, c_vp, c_sz], c_i),
+    "sabah_adamw_workspace": ([], c_sz),
+    "sabah_adamw_step": ([ctypes.POINTER(AdamWDesc), c_vp], c_i),
+    "sabah_adamw_moments_read": ([c_vp, c_vp, c_vp, c_vp, ctypes.c_longlong, c_vp, c_vp, c_vp], c_i),
+    "sabah_adamw_moments_write": ([c_vp, c_vp, ctypes.c_longlong, c_vp, c_vp, c_vp, c_vp, c_vp], c_i),
     # memory, copies, events and streams for the harness (the reference binds them, rt.py:70-107)
     "sabah_dev_alloc": ([c_sz], c_vp),
     "sabah_dev_free": ([c_vp], None),
