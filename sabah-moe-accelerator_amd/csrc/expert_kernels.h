@@ -118,14 +118,14 @@ __device__ inline void exp_store(uint8_t* p, xu4 r, int left) {
 // groups of another shape, or never made, sets the sticky error word and ends.
 constexpr int kExpHead = 16;
 constexpr uint32_t kExpMagic = 0x67727031u;
-constexpr int kExpSmall = 16, kExpTile = 128;     // rows of the two lists' tiles
+constexpr int kExpSmall = 16, kExpTile = 128, kExpLarge = 256;   // rows of the three lists' tiles
 constexpr int kExpChunk = 4096;                   // rows that a workgroup of k_expert_count / _place sorts
 constexpr int kExpMaxExperts = 4096;
 constexpr unsigned kErrExpertId = 1u, kErrExpertGroups = 5u;
 struct ExpertPlan {
     int n_rows, n_ids, n_experts, chunks;
-    size_t off, order, small, tiles, counts, words;   // in words from the buffer's start
-    int max_small, max_tiles;
+    size_t off, order, small, tiles, large, counts, words;   // in words from the buffer's start
+    int max_small, max_tiles, max_large;
 };
 inline ExpertPlan expert_plan(int n_ids, int n_tokens, int n_experts) {
     ExpertPlan p{};
@@ -136,6 +136,7 @@ inline ExpertPlan expert_plan(int n_ids, int n_tokens, int n_experts) {
     const int groups = p.n_rows < n_experts + 2 ? p.n_rows : n_experts + 2;
     p.max_small = p.n_rows / kExpSmall + groups;
     p.max_tiles = p.n_rows / kExpTile + groups;
+    p.max_large = p.n_rows / kExpLarge + groups;
     auto take = [&](size_t n) {
         const size_t at = p.words;
         p.words += (n + 3) / 4 * 4;
@@ -146,11 +147,12 @@ inline ExpertPlan expert_plan(int n_ids, int n_tokens, int n_experts) {
     p.order = take(p.n_rows);                         // the rows in that order
     p.small = take((size_t)p.max_small * 4);          // tiles (expert, first position, rows, 0); expert -1, -2: none, bad
     p.tiles = take((size_t)p.max_tiles * 4);
+    p.large = take((size_t)p.max_large * 4);
     p.counts = take(p.chunks > 1 ? (size_t)p.chunks * (n_experts + 2) : 0);
     return p;
 }
 // words of the head
-constexpr int kExpHeadMagic = 0, kExpHeadRows = 1, kExpHeadIds = 2, kExpHeadExperts = 3, kExpHeadSmall = 4, kExpHeadTiles = 5;
+constexpr int kExpHeadMagic = 0, kExpHeadRows = 1, kExpHeadIds = 2, kExpHeadExperts = 3, kExpHeadSmall = 4, kExpHeadTiles = 5, kExpHeadLarge = 6;
 
 struct ExpertGroupArgs {
     const uint8_t* ids;
@@ -180,18 +182,18 @@ __device__ inline void exp_read_keys(const ExpertGroupArgs& a, int chunk, int (&
     }
 }
 
-__device__ inline int exp_block_scan(int v, int* tmp, int& total) {    // exclusive, over kExpGroupThreads
+__device__ inline uint64_t exp_block_scan(uint64_t v, uint64_t* tmp, uint64_t& total) {    // exclusive, over kExpGroupThreads
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    int s = v;
+    uint64_t s = v;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(s, d);
+        const uint64_t o = __shfl_up((unsigned long long)s, d);
         if (lane >= d) s += o;
     }
     __syncthreads();
     if (lane == 63) tmp[wave] = s;
     __syncthreads();
-    int before = 0;
+    uint64_t before = 0;
     total = 0;
 #pragma unroll
     for (int w = 0; w < kExpGroupWaves; ++w) {
@@ -215,58 +217,66 @@ __global__ __launch_bounds__(kExpGroupThreads) void k_expert_count(ExpertGroupAr
     for (int e = threadIdx.x; e < keys; e += kExpGroupThreads) a.g[a.p.counts + (size_t)blockIdx.x * keys + e] = exp_lds[e];
 }
 
-// The keys' first positions and their tiles, from cnt(e), by one workgroup.  base(e, at): where key e begins
+__device__ inline void exp_head(const ExpertGroupArgs& a, int small, int tiles, int large) {
+    a.g[a.p.off + a.p.n_experts + 2] = a.p.n_rows;
+    a.g[kExpHeadMagic] = kExpMagic;
+    a.g[kExpHeadRows] = a.p.n_rows;
+    a.g[kExpHeadIds] = a.p.n_ids;
+    a.g[kExpHeadExperts] = a.p.n_experts;
+    a.g[kExpHeadSmall] = small;
+    a.g[kExpHeadTiles] = tiles;
+    a.g[kExpHeadLarge] = large;
+}
+constexpr int exp_tiles(int rows, int of) { return (rows + of - 1) / of; }
+
+// The keys' first positions and, where WRITE, their tiles, from cnt(e), by one workgroup.  base(e, at): where key e begins
 template <typename Count, typename Base>
-__device__ inline void exp_lists(const ExpertGroupArgs& a, int* tmp, Count cnt, Base base) {
+__device__ inline void exp_lists(const ExpertGroupArgs& a, uint64_t* tmp, bool write, Count cnt, Base base) {
     const int E = a.p.n_experts, keys = E + 2;
     const int seg = (keys + kExpGroupThreads - 1) / kExpGroupThreads;
     const int e0 = min(keys, (int)threadIdx.x * seg), e1 = min(keys, e0 + seg);
-    int rows = 0, small = 0, tiles = 0, total;
+    uint64_t one = 0, two = 0, total, total2 = 0;               // rows and small tiles, tiles and large ones: 32 bits each
     for (int e = e0; e < e1; ++e) {
         const int c = cnt(e);
-        rows += c;
-        small += (c + kExpSmall - 1) / kExpSmall;
-        tiles += (c + kExpTile - 1) / kExpTile;
+        one += (uint64_t)c | (uint64_t)exp_tiles(c, kExpSmall) << 32;
+        two += (uint64_t)exp_tiles(c, kExpTile) | (uint64_t)exp_tiles(c, kExpLarge) << 32;
     }
-    int at = exp_block_scan(rows, tmp, total);
-    int s = exp_block_scan(small, tmp, total);
-    const int n_small = total;
-    int t = exp_block_scan(tiles, tmp, total);
+    one = exp_block_scan(one, tmp, total);
+    if (write) two = exp_block_scan(two, tmp, total2);          // uniform
+    int at = (int)(uint32_t)one, s = (int)(one >> 32), t = (int)(uint32_t)two, l = (int)(two >> 32);
     int4* ls = reinterpret_cast<int4*>(a.g + a.p.small);
     int4* lt = reinterpret_cast<int4*>(a.g + a.p.tiles);
+    int4* ll = reinterpret_cast<int4*>(a.g + a.p.large);
     for (int e = e0; e < e1; ++e) {
         const int c = cnt(e), who = e < E ? e : E - 1 - e;
-        a.g[a.p.off + e] = at;
-        for (int o = 0; o < c; o += kExpSmall) ls[s++] = make_int4(who, at + o, min(kExpSmall, c - o), 0);
-        for (int o = 0; o < c; o += kExpTile) lt[t++] = make_int4(who, at + o, min(kExpTile, c - o), 0);
+        if (write) {
+            a.g[a.p.off + e] = at;
+            for (int o = 0; o < c; o += kExpSmall) ls[s++] = make_int4(who, at + o, min(kExpSmall, c - o), 0);
+            for (int o = 0; o < c; o += kExpTile) lt[t++] = make_int4(who, at + o, min(kExpTile, c - o), 0);
+            for (int o = 0; o < c; o += kExpLarge) ll[l++] = make_int4(who, at + o, min(kExpLarge, c - o), 0);
+            if (e == E + 1 && c) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrExpertId;
+        }
         base(e, at);
         at += c;
-        if (e == E + 1 && c) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrExpertId;
     }
-    if (threadIdx.x == 0) {
-        a.g[a.p.off + keys] = a.p.n_rows;
-        a.g[kExpHeadMagic] = kExpMagic;
-        a.g[kExpHeadRows] = a.p.n_rows;
-        a.g[kExpHeadIds] = a.p.n_ids;
-        a.g[kExpHeadExperts] = E;
-        a.g[kExpHeadSmall] = n_small;
-        a.g[kExpHeadTiles] = total;
-    }
+    if (write && threadIdx.x == 0) exp_head(a, (int)(total >> 32), (int)(uint32_t)total2, (int)(total2 >> 32));
 }
 
-// Several chunks: the counts of each become where its rows of a key begin
+// Many chunks: the counts of each become where its rows of a key begin
 __global__ __launch_bounds__(kExpGroupThreads) void k_expert_scan(ExpertGroupArgs a) {
-    __shared__ int tmp[kExpGroupWaves];
+    __shared__ uint64_t tmp[kExpGroupWaves];
     extern __shared__ int exp_lds[];
     const int keys = a.p.n_experts + 2;
     uint32_t* counts = a.g + a.p.counts;
     for (int e = threadIdx.x; e < keys; e += kExpGroupThreads) {
         int s = 0;
+#pragma unroll 16
         for (int c = 0; c < a.p.chunks; ++c) s += (int)counts[(size_t)c * keys + e];
         exp_lds[e] = s;
     }
     __syncthreads();
-    exp_lists(a, tmp, [&](int e) { return exp_lds[e]; }, [&](int e, int at) {
+    exp_lists(a, tmp, true, [&](int e) { return exp_lds[e]; }, [&](int e, int at) {
+#pragma unroll 16
         for (int c = 0; c < a.p.chunks; ++c) {
             const int n = (int)counts[(size_t)c * keys + e];
             counts[(size_t)c * keys + e] = (uint32_t)at;
@@ -275,18 +285,40 @@ __global__ __launch_bounds__(kExpGroupThreads) void k_expert_scan(ExpertGroupArg
     });
 }
 
-// The rows' places.  ALONE: the one chunk of a small call, whose lists are made here too.
-template <bool ALONE>
+// The rows' places.  kPlaceAlone: the one chunk of a small call, whose lists are made here too; kPlaceSum: of up to
+// kExpSumChunks chunks each adds up the others' counts by itself, and the first makes the lists (a launch less: 8 us);
+// kPlaceScanned: after k_expert_scan.
+constexpr int kPlaceAlone = 0, kPlaceSum = 1, kPlaceScanned = 2, kExpSumChunks = 64;
+template <int HOW>
 __global__ __launch_bounds__(kExpGroupThreads) void k_expert_place(ExpertGroupArgs a) {
-    extern __shared__ int exp_lds[];                  // [waves][words] counts of 16 bits; [keys] starts; scan
+    extern __shared__ uint64_t exp_place[];           // scan; [waves][words] counts of 16 bits; [keys] starts (and totals)
     const int keys = a.p.n_experts + 2, words = (keys + 1) / 2;
-    uint32_t* hist = reinterpret_cast<uint32_t*>(exp_lds);
-    int* start = exp_lds + kExpGroupWaves * words;
-    int* tmp = start + keys;
+    uint64_t* tmp = exp_place;
+    uint32_t* hist = reinterpret_cast<uint32_t*>(tmp + kExpGroupWaves);
+    int* start = reinterpret_cast<int*>(hist + kExpGroupWaves * words);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int e = threadIdx.x; e < kExpGroupWaves * words; e += kExpGroupThreads) hist[e] = 0;
     int key[kExpWaveSteps];
     exp_read_keys(a, blockIdx.x, key);
+    if constexpr (HOW == kPlaceSum) {
+        int* sum = start + keys;
+        const uint32_t* counts = a.g + a.p.counts;
+        for (int e = threadIdx.x; e < keys; e += kExpGroupThreads) {
+            int all = 0, before = 0;
+#pragma unroll 16
+            for (int c = 0; c < a.p.chunks; ++c) {
+                const int n = (int)counts[(size_t)c * keys + e];
+                all += n;
+                before += c < (int)blockIdx.x ? n : 0;
+            }
+            sum[e] = all;
+            start[e] = before;
+        }
+        __syncthreads();
+        exp_lists(a, tmp, blockIdx.x == 0, [&](int e) { return sum[e]; }, [&](int e, int at) { start[e] += at; });
+    } else if constexpr (HOW == kPlaceScanned) {
+        for (int e = threadIdx.x; e < keys; e += kExpGroupThreads) start[e] = (int)a.g[a.p.counts + (size_t)blockIdx.x * keys + e];
+    }
     __syncthreads();
     uint32_t* mine = hist + wave * words;
 #pragma unroll
@@ -302,18 +334,16 @@ __global__ __launch_bounds__(kExpGroupThreads) void k_expert_place(ExpertGroupAr
             hist[v * words + w] = sum;
             sum += c;
         }
-        if constexpr (ALONE) {
+        if constexpr (HOW == kPlaceAlone) {
             start[2 * w] = (int)(sum & 0xFFFFu);
             if (2 * w + 1 < keys) start[2 * w + 1] = (int)(sum >> 16);
         }
     }
     __syncthreads();
-    if constexpr (ALONE) {
-        exp_lists(a, tmp, [&](int e) { return start[e]; }, [&](int e, int at) { start[e] = at; });
-    } else {
-        for (int e = threadIdx.x; e < keys; e += kExpGroupThreads) start[e] = (int)a.g[a.p.counts + (size_t)blockIdx.x * keys + e];
+    if constexpr (HOW == kPlaceAlone) {
+        exp_lists(a, tmp, true, [&](int e) { return start[e]; }, [&](int e, int at) { start[e] = at; });
+        __syncthreads();
     }
-    __syncthreads();
     const int first = blockIdx.x * kExpChunk + wave * kExpWaveRows;
     uint16_t* taken = reinterpret_cast<uint16_t*>(mine);
     const int bits = 32 - __builtin_clz(keys);
@@ -334,6 +364,53 @@ __global__ __launch_bounds__(kExpGroupThreads) void k_expert_place(ExpertGroupAr
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the next step's lanes read what this one's left
         __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// At most 64 rows (decode): a lane has a row, and learns of the others from their lanes; every wave the same, each for its
+// share of the keys' first positions, the first wave for the rest.  No counts, no scans: 4 us where the general form takes 8.
+constexpr int kExpFewGroup = 64;
+__global__ __launch_bounds__(256) void k_expert_group_few(ExpertGroupArgs a) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, E = a.p.n_experts;
+    const bool some = lane < a.p.n_rows;
+    const int key = some ? exp_key(a, lane) : E + 2;
+    for (int e = threadIdx.x; e < E + 2; e += 256) {
+        int at = 0;
+        for (int j = 0; j < a.p.n_rows; ++j) at += __builtin_amdgcn_readlane(key, j) < e ? 1 : 0;
+        a.g[a.p.off + e] = at;
+    }
+    if (wave) return;
+    // rows before this one's key and with it; a key's first row writes its tiles (rows of a key: at most 64, one tile and
+    // up to four small ones)
+    int at = 0, before = 0, rows = 0, bad = 0;
+    for (int j = 0; j < a.p.n_rows; ++j) {
+        const int k = __builtin_amdgcn_readlane(key, j);
+        at += k < key ? 1 : 0;
+        rows += k == key ? 1 : 0;
+        before += k == key && j < lane ? 1 : 0;
+        bad |= k == E + 1;
+    }
+    static_assert(kExpFewGroup <= kExpTile, "a key's rows are one tile");
+    const bool leads = some && before == 0;
+    int s = 0, t = 0, small = 0, tiles = 0;
+    for (int j = 0; j < a.p.n_rows; ++j) {
+        if (!__builtin_amdgcn_readlane(leads ? 1 : 0, j)) continue;
+        const int k = __builtin_amdgcn_readlane(key, j), n = exp_tiles(__builtin_amdgcn_readlane(rows, j), kExpSmall);
+        small += n;
+        ++tiles;
+        s += k < key ? n : 0;
+        t += k < key ? 1 : 0;
+    }
+    if (some) a.g[a.p.order + at + before] = (uint32_t)lane;
+    if (leads) {
+        const int who = key < E ? key : E - 1 - key;
+        for (int o = 0; o < rows; o += kExpSmall) reinterpret_cast<int4*>(a.g + a.p.small)[s++] = make_int4(who, at + o, min(kExpSmall, rows - o), 0);
+        reinterpret_cast<int4*>(a.g + a.p.tiles)[t] = make_int4(who, at, rows, 0);
+        reinterpret_cast<int4*>(a.g + a.p.large)[t] = make_int4(who, at, rows, 0);
+    }
+    if (lane == 0) {
+        exp_head(a, small, tiles, tiles);
+        if (bad) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrExpertId;
     }
 }
 
@@ -593,14 +670,334 @@ __global__ __launch_bounds__(kExpThreads, 2) void k_expert_gemm(ExpertArgs a) {
     }
 }
 
+// The same tiles where every row of every operand begins at a multiple of 16 bytes and has a whole number of them:
+// both operands go from memory straight into LDS (1 KB a wave and instruction, no registers), the next stage's while the
+// matrix cores run on this one.  A lane's 16 bytes land at its own place of that KB, so the permutations of ExpGemm are made
+// by what each lane asks for.  Chunks past the summed axis come from `exp_zeros`; columns past the width
+// repeat the first and are not stored.
+// C: BM x BN tile, WM x WN waves, KB bytes of a contiguous row (or as many strided rows) a stage.
+static __device__ const uint32_t exp_zeros[4] = {0u, 0u, 0u, 0u};
+
+__device__ inline void exp_dma(const uint8_t* src, uint8_t* lds) {     // lds: the wave's; lane i fills lds + 16 i
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(src),
+                                     (__attribute__((address_space(3))) void*)(lds), 16, 0, 0);
+}
+// All but the last N of a wave's transfers are done, and its LDS reads, and that holds for all waves
+template <int N>
+__device__ inline void exp_stage_barrier() {
+    static_assert(N < 64, "vmcnt has 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// what may pass a transfer in the schedule: all but products and memory (LDS reads may)
+constexpr int kSchedBetween = 0x186;
+template <typename X, int MODE, int BM_, int BN_, int WM_, int WN_, int KB_, int S_>
+struct ExpFast {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = KB_, S = S_, NW = WM * WN, ES = (int)sizeof(typename X::S);
+    static constexpr int VEC = X::kVec, BK = KB / ES, STEPS = BK / (2 * VEC);          // of a stage
+    static constexpr bool TA = MODE == kModeDw, TB = MODE != kModeForward;
+    static constexpr int kA = BM * KB, kB = BN * KB;                                    // bytes of a stage (BK rows of BM values as well)
+    static constexpr int TRA = kA / 1024, NT = (kA + kB) / 1024 / NW;                   // transfers of A; of a wave
+    static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+    static constexpr int kStages = S * (kA + kB);
+    static constexpr int kWindow = 512;                    // rows of a weight gradient whose places are in LDS at a time
+    static constexpr int kLds = kStages + (MODE == kModeDw ? kWindow * 16 : 0);
+    static constexpr bool kLarge = BM == kExpLarge;
+    static_assert(MODE == kModeDw || BM == kExpTile || BM == kExpLarge, "one of the lists' tiles");
+    static_assert((kA + kB) % (1024 * NW) == 0, "whole transfers");
+    static_assert(NW % 2 == 0 && TRA % 2 == 0, "a lane's transfers are whole 16 rows apart, which the permutation repeats after");
+
+    // the chunk that lies at place p of a row, or the place of chunk p: the 16 lanes that are read at once (32 of 8
+    // bytes, 64 of 4) then lie in all 64 banks
+    static __device__ inline int swap_contiguous(int row, int p) { return KB == 128 ? p ^ ((row >> 1) & 7) : p ^ ((row >> 2) & 3); }
+    template <int COLS>
+    static __device__ inline int swap_strided(int row, int p) {
+        return ES == 4 ? p ^ ((row & 4) << 1) : COLS == 64 ? p ^ ((row & 2) << 1) : p ^ ((row & 3) << 2);
+    }
+    static __device__ inline xu4 contiguous(const uint8_t* t, int r0, int s) {
+        const int lane = threadIdx.x & 63, row = r0 + (lane & 31);
+        return *reinterpret_cast<const xu4*>(t + row * KB + (swap_contiguous(row, 2 * s + (lane >> 5)) << 4));
+    }
+    template <int COLS>
+    static __device__ inline xu4 strided(const uint8_t* t, int c0, int s) {
+        const int lane = threadIdx.x & 63;
+        xu4 r;
+        if constexpr (ES == 2) {
+            const int l = lane & 15, row = s * 16 + (lane >> 5) * 8 + (l >> 2), col = c0 + (lane & 16) + (l & 3) * 4;
+            const uint8_t* p = t + row * (COLS * ES) + (swap_strided<COLS>(row, col >> 3) << 4) + ((col & 4) << 1);
+            typedef __attribute__((address_space(3))) xs4 lds_xs4;
+            const xs4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_xs4*)(p));
+            const xs4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_xs4*)(p + 4 * COLS * ES));
+            __builtin_memcpy(&r, &lo, 8);
+            __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &hi, 8);
+        } else {
+            xf4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+            {
+                const int row = s * 8 + (lane >> 5) * 4 + j, col = c0 + (lane & 31);
+                v[j] = *reinterpret_cast<const float*>(t + row * (COLS * ES) + (swap_strided<COLS>(row, col >> 2) << 4) + (col & 3) * ES);
+            }
+            r = __builtin_bit_cast(xu4, v);
+        }
+        return r;
+    }
+};
+
+// The sum over `steps` stages.  Between two barriers lie the last products of a stage and the first of the next: their
+// operands are in registers when the barrier is reached (the next stage's first are read right after it), so the matrix
+// cores have work while the waves meet and LDS answers.  The transfers of stage t + S, into the buffer that the barrier frees,
+// go between those products: issued together they hold all waves up at once.  Stages past the end are
+// transferred too, as zeros: then S - 1 are always under way.  Rows: 32-row results of the wave that have rows at all.
+template <typename G, typename X, int Rows, typename Transfer>
+__device__ inline void exp_sum_rows(const uint8_t* tile, int steps, int wm, int wn, xf16 (&acc)[G::TM][G::TN], Transfer transfer) {
+    constexpr int S = G::S, P = G::STEPS, FIRST = G::NT / P;   // transfers that follow the barrier's first products
+    xu4 fa[2][G::TM], fb[2][G::TN];
+    auto fragments = [&](int t, int s, int to) {
+        const uint8_t* ta = tile + (t % S) * (G::kA + G::kB);
+        const uint8_t* tb = ta + G::kA;
+        if constexpr (Rows > 0) {
+#pragma unroll
+            for (int i = 0; i < Rows; ++i) {
+                if constexpr (G::TA) fa[to][i] = G::template strided<G::BM>(ta, wm + 32 * i, s);
+                else fa[to][i] = G::contiguous(ta, wm + 32 * i, s);
+            }
+#pragma unroll
+            for (int j = 0; j < G::TN; ++j) {
+                if constexpr (G::TB) fb[to][j] = G::template strided<G::BN>(tb, wn + 32 * j, s);
+                else fb[to][j] = G::contiguous(tb, wn + 32 * j, s);
+            }
+        }
+    };
+    // the products of operands `from`, with transfers [d0, d1) of stage t among them
+    auto products = [&](int from, int t, auto first, auto last) {
+        constexpr int d0 = decltype(first)::value, d1 = decltype(last)::value, ALL = Rows * G::TN;
+        if constexpr (Rows == 0) {
+#pragma unroll
+            for (int d = d0; d < d1; ++d) transfer(t, d);
+        }
+#pragma unroll
+        for (int i = 0; i < Rows; ++i)
+#pragma unroll
+            for (int j = 0; j < G::TN; ++j) {
+                // y and dx: the output's columns are the rows of the 32 x 32 result, so that a lane has four neighbours of them
+                acc[i][j] = G::TA ? X::mma32(fa[from][i], fb[from][j], acc[i][j]) : X::mma32(fb[from][j], fa[from][i], acc[i][j]);
+#pragma unroll
+                for (int d = d0; d < d1; ++d)
+                    if (i * G::TN + j == (d - d0) * ALL / (d1 - d0)) {
+                        __builtin_amdgcn_sched_barrier(kSchedBetween);
+                        transfer(t, d);
+                        __builtin_amdgcn_sched_barrier(kSchedBetween);
+                    }
+            }
+    };
+    static_assert(P == 2 || P == 4, "a stage's steps");
+#pragma unroll
+    for (int t = 0; t < S - 1; ++t)
+#pragma unroll
+        for (int j = 0; j < G::NT; ++j) transfer(t, j);
+    exp_stage_barrier<(S - 2) * G::NT>();
+    fragments(0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < FIRST; ++j) transfer(S - 1, j);
+    for (int t = 0; t < steps; ++t) {
+        fragments(t, 1, 1);
+        products(0, t + S - 1, std::integral_constant<int, FIRST>{}, std::integral_constant<int, P == 2 ? G::NT : 2 * FIRST>{});
+        if constexpr (P == 4) {
+            fragments(t, 2, 0);
+            products(1, t + S - 1, std::integral_constant<int, 2 * FIRST>{}, std::integral_constant<int, 3 * FIRST>{});
+            fragments(t, 3, 1);
+            products(0, t + S - 1, std::integral_constant<int, 3 * FIRST>{}, std::integral_constant<int, G::NT>{});
+        }
+        exp_stage_barrier<(S - 2) * G::NT>();
+        fragments(t + 1, 0, 0);
+        products(1, t + S, std::integral_constant<int, 0>{}, std::integral_constant<int, FIRST>{});
+    }
+    exp_stage_barrier<0>();                                 // nothing is under way, and the stages are free
+}
+template <typename G, typename X, typename Transfer>
+__device__ inline void exp_sum(const uint8_t* tile, int steps, int wm, int wn, int rows, xf16 (&acc)[G::TM][G::TN], Transfer transfer) {
+    if (rows > 32 * (G::TM - 1)) exp_sum_rows<G, X, G::TM>(tile, steps, wm, wn, acc, transfer);
+    else if (G::TM > 2 && rows > 64) exp_sum_rows<G, X, G::TM - 1>(tile, steps, wm, wn, acc, transfer);
+    else if (G::TM > 2 && rows > 32) exp_sum_rows<G, X, G::TM - 2>(tile, steps, wm, wn, acc, transfer);
+    else if (rows > 0) exp_sum_rows<G, X, 1>(tile, steps, wm, wn, acc, transfer);
+    else exp_sum_rows<G, X, 0>(tile, steps, wm, wn, acc, transfer);
+}
+
+// y and dx.  Transfer q of a stage fills its KB q, of A and then of B: a lane's 16 bytes come from src[j] + stage * step[j]
+// while their place on the summed axis, stage * BK + at[j], is inside, and else from exp_zeros.
+template <typename X, int MODE, int BM, int BN, int WM, int WN, int KB, int S, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void k_expert_fast(ExpertArgs a) {
+    typedef ExpFast<X, MODE, BM, BN, WM, WN, KB, S> G;
+    constexpr int ES = G::ES, VEC = G::VEC, BK = G::BK, NT = G::NT;
+    extern __shared__ __align__(16) uint8_t exp_tile[];
+    if (!exp_groups_fit(a)) return;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int width = MODE == kModeForward ? a.rows : a.k, K = MODE == kModeForward ? a.k : a.rows;
+    const int col_tiles = (width + BN - 1) / BN;
+    int work;
+    if (!exp_work(blockIdx.x, (int)a.g[G::kLarge ? kExpHeadLarge : kExpHeadTiles] * col_tiles, work)) return;
+    const int4 it = reinterpret_cast<const int4*>(a.g + (G::kLarge ? a.p.large : a.p.tiles))[work / col_tiles];
+    const int n0 = work % col_tiles * BN;
+    if (it.x < 0) {
+        exp_fill<X>(a, it, n0, BN, width);
+        return;
+    }
+    const uint32_t* order = a.g + a.p.order + it.y;
+    const uint8_t* w = a.w + (size_t)it.x * a.rows * a.k * ES;
+    constexpr int RC = 1024 / KB, CC = KB / 16;             // of a contiguous operand's transfer: rows, chunks of a row
+    constexpr int CB = BN * ES / 16, RB = 64 / CB;          // of a strided one's
+    uint64_t src[NT], step[NT];
+    int at[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int q = j * G::NW + wave, b = q - G::TRA;
+        if (q < G::TRA) {                                   // rows past the tile repeat its last and are not stored
+            const int m = q * RC + lane / CC;
+            const uint32_t row = order[min(m, it.z - 1)];
+            at[j] = G::swap_contiguous(m, lane % CC) * VEC;
+            src[j] = (uint64_t)((MODE == kModeForward ? exp_row_x(a, row) : exp_row_dy(a, row)) + at[j] * ES);
+            step[j] = KB;
+        } else if constexpr (!G::TB) {
+            const int n = b * RC + lane / CC;
+            at[j] = G::swap_contiguous(n, lane % CC) * VEC;
+            src[j] = (uint64_t)(w + ((size_t)min(n0 + n, a.rows - 1) * a.k + at[j]) * ES);
+            step[j] = KB;
+        } else {
+            const int r = b * RB + lane / CB, c = n0 + G::template swap_strided<BN>(r, lane % CB) * VEC;
+            at[j] = r;
+            src[j] = (uint64_t)(w + ((size_t)r * a.k + (c < a.k ? c : 0)) * ES);
+            step[j] = (uint64_t)BK * a.k * ES;
+        }
+    }
+    const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    uint32_t out[G::TM];                                    // rows of the lane's results
+#pragma unroll
+    for (int i = 0; i < G::TM; ++i) out[i] = order[min(wm + 32 * i + (lane & 31), it.z - 1)];
+    const uint8_t* zeros = reinterpret_cast<const uint8_t*>(exp_zeros);
+    xf16 acc[G::TM][G::TN] = {};
+    exp_sum<G, X>(exp_tile, (K + BK - 1) / BK, wm, wn, it.z - wm, acc, [&](int t, int j) {
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(src[j] + (uint64_t)t * step[j]);
+        exp_dma(t * BK + at[j] < K ? p : zeros, exp_tile + (t % S) * (G::kA + G::kB) + (j * G::NW + wave) * 1024);
+    });
+    // a lane has output row lane % 32, columns 8 (v / 4) + 4 (lane / 32) + v % 4
+#pragma unroll
+    for (int i = 0; i < G::TM; ++i) {
+        if (wm + 32 * i + (lane & 31) >= it.z) continue;
+        uint8_t* o = exp_row_out(a, out[i]);
+#pragma unroll
+        for (int j = 0; j < G::TN; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4) {
+                const int n = n0 + wn + 32 * j + 2 * v + 4 * (lane >> 5);
+                typename X::S s4[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s4[c] = X::put(acc[i][j][v + c]);
+                if (n < width) {                            // whole fours: rows are multiples of 16 bytes
+                    if constexpr (ES == 4) *reinterpret_cast<xu4*>(o + (size_t)n * ES) = __builtin_bit_cast(xu4, s4);
+                    else *reinterpret_cast<xu2*>(o + (size_t)n * ES) = __builtin_bit_cast(xu2, s4);
+                }
+            }
+    }
+}
+
+// dW: a tile of dy's columns by x's, summed over the rows of its expert.  Where the rows lie is kept in LDS, a window of them at a time.
+template <typename X, int BM, int BN, int WM, int WN, int KB, int S, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void k_expert_dw(ExpertArgs a) {
+    typedef ExpFast<X, kModeDw, BM, BN, WM, WN, KB, S> G;
+    constexpr int ES = G::ES, VEC = G::VEC, BK = G::BK, NT = G::NT;
+    extern __shared__ __align__(16) uint8_t exp_tile[];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int row_tiles = (a.rows + BM - 1) / BM, col_tiles = (a.k + BN - 1) / BN;
+    int work;
+    if (!exp_work(blockIdx.x, a.p.n_experts * row_tiles * col_tiles, work)) return;
+    const int expert = work / (row_tiles * col_tiles);
+    work -= expert * row_tiles * col_tiles;
+    const int m0 = work / col_tiles * BM, n0 = work % col_tiles * BN;
+    // read beside the head, not after it
+    const int first = (int)a.g[a.p.off + expert], count = (int)a.g[a.p.off + expert + 1] - first;
+    if (!exp_groups_fit(a)) return;
+    if (count == 0 && a.add) return;
+    const uint32_t* order = a.g + a.p.order + first;
+    constexpr int CA = BM * ES / 16, RA = 64 / CA, CB = BN * ES / 16, RB = 64 / CB;   // of a transfer: chunks of a row, rows
+    int src[NT], at[NT];                                    // bytes from a row's start, row of the stage
+    uint64_t* places = reinterpret_cast<uint64_t*>(exp_tile + G::kStages);   // of dy's and x's rows
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int q = j * G::NW + wave, b = q - G::TRA;
+        at[j] = q < G::TRA ? q * RA + lane / CA : b * RB + lane / CB;
+        const int c = q < G::TRA ? m0 + G::template swap_strided<BM>(at[j], lane % CA) * VEC : n0 + G::template swap_strided<BN>(at[j], lane % CB) * VEC;
+        src[j] = c < (q < G::TRA ? a.rows : a.k) ? c * ES : 0;
+    }
+    const uint8_t* zeros = reinterpret_cast<const uint8_t*>(exp_zeros);
+    int to = 0;
+    auto transfer = [&](int t, int j) {
+        const int q = j * G::NW + wave, r = t * BK + at[j];
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(places[2 * (r < to ? r : 0) + (q < G::TRA ? 0 : 1)]) + src[j];
+        exp_dma(r < to ? p : zeros, exp_tile + (t % S) * (G::kA + G::kB) + q * 1024);
+    };
+    const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    xf16 acc[G::TM][G::TN] = {};
+    for (int from = 0; from < count; from += G::kWindow) {
+        to = min(count - from, G::kWindow);
+        for (int r = tid; r < to; r += 64 * G::NW) {
+            const uint32_t row = order[from + r];
+            places[2 * r] = (uint64_t)exp_row_dy(a, row);
+            places[2 * r + 1] = (uint64_t)exp_row_x(a, row);
+        }
+        __syncthreads();
+        const int steps = (to + BK - 1) / BK;
+#pragma unroll
+        for (int t = 0; t < S - 1; ++t)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) transfer(t, j);
+        for (int t = 0; t < steps; ++t) {                   // stages past the end are zeros: S - 1 are always under way
+            exp_stage_barrier<(S - 2) * NT>();
+#pragma unroll
+            for (int j = 0; j < NT; ++j) transfer(t + S - 1, j);
+            const uint8_t* ta = exp_tile + (t % S) * (G::kA + G::kB);
+#pragma unroll
+            for (int s = 0; s < G::STEPS; ++s) {
+                xu4 fa[G::TM], fb[G::TN];
+#pragma unroll
+                for (int i = 0; i < G::TM; ++i) fa[i] = G::template strided<BM>(ta, wm + 32 * i, s);
+#pragma unroll
+                for (int j = 0; j < G::TN; ++j) fb[j] = G::template strided<BN>(ta + G::kA, wn + 32 * j, s);
+#pragma unroll
+                for (int i = 0; i < G::TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < G::TN; ++j) acc[i][j] = X::mma32(fa[i], fb[j], acc[i][j]);
+            }
+        }
+        exp_stage_barrier<0>();                             // nothing is under way, and the stages are free
+    }
+    // of a 32 x 32 result a lane has column lane % 32 and rows 8 (v / 4) + 4 (lane / 32) + v % 4
+    float* dw = a.dw + (size_t)expert * a.rows * a.k;
+#pragma unroll
+    for (int i = 0; i < G::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < G::TN; ++j) {
+            const int n = n0 + wn + 32 * j + (lane & 31);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int m = m0 + wm + 32 * i + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
+                if (m < a.rows && n < a.k) {
+                    float* o = dw + (size_t)m * a.k + n;
+                    *o = a.add ? *o + acc[i][j][v] : acc[i][j][v];
+                }
+            }
+        }
+}
+
 // Few rows: a workgroup has up to 16 rows of one expert and NT * 16 rows of its W; its waves share k.  W's rows go
 // from memory into MFMA operands (a lane has 16 bytes of row lane % 16), x's rows likewise from L2; the waves' sums meet
 // in LDS, added in the waves' order.
-constexpr int kExpRowsWaves = 8;
-template <typename X, int NT>
-__global__ __launch_bounds__(64 * kExpRowsWaves) void k_expert_rows(ExpertArgs a) {
+template <typename X, int NT, int NW>
+__global__ __launch_bounds__(64 * NW) void k_expert_rows(ExpertArgs a) {
     constexpr int ES = (int)sizeof(typename X::S), VEC = X::kVec, COLS = 16 * NT, STEP = 4 * VEC, U = 4;
-    __shared__ xf4 part[kExpRowsWaves][NT][64];
+    __shared__ xf4 part[NW][NT][64];
     if (!exp_groups_fit(a)) return;
     const int col_tiles = (a.rows + COLS - 1) / COLS;
     int work;
@@ -619,7 +1016,7 @@ __global__ __launch_bounds__(64 * kExpRowsWaves) void k_expert_rows(ExpertArgs a
     for (int t = 0; t < NT; ++t)
         pw[t] = a.w + ((size_t)it.x * a.rows + min(n0 + 16 * t + r, a.rows - 1)) * a.k * ES + q * 16;
     // each wave a run of steps
-    const int steps = (a.k + STEP - 1) / STEP, each = (steps + kExpRowsWaves - 1) / kExpRowsWaves;
+    const int steps = (a.k + STEP - 1) / STEP, each = (steps + NW - 1) / NW;
     const int s0 = min(steps, wave * each), s1 = min(steps, s0 + each);
     xf4 acc[NT] = {};
     int s = s0;
@@ -646,11 +1043,11 @@ __global__ __launch_bounds__(64 * kExpRowsWaves) void k_expert_rows(ExpertArgs a
     for (int t = 0; t < NT; ++t) part[wave][t][lane] = acc[t];
     __syncthreads();
     // a lane has four neighbouring columns of one row
-    for (int c = threadIdx.x; c < NT * 64; c += 64 * kExpRowsWaves) {
+    for (int c = threadIdx.x; c < NT * 64; c += 64 * NW) {
         const int t = c >> 6, l = c & 63;
         xf4 v = part[0][t][l];
 #pragma unroll
-        for (int w = 1; w < kExpRowsWaves; ++w) v += part[w][t][l];
+        for (int w = 1; w < NW; ++w) v += part[w][t][l];
         const int m = l & 15, n = n0 + 16 * t + 4 * (l >> 4);
         if (m >= it.z) continue;
         typename X::S* o = reinterpret_cast<typename X::S*>(exp_row_out(a, a.g[a.p.order + it.y + m])) + n;

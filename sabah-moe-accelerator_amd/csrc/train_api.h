@@ -220,17 +220,27 @@ SABAH_API int sabah_expert_group(const int32_t* d_ids, size_t ids_id_stride, siz
     a.err = g_err_dev;
     hipStream_t st = pick_stream(stream);
     const int keys = n_experts + 2;
-    const uint32_t lds = (uint32_t)(kExpGroupWaves * ((keys + 1) / 2) + keys + kExpGroupWaves) * 4;
-    static_assert((kExpGroupWaves * ((kExpMaxExperts + 3) / 2) + kExpMaxExperts + 2 + kExpGroupWaves) * 4 <= 160 * 1024, "a workgroup's LDS");
-    if (a.p.chunks > 1) {
-        const dim3 grid((unsigned)a.p.chunks);
-        hipLaunchKernelGGL(k_expert_count, grid, dim3(kExpGroupThreads), (uint32_t)keys * 4, st, a);
-        hipLaunchKernelGGL(k_expert_scan, dim3(1), dim3(kExpGroupThreads), (uint32_t)keys * 4, st, a);
-        if (!ck(fit_lds(k_expert_place<false>, (int)lds, (int)lds), "expert groups LDS")) return -1;
-        hipLaunchKernelGGL(k_expert_place<false>, grid, dim3(kExpGroupThreads), lds, st, a);
+    constexpr auto lds_of = [](int keys, bool sums) { return kExpGroupWaves * (8 + (keys + 1) / 2 * 4) + (sums ? 2 : 1) * keys * 4; };
+    static_assert(lds_of(kExpMaxExperts + 2, false) <= 160 * 1024 && lds_of(kExpMaxExperts + 2, true) <= 168 * 1024, "a workgroup's LDS");
+    const dim3 grid((unsigned)a.p.chunks), block(kExpGroupThreads);
+    if (a.p.n_rows <= kExpFewGroup) {
+        hipLaunchKernelGGL(k_expert_group_few, dim3(1), dim3(256), 0, st, a);
+    } else if (a.p.chunks == 1) {
+        const int lds = lds_of(keys, false);
+        if (!ck(fit_lds(k_expert_place<kPlaceAlone>, lds, lds), "expert groups LDS")) return -1;
+        hipLaunchKernelGGL(k_expert_place<kPlaceAlone>, grid, block, (uint32_t)lds, st, a);
     } else {
-        if (!ck(fit_lds(k_expert_place<true>, (int)lds, (int)lds), "expert groups LDS")) return -1;
-        hipLaunchKernelGGL(k_expert_place<true>, dim3(1), dim3(kExpGroupThreads), lds, st, a);
+        hipLaunchKernelGGL(k_expert_count, grid, block, (uint32_t)keys * 4, st, a);
+        const bool sums = a.p.chunks <= kExpSumChunks && lds_of(keys, true) <= g_max_lds;
+        const int lds = lds_of(keys, sums);
+        if (sums) {
+            if (!ck(fit_lds(k_expert_place<kPlaceSum>, lds, lds), "expert groups LDS")) return -1;
+            hipLaunchKernelGGL(k_expert_place<kPlaceSum>, grid, block, (uint32_t)lds, st, a);
+        } else {
+            hipLaunchKernelGGL(k_expert_scan, dim3(1), block, (uint32_t)keys * 4, st, a);
+            if (!ck(fit_lds(k_expert_place<kPlaceScanned>, lds, lds), "expert groups LDS")) return -1;
+            hipLaunchKernelGGL(k_expert_place<kPlaceScanned>, grid, block, (uint32_t)lds, st, a);
+        }
     }
     return ck(hipGetLastError(), "expert groups launch") ? 0 : -1;
 }
@@ -270,7 +280,7 @@ static int expert_grid(const char* what, long long works, dim3& grid) {
 }
 
 // Rows to an expert, on average, up to which a forward call streams its weights (k_expert_rows)
-constexpr int kExpFewRows = 16;
+constexpr int kExpFewRows = 10;
 
 template <typename X, int MODE>
 static int launch_expert_gemm(const char* what, const ExpertArgs& a, hipStream_t st) {
@@ -282,15 +292,64 @@ static int launch_expert_gemm(const char* what, const ExpertArgs& a, hipStream_t
     hipLaunchKernelGGL((k_expert_gemm<X, MODE>), grid, dim3(kExpThreads), G::kLdsAll, st, a);
     return ck(hipGetLastError(), what) ? 0 : -1;
 }
-template <typename X>
-static int launch_expert_mul(const ExpertArgs& a, hipStream_t st) {
-    if ((long long)a.p.n_rows > (long long)kExpFewRows * a.p.n_experts)
-        return launch_expert_gemm<X, kModeForward>("expert product launch", a, st);
+// whether every row of x, dy and out, and of the weights, is whole multiples of 16 bytes from an aligned start
+static bool expert_aligned(const ExpertArgs& a, int es) {
+    const size_t all = (size_t)(uintptr_t)a.w | (uintptr_t)a.x | (uintptr_t)a.dy | (uintptr_t)a.out | a.x_id | a.x_tok | a.dy_id |
+                       a.dy_tok | a.out_id | a.out_tok | (size_t)a.k * es | (size_t)a.rows * es;
+    return all % 16 == 0;
+}
+template <typename X, int MODE, int BM, int BN, int WM, int WN, int KB, int S, int OCC>
+static int launch_expert_fast(const char* what, const ExpertArgs& a, hipStream_t st) {
+    typedef ExpFast<X, MODE, BM, BN, WM, WN, KB, S> G;
+    const long long cols = ((MODE == kModeForward ? a.rows : a.k) + BN - 1) / BN;
+    dim3 grid;
+    if (expert_grid(what, (BM == kExpLarge ? a.p.max_large : a.p.max_tiles) * cols, grid)) return -1;
+    auto kernel = k_expert_fast<X, MODE, BM, BN, WM, WN, KB, S, OCC>;
+    if (!ck(fit_lds(kernel, G::kLds, G::kLds), what)) return -1;
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * G::NW), G::kLds, st, a);
+    return ck(hipGetLastError(), what) ? 0 : -1;
+}
+template <typename X, int BM, int BN, int WM, int WN, int KB, int S, int OCC>
+static int launch_expert_dw(const char* what, const ExpertArgs& a, hipStream_t st) {
+    typedef ExpFast<X, kModeDw, BM, BN, WM, WN, KB, S> G;
+    dim3 grid;
+    if (expert_grid(what, (long long)a.p.n_experts * ((a.rows + BM - 1) / BM) * ((a.k + BN - 1) / BN), grid)) return -1;
+    auto kernel = k_expert_dw<X, BM, BN, WM, WN, KB, S, OCC>;
+    if (!ck(fit_lds(kernel, G::kLds, G::kLds), what)) return -1;
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * G::NW), G::kLds, st, a);
+    return ck(hipGetLastError(), what) ? 0 : -1;
+}
+constexpr int kExpLargeRows = 384;
+template <typename X, int MODE>
+static int launch_expert_product(const char* what, const ExpertArgs& a, hipStream_t st) {
+    if (!expert_aligned(a, (int)sizeof(typename X::S))) return launch_expert_gemm<X, MODE>(what, a, st);
+    const int R = a.p.n_rows, E = a.p.n_experts, cols = ((MODE == kModeForward ? a.rows : a.k) + 255) / 256;
+    if constexpr (sizeof(typename X::S) == 4) {
+        if constexpr (MODE == kModeDw) return launch_expert_dw<X, 128, 64, 2, 2, 64, 2, 4>(what, a, st);
+        else return launch_expert_fast<X, MODE, 128, 128, 1, 4, 64, 4, 2>(what, a, st);
+    } else if constexpr (MODE == kModeDw) {
+        return launch_expert_dw<X, 128, 256, 2, 4, 64, 3, 4>(what, a, st);
+    } else {
+        if ((long long)(R / kExpTile + std::min(R, E)) * cols < g_num_cu * 7 / 10)
+            return launch_expert_fast<X, MODE, 128, 64, 2, 2, 64, 4, 3>(what, a, st);
+        if (MODE == kModeForward && R / kExpLargeRows >= E && (long long)(R / kExpLarge) * cols >= g_num_cu * 3 / 4)
+            return launch_expert_fast<X, MODE, 256, 256, 2, 4, 64, 3, 2>(what, a, st);
+        return launch_expert_fast<X, MODE, 128, 256, 2, 4, 64, 3, 4>(what, a, st);
+    }
+}
+template <typename X, int NW>
+static int launch_expert_rows(const ExpertArgs& a, hipStream_t st) {
     constexpr int NT = 2;
     dim3 grid;
     if (expert_grid("expert product", (long long)a.p.max_small * ((a.rows + 16 * NT - 1) / (16 * NT)), grid)) return -1;
-    hipLaunchKernelGGL((k_expert_rows<X, NT>), grid, dim3(64 * kExpRowsWaves), 0, st, a);
+    hipLaunchKernelGGL((k_expert_rows<X, NT, NW>), grid, dim3(64 * NW), 0, st, a);
     return ck(hipGetLastError(), "expert product launch") ? 0 : -1;
+}
+template <typename X>
+static int launch_expert_mul(const ExpertArgs& a, hipStream_t st) {
+    if ((long long)a.p.n_rows > (long long)kExpFewRows * a.p.n_experts)
+        return launch_expert_product<X, kModeForward>("expert product launch", a, st);
+    return (size_t)a.k * sizeof(typename X::S) >= 2048 ? launch_expert_rows<X, 8>(a, st) : launch_expert_rows<X, 4>(a, st);
 }
 
 SABAH_API int sabah_expert_mul(const sabah_expert_desc* experts, const void* d_x, size_t x_id_stride, int x_rows,
@@ -321,8 +380,8 @@ SABAH_API int sabah_expert_mul(const sabah_expert_desc* experts, const void* d_x
 
 template <typename X>
 static int launch_expert_back(const ExpertArgs& a, hipStream_t st) {
-    if (a.out && a.p.n_rows && launch_expert_gemm<X, kModeDx>("expert product's gradient launch", a, st)) return -1;
-    return a.dw ? launch_expert_gemm<X, kModeDw>("expert weights' gradient launch", a, st) : 0;
+    if (a.out && a.p.n_rows && launch_expert_product<X, kModeDx>("expert product's gradient launch", a, st)) return -1;
+    return a.dw ? launch_expert_product<X, kModeDw>("expert weights' gradient launch", a, st) : 0;
 }
 
 SABAH_API int sabah_expert_mul_backward(const sabah_expert_desc* experts, const void* d_x, size_t x_id_stride, int x_rows,

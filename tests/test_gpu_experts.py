@@ -103,7 +103,8 @@ def test_model_sizes(ex, k, rows, dtype):
         check(run(ex, *args, TYPES[dtype]), *args, TYPES[dtype], T != 30)
 
 
-@pytest.mark.parametrize("R_,E,K", [(1, 1, 1), (5, 4096, 5), (4096, 512, 8), (4097, 7, 1), (20000, 60, 10), (70000, 4096, 7), (9000, 2, 3)])
+@pytest.mark.parametrize("R_,E,K", [(1, 1, 1), (5, 4096, 5), (64, 3, 1), (60, 512, 10), (64, 70, 8), (65, 4, 5), (4096, 512, 8), (4097, 7, 1), (20000, 60, 10),
+                                     (70000, 4096, 7), (9000, 2, 3), (300000, 100, 3)])
 def test_groups_are_stable_and_whole(ex, R_, E, K):
     """The buffer's order, offsets and tiles against a stable sort, with -1 and bad ids at the end."""
     from sabah.runtime import rt
@@ -130,7 +131,7 @@ def test_groups_are_stable_and_whole(ex, R_, E, K):
     at = 16 + (E + 3 + 3) // 4 * 4
     assert torch.equal(words[at:at + n].long(), torch.argsort(key, stable=True))
     at += (n + 3) // 4 * 4
-    for rows, count in ((16, int(words[4])), (128, int(words[5]))):
+    for rows, count in ((16, int(words[4])), (128, int(words[5])), (256, int(words[6]))):
         want = [(e if e < E else E - 1 - e, int(start[e]) + o, min(rows, int(counts[e]) - o), 0)
                 for e in torch.nonzero(counts)[:, 0].tolist() for o in range(0, int(counts[e]), rows)]
         most = n // rows + min(n, E + 2)
