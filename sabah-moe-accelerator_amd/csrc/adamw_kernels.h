@@ -143,10 +143,14 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw_norm(AdamArgs a) {
 
 __global__ __launch_bounds__(1024) void k_adamw_begin(AdamArgs a) {
     __shared__ double tmp[16];
-    double c = a.grad_scale;
+    // the powers of both betas at once, in two lanes, while the sums arrive
+    const long long t = *a.step + 1;
+    const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
+    double s = a.norm && (int)threadIdx.x < a.parts ? a.part[threadIdx.x] : 0.0, c = a.grad_scale, rest = 0.0;
+    if (threadIdx.x < 64) rest = 1.0 - pow(threadIdx.x & 1 ? a.b2 : a.b1, (double)t);
+    const double rest2 = __shfl(rest, 1);
     bool skip = false;
     if (a.norm) {                                           // uniform
-        double s = (int)threadIdx.x < a.parts ? a.part[threadIdx.x] : 0.0;
         s = adam_block_sum(s, tmp);
         const double norm = sqrt(s) * a.grad_scale;
         skip = !(norm < __builtin_inf());                   // an infinite or NaN gradient: nothing changes
@@ -154,29 +158,27 @@ __global__ __launch_bounds__(1024) void k_adamw_begin(AdamArgs a) {
         if (threadIdx.x == 0) *a.norm = (float)norm;
     }
     if (threadIdx.x == 0) {
-        const long long t = *a.step + 1;
-        const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
-        AdamScalars s{};
-        s.c = c;
-        s.lr = lr;
-        s.rate = (float)(lr / (1.0 - pow(a.b1, (double)t)));
-        s.root = (float)(1.0 / sqrt(1.0 - pow(a.b2, (double)t)));
-        s.skip = skip;
-        *a.s = s;
+        AdamScalars r{};
+        r.c = c;
+        r.lr = lr;
+        r.rate = (float)(lr / rest);
+        r.root = (float)(1.0 / sqrt(rest2));
+        r.skip = skip;
+        *a.s = r;
         if (!skip) *a.step = t;
     }
 }
 
 // The nearest code to t = (code)^2 (m's), to t = (code)^4 (v's): f32's root, then its neighbours' borders in 64 bits
 __device__ inline int adam_code2(double t, int most) {
-    int k = min(most, (int)rintf(sqrtf((float)t)));
+    int k = min(most, (int)rintf(__builtin_amdgcn_sqrtf((float)t)));   // off by at most one, which the borders mend
     const double k2 = (double)(k * k) + 0.25;               // (k +- 1/2)^2 = k^2 +- k + 1/4
     if (t > k2 + (double)k) ++k;
     else if (t < k2 - (double)k) --k;
     return min(most, max(0, k));
 }
 __device__ inline int adam_code4(double t, int most) {
-    int k = min(most, (int)rintf(sqrtf(sqrtf((float)t))));
+    int k = min(most, (int)rintf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)t))));
     const double k2 = (double)(k * k) + 0.25, hi = k2 + (double)k, lo = k2 - (double)k;
     if (t > hi * hi) ++k;
     else if (k > 0 && t < lo * lo) --k;
@@ -281,8 +283,8 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw_step(AdamArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const double q = j < left ? (double)g[k][j] * s.c : 0.0;
-                dm[j] = dm[j] * a.b1 + q * (1.0 - a.b1);
-                dv[j] = dv[j] * a.b2 + q * q * (1.0 - a.b2);
+                dm[j] = __builtin_fma(dm[j], a.b1, q * (1.0 - a.b1));
+                dv[j] = __builtin_fma(dv[j], a.b2, q * q * (1.0 - a.b2));
                 m[k][j] = (float)dm[j];
                 v[k][j] = (float)dv[j];
             }
@@ -298,7 +300,16 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw_step(AdamArgs a) {
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[k][j] = p[k][j] * keep - m[k][j] / (sqrtf(v[k][j]) * s.root + eps) * s.rate;
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (BITS == 32) {
+                p[k][j] = p[k][j] * keep - m[k][j] / (sqrtf(v[k][j]) * s.root + eps) * s.rate;
+            } else {
+                // the instructions' roots and inverses, off by a step of f32: 8 bits' moments are off by 2^-7, and the step's
+                // own arithmetic is what this kernel waits for.  A v that overflows f32 has an infinite root: no change
+                const float r = __builtin_amdgcn_sqrtf(v[k][j]) * s.root + eps;
+                p[k][j] = p[k][j] * keep - m[k][j] * __builtin_amdgcn_rcpf(r) * s.rate;
+            }
+        }
         if (T.master) adam_store4<ExpF32>(reinterpret_cast<uint8_t*>(T.master), i, left, p[k]);
         if (!T.master || T.p_type != 0) adam_store(T.p_type, T.p, i, left, p[k]);
     }

@@ -10,7 +10,7 @@ static size_t float_size(int type) { return type == kTypeF32 ? 4 : 2; }
 // norms
 // ---------------------------------------------------------------------------
 // Tokens whose weight gradients one part adds up in f32, and the parts that fill the chip
-constexpr int kNormPartTokens = 64, kNormParts = 1024;
+constexpr int kNormPartTokens = 64, kNormParts = 768;
 static void norm_plan(int n_tokens, int& parts, int& per_part) {
     per_part = std::max(1, std::min(kNormPartTokens, (n_tokens + kNormParts - 1) / kNormParts));
     parts = (n_tokens + per_part - 1) / per_part;

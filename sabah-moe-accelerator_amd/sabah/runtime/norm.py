@@ -31,16 +31,28 @@ class BlockNorm:
         self.width, self.eps, self.scale, self.device = width, float(eps), float(scale), torch.device(device)
         self.w_after = torch.ones(width, dtype=torch.float32, device=device) if after else None
         self.w_before = torch.ones(width, dtype=torch.float32, device=device) if before else None
-        self._descs = {}
+        self.index = next((w.get_device() for w in (self.w_after, self.w_before) if w is not None), None)   # None: any
+        self._descs, self._space = {}, {}
 
     def ref(self, dtype: torch.dtype, after: bool = True):
         """The C descriptor for activations of a type; after: whether the call has a y."""
-        d = self._descs.get((dtype, after))
+        key = dtype, after, self.eps, self.scale
+        d = self._descs.get(key)
         if d is None:
             if dtype not in TYPES:
-                raise ValueError("norm: activations are float32, float16 or bfloat16, not %s" % dtype)
-            d = self._descs[dtype, after] = rt.NormDesc(
+                raise ValueError("block_norm: activations are float32, float16 or bfloat16, not %s" % dtype)
+            if len(self._descs) > 64:
+                self._descs.clear()
+            d = self._descs[key] = ctypes.byref(rt.NormDesc(
                 self.w_after.data_ptr() if after and self.w_after is not None else None,
-                self.w_before.data_ptr() if self.w_before is not None else None, TYPES[dtype], self.width, self.eps, self.scale)
-        d.eps, d.scale = self.eps, self.scale
-        return ctypes.byref(d)
+                self.w_before.data_ptr() if self.w_before is not None else None, TYPES[dtype], self.width, self.eps, self.scale))
+        return d
+
+    def space(self, lib, tokens: int) -> int:
+        """sabah_block_norm_workspace of a call, asked once for each size."""
+        n = self._space.get(tokens)
+        if n is None:
+            if len(self._space) > 4096:
+                self._space.clear()
+            n = self._space[tokens] = lib.sabah_block_norm_workspace(self.width, tokens)
+        return n
