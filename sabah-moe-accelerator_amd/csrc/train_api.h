@@ -28,23 +28,29 @@ static bool norm_rows_ok(const sabah_norm_desc* n, int n_tokens, const void* p, 
     return !p || (stride % float_size(n->type) == 0 && (stride >= n->width * float_size(n->type) || n_tokens <= 1));
 }
 
+// Waves of a row, 8 values a thread: 2,560 columns fill five of them and would leave three of eight idle
+template <typename F>
+static void norm_waves(int width, F go) {
+    if (width <= 512) go(std::integral_constant<int, 1>{});
+    else if (width <= 1024) go(std::integral_constant<int, 2>{});
+    else if (width <= 2048) go(std::integral_constant<int, 4>{});
+    else if (width <= 2560) go(std::integral_constant<int, 5>{});
+    else if (width <= 4096) go(std::integral_constant<int, 8>{});
+    else go(std::integral_constant<int, 16>{});
+}
 template <typename X>
 static void launch_block_norm(const NormArgs& a, hipStream_t st) {
-    const unsigned rows = (unsigned)a.n_tokens, four = (rows + 3) / 4;
-    if (a.width <= 512) hipLaunchKernelGGL((k_block_norm<X, 8, 1>), dim3(four), dim3(256), 0, st, a);
-    else if (a.width <= 1024) hipLaunchKernelGGL((k_block_norm<X, 16, 1>), dim3(four), dim3(256), 0, st, a);
-    else if (a.width <= 2048) hipLaunchKernelGGL((k_block_norm<X, 8, 4>), dim3(rows), dim3(256), 0, st, a);
-    else if (a.width <= 4096) hipLaunchKernelGGL((k_block_norm<X, 16, 4>), dim3(rows), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_block_norm<X, 16, 8>), dim3(rows), dim3(512), 0, st, a);
+    norm_waves(a.width, [&](auto w) {
+        constexpr int W = decltype(w)::value, kRows = norm_threads(W) / (64 * W);
+        hipLaunchKernelGGL((k_block_norm<X, 8, W>), dim3((unsigned)((a.n_tokens + kRows - 1) / kRows)), dim3(norm_threads(W)), 0, st, a);
+    });
 }
 template <typename X>
 static void launch_block_norm_back(const NormArgs& a, int parts, hipStream_t st) {
-    const unsigned n = (unsigned)parts;
-    if (a.width <= 512) hipLaunchKernelGGL((k_block_norm_back<X, 8, 1>), dim3((n + 3) / 4), dim3(256), 0, st, a);
-    else if (a.width <= 1024) hipLaunchKernelGGL((k_block_norm_back<X, 8, 2>), dim3(n), dim3(128), 0, st, a);
-    else if (a.width <= 2048) hipLaunchKernelGGL((k_block_norm_back<X, 8, 4>), dim3(n), dim3(256), 0, st, a);
-    else if (a.width <= 4096) hipLaunchKernelGGL((k_block_norm_back<X, 8, 8>), dim3(n), dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((k_block_norm_back<X, 8, 16>), dim3(n), dim3(1024), 0, st, a);
+    norm_waves(a.width, [&](auto w) {
+        constexpr int W = decltype(w)::value, kRows = norm_threads(W) / (64 * W);
+        hipLaunchKernelGGL((k_block_norm_back<X, 8, W>), dim3((unsigned)((parts + kRows - 1) / kRows)), dim3(norm_threads(W)), 0, st, a);
+    });
 }
 
 SABAH_API int sabah_block_norm(const sabah_norm_desc* norm, const void* d_x, size_t x_stride, const void* d_y,

@@ -63,7 +63,7 @@ FORMS = [(True, True, True, True), (False, True, False, True), (True, False, Tru
 
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("form", FORMS)
-@pytest.mark.parametrize("T,D", [(1, 1), (3, 5), (7, 511), (5, 640), (4, 1025), (130, 2048), (9, 2560), (6, 1000), (3, 4097), (2, 8189), (1, 8192)])
+@pytest.mark.parametrize("T,D", [(1, 1), (3, 5), (7, 511), (5, 640), (4, 1025), (130, 2048), (9, 2560), (5, 2559), (3, 2561), (6, 1000), (3, 4097), (2, 8189), (1, 8192)])
 def test_forward_and_backward(ex, T, D, form, dtype):
     n, t = make(T, D, TYPES[dtype], *form[:3], y=form[3])
     out, h = ex.block_norm(n, t["x"], t["y"], t["gate"])
