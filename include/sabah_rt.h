@@ -407,7 +407,7 @@ int sabah_expert_group(const int32_t *d_ids, size_t ids_id_stride, size_t ids_to
 /* Experts kept in a float type: one matrix of a projection for each. */
 typedef struct sabah_expert_desc {
     const void *w;                         /* device [n_experts][rows][k] */
-    int type, n_experts, k, rows;          /* k, rows <= 2^20 */
+    int type, n_experts, k, rows;          /* k, rows <= 2^20; more tiles than one launch takes are refused */
 } sabah_expert_desc;
 
 /* y[t][i] = W[ids[t][i]] x[t][i % x_rows] for the ids that d_groups was made from, with the same n_ids,

@@ -322,7 +322,7 @@ struct AdamMomentArgs {
     long long blocks;
 };
 __global__ __launch_bounds__(kAdamThreads) void k_adamw_decode(AdamMomentArgs a) {
-    const long long b = (long long)blockIdx.x * (kAdamThreads / 64) + (threadIdx.x >> 6);
+    const long long b = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * (kAdamThreads / 64) + (threadIdx.x >> 6);
     if (b >= a.blocks) return;
     const long long i = b * kAdamBlock + (threadIdx.x & 63) * 4;
     double m[4], v[4];
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw_decode(AdamMomentArgs a)
     adam_store4<ExpF32>(reinterpret_cast<uint8_t*>(a.v), i, 4, fv);
 }
 __global__ __launch_bounds__(kAdamThreads) void k_adamw_encode(AdamMomentArgs a) {
-    const long long b = (long long)blockIdx.x * (kAdamThreads / 64) + (threadIdx.x >> 6);
+    const long long b = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * (kAdamThreads / 64) + (threadIdx.x >> 6);
     if (b >= a.blocks) return;
     const long long i = b * kAdamBlock + (threadIdx.x & 63) * 4;
     float fm[4], fv[4], ms, vs;

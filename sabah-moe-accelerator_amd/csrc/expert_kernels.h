@@ -121,6 +121,9 @@ constexpr uint32_t kExpMagic = 0x67727031u;
 constexpr int kExpSmall = 16, kExpTile = 128, kExpLarge = 256;   // rows of the three lists' tiles
 constexpr int kExpChunk = 4096;                   // rows that a workgroup of k_expert_count / _place sorts
 constexpr int kExpMaxExperts = 4096;
+// Rows to an expert, on average, up to which a forward call streams its weights (k_expert_rows) and has small tiles.  us of
+// the two at 2,048 -> 768 of 128 experts in bf16: 72.6 and 86.1 at 2 rows, 95.7 and 101 at 8, 117 and 105 at 16
+constexpr int kExpFewRows = 10;
 constexpr unsigned kErrExpertId = 1u, kErrExpertGroups = 5u;
 struct ExpertPlan {
     int n_rows, n_ids, n_experts, chunks;
@@ -134,7 +137,7 @@ inline ExpertPlan expert_plan(int n_ids, int n_tokens, int n_experts) {
     p.n_experts = n_experts;
     p.chunks = (p.n_rows + kExpChunk - 1) / kExpChunk;
     const int groups = p.n_rows < n_experts + 2 ? p.n_rows : n_experts + 2;
-    p.max_small = p.n_rows / kExpSmall + groups;
+    p.max_small = p.n_rows <= (long long)kExpFewRows * n_experts ? p.n_rows / kExpSmall + groups : 0;
     p.max_tiles = p.n_rows / kExpTile + groups;
     p.max_large = p.n_rows / kExpLarge + groups;
     auto take = [&](size_t n) {
@@ -238,7 +241,7 @@ __device__ inline void exp_lists(const ExpertGroupArgs& a, uint64_t* tmp, bool w
     uint64_t one = 0, two = 0, total, total2 = 0;               // rows and small tiles, tiles and large ones: 32 bits each
     for (int e = e0; e < e1; ++e) {
         const int c = cnt(e);
-        one += (uint64_t)c | (uint64_t)exp_tiles(c, kExpSmall) << 32;
+        one += (uint64_t)c | (a.p.max_small ? (uint64_t)exp_tiles(c, kExpSmall) << 32 : 0);
         two += (uint64_t)exp_tiles(c, kExpTile) | (uint64_t)exp_tiles(c, kExpLarge) << 32;
     }
     one = exp_block_scan(one, tmp, total);
@@ -251,7 +254,8 @@ __device__ inline void exp_lists(const ExpertGroupArgs& a, uint64_t* tmp, bool w
         const int c = cnt(e), who = e < E ? e : E - 1 - e;
         if (write) {
             a.g[a.p.off + e] = at;
-            for (int o = 0; o < c; o += kExpSmall) ls[s++] = make_int4(who, at + o, min(kExpSmall, c - o), 0);
+            if (a.p.max_small)
+                for (int o = 0; o < c; o += kExpSmall) ls[s++] = make_int4(who, at + o, min(kExpSmall, c - o), 0);
             for (int o = 0; o < c; o += kExpTile) lt[t++] = make_int4(who, at + o, min(kExpTile, c - o), 0);
             for (int o = 0; o < c; o += kExpLarge) ll[l++] = make_int4(who, at + o, min(kExpLarge, c - o), 0);
             if (e == E + 1 && c) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrExpertId;
@@ -404,12 +408,13 @@ __global__ __launch_bounds__(256) void k_expert_group_few(ExpertGroupArgs a) {
     if (some) a.g[a.p.order + at + before] = (uint32_t)lane;
     if (leads) {
         const int who = key < E ? key : E - 1 - key;
-        for (int o = 0; o < rows; o += kExpSmall) reinterpret_cast<int4*>(a.g + a.p.small)[s++] = make_int4(who, at + o, min(kExpSmall, rows - o), 0);
+        if (a.p.max_small)
+            for (int o = 0; o < rows; o += kExpSmall) reinterpret_cast<int4*>(a.g + a.p.small)[s++] = make_int4(who, at + o, min(kExpSmall, rows - o), 0);
         reinterpret_cast<int4*>(a.g + a.p.tiles)[t] = make_int4(who, at, rows, 0);
         reinterpret_cast<int4*>(a.g + a.p.large)[t] = make_int4(who, at, rows, 0);
     }
     if (lane == 0) {
-        exp_head(a, small, tiles, tiles);
+        exp_head(a, a.p.max_small ? small : 0, tiles, tiles);
         if (bad) *reinterpret_cast<volatile unsigned int*>(a.err) = kErrExpertId;
     }
 }
@@ -434,6 +439,11 @@ struct ExpertArgs {
     unsigned int* err;
 };
 
+// a tile, the same for all lanes: what depends on it branches as one
+__device__ inline int4 exp_item(const ExpertArgs& a, size_t list, int i) {
+    const int4 it = reinterpret_cast<const int4*>(a.g + list)[i];
+    return make_int4(__builtin_amdgcn_readfirstlane(it.x), __builtin_amdgcn_readfirstlane(it.y), __builtin_amdgcn_readfirstlane(it.z), 0);
+}
 __device__ inline bool exp_groups_fit(const ExpertArgs& a) {
     const bool ok = a.g[kExpHeadMagic] == kExpMagic && a.g[kExpHeadRows] == (uint32_t)a.p.n_rows &&
                     a.g[kExpHeadIds] == (uint32_t)a.p.n_ids && a.g[kExpHeadExperts] == (uint32_t)a.p.n_experts;
@@ -456,7 +466,7 @@ __device__ inline uint8_t* exp_row_out(const ExpertArgs& a, uint32_t row) {
 // the same weights, and a tile's columns, which read the same rows, meet in one die's L2.  False: nothing left.
 __device__ inline bool exp_work(int id, int all, int& work) {
     const int each = (all + 7) / 8, q = id >> 3;
-    work = (id & 7) * each + q;
+    work = __builtin_amdgcn_readfirstlane((id & 7) * each + q);
     return q < each && work < all;
 }
 // rows without an expert (zeros), or with a bad id (NaN)
@@ -540,12 +550,12 @@ __global__ __launch_bounds__(kExpThreads, 2) void k_expert_gemm(ExpertArgs a) {
         work -= expert * row_tiles * col_tiles;
         m0 = work / col_tiles * BM;
         n0 = work % col_tiles * BN;
-        first = (int)a.g[a.p.off + expert];
-        count = (int)a.g[a.p.off + expert + 1] - first;
+        first = __builtin_amdgcn_readfirstlane(a.g[a.p.off + expert]);
+        count = __builtin_amdgcn_readfirstlane(a.g[a.p.off + expert + 1]) - first;
         if (count == 0 && a.add) return;
     } else {
         if (!exp_work(blockIdx.x, (int)a.g[kExpHeadTiles] * col_tiles, work)) return;
-        const int4 it = reinterpret_cast<const int4*>(a.g + a.p.tiles)[work / col_tiles];
+        const int4 it = exp_item(a, a.p.tiles, work / col_tiles);
         n0 = work % col_tiles * BN;
         if (it.x < 0) {
             exp_fill<X>(a, it, n0, BN, width);
@@ -839,7 +849,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_expert_fast(ExpertArgs a)
     const int col_tiles = (width + BN - 1) / BN;
     int work;
     if (!exp_work(blockIdx.x, (int)a.g[G::kLarge ? kExpHeadLarge : kExpHeadTiles] * col_tiles, work)) return;
-    const int4 it = reinterpret_cast<const int4*>(a.g + (G::kLarge ? a.p.large : a.p.tiles))[work / col_tiles];
+    const int4 it = exp_item(a, G::kLarge ? a.p.large : a.p.tiles, work / col_tiles);
     const int n0 = work % col_tiles * BN;
     if (it.x < 0) {
         exp_fill<X>(a, it, n0, BN, width);
@@ -917,7 +927,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_expert_dw(ExpertArgs a) {
     work -= expert * row_tiles * col_tiles;
     const int m0 = work / col_tiles * BM, n0 = work % col_tiles * BN;
     // read beside the head, not after it
-    const int first = (int)a.g[a.p.off + expert], count = (int)a.g[a.p.off + expert + 1] - first;
+    const int first = __builtin_amdgcn_readfirstlane(a.g[a.p.off + expert]);
+    const int count = __builtin_amdgcn_readfirstlane(a.g[a.p.off + expert + 1]) - first;
     if (!exp_groups_fit(a)) return;
     if (count == 0 && a.add) return;
     const uint32_t* order = a.g + a.p.order + first;
@@ -1002,7 +1013,7 @@ __global__ __launch_bounds__(64 * NW) void k_expert_rows(ExpertArgs a) {
     const int col_tiles = (a.rows + COLS - 1) / COLS;
     int work;
     if (!exp_work(blockIdx.x, (int)a.g[kExpHeadSmall] * col_tiles, work)) return;
-    const int4 it = reinterpret_cast<const int4*>(a.g + a.p.small)[work / col_tiles];
+    const int4 it = exp_item(a, a.p.small, work / col_tiles);
     const int n0 = work % col_tiles * COLS;
     if (it.x < 0) {
         exp_fill<X>(a, it, n0, COLS, a.rows);

@@ -99,8 +99,8 @@ __global__ __launch_bounds__(norm_threads(W)) void k_block_norm(NormArgs a) {
     constexpr int V = X::kVec, Q = PER / V;
     __shared__ float tmp[W];
     const int v = W == 1 ? (int)threadIdx.x & 63 : (int)threadIdx.x;
-    const long long t = W == 1 ? (long long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long long)blockIdx.x;
-    if (W == 1 && t >= a.n_tokens) return;
+    const long long group = (long long)blockIdx.y * gridDim.x + blockIdx.x, t = W == 1 ? group * 4 + (threadIdx.x >> 6) : group;
+    if (t >= a.n_tokens) return;                            // W > 1: the whole workgroup
     NormRow<X, PER, W> x, y;
     float wa[PER], wb[PER], e[V], f[V];
     x.load(a.x + (size_t)t * a.x_st, a.width, v);

@@ -42,7 +42,10 @@ template <typename X>
 static void launch_block_norm(const NormArgs& a, hipStream_t st) {
     norm_waves(a.width, [&](auto w) {
         constexpr int W = decltype(w)::value, kRows = norm_threads(W) / (64 * W);
-        hipLaunchKernelGGL((k_block_norm<X, 8, W>), dim3((unsigned)((a.n_tokens + kRows - 1) / kRows)), dim3(norm_threads(W)), 0, st, a);
+        // a launch takes fewer than 2^32 threads along x, and 2^24 tokens of a workgroup each may be more
+        constexpr unsigned kMost = 1u << 20;
+        const unsigned groups = (unsigned)((a.n_tokens + kRows - 1) / kRows);
+        hipLaunchKernelGGL((k_block_norm<X, 8, W>), dim3(std::min(groups, kMost), (groups + kMost - 1) / kMost), dim3(norm_threads(W)), 0, st, a);
     });
 }
 template <typename X>
@@ -279,21 +282,20 @@ static ExpertArgs expert_args(const sabah_expert_desc* E, const void* d_x, size_
     a.err = g_err_dev;
     return a;
 }
-static int expert_grid(const char* what, long long works, dim3& grid) {
-    if (works > 1ll << 30) return fail("%s: %lld tiles are too many for one call", what, works);
+// a launch takes fewer than 2^32 threads along x
+static int expert_grid(const char* what, long long works, int threads, dim3& grid) {
+    if (works > ((1ll << 32) - 1) / threads - 8) return fail("%s: %lld tiles are too many for one call", what, works);
     grid = dim3((unsigned)((works + 7) / 8 * 8));
     return 0;
 }
 
-// Rows to an expert, on average, up to which a forward call streams its weights (k_expert_rows)
-constexpr int kExpFewRows = 10;
 
 template <typename X, int MODE>
 static int launch_expert_gemm(const char* what, const ExpertArgs& a, hipStream_t st) {
     typedef ExpGemm<X, MODE> G;
     const long long cols = ((MODE == kModeForward ? a.rows : a.k) + G::BN - 1) / G::BN;
     dim3 grid;
-    if (expert_grid(what, (MODE == kModeDw ? (long long)a.p.n_experts * ((a.rows + G::BM - 1) / G::BM) : a.p.max_tiles) * cols, grid)) return -1;
+    if (expert_grid(what, (MODE == kModeDw ? (long long)a.p.n_experts * ((a.rows + G::BM - 1) / G::BM) : a.p.max_tiles) * cols, kExpThreads, grid)) return -1;
     if (!ck(fit_lds(k_expert_gemm<X, MODE>, G::kLdsAll, G::kLdsAll), what)) return -1;
     hipLaunchKernelGGL((k_expert_gemm<X, MODE>), grid, dim3(kExpThreads), G::kLdsAll, st, a);
     return ck(hipGetLastError(), what) ? 0 : -1;
@@ -309,7 +311,7 @@ static int launch_expert_fast(const char* what, const ExpertArgs& a, hipStream_t
     typedef ExpFast<X, MODE, BM, BN, WM, WN, KB, S> G;
     const long long cols = ((MODE == kModeForward ? a.rows : a.k) + BN - 1) / BN;
     dim3 grid;
-    if (expert_grid(what, (BM == kExpLarge ? a.p.max_large : a.p.max_tiles) * cols, grid)) return -1;
+    if (expert_grid(what, (BM == kExpLarge ? a.p.max_large : a.p.max_tiles) * cols, 64 * G::NW, grid)) return -1;
     auto kernel = k_expert_fast<X, MODE, BM, BN, WM, WN, KB, S, OCC>;
     if (!ck(fit_lds(kernel, G::kLds, G::kLds), what)) return -1;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * G::NW), G::kLds, st, a);
@@ -319,7 +321,7 @@ template <typename X, int BM, int BN, int WM, int WN, int KB, int S, int OCC>
 static int launch_expert_dw(const char* what, const ExpertArgs& a, hipStream_t st) {
     typedef ExpFast<X, kModeDw, BM, BN, WM, WN, KB, S> G;
     dim3 grid;
-    if (expert_grid(what, (long long)a.p.n_experts * ((a.rows + BM - 1) / BM) * ((a.k + BN - 1) / BN), grid)) return -1;
+    if (expert_grid(what, (long long)a.p.n_experts * ((a.rows + BM - 1) / BM) * ((a.k + BN - 1) / BN), 64 * G::NW, grid)) return -1;
     auto kernel = k_expert_dw<X, BM, BN, WM, WN, KB, S, OCC>;
     if (!ck(fit_lds(kernel, G::kLds, G::kLds), what)) return -1;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * G::NW), G::kLds, st, a);
@@ -347,7 +349,7 @@ template <typename X, int NW>
 static int launch_expert_rows(const ExpertArgs& a, hipStream_t st) {
     constexpr int NT = 2;
     dim3 grid;
-    if (expert_grid("expert product", (long long)a.p.max_small * ((a.rows + 16 * NT - 1) / (16 * NT)), grid)) return -1;
+    if (expert_grid("expert product", (long long)a.p.max_small * ((a.rows + 16 * NT - 1) / (16 * NT)), 64 * NW, grid)) return -1;
     hipLaunchKernelGGL((k_expert_rows<X, NT, NW>), grid, dim3(64 * NW), 0, st, a);
     return ck(hipGetLastError(), "expert product launch") ? 0 : -1;
 }
@@ -449,7 +451,7 @@ static int check_adamw_tensors(const sabah_adamw_tensor* t, int n, long long& ch
         all.push_back({g, g + t[i].n * float_size(t[i].g_type), false});
         if (m) all.push_back({m, m + t[i].n * 4, true});
     }
-    if (chunks > 1ll << 30) return fail("adamw: %lld values are too many for one step", values);
+    if (chunks >= 1 << 24) return fail("adamw: %lld values are too many for one step", values);
     std::sort(all.begin(), all.end(), [](const Range& x, const Range& y) { return x.lo < y.lo; });
     uintptr_t any = 0, written = 0;
     for (const Range& r : all) {
@@ -461,20 +463,29 @@ static int check_adamw_tensors(const sabah_adamw_tensor* t, int n, long long& ch
 }
 static size_t adamw_chunks_at(int n) { return align256((size_t)n * sizeof(AdamTensor)); }
 
+// the check keeps a list of the tensors' memory: without memory for it the call fails, as any other
+static int check_adamw_table(const sabah_adamw_tensor* t, int n, long long& chunks, long long& values) {
+    try {
+        return check_adamw_tensors(t, n, chunks, values);
+    } catch (const std::exception& e) {
+        return fail("adamw: %s", e.what());
+    }
+}
+
 SABAH_API size_t sabah_adamw_table_bytes(const sabah_adamw_tensor* tensors, int n_tensors, long long* n_values) {
     long long chunks, values;
     if (!n_values) {
         fail("adamw: null pointer");
         return 0;
     }
-    if (check_adamw_tensors(tensors, n_tensors, chunks, values)) return 0;
+    if (check_adamw_table(tensors, n_tensors, chunks, values)) return 0;
     *n_values = values;
     return adamw_chunks_at(n_tensors) + (size_t)chunks * sizeof(AdamChunk);
 }
 
 SABAH_API int sabah_adamw_table(const sabah_adamw_tensor* tensors, int n_tensors, void* table, size_t table_bytes) {
     long long chunks, values;
-    if (check_adamw_tensors(tensors, n_tensors, chunks, values)) return -1;
+    if (check_adamw_table(tensors, n_tensors, chunks, values)) return -1;
     const size_t need = adamw_chunks_at(n_tensors) + (size_t)chunks * sizeof(AdamChunk);
     if (!table || table_bytes != need) return fail("adamw: the table has %zu bytes (got %zu)", need, table_bytes);
     std::memset(table, 0, need);
@@ -502,7 +513,7 @@ SABAH_API int sabah_adamw_step(const sabah_adamw_desc* o, void* stream) {
     if (!(o->grad_scale > 0.0 && o->grad_scale < __builtin_inf())) return fail("adamw: grad_scale must be positive and finite");
     if (o->norm && !(o->max_norm > 0.0)) return fail("adamw: max_norm must be positive");
     const size_t at = o->n_tensors > 0 ? adamw_chunks_at(o->n_tensors) : 0;
-    if (o->n_tensors <= 0 || o->table_bytes < at || (o->table_bytes - at) % sizeof(AdamChunk) || (o->table_bytes - at) / sizeof(AdamChunk) > 1u << 30)
+    if (o->n_tensors <= 0 || o->table_bytes < at || (o->table_bytes - at) % sizeof(AdamChunk) || (o->table_bytes - at) / sizeof(AdamChunk) >= 1u << 24)
         return fail("adamw: %zu bytes are no table of %d tensors", o->table_bytes, o->n_tensors);
     if (o->table_bytes > at && (!o->m || !o->v || (o->bits == 8 && (!o->m_scale || !o->v_scale)))) return fail("adamw: null pointer");
     const size_t ws = sabah_adamw_workspace();
@@ -545,7 +556,7 @@ SABAH_API int sabah_adamw_step(const sabah_adamw_desc* o, void* stream) {
 
 static int adamw_moments(bool encode, void* m_code, void* v_code, float* m_scale, float* v_scale, long long n_values, float* m,
                          float* v, void* stream) {
-    if (n_values < 0 || n_values % kAdamBlock || n_values > 1ll << 40) return fail("adamw: %lld values are no whole blocks of %d", n_values, kAdamBlock);
+    if (n_values < 0 || n_values % kAdamBlock || n_values >= 1ll << 35) return fail("adamw: %lld values are no whole blocks of %d", n_values, kAdamBlock);
     if (n_values && (!m_code || !v_code || !m_scale || !v_scale || !m || !v)) return fail("adamw: null pointer");
     if (((uintptr_t)m_code | (uintptr_t)v_code | (uintptr_t)m | (uintptr_t)v) % 16) return fail("adamw: moments must be 16-byte aligned");
     if (g_device < 0) return fail("sabah_rt_init has not been called");
@@ -554,7 +565,9 @@ static int adamw_moments(bool encode, void* m_code, void* v_code, float* m_scale
     OnDevice dev;
     if (!dev.ok) return -1;
     const AdamMomentArgs a{static_cast<uint8_t*>(m_code), static_cast<uint8_t*>(v_code), m_scale, v_scale, m, v, n_values / kAdamBlock};
-    const dim3 grid((unsigned)((a.blocks + 3) / 4));
+    constexpr long long kMost = 1 << 20;                   // fewer than 2^32 threads along x
+    const long long groups = (a.blocks + 3) / 4;
+    const dim3 grid((unsigned)std::min(groups, kMost), (unsigned)((groups + kMost - 1) / kMost));
     if (encode) hipLaunchKernelGGL(k_adamw_encode, grid, dim3(kAdamThreads), 0, pick_stream(stream), a);
     else hipLaunchKernelGGL(k_adamw_decode, grid, dim3(kAdamThreads), 0, pick_stream(stream), a);
     return ck(hipGetLastError(), "adamw moments launch") ? 0 : -1;

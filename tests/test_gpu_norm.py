@@ -168,6 +168,21 @@ def test_nan_and_infinity_stay_in_their_rows(ex):
     assert (dy[12] == 0).all() and dgate[12] == 0 and dgate[13] == 0
 
 
+def test_more_threads_than_a_launch_takes_along_x(ex):
+    """2^22 + 3 tokens of 1,024 threads each are more than 2^32."""
+    from sabah.runtime.norm import BlockNorm
+    T, D = (1 << 22) + 3, 4097
+    n = BlockNorm(D, after=False, eps=EPS, device=DEV)
+    x = torch.empty(T, D, dtype=torch.bfloat16, device=DEV)
+    x.fill_(2.0)
+    x[T - 1] = 4.0
+    _, h = ex.block_norm(n, x)
+    for rows in (h[:2], h[(1 << 20) - 1:(1 << 20) + 2], h[T - 2:]):
+        assert (rows == 1).all()                              # of equal values: rounded to bf16, 1 exactly
+    del x, h
+    torch.cuda.empty_cache()
+
+
 def test_rows_of_zeros(ex):
     """The mean is zero and eps alone divides."""
     n, t = make(4, 100, torch.float32, True, True, False)
