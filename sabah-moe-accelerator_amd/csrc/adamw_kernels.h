@@ -11,7 +11,9 @@
 //
 // k_adamw_norm:  the gradients' sum of squares in 64 bits, by a fixed number of workgroups, in a fixed order.
 // k_adamw_begin: the norm, the step's number and what depends on them, by one wave.
-// k_adamw_step:  2,048 values of one tensor to a workgroup; every state is read and written once, which bounds it.
+// k_adamw_step:  2,048 values of one tensor to a workgroup; every state is read and written once, which bounds it: 604 M values
+//   in f32 3,180 us, 5.3 TB/s; 302 M in bf16 with master copies and 8-bit moments 1,080 us, 5.0 TB/s (1,430 with f32's
+//   correctly rounded roots and division, which the 64-bit codes do not need: they are found by their borders).
 #pragma once
 #include "balance_kernels.h"   // row_max
 #include "expert_kernels.h"    // storage types

@@ -4,10 +4,16 @@
 //   backward   dx_r = W[e_r]^T dy_r;   dW[e] (+)= sum over the rows of e of dy_r x_r^T
 // Products are exact in f32, sums are f32 on the matrix cores; y and dx are rounded once, dW is f32.
 //
-// k_expert_count, _scan, _place: the rows in expert order, stable and without an order that depends on
+// k_expert_group_few, _count, _scan, _place: the rows in expert order, stable and without an order that depends on
 //   atomics, so the same ids give the same bits; cut into tiles of one expert.
-// k_expert_gemm:  a tile of 128 rows by 128 columns, both operands staged through LDS.
-// k_expert_rows:  up to 16 rows of one expert (decode, few tokens): W streamed from HBM into MFMA operands.
+// k_expert_rows:  up to 16 rows of one expert (decode, few tokens): W streamed from HBM into MFMA operands.  HBM bounds it:
+//   47 tokens of 8 of 128 experts (385 MB) in 79 us, the rate of a large copy.
+// k_expert_fast, k_expert_dw: tiles whose operands go from memory straight into LDS.  Bounds, at 2,048 -> 768 in bf16:
+//   over 8 experts of 8,192 rows 211 us (976 TFLOP/s; the same products with nothing to load 148, the loads alone 139:
+//   what is left is the two getting in each other's way); over 128 experts of 512 rows the weights' 402 MB come at half the
+//   rate of a copy, because two tiles ask for the same bytes at once, which leaves half as many different ones under way.
+//   dW of 128 experts writes 805 MB: 338 us, where the sums alone take 214 - 239 and the loads alone 140.
+// k_expert_gemm:  the same products for rows at any alignment, staged through registers.
 #pragma once
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -483,7 +489,8 @@ __device__ inline void exp_fill(const ExpertArgs& a, const int4& it, int col0, i
 constexpr int kExpThreads = 256;
 constexpr int kModeForward = 0, kModeDx = 1, kModeDw = 2;
 
-// A tile of BM x BN outputs, four waves of (BM / 2) x (BN / 2), the summed axis in steps of 128 bytes.
+// Rows at any alignment and of any length.  A tile of BM x BN outputs, four waves of (BM / 2) x (BN / 2), the summed axis in steps of
+// 128 bytes (8,191 tokens, top-8 of 128, 2,048 -> 768 in bf16: 368 us, where k_expert_fast takes 260).
 //   forward: rows of x by rows of W;  dx: rows of dy by columns of W;  dw: columns of dy by columns of x, summed over a
 //   group's rows.
 // An operand whose summed axis is contiguous in memory lies in LDS as rows of 128 bytes, its 16-byte chunks
@@ -680,7 +687,7 @@ __global__ __launch_bounds__(kExpThreads, 2) void k_expert_gemm(ExpertArgs a) {
     }
 }
 
-// The same tiles where every row of every operand begins at a multiple of 16 bytes and has a whole number of them:
+// Where every row of every operand begins at a multiple of 16 bytes and has a whole number of them:
 // both operands go from memory straight into LDS (1 KB a wave and instruction, no registers), the next stage's while the
 // matrix cores run on this one.  A lane's 16 bytes land at its own place of that KB, so the permutations of ExpGemm are made
 // by what each lane asks for.  Chunks past the summed axis come from `exp_zeros`; columns past the width
@@ -1002,7 +1009,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_expert_dw(ExpertArgs a) {
         }
 }
 
-// Few rows: a workgroup has up to 16 rows of one expert and NT * 16 rows of its W; its waves share k.  W's rows go
+// Few rows: a workgroup has up to 16 rows of one expert and NT * 16 rows of its W; its NW waves share k (8 where each then has
+// four loads of 64 bytes a row to make at once, k of 1,024 values of 16 bits; 4 below: one token at 768 -> 2,048 9.4 us against
+// 10.3, 64 tokens 225 against 249; at 2,048 -> 768 8.1 with 8, 8.6 with 4).  W's rows go
 // from memory into MFMA operands (a lane has 16 bytes of row lane % 16), x's rows likewise from L2; the waves' sums meet
 // in LDS, added in the waves' order.
 template <typename X, int NT, int NW>

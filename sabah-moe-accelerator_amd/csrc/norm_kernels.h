@@ -6,7 +6,10 @@
 //              dw_before = sum over tokens of dh u;  with dn = scale sigmoid(gate) d the same rule gives dy and dw_after
 //              from y, and dgate = sigmoid (1 - sigmoid) scale sum(d n(y))
 // A row is held in registers by one wave or by a workgroup from its loads to its stores: each input is read and
-// each output written once, which is what bounds it.  Sums are f32, of rounded inputs; x', h, dx and dy are rounded once.
+// each output written once, which is what bounds it (4,001 tokens of 2,560 in bf16 forward 15.2 us, 5.4 TB/s with the
+// last-level cache's help; 16,384 of 2,048 backward 91 us, 4.4 TB/s, and 6 for the weights' sums; a large copy 4.86).  8 values a
+// thread: with 16 a row of 2,560 kept 4,096 places, 19.0 us, and the backward spilled.  Loading the next token's rows
+// ahead changed nothing (87 us), nor did 512 or 2,048 parts (96, 84 + 13).  Sums are f32, of rounded inputs; x', h, dx and dy are rounded once.
 #pragma once
 #include "balance_kernels.h"   // row_reduce
 #include "expert_kernels.h"    // storage types

@@ -327,6 +327,14 @@ static int launch_expert_dw(const char* what, const ExpertArgs& a, hipStream_t s
     hipLaunchKernelGGL(kernel, grid, dim3(64 * G::NW), G::kLds, st, a);
     return ck(hipGetLastError(), what) ? 0 : -1;
 }
+// Which tile, of 16-bit types (us in bf16, 8 experts unless said; rows to an expert):
+//   128 x 64   while tiles of 128 x 256 are too few for the card: forward 2,048 -> 768 at 256 rows 20.1 against 33.6, at 512
+//              32.4 and 35.1, at 1,024 (216 tiles) 61.8 and 40.4; dx at 128 rows 20.3 and 25.2, at 512 (288 tiles) 42.3 and 34.7
+//   256 x 256  forward, from 384 rows and three quarters of the card's tiles: of 128 experts at 256 rows 188 against 184, at
+//              512 270 and 315; at 8,192 rows 265 and 291, at 1,024 (60 tiles) 56 and 40.  Of dx, whose sums are shorter, 421 and 386
+//   128 x 256  else, and for dW: 338 against 356 with 256 x 256, 346 with 128 x 128; few tiles are not faster in 128 x 64 (14.4, 15.4)
+// f32's products take 64 cycles where loads take few: 128 x 128 with all four waves on all rows, so that a last tile's missing rows
+// are missing from each (600 rows of 8 experts: dx 53 us; dW in 128 x 64 46 - 52, in 128 x 128 50 - 58).
 constexpr int kExpLargeRows = 384;
 template <typename X, int MODE>
 static int launch_expert_product(const char* what, const ExpertArgs& a, hipStream_t st) {
