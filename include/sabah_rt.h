@@ -376,7 +376,8 @@ int sabah_lora_backward(const sabah_lora_desc *lora, const float *d_x, size_t x_
  * stream, and before the next one.  With n(v; w) = v / sqrt(mean(v^2) + eps) * w for each row of `width` values:
  *   out[t] = x[t] + scale * sigmoid(gate[t]) * n(y[t]; w_after)   (w_after NULL: y itself; gate NULL: 1)
  *   h[t]   = n(out[t]; w_before), of out as it is stored          (w_before NULL: no h)
- * y NULL: only h, of x.  Rows are strides (bytes) apart; out may be x itself.  width <= 8192, n_tokens <= 2^24. */
+ * y NULL: only h, of x.  Rows are strides (bytes) apart; out may be x itself.  Squares and sums are f32 (values beyond
+ * 1.8e19 overflow them).  width <= 8192, n_tokens <= 2^24. */
 typedef struct sabah_norm_desc {
     const float *w_after, *w_before;       /* device [width], or NULL */
     int type, width;
@@ -456,7 +457,7 @@ typedef struct sabah_adamw_desc {
     int n_tensors, bits;                   /* 32 or 8 */
     void *m, *v;                           /* device, 16-byte aligned */
     float *m_scale, *v_scale;              /* bits 8: device [n_values / 256] */
-    double lr, beta1, beta2, eps, grad_scale, max_norm;
+    double lr, beta1, beta2, eps, grad_scale, max_norm;   /* eps: at least f32's smallest normal number */
     const float *d_lr;                     /* device, or NULL: lr; for captured steps */
     long long *step;                       /* device: steps made, 0 before the first; counted here */
     float *norm;                           /* device [1]: the gradients' norm, NULL: not wanted and not clipped */

@@ -103,6 +103,29 @@ __device__ inline xu4 exp_load(const uint8_t* p, int left) {
     }
     return r;
 }
+// The same from column c of a row of `width` >= kVec, without a branch for each value: a chunk that the row ends in, or one past
+// it, is read as the row's last kVec values (exp_last) and shifted down by what lies past the end (exp_over bytes).
+template <typename X>
+__device__ inline xu4 exp_last(const uint8_t* row, int c, int width) {
+    return *reinterpret_cast<const xu4u*>(row + (size_t)min(c, width - X::kVec) * sizeof(typename X::S));
+}
+template <typename X>
+__device__ inline int exp_over(int c, int width) {
+    return max(0, min(c + X::kVec - width, X::kVec)) * (int)sizeof(typename X::S);
+}
+__device__ inline xu4 exp_shift(xu4 r, int over) {
+    if (over) {
+        if (over & 8) r = xu4{r[2], r[3], 0u, 0u};
+        if (over & 4) r = xu4{r[1], r[2], r[3], 0u};
+        if (over & 2) r = xu4{r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16, r[3] >> 16};
+        if (over & 16) r = xu4{0u, 0u, 0u, 0u};
+    }
+    return r;
+}
+template <typename X>
+__device__ inline xu4 exp_chunk(const uint8_t* row, int c, int width) {
+    return exp_shift(exp_last<X>(row, c, width), exp_over<X>(c, width));
+}
 template <typename X>
 __device__ inline void exp_store(uint8_t* p, xu4 r, int left) {
     if (left >= X::kVec) {
@@ -490,11 +513,12 @@ constexpr int kExpThreads = 256;
 constexpr int kModeForward = 0, kModeDx = 1, kModeDw = 2;
 
 // Rows at any alignment and of any length.  A tile of BM x BN outputs, four waves of (BM / 2) x (BN / 2), the summed axis in steps of
-// 128 bytes (8,191 tokens, top-8 of 128, 2,048 -> 768 in bf16: 368 us, where k_expert_fast takes 260).
+// 128 bytes (4,096 tokens, top-8 of 128, 2,047 -> 767 in bf16: 315 us, where k_expert_fast takes 192 for one column more).
+// All loads of a stage are under way before any of them is looked at: with chunks completed as they were loaded gradients took 2.5 times as long.
 //   forward: rows of x by rows of W;  dx: rows of dy by columns of W;  dw: columns of dy by columns of x, summed over a
 //   group's rows.
 // An operand whose summed axis is contiguous in memory lies in LDS as rows of 128 bytes, its 16-byte chunks
-// permuted by the row's low bits (any 8 neighbouring lanes of a read then cover all banks); one whose summed axis is
+// permuted by the row's bits (the 16 lanes that are read at once then lie in all 64 banks); one whose summed axis is
 // strided lies as BK rows of the tile's columns, and its fragments are transposed as they are read
 // (ds_read_b64_tr_b16: 16 lanes read a 4 x 16 block and get its columns); f32 values are read one by one.
 template <typename X, int MODE>
@@ -508,9 +532,9 @@ struct ExpGemm {
     static constexpr int kLdsAll = MODE == kModeDw || kLds >= BM * kOutStride ? kLds : BM * kOutStride;
     static constexpr int CPR = 128 * ES / 16;         // 16-byte chunks of a strided operand's row
 
-    static __device__ inline int at_contiguous(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+    static __device__ inline int at_contiguous(int row, int chunk) { return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4); }
     static __device__ inline int at_strided(int row, int chunk) {
-        return row * (128 * ES) + ((ES == 2 ? chunk ^ ((row & 3) << 1) : chunk) << 4);
+        return row * (128 * ES) + ((ES == 2 ? chunk ^ ((row & 3) << 2) : chunk ^ ((row & 4) << 1)) << 4);
     }
     // the fragment of 32 rows (or columns) from r0, step s of the tile's
     static __device__ inline xu4 contiguous(const uint8_t* t, int r0, int s) {
@@ -531,8 +555,10 @@ struct ExpGemm {
         } else {
             xf4 v;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                v[j] = *reinterpret_cast<const float*>(t + (s * 8 + (lane >> 5) * 4 + j) * (128 * ES) + (c0 + (lane & 31)) * ES);
+            for (int j = 0; j < 4; ++j) {
+                const int col = c0 + (lane & 31);
+                v[j] = *reinterpret_cast<const float*>(t + at_strided(s * 8 + (lane >> 5) * 4 + j, col >> 2) + (col & 3) * ES);
+            }
             r = __builtin_bit_cast(xu4, v);
         }
         return r;
@@ -587,38 +613,49 @@ __global__ __launch_bounds__(kExpThreads, 2) void k_expert_gemm(ExpertArgs a) {
         for (int i = 0; i < NL; ++i) {                // rows past the tile repeat its first and are not stored
             const int m = rc + 32 * i;
             const uint32_t row = order[m < count ? m : 0];
-            pa[i] = (MODE == kModeForward ? exp_row_x(a, row) : exp_row_dy(a, row)) + cc * 16;
+            pa[i] = MODE == kModeForward ? exp_row_x(a, row) : exp_row_dy(a, row);
         }
     }
     if constexpr (MODE == kModeForward) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) pb[i] = w + (size_t)min(n0 + rc + 32 * i, a.rows - 1) * a.k * ES + cc * 16;
+        for (int i = 0; i < NL; ++i) pb[i] = w + (size_t)min(n0 + rc + 32 * i, a.rows - 1) * a.k * ES;
     }
     xu4 ra[NL], rb[NL];
-    auto load = [&](int k0) {
+    // f(row, column, width): a chunk, as it is loaded
+    auto load_by = [&](int k0, auto f) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            if constexpr (MODE != kModeDw) ra[i] = exp_load<X>(pa[i] + (size_t)k0 * ES, K - k0 - cc * VEC);
-            if constexpr (MODE == kModeForward) rb[i] = exp_load<X>(pb[i] + (size_t)k0 * ES, K - k0 - cc * VEC);
-            if constexpr (MODE == kModeDx) {
-                const int n = k0 + rs + RPI * i, col = n0 + cs * VEC;
-                rb[i] = exp_load<X>(w + ((size_t)n * a.k + col) * ES, n < K ? a.k - col : 0);
-            }
+            if constexpr (MODE != kModeDw) ra[i] = f(pa[i], k0 + cc * VEC, K);
+            if constexpr (MODE == kModeForward) rb[i] = f(pb[i], k0 + cc * VEC, K);
+            if constexpr (MODE == kModeDx) rb[i] = f(w + (size_t)min(k0 + rs + RPI * i, K - 1) * a.k * ES, n0 + cs * VEC, a.k);
             if constexpr (MODE == kModeDw) {
-                const int r = k0 + rs + RPI * i, ca = m0 + cs * VEC, cb = n0 + cs * VEC;
+                const int r = k0 + rs + RPI * i;
                 const uint32_t row = order[r < K ? r : 0];
-                ra[i] = exp_load<X>(exp_row_dy(a, row) + (size_t)ca * ES, r < K ? a.rows - ca : 0);
-                rb[i] = exp_load<X>(exp_row_x(a, row) + (size_t)cb * ES, r < K ? a.k - cb : 0);
+                ra[i] = f(exp_row_dy(a, row), m0 + cs * VEC, a.rows);
+                rb[i] = f(exp_row_x(a, row), n0 + cs * VEC, a.k);
             }
         }
     };
-    auto stage = [&](int buf) {
+    const bool narrow = min(a.k, a.rows) < VEC;             // rows shorter than a load go value by value
+    auto load = [&](int k0) {
+        if (narrow)
+            load_by(k0, [](const uint8_t* row, int c, int width) { return exp_load<X>(row + (size_t)c * ES, width - c); });
+        else
+            load_by(k0, [](const uint8_t* row, int c, int width) { return exp_last<X>(row, c, width); });
+    };
+    // what lies past a row's end, or past the sum's rows, becomes zeros on the way to LDS, when all loads are under way
+    const int over_a = narrow ? 0 : exp_over<X>(m0 + cs * VEC, a.rows), over_b = narrow ? 0 : exp_over<X>(n0 + cs * VEC, a.k);
+    auto stage = [&](int buf, int k0) {
         uint8_t* ta = exp_tile + buf * 2 * G::kSide;
         uint8_t* tb = ta + G::kSide;
+        const int over_k = narrow ? 0 : exp_over<X>(k0 + cc * VEC, K);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            *reinterpret_cast<xu4*>(ta + (G::TA ? G::at_strided(rs + RPI * i, cs) : G::at_contiguous(rc + 32 * i, cc))) = ra[i];
-            *reinterpret_cast<xu4*>(tb + (G::TB ? G::at_strided(rs + RPI * i, cs) : G::at_contiguous(rc + 32 * i, cc))) = rb[i];
+            const int past = k0 + rs + RPI * i < K ? 0 : 16;
+            *reinterpret_cast<xu4*>(ta + (G::TA ? G::at_strided(rs + RPI * i, cs) : G::at_contiguous(rc + 32 * i, cc))) =
+                exp_shift(ra[i], G::TA ? max(over_a, past) : over_k);
+            *reinterpret_cast<xu4*>(tb + (G::TB ? G::at_strided(rs + RPI * i, cs) : G::at_contiguous(rc + 32 * i, cc))) =
+                exp_shift(rb[i], G::TB ? max(over_b, past) : over_k);
         }
     };
     const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
@@ -626,7 +663,7 @@ __global__ __launch_bounds__(kExpThreads, 2) void k_expert_gemm(ExpertArgs a) {
     const int steps = (K + BK - 1) / BK;
     if (steps) {
         load(0);
-        stage(0);
+        stage(0, 0);
         __syncthreads();
     }
     for (int t = 0; t < steps; ++t) {
@@ -646,7 +683,7 @@ __global__ __launch_bounds__(kExpThreads, 2) void k_expert_gemm(ExpertArgs a) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) acc[i][j] = X::mma32(fa[i], fb[j], acc[i][j]);
         }
-        if (t + 1 < steps) stage((t + 1) & 1);
+        if (t + 1 < steps) stage((t + 1) & 1, (t + 1) * BK);
         __syncthreads();
     }
     // of a 32 x 32 result a lane has column lane % 32 and rows 8 (v / 4) + 4 (lane / 32) + v % 4

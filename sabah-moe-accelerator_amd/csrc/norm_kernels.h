@@ -49,21 +49,12 @@ __device__ inline xu4 norm_pack(const float* v) {
 template <typename X, int W>
 __device__ inline int norm_col(int v, int q) { return (64 * W * q + v) * X::kVec; }
 
-// kVec values from column c of a row, zeros past its width.  A chunk that the row ends in, or one past it, is
-// read as the row's last kVec values and shifted: one load all the same, and no branch for each value.  Only a row
-// narrower than a load (NARROW: where one wave has it) goes value by value.
+// kVec values from column c of a row, zeros past its width.  Only a row narrower than a load (NARROW: where one wave has
+// it) goes value by value.
 template <typename X, bool NARROW>
 __device__ inline xu4 norm_chunk(const uint8_t* row, int c, int width) {
     if (NARROW && width < X::kVec) return exp_load<X>(row + (size_t)c * sizeof(typename X::S), width - c);
-    xu4 r = *reinterpret_cast<const xu4u*>(row + (size_t)min(c, width - X::kVec) * sizeof(typename X::S));
-    if (c > width - X::kVec) {
-        const int over = min(c + X::kVec - width, X::kVec) * (int)sizeof(typename X::S);   // bytes to shift out
-        if (over & 8) r = xu4{r[2], r[3], 0u, 0u};
-        if (over & 4) r = xu4{r[1], r[2], r[3], 0u};
-        if (over & 2) r = xu4{r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16, r[3] >> 16};
-        if (over & 16) r = xu4{0u, 0u, 0u, 0u};
-    }
-    return r;
+    return exp_chunk<X>(row, c, width);
 }
 template <typename X, int PER, int W>
 struct NormRow {

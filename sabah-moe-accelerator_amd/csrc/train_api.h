@@ -516,7 +516,8 @@ SABAH_API int sabah_adamw_step(const sabah_adamw_desc* o, void* stream) {
     if (o->bits != 32 && o->bits != 8) return fail("adamw: moments of %d bits, expected 32 or 8", o->bits);
     if ((uintptr_t)o->m % 16 || (uintptr_t)o->v % 16 || (uintptr_t)o->table % 16) return fail("adamw: the table and the moments must be 16-byte aligned");
     if (!(o->beta1 >= 0.0 && o->beta1 < 1.0 && o->beta2 >= 0.0 && o->beta2 < 1.0)) return fail("adamw: betas %g, %g outside [0, 1)", o->beta1, o->beta2);
-    if (!(o->eps > 0.0 && o->eps < __builtin_inf())) return fail("adamw: eps must be positive and finite");
+    // the step adds it in f32: what vanishes there would divide 0 by 0
+    if (!(o->eps >= 1.2e-38 && o->eps < 3.4e38)) return fail("adamw: eps %g outside f32's positive numbers", o->eps);
     if (!(o->lr >= 0.0 && o->lr < __builtin_inf())) return fail("adamw: lr must be finite and not negative");
     if (!(o->grad_scale > 0.0 && o->grad_scale < __builtin_inf())) return fail("adamw: grad_scale must be positive and finite");
     if (o->norm && !(o->max_norm > 0.0)) return fail("adamw: max_norm must be positive");

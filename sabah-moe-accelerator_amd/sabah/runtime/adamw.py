@@ -91,8 +91,13 @@ class AdamW:
                                  self.workspace.numel())
         self.ref = ctypes.byref(self.desc)
 
+    def _on_gpu(self) -> None:
+        if self.index < 0:
+            raise ValueError("adamw: the tensors are on %s, not on a GPU" % self.device)
+
     def step(self, grad_scale: float = 1.0) -> None:
         """One step on torch's current stream.  grad_scale: what the gradients are multiplied by first (one over a loss scale)."""
+        self._on_gpu()
         d = self.desc
         if not isinstance(self.lr, torch.Tensor):
             d.lr = self.lr
@@ -105,6 +110,7 @@ class AdamW:
         """(m, v) as flat f32 values: the state itself with 32 bits, with 8 bits what the codes stand for."""
         if self.bits == 32:
             return self.m, self.v
+        self._on_gpu()
         m = torch.empty(self.n_values, dtype=torch.float32, device=self.device)
         v = torch.empty(self.n_values, dtype=torch.float32, device=self.device)
         rt.check(rt.lib().sabah_adamw_moments_read(
@@ -114,6 +120,8 @@ class AdamW:
 
     def load_moments(self, m: torch.Tensor, v: torch.Tensor, step: int) -> None:
         """Flat f32 moments in the layout of moments() (zeros between the tensors) and the number of steps made: a checkpoint's."""
+        if step < 0:
+            raise ValueError("adamw: %d steps made" % step)
         for t in (m, v):
             if t.dtype != torch.float32 or t.shape != (self.n_values,) or not t.is_contiguous() or t.get_device() != self.index:
                 raise ValueError("adamw: moments %s %s, expected contiguous f32 [%d] on %s"
@@ -122,6 +130,7 @@ class AdamW:
             self.m.copy_(m)
             self.v.copy_(v)
         else:
+            self._on_gpu()
             rt.check(rt.lib().sabah_adamw_moments_write(
                 m.data_ptr(), v.data_ptr(), self.n_values, self.m.data_ptr(), self.v.data_ptr(), self.m_scale.data_ptr(),
                 self.v_scale.data_ptr(), torch._C._cuda_getCurrentRawStream(self.index)), "adamw moments")

@@ -185,7 +185,7 @@ def step(**kw):
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(table=None), "null"), (dict(step=None), "null"), (dict(m=None), "null"), (dict(v_scale=None), "null"), (dict(bits=16), "bits"),
-    (dict(m=2 * P + 4), "aligned"), (dict(beta1=1.0), "betas"), (dict(beta2=-0.1), "betas"), (dict(eps=0.0), "eps"),
+    (dict(m=2 * P + 4), "aligned"), (dict(beta1=1.0), "betas"), (dict(beta2=-0.1), "betas"), (dict(eps=0.0), "eps"), (dict(eps=1e-60), "eps"),
     (dict(lr=float("nan")), "lr"), (dict(lr=-1.0), "lr"), (dict(grad_scale=0.0), "grad_scale"), (dict(max_norm=0.0), "max_norm"),
     (dict(table_bytes=260), "table"), (dict(table_bytes=100), "table"), (dict(n_tensors=0), "table"),
     (dict(workspace=None), "workspace"), (dict(workspace_bytes=64), "workspace"), (dict(workspace=8 * P + 8), "workspace")])
@@ -269,3 +269,8 @@ def test_adamw_tensors():
     for bad in (torch.zeros(767), torch.zeros(768, dtype=torch.float64)):
         with pytest.raises(ValueError, match="moments"):
             a.load_moments(bad, bad, 0)
+    with pytest.raises(ValueError, match="steps"):
+        a.load_moments(torch.zeros(768), torch.zeros(768), -1)
+    for call in (a.step, a.moments, lambda: a.load_moments(torch.zeros(768), torch.zeros(768), 0)):
+        with pytest.raises(ValueError, match="GPU"):           # kernels are never given a host address
+            call()
