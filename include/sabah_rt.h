@@ -369,7 +369,8 @@ int sabah_lora_backward(const sabah_lora_desc *lora, const float *d_x, size_t x_
 /* ---- training a block's own weights ---------------------------------------- */
 
 /* No reference counterpart, like the adapters, whose rules on scratch, captures, streams, devices and
- * equal bits hold here too.  type: F32 0, F16 1 or BF16 30, of the activations (and an expert's
+ * equal bits hold here too.  A result shares memory with no other tensor of its call where nothing else is said, nor
+ * its rows with each other: rows of activations and experts' matrices that do are refused.  type: F32 0, F16 1 or BF16 30, of the activations (and an expert's
  * weights); other tensors are f32 where nothing else is said. */
 
 /* The norms around a block: after it, with the block's gate and the scale of its branch on the residual

@@ -6,6 +6,23 @@
 static bool float_type(int type) { return type == kTypeF32 || type == kTypeF16 || type == kTypeBF16; }
 static size_t float_size(int type) { return type == kTypeF32 ? 4 : 2; }
 
+// Memory of a tensor: n rows of `bytes`, `stride` apart (what is written may be no other tensor's memory)
+struct MemRows {
+    const void* p;
+    size_t stride, bytes;
+    int n;
+};
+static bool rows_meet(const MemRows& x, const MemRows& y) {
+    if (!x.p || !y.p || x.n <= 0 || y.n <= 0) return false;
+    const bool swap = (uintptr_t)x.p > (uintptr_t)y.p;
+    const MemRows &a = swap ? y : x, &b = swap ? x : y;
+    const size_t off = (uintptr_t)b.p - (uintptr_t)a.p;
+    if (off >= (size_t)(a.n - 1) * a.stride + a.bytes) return false;
+    // one within the other's span: apart only as columns of rows of one length
+    if (a.n == 1 || b.n == 1 || a.stride != b.stride || a.bytes > a.stride || b.bytes > b.stride) return true;
+    return off % a.stride < a.bytes || off % a.stride + b.bytes > a.stride;
+}
+
 // ---------------------------------------------------------------------------
 // norms
 // ---------------------------------------------------------------------------
@@ -26,6 +43,10 @@ static int check_norm(const char* what, const sabah_norm_desc* n, int n_tokens) 
 }
 static bool norm_rows_ok(const sabah_norm_desc* n, int n_tokens, const void* p, size_t stride) {
     return !p || (stride % float_size(n->type) == 0 && (stride >= n->width * float_size(n->type) || n_tokens <= 1));
+}
+
+static MemRows norm_mem(const sabah_norm_desc* n, int n_tokens, const void* p, size_t stride) {
+    return {p, stride, n->width * float_size(n->type), n_tokens};
 }
 
 // Waves of a row, 8 values a thread: 2,560 columns fill five of them and would leave three of eight idle
@@ -66,9 +87,12 @@ SABAH_API int sabah_block_norm(const sabah_norm_desc* norm, const void* d_x, siz
     if (!norm_rows_ok(norm, n_tokens, d_x, x_stride) || !norm_rows_ok(norm, n_tokens, d_y, y_stride) ||
         !norm_rows_ok(norm, n_tokens, d_out, out_stride) || !norm_rows_ok(norm, n_tokens, d_h, h_stride))
         return fail("block norm: a stride below a row of %d values, or no multiple of one", norm->width);
-    if (n_tokens && norm->w_before && (d_h == d_x || d_h == d_y || d_h == d_out)) return fail("block norm: h would overwrite x, y or out");
-    if (n_tokens && d_y && (d_out == d_y || (d_out == d_x && n_tokens > 1 && out_stride != x_stride)))
-        return fail("block norm: out would overwrite y, or x at another stride");
+    const MemRows x = norm_mem(norm, n_tokens, d_x, x_stride), y = norm_mem(norm, n_tokens, d_y, y_stride);
+    const MemRows out = norm_mem(norm, n_tokens, d_y ? d_out : nullptr, out_stride);
+    const MemRows h = norm_mem(norm, n_tokens, norm->w_before ? d_h : nullptr, h_stride);
+    if (rows_meet(h, x) || rows_meet(h, y) || rows_meet(h, out)) return fail("block norm: h would overwrite x, y or out");
+    const bool in_place = d_out == d_x && (n_tokens <= 1 || out_stride == x_stride);
+    if (rows_meet(out, y) || (!in_place && rows_meet(out, x))) return fail("block norm: out would overwrite y, or rows of x other than its own");
     if (g_device < 0) return fail("sabah_rt_init has not been called");
     if (!check_sticky()) return -1;
     if (n_tokens == 0) return 0;
@@ -124,10 +148,17 @@ SABAH_API int sabah_block_norm_backward(const sabah_norm_desc* norm, const void*
         !norm_rows_ok(norm, n_tokens, d_dout, dout_stride) || !norm_rows_ok(norm, n_tokens, d_dh, dh_stride) ||
         !norm_rows_ok(norm, n_tokens, d_dx, dx_stride) || !norm_rows_ok(norm, n_tokens, d_dy, dy_stride))
         return fail("block norm backward: a stride below a row of %d values, or no multiple of one", norm->width);
-    if (n_tokens && ((before && (d_dx == d_out || d_dx == d_y || d_dx == d_dh)) || (after && (d_dy == d_out || d_dy == d_y || d_dy == d_dh || d_dy == d_dout || d_dy == d_dx))))
+    const MemRows out = norm_mem(norm, n_tokens, d_out, out_stride), y = norm_mem(norm, n_tokens, d_y, y_stride);
+    const MemRows dout = norm_mem(norm, n_tokens, d_dout, dout_stride), dh = norm_mem(norm, n_tokens, before ? d_dh : nullptr, dh_stride);
+    const MemRows dx = norm_mem(norm, n_tokens, before ? d_dx : nullptr, dx_stride), dy = norm_mem(norm, n_tokens, d_dy, dy_stride);
+    if (rows_meet(dx, out) || rows_meet(dx, y) || rows_meet(dx, dh) || rows_meet(dy, out) || rows_meet(dy, y) || rows_meet(dy, dh) ||
+        rows_meet(dy, dout) || rows_meet(dy, dx))
         return fail("block norm backward: dx or dy would overwrite an input, or each other");
-    if (n_tokens > 1 && before && d_dx == d_dout && dx_stride != dout_stride)
-        return fail("block norm backward: dx in place of dout needs its stride");
+    if (!(d_dx == d_dout && (n_tokens <= 1 || dx_stride == dout_stride)) && rows_meet(dx, dout))
+        return fail("block norm backward: dx in place of dout needs its stride and its rows");
+    const size_t dw_bytes = norm->width * sizeof(float);
+    if (norm->w_after && before && rows_meet({d_dw_after, 0, dw_bytes, 1}, {d_dw_before, 0, dw_bytes, 1}))
+        return fail("block norm backward: dw_after and dw_before would overwrite each other");
     int parts, per_part;
     norm_plan(n_tokens, parts, per_part);
     const size_t part = align256((size_t)std::max(1, parts) * norm->width * 4);
@@ -267,6 +298,20 @@ static int check_experts(const char* what, const sabah_expert_desc* E, const voi
         return fail("%s: strides are in bytes and whole values", what);
     return 0;
 }
+// rows [n_tokens][n_ids] of `bytes`, the longer stride outside; own: whether the rows are apart from each other
+static MemRows expert_mem(const void* p, size_t id, size_t tok, int n_ids, int n_tokens, size_t bytes, bool* own = nullptr) {
+    if (n_ids == 1) id = 0;
+    if (n_tokens <= 1) tok = 0;
+    const bool tokens = tok >= id;
+    const size_t outer = tokens ? tok : id, inner = tokens ? id : tok;
+    const int n = tokens ? n_tokens : n_ids, m = tokens ? n_ids : n_tokens;
+    const MemRows r{p, outer, (size_t)(m - 1) * inner + bytes, n_tokens ? n : 0};
+    if (own) *own = (m <= 1 || inner >= bytes) && (n <= 1 || outer >= r.bytes);
+    return r;
+}
+static MemRows expert_weights(const sabah_expert_desc* E, const void* p, size_t value) {
+    return {p, 0, (size_t)E->n_experts * E->rows * E->k * value, 1};
+}
 static ExpertArgs expert_args(const sabah_expert_desc* E, const void* d_x, size_t x_id_stride, int x_rows, size_t x_token_stride,
                               const void* d_groups, int n_ids, int n_tokens) {
     ExpertArgs a{};
@@ -375,7 +420,12 @@ SABAH_API int sabah_expert_mul(const sabah_expert_desc* experts, const void* d_x
     if (n_tokens && !d_y) return fail("expert product: null pointer");
     if (y_id_stride % float_size(experts->type) || y_token_stride % float_size(experts->type))
         return fail("expert product: strides are in bytes and whole values");
-    if (n_tokens && d_y == d_x) return fail("expert product: y would overwrite x");
+    const size_t es = float_size(experts->type);
+    bool own;
+    const MemRows x = expert_mem(d_x, x_id_stride, x_token_stride, x_rows, n_tokens, experts->k * es);
+    const MemRows y = expert_mem(d_y, y_id_stride, y_token_stride, n_ids, n_tokens, experts->rows * es, &own);
+    if (n_tokens && !own) return fail("expert product: rows of y overlap");
+    if (rows_meet(y, x) || rows_meet(y, expert_weights(experts, experts->w, es))) return fail("expert product: y would overwrite x or the weights");
     ExpertArgs a = expert_args(experts, d_x, x_id_stride, x_rows, x_token_stride, d_groups, n_ids, n_tokens);
     if (check_groups_buffer("expert product", a.p, d_groups, groups_bytes)) return -1;
     if (g_device < 0) return fail("sabah_rt_init has not been called");
@@ -410,7 +460,15 @@ SABAH_API int sabah_expert_mul_backward(const sabah_expert_desc* experts, const 
     const size_t es = float_size(experts->type);
     if (dy_id_stride % es || dy_token_stride % es || dx_id_stride % es || dx_token_stride % es)
         return fail("expert product backward: strides are in bytes and whole values");
-    if (n_tokens && d_dx && (d_dx == d_x || d_dx == d_dy)) return fail("expert product backward: dx would overwrite x or dy");
+    bool own;
+    const MemRows x = expert_mem(d_x, x_id_stride, x_token_stride, x_rows, n_tokens, experts->k * es);
+    const MemRows dy = expert_mem(d_dy, dy_id_stride, dy_token_stride, n_ids, n_tokens, experts->rows * es);
+    const MemRows dx = expert_mem(d_dx, dx_id_stride, dx_token_stride, n_ids, n_tokens, experts->k * es, &own);
+    const MemRows w = expert_weights(experts, experts->w, es), dw = expert_weights(experts, d_dw, sizeof(float));
+    if (n_tokens && d_dx && !own) return fail("expert product backward: rows of dx overlap");
+    if (rows_meet(dx, x) || rows_meet(dx, dy) || rows_meet(dx, w)) return fail("expert product backward: dx would overwrite x, dy or the weights");
+    if (rows_meet(dw, x) || rows_meet(dw, dy) || rows_meet(dw, w) || rows_meet(dw, dx))
+        return fail("expert product backward: dw would overwrite x, dy, dx or the weights");
     ExpertArgs a = expert_args(experts, d_x, x_id_stride, x_rows, x_token_stride, d_groups, n_ids, n_tokens);
     if (check_groups_buffer("expert product backward", a.p, d_groups, groups_bytes)) return -1;
     if (g_device < 0) return fail("sabah_rt_init has not been called");

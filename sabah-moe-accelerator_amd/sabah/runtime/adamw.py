@@ -21,10 +21,11 @@ class AdamW:
     float32, float16 or bfloat16, kept by reference: write new gradients into the same tensors):
         g = c * grad;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
         p = p (1 - lr decay) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
-    lr: a number, or a float32 tensor [1] on the device, read by the step itself (a captured one follows it).
+    lr: a number, or a float32 tensor [1] on the device, read by the step itself (a captured one follows it).  `lr` and
+    `max_norm` may be set between steps, lr from a number to a tensor too, a max_norm only where there was one.
     weight_decay: a number, or one for each tensor.  bits: 32 or 8, of the moments; 8 are codes with a scale for each
     256 values (sabah_adamw_desc in include/sabah_rt.h), a quarter of the memory.  master: tensors of 16 bits have a
-    float32 copy, which is what steps change; without it small steps are lost in the tensor's rounding.  max_norm: the
+    float32 copy, which is what steps read and change (new values go into the copy too); without it small steps are lost in the tensor's rounding.  max_norm: the
     gradients are scaled down to that norm; a step whose norm is infinite or NaN changes nothing (`grad_norm`
     [1] says it); None: neither.
 
@@ -48,10 +49,8 @@ class AdamW:
                                  % (tuple(p.shape), p.dtype, tuple(g.shape), g.dtype, self.device))
         if self.index >= 0:
             rt.init(self.index)
-        self.bits, self.max_norm = bits, max_norm
-        self.lr = lr
-        if isinstance(lr, torch.Tensor) and (lr.dtype != torch.float32 or lr.numel() != 1 or lr.get_device() != self.index):
-            raise ValueError("adamw: lr is %s %s, expected float32 [1] on %s" % (tuple(lr.shape), lr.dtype, self.device))
+        self.bits, self.max_norm, self.lr = bits, max_norm, lr
+        self._rate()
         self.starts, self.n_values = [], 0
         for p in self.params:
             self.starts.append(self.n_values)
@@ -82,11 +81,10 @@ class AdamW:
         rt.check(lib.sabah_adamw_table(ts, n, host.data_ptr(), size), "adamw")
         self.table = host.to(dev)
         self.workspace = torch.empty(lib.sabah_adamw_workspace(), dtype=torch.uint8, device=dev)
-        on_device = isinstance(lr, torch.Tensor)
         self.desc = rt.AdamWDesc(self.table.data_ptr(), size, n, bits, self.m.data_ptr(), self.v.data_ptr(),
                                  self.m_scale.data_ptr() if bits == 8 else None, self.v_scale.data_ptr() if bits == 8 else None,
-                                 0.0 if on_device else float(lr), betas[0], betas[1], eps, 1.0, max_norm or 0.0,
-                                 lr.data_ptr() if on_device else None, self.step_count.data_ptr(),
+                                 self._rate()[0], betas[0], betas[1], eps, 1.0, max_norm or 0.0,
+                                 self._rate()[1], self.step_count.data_ptr(),
                                  self.grad_norm.data_ptr() if max_norm is not None else None, self.workspace.data_ptr(),
                                  self.workspace.numel())
         self.ref = ctypes.byref(self.desc)
@@ -95,12 +93,23 @@ class AdamW:
         if self.index < 0:
             raise ValueError("adamw: the tensors are on %s, not on a GPU" % self.device)
 
+    def _rate(self):
+        """(lr, d_lr) of the C descriptor."""
+        lr = self.lr
+        if not isinstance(lr, torch.Tensor):
+            return float(lr), None
+        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.get_device() != self.index:
+            raise ValueError("adamw: lr is %s %s, expected float32 [1] on %s" % (tuple(lr.shape), lr.dtype, self.device))
+        return 0.0, lr.data_ptr()
+
     def step(self, grad_scale: float = 1.0) -> None:
         """One step on torch's current stream.  grad_scale: what the gradients are multiplied by first (one over a loss scale)."""
         self._on_gpu()
+        if (self.max_norm is None) != (self.grad_norm is None):
+            raise ValueError("adamw: max_norm %r, the steps were made %s one" % (self.max_norm, "with" if self.max_norm is None else "without"))
         d = self.desc
-        if not isinstance(self.lr, torch.Tensor):
-            d.lr = self.lr
+        d.lr, d.d_lr = self._rate()
+        d.max_norm = self.max_norm or 0.0
         d.grad_scale = grad_scale
         rc = rt.lib().sabah_adamw_step(self.ref, torch._C._cuda_getCurrentRawStream(self.index))
         if rc:

@@ -238,6 +238,29 @@ def test_captured_steps_follow_gradients_and_rate(hip_rt, bits):
             assert torch.equal(x, y)
 
 
+def test_rate_and_norm_set_between_steps(hip_rt):
+    """What lr and max_norm are when step() is called counts: each step equals that of an optimizer made with them."""
+    from sabah.runtime.adamw import AdamW
+    g = torch.Generator().manual_seed(6)
+    start, grad = torch.randn(700, generator=g), torch.randn(700, generator=g).to(DEV)
+    a = AdamW([start.to(DEV)], [grad], lr=1e-2, max_norm=1.0)
+    for lr, max_norm in ((torch.tensor([3e-2], device=DEV), 1.0), (5e-3, 4.0), (torch.tensor([1e-3], device=DEV), 0.5)):
+        b = AdamW([a.params[0].clone()], [grad], lr=lr, max_norm=max_norm)
+        b.load_moments(a.m, a.v, int(a.step_count.item()))
+        a.lr, a.max_norm = lr, max_norm
+        a.step()
+        b.step()
+        torch.cuda.synchronize()
+        for x, y in zip(a.params + [a.m, a.v, a.grad_norm], b.params + [b.m, b.v, b.grad_norm]):
+            assert torch.equal(x, y)
+    a.max_norm = None
+    with pytest.raises(ValueError, match="max_norm"):
+        a.step()
+    a.max_norm, a.lr = 1.0, torch.zeros(2, device=DEV)
+    with pytest.raises(ValueError, match="lr"):
+        a.step()
+
+
 def test_a_longer_run_of_8_bits_stays_near_32(hip_rt):
     """A noisy quadratic: with 8 bits the weights come as near to its minimum as with 32 (within twice the distance)."""
     far = {}

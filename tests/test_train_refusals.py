@@ -82,6 +82,28 @@ def test_norms_refuse_their_own_arguments():
     assert rt.lib().sabah_block_norm_workspace(0, 3) == 0
 
 
+# three rows of 128 bytes at P, 2 P ..: one value, the last byte's and other rows' overlaps, and columns of one buffer
+@pytest.mark.parametrize("kw,msg", [
+    (dict(out=P + 2), "overwrite"), (dict(out=P + 128), "overwrite"), (dict(out=2 * P - 382), "overwrite"), (dict(out=2 * P - 384), None),
+    (dict(out=2 * P + 382), "overwrite"), (dict(out=2 * P + 384), None), (dict(out=P), None), (dict(h=P + 382), "overwrite"),
+    (dict(h=3 * P + 2), "overwrite"), (dict(x=P, xs=512, out=P + 128, os=512, y=P + 256, ys=512, h=P + 384, hs=512), None),
+    (dict(x=P, xs=512, h=P + 126, hs=512), "overwrite"), (dict(x=P, xs=512, h=P + 386, hs=512), "overwrite"),
+    (dict(x=P, xs=512, h=P + 384 + 512, hs=512), None), (dict(x=P, xs=512, h=P + 128, hs=256), "overwrite"),
+    (dict(x=P, xs=512, h=P + 128, hs=256, T=1), None), (dict(x=P, h=P + 126, T=1), "overwrite"), (dict(x=P, h=P + 2, T=0), None)])
+def test_norms_refuse_results_over_other_rows(kw, msg):
+    if torch.cuda.device_count():
+        pytest.skip("with a device an accepted call would use the addresses")
+    fails(norm(norm_desc(), **kw), msg or "sabah_rt_init")
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(dx=P + 2), "overwrite"), (dict(dx=4 * P + 128), "overwrite"), (dict(dy=3 * P + 382), "overwrite"), (dict(dy=5 * P + 2), "overwrite"),
+    (dict(dx=3 * P), None), (dict(dx=3 * P + 128), "in place"), (dict(dwb=7 * P), "each other"), (dict(dwb=7 * P + 252), "each other"),
+    (dict(dwb=7 * P + 256), None)])
+def test_norms_backward_refuses_results_over_other_rows(kw, msg):
+    fails(norm_back(norm_desc(), **kw, ws=None), msg or "workspace")       # the check that follows
+
+
 # ---- experts -----------------------------------------------------------------
 def expert_desc(**kw):
     from sabah.runtime import rt
@@ -135,6 +157,26 @@ def test_experts_refuse_their_own_arguments():
     fails(group(T=-1), "rows")
     fails(group(ng=n - 1), "groups")
     fails(group(g=2 * P + 4), "groups")
+
+
+# x: three rows of 128 bytes at P (the weights' 24,576 lie at 32 P); y: [3][2] rows of 96 bytes
+@pytest.mark.parametrize("kw,msg", [
+    (dict(yi=94), "overlap"), (dict(yt=190), "overlap"), (dict(yi=0), "overlap"), (dict(yt=0), "overlap"), (dict(yi=288, yt=96), None),
+    (dict(yi=286, yt=96), "overlap"), (dict(n=1, yi=0, yt=96), None), (dict(T=1, yt=0), None), (dict(y=P + 382), "overwrite"),
+    (dict(y=P + 384), None), (dict(xt=512, y=P + 128, yt=512), None), (dict(xt=512, y=P + 126, yt=512), "overwrite"),
+    (dict(xt=512, y=P + 322, yt=512), "overwrite"), (dict(xt=0, y=P + 126), "overwrite"), (dict(xt=0, y=P + 128), None),
+    (dict(y=32 * P + 24574), "overwrite"), (dict(y=32 * P + 24576), None)])
+def test_experts_refuse_results_over_other_rows(kw, msg):
+    fails(mul(expert_desc(w=32 * P), **kw, g=None), msg or "groups must")  # the check that follows
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(di=126), "overlap"), (dict(dt=254), "overlap"), (dict(dx=P + 382), "overwrite"), (dict(dx=3 * P + 574), "overwrite"),
+    (dict(dx=3 * P + 576), None), (dict(dx=32 * P), "overwrite"), (dict(dw=32 * P + 24572), "overwrite"), (dict(dw=4 * P + 764), "overwrite"),
+    (dict(dw=4 * P + 768), None), (dict(dw=3 * P), "overwrite"), (dict(dw=None), None), (dict(dx=None, di=0, dt=0), None),
+    (dict(T=0, dx=None, dw=32 * P), "overwrite")])
+def test_experts_backward_refuses_results_over_other_rows(kw, msg):
+    fails(mul_back(expert_desc(w=32 * P), **kw, g=None), msg or "groups must")
 
 
 # ---- AdamW -------------------------------------------------------------------
