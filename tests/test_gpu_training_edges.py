@@ -1,0 +1,45 @@
+"""A block's norms, experts' products and AdamW where the training tests' ordinary values do not reach, against the 64-bit
+forms of train_refs."""
+import math
+
+import pytest
+import torch
+
+import train_refs as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = {"f32": F32, "f16": F16, "bf16": BF16}
+
+
+@pytest.fixture(scope="module")
+def ex(hip_rt):
+    from sabah.runtime.bank import ExpertBank
+    from sabah.runtime.executor import MoEExecutor
+    return MoEExecutor(ExpertBank(1, 8, 256, 256, {"gate": 21, "up": 21, "down": 21}, device=DEV))
+
+
+# ---- norms -------------------------------------------------------------------
+@pytest.mark.parametrize("after", [True, False])
+@pytest.mark.parametrize("D", [24, 700])
+def test_gates_far_from_zero(ex, after, D):
+    """dgate has sigmoid(-gate), which is far below the steps of 1 - sigmoid(gate) where a gate is wide open."""
+    from sabah.runtime.norm import BlockNorm
+    eps, scale = 1e-6, 0.5
+    gate = torch.linspace(-87.0, 87.0, 349)
+    T = gate.numel()
+    g = torch.Generator().manual_seed(3)
+    n = BlockNorm(D, after=after, before=True, eps=eps, scale=scale, device=DEV)
+    x, y, dout, dh = (torch.randn(T, D, generator=g) for _ in range(4))
+    out, _ = ex.block_norm(n, x.to(DEV), y.to(DEV), gate.to(DEV))
+    _, _, dgate, _, _ = ex.block_norm_backward(n, out, y.to(DEV), gate.to(DEV), dout=dout.to(DEV), dh=dh.to(DEV))
+    one = torch.ones(D)
+    d, tol = R.norm_back(out.cpu(), None, None, None, one, dout, dh, eps, scale)["dx"]
+    branch = y.double()
+    if after:
+        branch = branch / torch.sqrt(branch.square().mean(1, keepdim=True) + eps)
+    c = scale * torch.sigmoid(gate.double()) * torch.sigmoid(-gate.double())
+    size = (tol / (80 * R.U) * branch.abs()).sum(1)
+    # the bound of train_refs (an exp and a quotient more are within it), and steps of 2^-149 where factors are below 2^-126
+    R.close(dgate, c * (d * branch).sum(1), 200 * R.U * c * size + 2.0 ** -147 * (1 + size), "dgate")
