@@ -265,7 +265,7 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw_step(AdamArgs a) {
         }
     }
     const float keep = (float)(1.0 - s.lr * T.decay), eps = (float)a.eps;
-    const float b1 = (float)a.b1, n1 = (float)(1.0 - a.b1), b2 = (float)a.b2, n2 = (float)(1.0 - a.b2), c = (float)s.c;
+    const float b1 = (float)a.b1, n1 = (float)(1.0 - a.b1), b2 = (float)a.b2, n2 = (float)(1.0 - a.b2);
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
         const long long i = first + (k * kAdamThreads + (int)threadIdx.x) * 4;
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw_step(AdamArgs a) {
         if constexpr (BITS == 32) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float q = g[k][j] * c;
+                const float q = (float)((double)g[k][j] * s.c);   // s.c may lie outside f32's numbers
                 m[k][j] = m[k][j] * b1 + q * n1;
                 v[k][j] = v[k][j] * b2 + q * q * n2;
             }

@@ -43,3 +43,33 @@ def test_gates_far_from_zero(ex, after, D):
     size = (tol / (80 * R.U) * branch.abs()).sum(1)
     # the bound of train_refs (an exp and a quotient more are within it), and steps of 2^-149 where factors are below 2^-126
     R.close(dgate, c * (d * branch).sum(1), 200 * R.U * c * size + 2.0 ** -147 * (1 + size), "dgate")
+
+
+# ---- AdamW -------------------------------------------------------------------
+def adamw(p, grad, **kw):
+    from sabah.runtime.adamw import AdamW
+    return AdamW([p.to(DEV)], [grad.to(DEV)], **{**dict(lr=3e-3, betas=(0.9, 0.99), weight_decay=0.0), **kw})
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("size,scale,max_norm", [(1e38, 1.0, 1e-4), (1e38, 1.0, 1e-9), (1e38, 1e-42, None), (1e-39, 1e39, None), (1e-39, 1e41, 10.0)])
+def test_factors_of_the_gradients_beyond_f32(hip_rt, size, scale, max_norm, bits):
+    """What gradients are multiplied by may lie outside f32's numbers where the products do not."""
+    g = torch.Generator().manual_seed(2)
+    grad = torch.randn(700, generator=g).clamp(-3, 3) * size
+    p = torch.randn(700, generator=g)
+    opt = adamw(p, grad, bits=bits, max_norm=max_norm)
+    opt.step(grad_scale=scale)
+    torch.cuda.synchronize()
+    c = scale
+    if max_norm is not None:
+        c *= min(1.0, max_norm / (scale * grad.double().norm().item() + 1e-6))
+    want, m, v, step = R.adamw(p, grad, torch.zeros(700), torch.zeros(700), 1, 3e-3, (0.9, 0.99), 1e-8, 0.0, c)
+    q = grad.double().abs() * c
+    tm, tv = 6 * R.U * q + 1e-44, 8 * R.U * q * q + 1e-44
+    if bits == 32:
+        R.close(opt.m[:700], m, tm, "m")
+        R.close(opt.v[:700], v, tv, "v")
+    # m's error, half of v's relative one, 12 roundings of the step and 3 of the rest; one more where the whole step is tiny
+    tp = step.abs() * (12 * R.U + tm / m.abs().clamp(min=1e-300) + tv / v.clamp(min=1e-300)).clamp(max=1) + 3 * R.U * (p.double().abs() + step.abs())
+    R.close(opt.params[0], want, tp, "p")
