@@ -431,7 +431,8 @@ int sabah_expert_mul_backward(const sabah_expert_desc *experts, const void *d_x,
  *   g = c * grad;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
  *   p = p (1 - lr decay) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
  * with c = grad_scale, times min(1, max_norm / (norm + 1e-6)) where the norm of all gradients (times grad_scale) is wanted.
- * A step whose norm is infinite or NaN changes nothing but the norm.  Tensors of 16 bits may have a master copy
+ * A step whose norm is infinite or NaN changes nothing but the norm; a finite one that f32 cannot hold is reported as f32's
+ * largest number.  Tensors of 16 bits may have a master copy
  * in f32, which is then what the step reads and writes; the tensor is its rounded copy. */
 typedef struct sabah_adamw_tensor {
     void *p;                               /* n values of p_type */

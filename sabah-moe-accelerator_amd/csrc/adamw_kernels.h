@@ -22,6 +22,7 @@ namespace sabah {
 
 constexpr int kAdamBlock = 256, kAdamChunk = 2048, kAdamThreads = 256;
 constexpr int kAdamNormGroups = 1024;
+constexpr float kAdamMost = 3.4028234663852886e38f;  // f32's largest number
 
 // A tensor as the device sees it; m and v begin at `at` of the flat moments, a multiple of kAdamBlock
 struct AdamTensor {
@@ -157,7 +158,7 @@ __global__ __launch_bounds__(1024) void k_adamw_begin(AdamArgs a) {
         const double norm = sqrt(s) * a.grad_scale;
         skip = !(norm < __builtin_inf());                   // an infinite or NaN gradient: nothing changes
         c *= fmin(1.0, a.max_norm / (norm + 1e-6));
-        if (threadIdx.x == 0) *a.norm = (float)norm;
+        if (threadIdx.x == 0) *a.norm = skip ? (float)norm : fminf(kAdamMost, (float)norm);   // infinite or NaN: not made
     }
     if (threadIdx.x == 0) {
         AdamScalars r{};
@@ -187,7 +188,6 @@ __device__ inline int adam_code4(double t, int most) {
     return min(most, max(0, k));
 }
 constexpr double kAdamM2 = 127.0 * 127.0, kAdamV4 = 255.0 * 255.0 * 255.0 * 255.0;
-constexpr float kAdamMost = 3.4028234663852886e38f;
 
 // Four neighbours a lane, a block of 256 a wave: the codes and the scales of m and v
 __device__ inline float adam_block_max(float v) {

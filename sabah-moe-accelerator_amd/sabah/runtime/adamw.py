@@ -27,7 +27,7 @@ class AdamW:
     256 values (sabah_adamw_desc in include/sabah_rt.h), a quarter of the memory.  master: tensors of 16 bits have a
     float32 copy, which is what steps read and change (new values go into the copy too); without it small steps are lost in the tensor's rounding.  max_norm: the
     gradients are scaled down to that norm; a step whose norm is infinite or NaN changes nothing (`grad_norm`
-    [1] says it); None: neither.
+    [1] says it: it is infinite or NaN after such steps alone, and at most f32's largest number after others); None: neither.
 
     `step_count` [1] int64, `m`, `v` (and `m_scale`, `v_scale`, `master`) are the state, on the device.  In the flat ones each tensor
     begins at a multiple of 256: tensor i at `starts[i]`."""

@@ -73,3 +73,21 @@ def test_factors_of_the_gradients_beyond_f32(hip_rt, size, scale, max_norm, bits
     # m's error, half of v's relative one, 12 roundings of the step and 3 of the rest; one more where the whole step is tiny
     tp = step.abs() * (12 * R.U + tm / m.abs().clamp(min=1e-300) + tv / v.clamp(min=1e-300)).clamp(max=1) + 3 * R.U * (p.double().abs() + step.abs())
     R.close(opt.params[0], want, tp, "p")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_finite_norm_beyond_f32(hip_rt, bits):
+    """A step that is made says so: its norm, which f32 cannot hold, is f32's largest number and not infinite."""
+    grad = torch.tensor([3e38, -3e38, 1e38])
+    opt = adamw(torch.zeros(3), grad, bits=bits, max_norm=1.0)
+    opt.step()
+    torch.cuda.synchronize()
+    assert opt.step_count.item() == 1 and opt.grad_norm.item() == torch.finfo(F32).max
+    want, _, _, step = R.adamw(torch.zeros(3), grad, torch.zeros(3), torch.zeros(3), 1, 3e-3, (0.9, 0.99), 1e-8, 0.0,
+                               1.0 / grad.double().norm().item())
+    R.close(opt.params[0], want, 20 * R.U * step.abs(), "p")
+    for bad in (float("inf"), float("nan")):
+        opt.grads[0][1] = bad
+        opt.step()
+        torch.cuda.synchronize()
+        assert opt.step_count.item() == 1 and not opt.grad_norm.isfinite().item()
