@@ -91,3 +91,15 @@ def test_a_finite_norm_beyond_f32(hip_rt, bits):
         opt.step()
         torch.cuda.synchronize()
         assert opt.step_count.item() == 1 and not opt.grad_norm.isfinite().item()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("lr,decay", [(1e-5, 0.01), (3e-5, 0.01), (1e-4, 0.1), (1e-2, 0.1)])
+def test_a_small_decay_is_not_rounded_to_steps_of_one(hip_rt, lr, decay, bits):
+    """p (1 - lr decay) rounded once: lr decay next to 1 would be a whole number of steps of 2^-24."""
+    p = 1 + torch.rand(5000, generator=torch.Generator().manual_seed(4))
+    opt = adamw(p, torch.zeros(5000), lr=lr, weight_decay=decay, bits=bits)
+    opt.step()
+    torch.cuda.synchronize()
+    # the sum's rounding, half a step of numbers below 2, and those of lr decay and its product
+    R.close(opt.params[0], p.double() * (1 - lr * decay), R.U * (1 + 4 * p.double() * lr * decay), "p")
