@@ -103,3 +103,17 @@ def test_a_small_decay_is_not_rounded_to_steps_of_one(hip_rt, lr, decay, bits):
     torch.cuda.synchronize()
     # the sum's rounding, half a step of numbers below 2, and those of lr decay and its product
     R.close(opt.params[0], p.double() * (1 - lr * decay), R.U * (1 + 4 * p.double() * lr * decay), "p")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("size", [1e-12, 1e-17, 1e-18, 1e-19, 1e-20])
+def test_squares_below_f32_normal_numbers(hip_rt, size, bits):
+    """v of gradients whose squares are below 2^-126 still divides m, down to f32's steps of 2^-149."""
+    g = torch.Generator().manual_seed(5)
+    grad = (1 + torch.rand(700, generator=g)) * size * torch.where(torch.rand(700, generator=g) < 0.5, -1.0, 1.0)
+    opt = adamw(torch.zeros(700), grad, bits=bits, eps=1e-30)
+    opt.step()
+    torch.cuda.synchronize()
+    want, m, v, step = R.adamw(torch.zeros(700), grad, torch.zeros(700), torch.zeros(700), 1, 3e-3, (0.9, 0.99), 1e-30, 0.0, 1.0)
+    # f32's steps of a square, its product and v: 3 of 2^-149, of which the root takes half
+    R.close(opt.params[0], want, step.abs() * (16 * R.U + 3 * 2.0 ** -149 / v), "p")
