@@ -60,7 +60,7 @@ class AdamW:
         if master and any(p.dtype != torch.float32 for p in self.params):
             self.master = torch.zeros(self.n_values, dtype=torch.float32, device=dev)
             for p, at in zip(self.params, self.starts):
-                self.master[at:at + p.numel()].copy_(p.reshape(-1))
+                self.master[at:at + p.numel()].copy_(p.detach().reshape(-1))
         self.m = torch.zeros(self.n_values, dtype=torch.float32 if bits == 32 else torch.int8, device=dev)
         self.v = torch.zeros(self.n_values, dtype=torch.float32 if bits == 32 else torch.uint8, device=dev)
         self.m_scale = torch.zeros(blocks, dtype=torch.float32, device=dev) if bits == 8 else None
