@@ -16,6 +16,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <numeric>
 #include <unordered_set>
 #include <vector>
 

@@ -6,19 +6,33 @@
 static bool float_type(int type) { return type == kTypeF32 || type == kTypeF16 || type == kTypeBF16; }
 static size_t float_size(int type) { return type == kTypeF32 ? 4 : 2; }
 
-// Memory of a tensor: n rows of `bytes`, `stride` apart (what is written may be no other tensor's memory)
+// Memory of a tensor: n rows of `bytes`, `stride` apart (what is written may be no other tensor's memory); a row may itself be
+// m parts of `part` bytes, `inner` apart
 struct MemRows {
     const void* p;
     size_t stride, bytes;
     int n;
+    size_t inner = 0, part = 0;
+    int m = 1;
 };
+// Whether parts are apart as columns of one buffer are: every stride is a multiple of s, and modulo s they do not meet
+static bool parts_apart(const MemRows& a, const MemRows& b, size_t off) {
+    size_t s = 0;
+    for (const MemRows* r : {&a, &b}) {
+        if (r->n > 1) s = std::gcd(s, r->stride);
+        if (r->m > 1) s = std::gcd(s, r->inner);
+    }
+    const size_t first = a.m > 1 ? a.part : a.bytes, second = b.m > 1 ? b.part : b.bytes;
+    return s && first <= s && second <= s && off % s >= first && off % s + second <= s;
+}
 static bool rows_meet(const MemRows& x, const MemRows& y) {
     if (!x.p || !y.p || x.n <= 0 || y.n <= 0) return false;
     const bool swap = (uintptr_t)x.p > (uintptr_t)y.p;
     const MemRows &a = swap ? y : x, &b = swap ? x : y;
     const size_t off = (uintptr_t)b.p - (uintptr_t)a.p;
     if (off >= (size_t)(a.n - 1) * a.stride + a.bytes) return false;
-    // one within the other's span: apart only as columns of rows of one length
+    // one within the other's span: apart only as columns of rows of one length, or of their parts
+    if ((a.m > 1 || b.m > 1) && parts_apart(a, b, off)) return false;
     if (a.n == 1 || b.n == 1 || a.stride != b.stride || a.bytes > a.stride || b.bytes > b.stride) return true;
     return off % a.stride < a.bytes || off % a.stride + b.bytes > a.stride;
 }
@@ -305,7 +319,7 @@ static MemRows expert_mem(const void* p, size_t id, size_t tok, int n_ids, int n
     const bool tokens = tok >= id;
     const size_t outer = tokens ? tok : id, inner = tokens ? id : tok;
     const int n = tokens ? n_tokens : n_ids, m = tokens ? n_ids : n_tokens;
-    const MemRows r{p, outer, (size_t)(m - 1) * inner + bytes, n_tokens ? n : 0};
+    const MemRows r{p, outer, (size_t)(m - 1) * inner + bytes, n_tokens ? n : 0, inner, bytes, m};
     if (own) *own = (m <= 1 || inner >= bytes) && (n <= 1 || outer >= r.bytes);
     return r;
 }

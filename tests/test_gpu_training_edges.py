@@ -117,3 +117,25 @@ def test_squares_below_f32_normal_numbers(hip_rt, size, bits):
     want, m, v, step = R.adamw(torch.zeros(700), grad, torch.zeros(700), torch.zeros(700), 1, 3e-3, (0.9, 0.99), 1e-30, 0.0, 1.0)
     # f32's steps of a square, its product and v: 3 of 2^-149, of which the root takes half
     R.close(opt.params[0], want, step.abs() * (16 * R.U + 3 * 2.0 ** -149 / v), "p")
+
+
+# ---- experts -----------------------------------------------------------------
+@pytest.mark.parametrize("T", [5, 200])
+def test_inputs_and_results_as_columns_of_one_buffer(ex, T):
+    """x beside y and dy beside dx in the rows of [T, slots, k + rows]: the same as apart, and nothing else changes."""
+    from sabah.runtime.experts import FloatExperts
+    g = torch.Generator().manual_seed(8)
+    k, rows = 72, 88
+    e = FloatExperts(4, k, rows, dtype=BF16, device=DEV)
+    e.w.copy_(torch.randint(-3, 4, (4, rows, k), generator=g))
+    ids = torch.randint(-1, 4, (T, 2), generator=g, dtype=torch.int32).to(DEV)
+    x, dy = (torch.randint(-3, 4, (T, 2, n), generator=g).to(BF16).to(DEV) for n in (k, rows))
+    groups = ex.group_rows(ids, 4)
+    want = ex.expert_mul(e, x, groups), ex.expert_mul_backward(e, x, groups, dy)
+    buf = torch.full((T, 2, k + rows), 9.0, dtype=BF16, device=DEV)
+    buf[:, :, :k] = x
+    y = ex.expert_mul(e, buf[:, :, :k], groups, out=buf[:, :, k:])
+    assert torch.equal(y, want[0]) and torch.equal(buf[:, :, :k], x)
+    buf[:, :, k:] = dy
+    dx, dw = ex.expert_mul_backward(e, x, groups, buf[:, :, k:], dx=buf[:, :, :k])
+    assert torch.equal(dx, want[1][0]) and torch.equal(dw, want[1][1]) and torch.equal(buf[:, :, k:], dy)
