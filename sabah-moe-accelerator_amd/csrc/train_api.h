@@ -250,6 +250,20 @@ static int check_groups_buffer(const char* what, const ExpertPlan& p, const void
     return 0;
 }
 
+// rows [n_tokens][n_ids] of `bytes`, the longer stride outside; own: whether the rows are apart from each other
+static MemRows expert_mem(const void* p, size_t id, size_t tok, int n_ids, int n_tokens, size_t bytes, bool* own = nullptr) {
+    if (n_ids == 1) id = 0;
+    if (n_tokens <= 1) tok = 0;
+    const bool tokens = tok >= id;
+    const size_t outer = tokens ? tok : id, inner = tokens ? id : tok;
+    const int n = tokens ? n_tokens : n_ids, m = tokens ? n_ids : n_tokens;
+    const MemRows r{p, outer, (size_t)(m - 1) * inner + bytes, n_tokens ? n : 0, inner, bytes, m};
+    if (own) *own = (m <= 1 || inner >= bytes) && (n <= 1 || outer >= r.bytes);
+    return r;
+}
+// the groups' memory: kernels take rows' numbers and tiles from it, so nothing else may be written there
+static MemRows groups_mem(const ExpertPlan& p, const void* d_groups) { return {d_groups, 0, p.words * 4, 1}; }
+
 SABAH_API size_t sabah_expert_groups_bytes(int n_ids, int n_tokens, int n_experts) {
     if (check_groups("expert groups", n_ids, n_tokens, n_experts)) return 0;
     return expert_plan(n_ids, n_tokens, n_experts).words * 4;
@@ -263,6 +277,8 @@ SABAH_API int sabah_expert_group(const int32_t* d_ids, size_t ids_id_stride, siz
     ExpertGroupArgs a{};
     a.p = expert_plan(n_ids, n_tokens, n_experts);
     if (check_groups_buffer("expert groups", a.p, d_groups, groups_bytes)) return -1;
+    if (rows_meet(groups_mem(a.p, d_groups), expert_mem(d_ids, ids_id_stride, ids_token_stride, n_ids, n_tokens, 4)))
+        return fail("expert groups: the groups would overwrite the ids");
     if (g_device < 0) return fail("sabah_rt_init has not been called");
     if (!check_sticky()) return -1;
     OnDevice dev;
@@ -311,17 +327,6 @@ static int check_experts(const char* what, const sabah_expert_desc* E, const voi
     if (x_id_stride % float_size(E->type) || x_token_stride % float_size(E->type))
         return fail("%s: strides are in bytes and whole values", what);
     return 0;
-}
-// rows [n_tokens][n_ids] of `bytes`, the longer stride outside; own: whether the rows are apart from each other
-static MemRows expert_mem(const void* p, size_t id, size_t tok, int n_ids, int n_tokens, size_t bytes, bool* own = nullptr) {
-    if (n_ids == 1) id = 0;
-    if (n_tokens <= 1) tok = 0;
-    const bool tokens = tok >= id;
-    const size_t outer = tokens ? tok : id, inner = tokens ? id : tok;
-    const int n = tokens ? n_tokens : n_ids, m = tokens ? n_ids : n_tokens;
-    const MemRows r{p, outer, (size_t)(m - 1) * inner + bytes, n_tokens ? n : 0, inner, bytes, m};
-    if (own) *own = (m <= 1 || inner >= bytes) && (n <= 1 || outer >= r.bytes);
-    return r;
 }
 static MemRows expert_weights(const sabah_expert_desc* E, const void* p, size_t value) {
     return {p, 0, (size_t)E->n_experts * E->rows * E->k * value, 1};
@@ -442,6 +447,7 @@ SABAH_API int sabah_expert_mul(const sabah_expert_desc* experts, const void* d_x
     if (rows_meet(y, x) || rows_meet(y, expert_weights(experts, experts->w, es))) return fail("expert product: y would overwrite x or the weights");
     ExpertArgs a = expert_args(experts, d_x, x_id_stride, x_rows, x_token_stride, d_groups, n_ids, n_tokens);
     if (check_groups_buffer("expert product", a.p, d_groups, groups_bytes)) return -1;
+    if (rows_meet(y, groups_mem(a.p, d_groups))) return fail("expert product: y would overwrite the groups");
     if (g_device < 0) return fail("sabah_rt_init has not been called");
     if (!check_sticky()) return -1;
     if (n_tokens == 0) return 0;
@@ -485,6 +491,8 @@ SABAH_API int sabah_expert_mul_backward(const sabah_expert_desc* experts, const 
         return fail("expert product backward: dw would overwrite x, dy, dx or the weights");
     ExpertArgs a = expert_args(experts, d_x, x_id_stride, x_rows, x_token_stride, d_groups, n_ids, n_tokens);
     if (check_groups_buffer("expert product backward", a.p, d_groups, groups_bytes)) return -1;
+    if (rows_meet(dx, groups_mem(a.p, d_groups)) || rows_meet(dw, groups_mem(a.p, d_groups)))
+        return fail("expert product backward: dx or dw would overwrite the groups");
     if (g_device < 0) return fail("sabah_rt_init has not been called");
     if (!check_sticky()) return -1;
     OnDevice dev;

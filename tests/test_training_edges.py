@@ -37,3 +37,28 @@ def test_experts_take_columns_of_one_buffer(kw, msg):
     back = dict(dx=v.get("x", P), di=v["xi"], dt=v["xt"], y=v["y"], yi=v["yi"], yt=v["yt"], xi=128, xr=2, xt=256)
     if v["xr"] == 2:
         fails(mul_back(expert_desc(w=32 * P), **back, x=8 * P, dw=None, g=None), msg or "groups must")
+
+
+def group(ids=P, g=2 * P, si=4, st=8, T=3):
+    from sabah.runtime import rt
+    return rt.lib().sabah_expert_group(ids, si, st, 2, T, 4, g, 1 << 40, None)
+
+
+# groups of [3][2] rows over 4 experts at 2 P; y, dx and ids of 3 tokens' two rows, dw of 49,152 bytes
+@pytest.mark.parametrize("call,own,msg", [
+    (mul, dict(y=2 * P), "groups"), (mul, dict(y=2 * P - 574), "groups"), (mul, dict(y=2 * P - 576), None), (mul, dict(y=2 * P + 16), "groups"),
+    (mul_back, dict(dx=2 * P - 766), "groups"), (mul_back, dict(dx=2 * P - 768), None), (mul_back, dict(dx=None, dw=2 * P), "groups"),
+    (mul_back, dict(dw=2 * P - 49148), "groups"), (mul_back, dict(dw=2 * P - 49152), None),
+    (group, dict(ids=2 * P), "ids"), (group, dict(ids=2 * P - 20), "ids"), (group, dict(ids=2 * P - 24), None), (group, dict(ids=2 * P, T=0), None)])
+def test_nothing_is_written_over_the_groups(call, own, msg):
+    """Rows' numbers that were overwritten would send kernels anywhere."""
+    from sabah.runtime import rt
+    n = rt.lib().sabah_expert_groups_bytes(2, 3, 4)
+    if msg is None and torch.cuda.device_count():
+        pytest.skip("with a device an accepted call would use the addresses")
+    rc = call(**own) if call is group else call(expert_desc(w=32 * P), **{**dict(x=8 * P, y=9 * P, g=2 * P), **own})
+    fails(rc, msg or "sabah_rt_init")
+    if call is not group and "y" in own and own["y"] == 2 * P:           # the groups' last bytes, and what follows them
+        fails(mul(expert_desc(w=32 * P), x=8 * P, y=2 * P + n - 2), "groups")
+        if not torch.cuda.device_count():
+            fails(mul(expert_desc(w=32 * P), x=8 * P, y=2 * P + n), "sabah_rt_init")
