@@ -593,7 +593,9 @@ SABAH_API size_t sabah_adamw_workspace(void) { return align256(kAdamNormGroups *
 
 SABAH_API int sabah_adamw_step(const sabah_adamw_desc* o, void* stream) {
     if (!o || !o->table || !o->step) return fail("adamw: null pointer");
-    if (o->bits != 32 && o->bits != 8) return fail("adamw: moments of %d bits, expected 32 or 8", o->bits);
+    const bool unbiased = o->bits == (8 | SABAH_ADAMW_UNBIASED);
+    const int bits = unbiased ? 8 : o->bits;
+    if (bits != 32 && bits != 8) return fail("adamw: moments of %d bits, expected 32 or 8", o->bits);
     if ((uintptr_t)o->m % 16 || (uintptr_t)o->v % 16 || (uintptr_t)o->table % 16) return fail("adamw: the table and the moments must be 16-byte aligned");
     if (!(o->beta1 >= 0.0 && o->beta1 < 1.0 && o->beta2 >= 0.0 && o->beta2 < 1.0)) return fail("adamw: betas %g, %g outside [0, 1)", o->beta1, o->beta2);
     // the step adds it in f32: what vanishes there would divide 0 by 0
@@ -604,7 +606,7 @@ SABAH_API int sabah_adamw_step(const sabah_adamw_desc* o, void* stream) {
     const size_t at = o->n_tensors > 0 ? adamw_chunks_at(o->n_tensors) : 0;
     if (o->n_tensors <= 0 || o->table_bytes < at || (o->table_bytes - at) % sizeof(AdamChunk) || (o->table_bytes - at) / sizeof(AdamChunk) >= 1u << 24)
         return fail("adamw: %zu bytes are no table of %d tensors", o->table_bytes, o->n_tensors);
-    if (o->table_bytes > at && (!o->m || !o->v || (o->bits == 8 && (!o->m_scale || !o->v_scale)))) return fail("adamw: null pointer");
+    if (o->table_bytes > at && (!o->m || !o->v || (bits == 8 && (!o->m_scale || !o->v_scale)))) return fail("adamw: null pointer");
     const size_t ws = sabah_adamw_workspace();
     if (!o->workspace || o->workspace_bytes < ws || (uintptr_t)o->workspace % 16)
         return fail("adamw: the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", ws, o->workspace_bytes);
@@ -616,7 +618,7 @@ SABAH_API int sabah_adamw_step(const sabah_adamw_desc* o, void* stream) {
     a.tensors = static_cast<const AdamTensor*>(o->table);
     a.chunks = reinterpret_cast<const AdamChunk*>(static_cast<const uint8_t*>(o->table) + at);
     a.n_chunks = (int)((o->table_bytes - at) / sizeof(AdamChunk));
-    a.bits = o->bits;
+    a.bits = bits;
     a.m = o->m;
     a.v = o->v;
     a.m_scale = o->m_scale;
@@ -637,8 +639,10 @@ SABAH_API int sabah_adamw_step(const sabah_adamw_desc* o, void* stream) {
     if (a.norm && a.parts) hipLaunchKernelGGL(k_adamw_norm, dim3((unsigned)a.parts), dim3(kAdamThreads), 0, st, a);
     hipLaunchKernelGGL(k_adamw_begin, dim3(1), dim3(a.norm ? 1024 : 64), 0, st, a);
     if (a.n_chunks) {
-        if (a.bits == 32) hipLaunchKernelGGL(k_adamw_step<32>, dim3((unsigned)a.n_chunks), dim3(kAdamThreads), 0, st, a);
-        else hipLaunchKernelGGL(k_adamw_step<8>, dim3((unsigned)a.n_chunks), dim3(kAdamThreads), 0, st, a);
+        const dim3 grid((unsigned)a.n_chunks), block(kAdamThreads);
+        if (bits == 32) hipLaunchKernelGGL((k_adamw_step<32, false>), grid, block, 0, st, a);
+        else if (!unbiased) hipLaunchKernelGGL((k_adamw_step<8, false>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((k_adamw_step<8, true>), grid, block, 0, st, a);
     }
     return ck(hipGetLastError(), "adamw launch") ? 0 : -1;
 }

@@ -75,6 +75,9 @@ class ExpertDesc(ctypes.Structure):
     _fields_ = [("w", c_vp), ("type", c_i), ("n_experts", c_i), ("k", c_i), ("rows", c_i)]
 
 
+ADAMW_UNBIASED = 0x100                          # SABAH_ADAMW_UNBIASED
+
+
 class AdamWTensor(ctypes.Structure):
     """sabah_adamw_tensor (include/sabah_rt.h)."""
     _fields_ = [("p", c_vp), ("g", c_vp), ("master", c_vp), ("decay", ctypes.c_double), ("n", ctypes.c_longlong),

@@ -139,3 +139,125 @@ def test_inputs_and_results_as_columns_of_one_buffer(ex, T):
     buf[:, :, k:] = dy
     dx, dw = ex.expert_mul_backward(e, x, groups, buf[:, :, k:], dx=buf[:, :, :k])
     assert torch.equal(dx, want[1][0]) and torch.equal(dw, want[1][1]) and torch.equal(buf[:, :, k:], dy)
+
+
+# ---- unbiased moments of 8 bits ------------------------------------------------
+def unbiased(p, grad, **kw):
+    return adamw(p, grad, bits=8, unbiased=True, **kw)
+
+
+def test_unbiased_codes_are_the_two_around_a_value_in_proportion(hip_rt):
+    """Against the 64-bit values of the same step: below or above, by shares that fit (six standard deviations of that many
+    independent choices), another choice in another step, and codes that a value hits exactly kept."""
+    n = 1 << 16
+    g = torch.Generator().manual_seed(11)
+    opt = unbiased(torch.zeros(n), torch.randn(n, generator=g), betas=(0.9, 0.999))
+    for _ in range(3):
+        opt.step()
+    kept = [t.clone() for t in (opt.m, opt.v, opt.m_scale, opt.v_scale)]
+    ups = []
+    for steps in (3, 4):
+        for t, k in zip((opt.m, opt.v, opt.m_scale, opt.v_scale), kept):
+            t.copy_(k)
+        opt.step_count.fill_(steps)
+        opt.step()
+        torch.cuda.synchronize()
+        m0 = R.m_value(kept[0].cpu()).reshape(-1, 256) * kept[2].cpu().double()[:, None]
+        v0 = R.v_value(kept[1].cpu()).reshape(-1, 256) * kept[3].cpu().double()[:, None]
+        grad = opt.grads[0].cpu().double().reshape(-1, 256)
+        m, v = 0.9 * m0 + 0.1 * grad, 0.999 * v0 + 0.001 * grad * grad
+        for x, scale, code, top, power in ((m, opt.m_scale, opt.m, 127, 2), (v, opt.v_scale, opt.v, 255, 4)):
+            s = scale.cpu()
+            # 0.9 s + 0.1 g of f32's numbers is often half way between two of them, where an error of 64 bits decides: half a step
+            assert ((s.double() - x.abs().amax(1)).abs() <= R.U * (1 + 1e-6) * s.double()).all()
+            t = (x.abs() / s.double()[:, None]).clamp(max=1) * top ** power
+            low = torch.floor((t * (1 + 1e-12)).pow(1 / power)).clamp(max=top - 1)
+            share = ((t - low ** power) / ((low + 1) ** power - low ** power)).clamp(0, 1)
+            code = code.cpu().reshape(-1, 256).double()
+            assert ((code == 0) | (torch.sign(code) == torch.sign(x))).all()
+            up = code.abs() - low
+            edge = (share < 1e-9) | (share > 1 - 1e-9) | ((low == 0) if power == 4 else (low < 0))   # v above 0 never becomes 0
+            assert (((up == 0) | (up == 1)) | edge).all() and (up[share > 1 - 1e-9] == 1).all()
+            if power == 4:
+                assert (code[x > 0] >= 1).all()
+            u, q = up[~edge], share[~edge]
+            assert (u - q).sum().abs() <= 6 * (q * (1 - q)).sum().sqrt()
+            for part in (q < 0.1, q > 0.9):                 # and where one of them is likely
+                assert (u - q)[part].sum().abs() <= 6 * (q * (1 - q))[part].sum().sqrt()
+            ups.append((up, share))
+    for a, b in ((0, 2), (1, 3), (0, 1)):                  # m in two steps, v in two steps, m and v: no common choice
+        (x, p), (y, q) = ups[a], ups[b]
+        r = (x - p) * (y - q)
+        assert r.sum().abs() <= 6 * (p * (1 - p) * q * (1 - q)).sum().sqrt() + 1e-3 * n ** 0.5
+
+
+@pytest.mark.parametrize("largest", [False, True])
+def test_unbiased_second_moments_over_thousands_of_steps(hip_rt, largest):
+    """The mean of v against the unrounded recurrence, at beta2 = 0.999: even noise; and one value of each block that stays
+    while the gradients of the others become a tenth.  A step moves v by 0.001 of itself; the choice between two codes 4 / k
+    apart then has a variance of at most 0.004 / k of v^2, which later steps forget by 0.998: 2 / k.  While v falls, nothing is forgotten
+    relative to v: 6,000 times 0.004 / k more.  k >= 128 under even noise (all values within 16 times), >= 80 at the end of the fall.  Over n values six
+    standard deviations of their mean; the values' choices are independent."""
+    n = 64 * 256
+    g = torch.Generator(device=DEV).manual_seed(12)
+    grad = torch.zeros(n, device=DEV)
+    opt = unbiased(torch.zeros(n), grad, betas=(0.9, 0.999))
+    grad, want = opt.grads[0], torch.zeros(n, dtype=torch.float64, device=DEV)
+    first = torch.arange(n, device=DEV) % 256 == 0
+    for step in range(8000 if largest else 5000):
+        grad.normal_(generator=g)
+        if largest and step >= 2000:
+            grad.mul_(torch.where(first, 1.0, 0.1))
+        opt.step()
+        want.mul_(0.999).add_(grad.double().square(), alpha=0.001)
+    v = opt.moments()[1].double()
+    far = (v[~first].mean() / want[~first].mean() - 1).abs().item()
+    spread = math.sqrt(2 / 80 + 6000 * 0.004 / 80) if largest else math.sqrt(2 / 128)
+    assert far <= 6 * spread / math.sqrt(n - 64), far
+
+
+def test_unbiased_steps_repeat_and_replay(hip_rt):
+    """The same bits from the same state, eager or replayed; a step by R.adamw's rule from the values of the codes."""
+    from sabah.runtime.adamw import AdamW
+    g = torch.Generator().manual_seed(13)
+    sizes = [1, 255, 257, 5000]
+    start, gs = [torch.randn(n, generator=g).to(BF16) for n in sizes], [torch.randn(n, generator=g).to(DEV) for n in sizes]
+    a, b = (AdamW([t.to(DEV) for t in start], gs, bits=8, unbiased=True, max_norm=3.0, master=True) for _ in range(2))
+    a.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    b.step()
+    for i in range(3):
+        for t in gs:
+            t.mul_(-0.9)
+        m0, v0 = (t.clone() for t in b.moments())
+        p0 = b.master.clone()
+        graph.replay()
+        b.step()
+        torch.cuda.synchronize()
+        for x, y in zip(a.params + [a.m, a.v, a.m_scale, a.v_scale, a.master, a.grad_norm, a.step_count],
+                        b.params + [b.m, b.v, b.m_scale, b.v_scale, b.master, b.grad_norm, b.step_count]):
+            assert torch.equal(x, y)
+        c = min(1.0, 3.0 / (math.sqrt(sum(t.double().square().sum().item() for t in gs)) + 1e-6))
+        for j, (n, at) in enumerate(zip(sizes, b.starts)):
+            rows = slice(at, at + n)
+            want, _, v, step = R.adamw(p0[rows].cpu(), gs[j].cpu(), m0[rows].cpu(), v0[rows].cpu(), i + 2, 1e-3, (0.9, 0.999), 1e-8, 0.01, c)
+            q = gs[j].cpu().double().abs() * c
+            tm = 6 * R.U * (m0[rows].cpu().double().abs() + q) + 1e-44
+            scale = 1e-3 / (1 - 0.9 ** (i + 2)) / ((v / (1 - 0.999 ** (i + 2))).sqrt() + 1e-8)
+            R.close(b.master[rows], want, scale * tm + 20 * R.U * step.abs() + 3 * R.U * (p0[rows].cpu().double().abs() + step.abs()), "p")
+
+
+def test_unbiased_moments_of_zeros_and_nan(hip_rt):
+    """Values without a gradient keep moments of 0; a NaN becomes its block's; other blocks and what lies behind the tensor stay."""
+    grad = torch.zeros(1000)
+    grad[256:512], grad[600] = 1.0, float("nan")
+    opt = unbiased(torch.ones(1000), grad)
+    for _ in range(3):
+        opt.step()
+    torch.cuda.synchronize()
+    m, v = (t.cpu() for t in opt.moments())
+    assert (m[:256] == 0).all() and (v[:256] == 0).all() and (opt.params[0][:256] == 1).all()
+    assert (opt.m[256:512] == 127).all() and (opt.v[256:512] == 255).all()      # all at the block's largest: exact
+    assert m[512:768].isnan().all() and (m[768:] == 0).all() and (v[768:] == 0).all()
