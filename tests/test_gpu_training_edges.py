@@ -261,3 +261,70 @@ def test_unbiased_moments_of_zeros_and_nan(hip_rt):
     assert (m[:256] == 0).all() and (v[:256] == 0).all() and (opt.params[0][:256] == 1).all()
     assert (opt.m[256:512] == 127).all() and (opt.v[256:512] == 255).all()      # all at the block's largest: exact
     assert m[512:768].isnan().all() and (m[768:] == 0).all() and (v[768:] == 0).all()
+
+
+# ---- experts: stages and the ends of the types --------------------------------
+def products(ex, w, x, ids, dy):
+    """(y, dx, dw) on the device."""
+    from sabah.runtime import rt
+    from sabah.runtime.experts import FloatExperts
+    e = FloatExperts(w.shape[0], w.shape[2], w.shape[1], dtype=w.dtype, device=DEV)
+    e.w.copy_(w)
+    groups = ex.group_rows(ids.to(DEV), e.n_experts)
+    y = ex.expert_mul(e, x.to(DEV), groups)
+    dx, dw = ex.expert_mul_backward(e, x.to(DEV), groups, dy.to(DEV))
+    torch.cuda.synchronize()
+    rt.check(rt.lib().sabah_rt_check_errors(), "experts")
+    return y, dx, dw
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("last,k", [(1, 640), (33, 648), (70, 1024), (100, 72), (129, 640), (225, 1000)])
+def test_sums_of_many_stages_in_tiles_of_256_rows(ex, last, k, dtype):
+    """Two experts of more than 384 rows each on average and 24 x 8 tiles: the largest form, its three stages used again and again, by
+    tiles of all numbers of 32-row results.  Whole numbers: sums are exact, results equal."""
+    from sabah.runtime.experts import FloatExperts
+    g = torch.Generator().manual_seed(last)
+    T, rows = 6144 + last, 2048
+    w = torch.randint(-3, 4, (2, rows, k), generator=g).to(TYPES[dtype])
+    x = torch.randint(-3, 4, (T, k), generator=g).to(TYPES[dtype])
+    ids = torch.zeros(T, 1, dtype=torch.int32)
+    ids[torch.randperm(T, generator=g)[:last]] = 1
+    e = FloatExperts(2, k, rows, dtype=TYPES[dtype], device=DEV)
+    e.w.copy_(w)
+    y = ex.expert_mul(e, x.to(DEV), ex.group_rows(ids.to(DEV), 2))
+    torch.cuda.synchronize()
+    want = torch.empty(T, rows, dtype=torch.float64)
+    for i in (0, 1):
+        at = ids[:, 0] == i
+        want[at] = x[at].double() @ w[i].double().t()
+    assert torch.equal(y[:, 0].cpu(), want.to(TYPES[dtype]))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("T,k,rows", [(5, 64, 96), (5, 63, 35), (90, 72, 128), (90, 71, 35)])
+@pytest.mark.parametrize("what", ["subnormal", "large and small"])
+def test_products_at_the_ends_of_their_types(ex, T, k, rows, dtype, what):
+    """Operands below the type's normal numbers, and factors far from 1 whose products are not; in the streamed, the direct and
+    the staged form.  Every product is a whole number of one unit and each sum exact in f32, so results equal."""
+    t = TYPES[dtype]
+    g = torch.Generator().manual_seed(7)
+    ids = torch.randint(0, 3, (T, 2), generator=g, dtype=torch.int32)
+    step = torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    up = {"f32": 100, "f16": 12, "bf16": 100}[dtype]
+    a, b = (step, 1.0) if what == "subnormal" else (2.0 ** up, 2.0 ** -up)
+
+    def whole(*shape):
+        return torch.randint(-3, 4, shape, generator=g).double()
+    for small in ("w", "x"):                       # which operand has the far values; dy goes with the other one's
+        w = (whole(3, rows, k) * (a if small == "w" else b)).to(t)
+        x = (whole(T, 1, k) * (a if small == "x" else b)).to(t)
+        dy = (whole(T, 2, rows) * (a if small == "x" else b)).to(t)
+        y, dx, _ = products(ex, w, x, ids, dy)
+        assert torch.equal(y.cpu(), R.expert_mul(w, x, ids)[0].to(t)), ("y", small)
+        (wx, _), _ = R.expert_back(w, x, ids, dy)
+        assert torch.equal(dx.cpu(), wx.to(t)), ("dx", small)
+        dy = whole(T, 2, rows).mul(b if small == "x" else a).to(t)
+        _, _, dw = products(ex, w, x, ids, dy)
+        _, (ww, _) = R.expert_back(w, x, ids, dy)
+        assert torch.equal(dw.cpu().double(), ww), ("dw", small)
