@@ -10,13 +10,14 @@
 // b2 = 0.999 a v below its block's largest decays with the block's scale alone (a step of 0.1 %, half a code is 0.8 % at least), and
 // only squares of many times v raise it.  So v comes out too large over some thousand steps: 1.1 times after 2,000 of even
 // noise, 1.4 after 5,000 (single blocks 2.5); 45 times where all but one gradient of a block became a tenth.
-// UNBIASED codes take the lower or the upper of the two codes around a value in proportion to where it lies between them, so that moments are right in the mean at
-// any b1 and b2 (both: an m that the nearest code holds up would be divided by a v that goes on falling), with a noise of at
-// most sqrt(2 / code) of v, 9 % near the block's largest.  The choice is a hash of the step's number and the value's place, so
-// that a state and a gradient give the same bits again (302 M values in bf16 with master copies: 1,400 us a step, 1,217 with the nearest).
+// UNBIASED codes take the lower or the upper of the two codes around a value in proportion to where it lies between them, so
+// that moments are right in the mean at any b1 and b2 (both: an m that the nearest code holds up would be divided by a v that
+// goes on falling), with a noise of at most sqrt(2 / code) of v, 9 % near the block's largest.  The choice is a hash of the step's
+// number and the value's place, so that a state and a gradient give the same bits again (302 M values in bf16 with master
+// copies: 1,400 us a step, 1,217 with the nearest codes).
 //
 // k_adamw_norm:  the gradients' sum of squares in 64 bits, by a fixed number of workgroups, in a fixed order.
-// k_adamw_begin: the norm, the step's number and what depends on them, by one wave.
+// k_adamw_begin: the norm, the step's number and what depends on them, by one workgroup (of one wave where no norm is wanted).
 // k_adamw_step:  2,048 values of one tensor to a workgroup; every state is read and written once, which bounds it: 604 M values
 //   in f32 3,180 us, 5.3 TB/s; 302 M in bf16 with master copies and 8-bit moments 1,080 us, 5.0 TB/s (1,430 with f32's
 //   correctly rounded roots and division, which the 64-bit codes do not need: they are found by their borders).
@@ -284,8 +285,6 @@ __device__ inline void adam_roots(const float (&v)[4], float (&r)[4]) {
             if (v[j] < 0x1p-126f) r[j] = __builtin_amdgcn_sqrtf(v[j] * 0x1p64f) * 0x1p-32f;
     }
 }
-
-__device__ inline void adam_codes_load(const uint8_t* p, uint32_t& c) { c = *reinterpret_cast<const uint32_t*>(p); }
 
 template <int BITS, bool UNBIASED>
 __global__ __launch_bounds__(kAdamThreads) void k_adamw_step(AdamArgs a) {

@@ -63,7 +63,8 @@ static MemRows norm_mem(const sabah_norm_desc* n, int n_tokens, const void* p, s
     return {p, stride, n->width * float_size(n->type), n_tokens};
 }
 
-// Waves of a row, 8 values a thread: 2,560 columns fill five of them and would leave three of eight idle
+// Waves of a row, 8 values a thread: 2,560 columns fill five of them and would leave three of eight idle (19.0 us against 15.2 for
+// 4,001 tokens in bf16).  Other widths between two counts leave up to half of the waves idle: no forms of their own so far
 template <typename F>
 static void norm_waves(int width, F go) {
     if (width <= 512) go(std::integral_constant<int, 1>{});
@@ -291,7 +292,7 @@ SABAH_API int sabah_expert_group(const int32_t* d_ids, size_t ids_id_stride, siz
     hipStream_t st = pick_stream(stream);
     const int keys = n_experts + 2;
     constexpr auto lds_of = [](int keys, bool sums) { return kExpGroupWaves * (8 + (keys + 1) / 2 * 4) + (sums ? 2 : 1) * keys * 4; };
-    static_assert(lds_of(kExpMaxExperts + 2, false) <= 160 * 1024 && lds_of(kExpMaxExperts + 2, true) <= 168 * 1024, "a workgroup's LDS");
+    static_assert(lds_of(kExpMaxExperts + 2, false) <= 160 * 1024, "a workgroup's LDS");   // with sums 4,096 experts have more: below
     const dim3 grid((unsigned)a.p.chunks), block(kExpGroupThreads);
     if (a.p.n_rows <= kExpFewGroup) {
         hipLaunchKernelGGL(k_expert_group_few, dim3(1), dim3(256), 0, st, a);
@@ -391,12 +392,14 @@ static int launch_expert_dw(const char* what, const ExpertArgs& a, hipStream_t s
     hipLaunchKernelGGL(kernel, grid, dim3(64 * G::NW), G::kLds, st, a);
     return ck(hipGetLastError(), what) ? 0 : -1;
 }
-// Which tile, of 16-bit types (us in bf16, 8 experts unless said; rows to an expert):
-//   128 x 64   while tiles of 128 x 256 are too few for the card: forward 2,048 -> 768 at 256 rows 20.1 against 33.6, at 512
-//              32.4 and 35.1, at 1,024 (216 tiles) 61.8 and 40.4; dx at 128 rows 20.3 and 25.2, at 512 (288 tiles) 42.3 and 34.7
-//   256 x 256  forward, from 384 rows and three quarters of the card's tiles: of 128 experts at 256 rows 188 against 184, at
-//              512 270 and 315; at 8,192 rows 265 and 291, at 1,024 (60 tiles) 56 and 40.  Of dx, whose sums are shorter, 421 and 386
-//   128 x 256  else, and for dW: 338 against 356 with 256 x 256, 346 with 128 x 128; few tiles are not faster in 128 x 64 (14.4, 15.4)
+// Which tile, of 16-bit types (us in bf16, 8 experts unless said, 2,048 -> 768; rows to an expert):
+//   128 x 64   while tiles of 128 x 256 are too few for the card: forward at 256 rows 20.4 against 32.5, at 512 30.2 and 33.8,
+//              at 1,024 (216 tiles) 48.7 and 36.8; dx at 128 rows 13.8 and 18.8, at 512 (288 tiles) 40.7 and 26.8
+//   256 x 256  forward, from 384 rows and three quarters of the card's tiles: of 128 experts at 256 rows 186 against 168, at 384
+//              208 and 225, at 512 259 and 279; at 8,192 rows 210 and 240, at 2,048 58 and 67, at 1,024 (96 tiles) 54 and 37.  Of
+//              dx, whose sums are shorter, 353 and 330 (128 experts, 512 rows)
+//   128 x 256  else, and for dW: 338 against 356 with 256 x 256, 346 with 128 x 128 (128 experts, 256 rows, 768 -> 2,048); few tiles
+//              are not faster in 128 x 64 (14.4, 15.4)
 // f32's products take 64 cycles where loads take few: 128 x 128 with all four waves on all rows, so that a last tile's missing rows
 // are missing from each (600 rows of 8 experts: dx 53 us; dW in 128 x 64 46 - 52, in 128 x 128 50 - 58).
 constexpr int kExpLargeRows = 384;
