@@ -214,8 +214,12 @@ __global__ __launch_bounds__(norm_threads(W)) void k_block_norm_back(NormArgs a)
             o.store(a.dx + (size_t)t * a.dx_st, a.width, v);
         }
         if (a.dy) {
-            float c = a.scale, r = 0.0f, m = 0.0f;
-            if (a.gate) c *= norm_sigmoid(a.gate[t]);
+            float c = a.scale, shut = 0.0f, r = 0.0f, m = 0.0f;
+            if (a.gate) {
+                const float g = a.gate[t], e = expf(-g), sg = 1.0f / (1.0f + e);
+                c *= sg;
+                shut = g > 0.0f ? e * sg : 1.0f - sg;           // sigmoid(-gate)
+            }
             if (read_y) {
                 float syy = 0.0f, sdy = 0.0f;
 #pragma unroll
@@ -233,7 +237,7 @@ __global__ __launch_bounds__(norm_threads(W)) void k_block_norm_back(NormArgs a)
                     sdy *= r;                                   // sum(d n(y))
                     m = sdy * inv;
                 }
-                if (a.gate && v == 0) a.dgate[t] = norm_sigmoid(-a.gate[t]) * c * sdy;
+                if (a.gate && v == 0) a.dgate[t] = shut * c * sdy;
             }
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
