@@ -14,12 +14,12 @@
 // that moments are right in the mean at any b1 and b2 (both: an m that the nearest code holds up would be divided by a v that
 // goes on falling), with a noise of at most sqrt(2 / code) of v, 9 % near the block's largest.  The choice is a hash of the step's
 // number and the value's place, so that a state and a gradient give the same bits again (302 M values in bf16 with master
-// copies: 1,400 us a step, 1,217 with the nearest codes).
+// copies: 1,374 us, 1,098 with the nearest codes).
 //
 // k_adamw_norm:  the gradients' sum of squares in 64 bits, by a fixed number of workgroups, in a fixed order.
 // k_adamw_begin: the norm, the step's number and what depends on them, by one workgroup (of one wave where no norm is wanted).
 // k_adamw_step:  2,048 values of one tensor to a workgroup; every state is read and written once, which bounds it: 604 M values
-//   in f32 3,180 us, 5.3 TB/s; 302 M in bf16 with master copies and 8-bit moments 1,080 us, 5.0 TB/s (1,430 with f32's
+//   in f32 3,180 us, 5.3 TB/s; 302 M in bf16 with master copies and 8-bit moments 1,098 us, 4.9 TB/s (1,430 with f32's
 //   correctly rounded roots and division, which the 64-bit codes do not need: they are found by their borders).
 #pragma once
 #include "balance_kernels.h"   // row_max

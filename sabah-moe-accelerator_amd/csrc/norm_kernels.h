@@ -7,8 +7,8 @@
 //              from y, and dgate = sigmoid(gate) sigmoid(-gate) scale sum(d n(y)): 1 - sigmoid(gate) in f32 would have lost 6 % at a
 //              gate of 16 and all of it from 17
 // A row is held in registers by one wave or by a workgroup from its loads to its stores: each input is read and
-// each output written once, which is what bounds it (4,001 tokens of 2,560 in bf16 forward 15.2 us, 5.4 TB/s with the
-// last-level cache's help; 16,384 of 2,048 backward 91 us, 4.4 TB/s, and 6 for the weights' sums; a large copy 4.86).  8 values a
+// each output written once, which is what bounds it (4,001 tokens of 2,560 in bf16 forward 15.5 us, 5.3 TB/s with the
+// last-level cache's help; 16,384 of 2,048 backward 92 us, 4.4 TB/s, and 6 for the weights' sums; a large copy 4.86).  8 values a
 // thread: with 16 a row of 2,560 kept 4,096 places, 19.0 us, and the backward spilled.  Loading the next token's rows
 // ahead changed nothing (87 us), nor did 512 or 2,048 parts (96, 84 + 13).  Sums are f32, of rounded inputs; x', h, dx and dy are rounded once.
 #pragma once
