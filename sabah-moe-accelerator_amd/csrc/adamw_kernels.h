@@ -152,7 +152,7 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw_norm(AdamArgs a) {
     if (threadIdx.x == 0) a.part[blockIdx.x] = s;
 }
 
-// 64 bits of a number, by the finalizer of Stafford's variant 13 (the output function of the SplitMix64 generator)
+// 64 bits of a number: the SplitMix64 generator's output after it (Steele, Lea and Flood, 2014)
 __device__ inline uint64_t adam_mix(uint64_t z) {
     z += 0x9E3779B97F4A7C15ull;
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
